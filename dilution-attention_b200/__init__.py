@@ -15,7 +15,7 @@ After the first import it is also registered as `dilution_attention_b200`.
 
 import sys as _sys
 
-from . import _lib, kernels, kernels_bid, layers, partition  # noqa: F401
+from . import _lib, kernels, kernels_bid, layers, masked, partition, serving  # noqa: F401
 from .kernels import (  # noqa: F401
     dilution_attention,
     dilution_attention_forward,
@@ -34,6 +34,13 @@ from .layers import (  # noqa: F401
     split_heads_rope,
     uninstall_layers,
 )
+from .masked import softmax_attention  # noqa: F401
+from .serving import (  # noqa: F401
+    dilution_tree_step,
+    evict_cache,
+    softmax_tree_step,
+    tree_accept,
+)
 
 _sys.modules.setdefault("dilution_attention_b200", _sys.modules[__name__])
 
@@ -42,4 +49,5 @@ __all__ = [
     "dilution_attention_reference", "dilution_attention_host", "dilution_decode_step",
     "dilution_decode_append_step", "softmax_attention_forward", "softmax_decode_append_step",
     "split_heads_rope", "install", "uninstall", "install_layers", "uninstall_layers", "layers", "GraphedDecode",
+    "masked", "serving", "softmax_attention", "softmax_tree_step", "dilution_tree_step", "tree_accept", "evict_cache",
 ]

@@ -58,6 +58,17 @@ SIGNATURES = {
     "dilution_variant_backward": (_I, [_P, _P, _P, _I, _I, _L, _L, _I, _F, _F, _I, _I, _F,
                                        _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "dilution_variant_decode": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _F, _F, _I, _I, _F, _P, _P, _P, _P]),
+    "dilution_attend_ranges_bytes": (_Z, [_L, _L]),
+    "dilution_attend_forward": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _I, _F, _F, _P, _P, _P, _P, _P, _P, _P]),
+    "dilution_attend_backward": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _I, _F, _F, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                      _P]),
+    "dilution_tree_scratch_bytes": (_Z, [_L, _L, _I, _I, _L, _I]),
+    "dilution_tree_softmax": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _I, _I, _L, _L, _P, _I, _F, _F, _P, _P, _L, _P, _P, _P,
+                                   _P]),
+    "dilution_tree_dilute": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _I, _L, _L, _P, _I, _F, _F, _P, _P, _L, _P, _P, _P, _P]),
+    "dilution_tree_accept": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _I, _I, _L, _L, _P, _I, _F, _F, _P, _P, _L, _P, _P, _L, _I,
+                                  _P, _P, _P]),
+    "dilution_evict": (_I, [_P, _P, _P, _I, _L, _L, _L, _I, _P, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P]),
 }
 # codes of the reference's BID_TYPES (kernels_bid.py:84) for the bids that are built
 BID = {"softmax": 0, "relu": 1, "relu2": 2, "softplus": 3, "minshift": 4, "sigmoid": 5, "expshift": 6, "sigshift": 7}

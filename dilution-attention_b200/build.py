@@ -2,16 +2,18 @@
 
     python dilution-attention_b200/build.py [--force]
 
-The library is rebuilt only when a source under csrc/ or include/ is newer than
-the existing .so.  nvcc cross-compiles without a GPU.
+A translation unit is compiled again only when it or a file that it includes is newer than its
+object.  nvcc cross-compiles without a GPU.
 """
 
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -21,21 +23,34 @@ LIB = os.path.join(HERE, "libdilution_b200.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xptxas=-v",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
+UNITS = ("abi.cu", "operators.cu")     # one object each, next to its source
 
 
-def _sources():
-    files = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh"))]
-    files.append(os.path.join(ROOT, "include", "dilution_b200.h"))
-    return files
+def _includes(path, seen=None):
+    """The file and every file of this repository that it includes."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path in seen or not os.path.exists(path):
+        return seen
+    seen.add(path)
+    with open(path) as f:
+        for name in re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M):
+            _includes(os.path.join(os.path.dirname(path), name), seen)
+    return seen
+
+
+def _object(unit):
+    return os.path.join(CSRC, unit.replace(".cu", ".o"))
+
+
+def _stale(target, sources):
+    return not os.path.exists(target) or any(os.path.getmtime(f) > os.path.getmtime(target) for f in sources)
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
-        return True
-    built = os.path.getmtime(LIB)
-    return any(os.path.getmtime(f) > built for f in _sources())
+    return any(_stale(LIB, _includes(os.path.join(CSRC, unit))) for unit in UNITS)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -44,11 +59,17 @@ def build(force: bool = False, verbose: bool = False) -> str:
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     if not os.path.exists(nvcc):
         raise RuntimeError("nvcc not found: cannot build libdilution_b200.so")
-    cmd = [nvcc, *NVCC_FLAGS, "-o", LIB, os.path.join(CSRC, "abi.cu"), "-lcuda"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or proc.returncode != 0:
-        sys.stderr.write(proc.stdout + proc.stderr)
-    if proc.returncode != 0:
+
+    def run(cmd):
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose or proc.returncode != 0:
+            sys.stderr.write(proc.stdout + proc.stderr)
+        return proc.returncode
+
+    units = [u for u in UNITS if force or _stale(_object(u), _includes(os.path.join(CSRC, u)))]
+    with ThreadPoolExecutor() as pool:
+        codes = list(pool.map(lambda u: run([nvcc, *NVCC_FLAGS, "-c", "-o", _object(u), os.path.join(CSRC, u)]), units))
+    if any(codes) or run([nvcc, *NVCC_FLAGS, "-shared", "-o", LIB, *map(_object, UNITS), "-lcuda"]):
         raise RuntimeError("nvcc failed building libdilution_b200.so")
     return LIB
 

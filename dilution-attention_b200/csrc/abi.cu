@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/dilution_b200.h"
+#include "abi_internal.h"
 #include "decode_kernels.cuh"
 #include "layer_kernels.cuh"
 #include "simt_kernels.cuh"
@@ -473,6 +474,21 @@ int check_carry_rows(const char* fn, int dtype, int precision, int d, int64_t q_
 }
 }  // namespace
 
+namespace dil {
+
+int abi_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int abi_check_launch(const char* what) { return check_launch(what); }
+LaunchMark::LaunchMark(const char* name, cudaStream_t st) : prof_(new Prof(name, st)) {}
+LaunchMark::~LaunchMark() { delete static_cast<Prof*>(prof_); }
+
+}  // namespace dil
+
 extern "C" {
 
 int dilution_carry_rows(int dtype, int precision, int d, int training) {
@@ -490,6 +506,8 @@ int dilution_device_status(void) {
 #ifdef DILUTION_TENSOR_PATH
   int v = 0;
   if (dil::tc::read_status(&v) != 0) return fail(DILUTION_ERR_CUDA, "dilution_device_status: could not read the status word");
+  if (v == 0 && dil::operators_read_status(&v) != 0)
+    return fail(DILUTION_ERR_CUDA, "dilution_device_status: could not read the status word");
   if (v != 0) return fail(DILUTION_ERR_DEVICE, "a kernel gave up a bounded wait (code %d)", v);
 #endif
   return DILUTION_OK;

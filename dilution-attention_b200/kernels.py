@@ -704,7 +704,7 @@ def _fused_step_cache(self, x1, cache):
         from . import layers
         q1, k1, v1 = layers.split_heads_at(self, x1, cache)
     else:
-        q1, k1, v1 = self._split_heads(x1, offset=cache["len"])
+        q1, k1, v1 = self._split_heads(x1, offset=cache["len"] + cache.get("evicted", 0))
     y = dilution_decode_append_step(q1, k1, v1, cache).to(q1.dtype)
     return self._merge_heads(y, batch, 1)
 

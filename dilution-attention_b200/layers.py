@@ -198,6 +198,8 @@ class GraphedDecode:
         self.position = caches[0]["len"]
         if any(c["len"] != self.position for c in caches):
             raise ValueError("all layers' caches must hold the same number of tokens")
+        if model.config.positional != "none" and any(c.get("evicted") for c in caches):
+            raise ValueError("a recorded step rotates by the cache's length, which evicted keys are missing from")
         self.pos_dev = torch.tensor([self.position], device=dev, dtype=torch.int32)
         for c in caches:
             c["pos_dev"] = self.pos_dev
@@ -303,7 +305,7 @@ def _softmax_step_cache(self, x1, cache):
     if cache.get("pos_dev") is not None:       # the position lives on the device (a captured step)
         q1, k1, v1 = split_heads_at(self, x1, cache)
         return self._merge_heads(softmax_decode_append_step(q1, k1, v1, cache), batch, 1)
-    q1, k1, v1 = self._split_heads(x1, offset=cache["len"])
+    q1, k1, v1 = self._split_heads(x1, offset=cache["len"] + cache.get("evicted", 0))
     if q1.dtype not in (torch.float32, torch.bfloat16) or cache["k"].dtype != q1.dtype:
         t = self._append_kv(cache, k1, v1)
         y = torch.nn.functional.scaled_dot_product_attention(q1, cache["k"][:, :, :t], cache["v"][:, :, :t])

@@ -393,6 +393,64 @@ int dilution_variant_decode(const void* q1, const void* k1, const void* v1, void
                             float eps, int bid, int share, float shift, float* committed, void* out, void* scratch,
                             void* stream);
 
+/* ---- masked softmax attention (no counterpart in the reference, whose softmax layers are causal only) -----------
+ * q, out (batch, heads, t, d); k, v (batch, kv_heads, t, d), query head h on key head h / (heads / kv_heads); dtype
+ * of all of them DILUTION_F32 or DILUTION_BF16, 16-byte aligned.  Scores scale q.k, through cap * tanh(x / cap) if cap > 0,
+ * minus slopes[h] * |i - j| if slopes (heads fp32) is not NULL.  Query i of a sequence sees key j where j <= i, or
+ * j < prefix[b] if prefix (batch) is not NULL, and where documents (batch, t), if not NULL, gives both the same id >= 0.  A
+ * query that sees no key has out = 0 and lse = +inf.  With documents, `ranges` is a buffer of
+ * dilution_attend_ranges_bytes(batch, t) that the forward fills and the backward reads.  lse (batch, heads, t) fp32: log2 of
+ * the sum of 2^(score log2 e), or NULL.
+ * The backward takes what the forward wrote, dout like out, and delta (batch, heads, t) fp32 as scratch; dq, dk, dv are like
+ * q, k, v.  All results repeat bit for bit. */
+size_t dilution_attend_ranges_bytes(int64_t batch, int64_t t);
+int dilution_attend_forward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
+                            int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
+                            const int* documents, const int* prefix, void* ranges, void* out, float* lse, void* stream);
+int dilution_attend_backward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
+                             int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
+                             const int* documents, const int* prefix, const void* ranges, const void* out, const float* lse,
+                             const void* dout, float* delta, void* dq, void* dk, void* dv, void* stream);
+
+/* ---- draft trees over a cache -------------------------------------------------------------------------------------
+ * `nodes` (1 to 64) drafted tokens of each sequence: q, out (batch, kv_heads * group, nodes, d), k_new, v_new
+ * (batch, kv_heads, nodes, d), caches (batch, kv_heads, capacity, d) of which the first `length` rows (or *length_dev, held
+ * inside the cache, if that is not NULL) are valid.  parents: int32, parent_stride apart for each sequence (0: one tree for
+ * all), the earlier node that a node follows; anything else makes it follow the last cached token.  Node x sees the cached
+ * keys, its ancestors and itself, at position length + its depth.  lse (batch, heads, nodes) fp32 out: log2 of the sum of
+ * 2^(score log2 e).  Scratch of dilution_tree_scratch_bytes(batch, kv_heads, group, nodes, length, d) bytes (the capacity in
+ * place of the length with length_dev).  The caches are only read.
+ *   dilution_tree_softmax: softmax attention, scores capped and biased as in dilution_attend_forward.
+ *   dilution_tree_dilute : the dilution operator: each node's bids meet committed (batch, heads, capacity) fp32 plus the bids of
+ *                          its ancestors, as a chain of dilution_decode steps along its branch would.
+ *   dilution_tree_accept : rows of k_new, v_new of the nodes path[0 .. accepted) (path_stride apart for each sequence, indices
+ *                          held inside the tree) go to cache rows length, length + 1, ...; if committed (batch, kv_heads,
+ *                          capacity) is not NULL, advanced (which may be committed) is committed plus the bids of those nodes,
+ *                          and of one another for their own keys, from q and the step's lse. */
+size_t dilution_tree_scratch_bytes(int64_t batch, int64_t kv_heads, int group, int nodes, int64_t length, int d);
+int dilution_tree_softmax(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache, int dtype,
+                          int64_t batch, int64_t kv_heads, int group, int nodes, int64_t capacity, int64_t length,
+                          const int* length_dev, int d, float scale, float cap, const float* slopes, const int* parents,
+                          int64_t parent_stride, float* lse, void* out, void* scratch, void* stream);
+int dilution_tree_dilute(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache, int dtype,
+                         int64_t batch, int64_t heads, int nodes, int64_t capacity, int64_t length, const int* length_dev, int d,
+                         float scale, float eps, const float* committed, const int* parents, int64_t parent_stride, float* lse,
+                         void* out, void* scratch, void* stream);
+int dilution_tree_accept(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, int dtype,
+                         int64_t batch, int64_t kv_heads, int group, int nodes, int64_t capacity, int64_t length,
+                         const int* length_dev, int d, float scale, float cap, const float* slopes, const int* parents,
+                         int64_t parent_stride, const float* lse, const int* path, int64_t path_stride, int accepted,
+                         const float* committed, float* advanced, void* stream);
+
+/* ---- eviction ----------------------------------------------------------------------------------------------------------
+ * Of each of n rows of a cache (n, capacity, d) with `length` valid keys, `keep` stay: the first `sinks`, the last `recent`
+ * and those of the highest scores (n, score_stride) between them (NaN above every number, equal ones the earlier first), in
+ * their order.  k_out, v_out (n, new_capacity, d) and, if committed is not NULL, committed_out (n, new_capacity) get their
+ * rows and zeros behind them; index (n, keep) their positions. */
+int dilution_evict(const void* k_cache, const void* v_cache, const float* committed, int dtype, int64_t n, int64_t capacity,
+                   int64_t length, int d, const float* scores, int64_t score_stride, int64_t keep, int64_t recent, int64_t sinks,
+                   int64_t new_capacity, void* k_out, void* v_out, float* committed_out, int* index, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
