@@ -10,12 +10,20 @@
 #include "attend_simt.cuh"
 #include "evict_kernels.cuh"
 #include "once_per_device.cuh"
+#include "tc_attend.cuh"
 #include "tree_simt.cuh"
 
 namespace dil {
 
 int operators_read_status(int* code) {
-  *code = 0;
+  int v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return 3;
+  if (cudaMemcpyFromSymbol(&v, tc::g_attend_status, sizeof(int)) != cudaSuccess) return 3;
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(tc::g_attend_status, &zero, sizeof(int));
+  }
+  *code = v;
   return 0;
 }
 
@@ -113,6 +121,67 @@ template <typename T, int D> int simt_backward(const attend::Args& a, cudaStream
   attend::simt_dq_kernel<T, D><<<grid, attend::kSimtThreads, smem, st>>>(a);
   return abi_check_launch("attend_dq");
 }
+
+// ---- the same on the tensor cores
+struct AttendMaps {
+  CUtensorMap q, k, v, dout;
+};
+int attend_maps(AttendMaps& m, const attend::Args& a, int d, int q_box, int k_box) {
+  const int64_t nq = (int64_t)a.batch * a.heads, nk = (int64_t)a.batch * a.kv_heads;
+  if (!tc::attend_map(&m.q, a.q, nq, a.t, d, q_box) || !tc::attend_map(&m.k, a.k, nk, a.t, d, k_box) ||
+      !tc::attend_map(&m.v, a.v, nk, a.t, d, k_box) || (a.dout && !tc::attend_map(&m.dout, a.dout, nq, a.t, d, q_box)))
+    return abi_fail(DILUTION_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  return DILUTION_OK;
+}
+// f(bool_constant<cap>, bool_constant<bias>)
+template <typename F> int with_score(const attend::Args& a, F f) {
+  if (a.cap > 0.f) return a.slopes ? f(std::true_type(), std::true_type()) : f(std::true_type(), std::false_type());
+  return a.slopes ? f(std::false_type(), std::true_type()) : f(std::false_type(), std::false_type());
+}
+
+template <int D, int NT> int tc_forward(const attend::Args& a, cudaStream_t st) {
+  using F = tc::AttendForward<D, NT>;
+  AttendMaps m;
+  if (int rc = attend_maps(m, a, D, 128, 64)) return rc;
+  return with_score(a, [&](auto cap, auto bias) {
+    auto kernel = tc::attend_forward_kernel<D, NT, cap(), bias()>;
+    if (int rc = opt_in(kernel, F::kBytes)) return rc;
+    LaunchMark mark("attend_forward", st);
+    const unsigned grid = (unsigned)((int64_t)a.batch * a.heads * ((a.t + 128 * NT - 1) / (128 * NT)));
+    kernel<<<grid, F::kThreads, F::kBytes, st>>>(m.q, m.k, m.v, a);
+    return abi_check_launch("attend_forward");
+  });
+}
+
+template <int D, int STAY> int tc_backward_half(const attend::Args& a, const AttendMaps& m, const float2* stats, cudaStream_t st) {
+  using F = tc::AttendBackward<D, STAY>;
+  return with_score(a, [&](auto cap, auto bias) {
+    auto kernel = tc::attend_backward_kernel<D, STAY, cap(), bias()>;
+    if (int rc = opt_in(kernel, F::kBytes)) return rc;
+    LaunchMark mark(STAY ? "attend_dkv" : "attend_dq", st);
+    const unsigned grid = (unsigned)((int64_t)a.batch * (STAY ? a.kv_heads : a.heads) * ((a.t + 127) / 128));
+    kernel<<<grid, F::kThreads, F::kBytes, st>>>(m.q, m.dout, m.k, m.v, a, stats);
+    return abi_check_launch("attend_backward");
+  });
+}
+
+template <int D> int tc_backward(const attend::Args& a, float2* stats, cudaStream_t st) {
+  AttendMaps m;
+  if (int rc = attend_maps(m, a, D, 64, 64)) return rc;
+  {
+    LaunchMark mark("attend_delta", st);
+    const int64_t threads = (int64_t)a.batch * a.heads * ((a.t + 63) / 64 * 64) * (D / 8);
+    tc::attend_stats_kernel<D><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a, stats);
+    if (int rc = abi_check_launch("attend_delta")) return rc;
+  }
+  if (int rc = tc_backward_half<D, 1>(a, m, stats, st)) return rc;
+  return tc_backward_half<D, 0>(a, m, stats, st);
+}
+
+bool on_tensor_cores(int dtype, int d) { return dtype == DILUTION_BF16 && (d == 64 || d == 128); }
+
+// delta (batch * heads, t) fp32, then (lse, delta) padded to half tiles.
+size_t delta_bytes(int64_t batch, int64_t heads, int64_t t) { return (size_t)((batch * heads * t * 4 + 255) / 256 * 256); }
 
 attend::Args attend_args(const void* q, const void* k, const void* v, int64_t batch, int64_t heads, int64_t kv_heads, int64_t t,
                          float scale, float cap, const float* slopes, const int* documents, const int* prefix, void* ranges,
@@ -252,6 +321,10 @@ size_t dilution_attend_ranges_bytes(int64_t batch, int64_t t) {
   return batch < 1 || t < 1 ? 0 : (size_t)(batch * doc_spans(t)) * sizeof(attend::DocRange);
 }
 
+size_t dilution_attend_scratch_bytes(int64_t batch, int64_t heads, int64_t t) {
+  return batch < 1 || heads < 1 || t < 1 ? 0 : delta_bytes(batch, heads, t) + (size_t)(batch * heads * ((t + 63) / 64 * 64)) * 8;
+}
+
 int dilution_attend_forward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
                             int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
                             const int* documents, const int* prefix, void* ranges, void* out, float* lse, void* stream) {
@@ -259,23 +332,31 @@ int dilution_attend_forward(const void* q, const void* k, const void* v, int dty
   if (int rc = check_attend("dilution_attend_forward", a, dtype, d)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = launch_ranges(a, st)) return rc;
+  if (on_tensor_cores(dtype, d)) {
+    if (d == 128) return tc_forward<128, 1>(a, st);
+    return (int64_t)a.batch * a.heads * ((a.t + 255) / 256) >= 148 ? tc_forward<64, 2>(a, st) : tc_forward<64, 1>(a, st);
+  }
   return with_type(dtype, d, [&](auto type, auto dim) { return simt_forward<decltype(type), dim()>(a, st); });
 }
 
 int dilution_attend_backward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
                              int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
                              const int* documents, const int* prefix, const void* ranges, const void* out, const float* lse,
-                             const void* dout, float* delta, void* dq, void* dk, void* dv, void* stream) {
+                             const void* dout, void* scratch, void* dq, void* dk, void* dv, void* stream) {
   attend::Args a = attend_args(q, k, v, batch, heads, kv_heads, t, scale, cap, slopes, documents, prefix,
                                const_cast<void*>(ranges), const_cast<void*>(out), const_cast<float*>(lse));
   a.dout = dout;
-  a.delta = delta;
+  a.delta = (float*)scratch;
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
   if (int rc = check_attend("dilution_attend_backward", a, dtype, d)) return rc;
-  if (!lse || !dout || !delta || !dq || !dk || !dv) return abi_fail(DILUTION_ERR_ARG, "dilution_attend_backward: null pointer");
+  if (!lse || !dout || !scratch || !dq || !dk || !dv || misaligned({scratch})) return abi_fail(DILUTION_ERR_ARG, "dilution_attend_backward: null or misaligned pointer");
   cudaStream_t st = (cudaStream_t)stream;
+  if (on_tensor_cores(dtype, d)) {
+    float2* stats = (float2*)((char*)scratch + delta_bytes(batch, heads, t));
+    return d == 128 ? tc_backward<128>(a, stats, st) : tc_backward<64>(a, stats, st);
+  }
   return with_type(dtype, d, [&](auto type, auto dim) { return simt_backward<decltype(type), dim()>(a, st); });
 }
 

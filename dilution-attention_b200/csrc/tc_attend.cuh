@@ -1,0 +1,769 @@
+// Softmax attention with caps, biases and masks (attend_common.cuh) on the tensor cores: bf16 heads of 64 and 128.
+// Operand tiles come in by TMA, products are tcgen05.mma with accumulators in TMEM, and the values that a thread forms
+// (P~, dS) go back into TMEM over the scores it has read, as the A operand of the next product.  A warp of its own issues
+// every copy and MMA.  Which pairs of tiles have anything to do is asked of the documents' ranges, never of a list.
+//
+//   forward : a CTA's query tiles of 128 (two of heads of 64, one of 128) walk over half tiles of 64 keys; two warpgroups per query
+//             tile take them in turn.  lane = query: reference, sum and accumulator of a row belong to one thread and
+//             warpgroup, and are merged once at the end.
+//   backward: one kernel for both halves.  A tile of 128 stays (dq: queries with their dout; dk, dv: keys with their values),
+//             half tiles of 64 of the other kind stream past; kWg warpgroups take them in turn, and accumulators in TMEM
+//             are shared by all of them.  dq: lane = query.  dk, dv: lane = key, and nothing is reduced across CTAs: the heads
+//             that share a key head stream past one after the other.  So scores are formed twice, seven products in
+//             place of five, and no result depends on an order of atomic additions.
+//
+// What bounds them, per pair of tiles of 128 x 64: 512 cycles for one exponential a score on the special-function unit (16 a
+// clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.
+#pragma once
+
+#include "attend_common.cuh"
+#include "tc_common.cuh"
+
+namespace dil {
+namespace tc {
+
+__device__ int g_attend_status = 0;        // first bounded wait that ran out (0 = none)
+
+using attend::Row;
+
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Head sizes: D / 64 sub-tiles of 64 features (tc_common.cuh).
+template <int D> constexpr int kForm = D == 128 ? kWide128 : kNarrow;
+
+// ---- which pairs of tiles ------------------------------------------------------------------------
+struct Docs {
+  int lo, hi, id;          // smallest and largest id, and the one id of all tokens or -1
+};
+__device__ __forceinline__ Docs docs_of(const Row& r, int i0, int i1) {
+  Docs d{INT_MAX, -1, -1};
+  bool pure = true;
+  for (int s = i0 / attend::kSpan; s <= min(i1, r.t - 1) / attend::kSpan; ++s) {
+    const attend::DocRange x = r.ranges[s];
+    d.lo = min(d.lo, x.lo);
+    d.hi = max(d.hi, x.hi);
+    pure = pure && x.pure;
+  }
+  if (pure && d.lo == d.hi) d.id = d.lo;
+  return d;
+}
+// 0: no query of [i0, i1] sees a key of [j0, j1]; 2: each sees each; 1: masks decide.  BIAS: distances of one sign only are
+// left to the kernels' common path.  Rows behind the last token count as seen where they do no harm: queries, and keys
+// of a tile that stays; j1 is the last key that matters then.
+template <bool BIAS>
+__device__ __forceinline__ int pair_state(const Row& r, int i0, int i1, const Docs& di, int j0, int j1, const Docs& dj) {
+  if (j0 > i1 && j0 >= r.prefix) return 0;
+  if (r.ranges != nullptr) {
+    if (di.hi < dj.lo || dj.hi < di.lo) return 0;
+    if (di.id < 0 || di.id != dj.id) return 1;
+  }
+  if (j1 >= r.t || (BIAS && j1 > i0)) return 1;
+  return j1 <= i0 || j1 < r.prefix ? 2 : 1;
+}
+
+// ---- scores ----------------------------------------------------------------------------------------
+// tanh of two values, |x| <= 1: x + x^3 P(x^2) with a least-maximum fit of degree 5, 1.6e-7 relative.  Nine packed instructions,
+// where the two special-function operations of a value take 16 cycles of a warp's quarter.
+__device__ __forceinline__ float2 tanh_poly2(float2 x) {
+  auto both = [](float c) { return make_float2(c, c); };
+  const float2 y = mul2(x, x);
+  float2 p = fma2(y, both(0.0010702026775106788f), both(-0.006294633727520704f));
+  p = fma2(p, y, both(0.02039860375225544f));
+  p = fma2(p, y, both(-0.053518135100603104f));
+  p = fma2(p, y, both(0.133268341422081f));
+  p = fma2(p, y, both(-0.3333301842212677f));
+  p = mul2(p, y);
+  return fma2(x, p, x);
+}
+// v = tanh(v * pre) of N products q . k.  pre: scale / cap.
+template <int N> __device__ __forceinline__ void cap_scores(float* v, float pre) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; e += 2) top = fmaxf(top, fmaxf(fabsf(v[e]), fabsf(v[e + 1])));
+  // (fmaxf passes over a NaN, which comes through either form)
+  if (__any_sync(0xffffffffu, top * pre > 1.f)) {
+    const float twice = pre * 2.f * kLog2e;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = fmaf(-2.f, fast_rcp(1.f + fast_exp2(v[e] * twice)), 1.f);
+  } else {
+    const float2 pp = make_float2(pre, pre);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float2 t = tanh_poly2(mul2(make_float2(v[e], v[e + 1]), pp));
+      v[e] = t.x;
+      v[e + 1] = t.y;
+    }
+  }
+}
+
+// ---- forward -----------------------------------------------------------------------------------------
+template <int D, int NT> struct AttendForward {
+  static constexpr int kThreads = 256 * NT + 32;
+  static constexpr int kRing = D == 64 && NT == 1 ? 5 : D == 64 ? 8 : 5;           // half tiles of K and V
+  static constexpr uint32_t kTile = Rows<kForm<D>>::kBytes, kHalf = kTile / 2;
+  // Q[NT] | K[ring] | V[ring] | merge statistics [NT][2][128] float2 | flags [NT][128] | barriers + control
+  static constexpr int kOperands = (int)(NT * kTile + 2 * kRing * kHalf);
+  static constexpr int kStats = NT * 2 * 128 * 8, kFlags = NT * 128 * 4;
+  static constexpr int kBytes = kOperands + kStats + kFlags + 256 + 1024;
+  static constexpr int kWgCols = 64 + D;
+  static constexpr int kTmem = 2 * NT * kWgCols <= 256 ? 256 : 512;
+  static_assert(2 * NT * kWgCols <= kTmem, "the warpgroups' columns fit the allocation");
+  static_assert(NT * 128 * D * 4 <= (int)(2 * kRing * kHalf), "the merge area fits the ring");
+};
+
+constexpr float kAttendLimit = 1099511627776.f;      // 2^40: a half tile whose P~ sum to more moves the reference
+
+// A warpgroup's step over the 64 scores of keys j0 .. at tS: P~ = 2^(z - reference) as bf16 over the scores, their sum
+// into s.  The reference is the maximum of the first half tile that a row sees and moves where a later one's P~ sum to more
+// than 2^40; only then is the accumulator rescaled.  bf16 has the range of fp32: P~ below that limit keeps 8 bits.
+template <int D, bool CAP, bool BIAS>
+__device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row& r, float lin, float pre, int j0, int i, bool edge,
+                                             float& ref, float& s) {
+  float v[64];
+  uint32_t pw[32];
+  float ps;
+  auto fetch = [&]() {
+    tmem_ld32(tS, v);
+    tmem_ld32(tS + 32, v + 32);
+    tmem_ld_wait(v);
+    tmem_ld_wait(v + 32);
+    if (CAP) cap_scores<64>(v, pre);
+  };
+  // P~ of scores mul * v + add + step * e
+  auto exponentials = [&](float mul, float add, float step) {
+    const float2 mm = make_float2(mul, mul);
+    float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+#pragma unroll
+    for (int e = 0; e < 64; e += 4) {
+      float2 o0 = make_float2(add, add), o1 = o0;
+      if (BIAS) {
+        o0 = fma2(make_float2(step, step), make_float2((float)e, (float)(e + 1)), o0);
+        o1 = fma2(make_float2(step, step), make_float2((float)(e + 2), (float)(e + 3)), o1);
+      }
+      const float2 z0 = fma2(make_float2(v[e], v[e + 1]), mm, o0), z1 = fma2(make_float2(v[e + 2], v[e + 3]), mm, o1);
+      const float2 p0 = make_float2(fast_exp2(z0.x), fast_exp2(z0.y)), p1 = make_float2(fast_exp2(z1.x), fast_exp2(z1.y));
+      a0 = add2(a0, p0);
+      a1 = add2(a1, p1);
+      pw[e >> 1] = pack_pair(p0.x, p0.y);
+      pw[(e >> 1) + 1] = pack_pair(p1.x, p1.y);
+    }
+    const float2 a = add2(a0, a1);
+    ps = a.x + a.y;
+  };
+  fetch();
+  bool slow = edge || __any_sync(0xffffffffu, ref == -INFINITY);
+  if (!slow) {
+    exponentials(lin, (BIAS ? r.slope2 * (float)(j0 - i) : 0.f) - ref, r.slope2);
+    slow = __any_sync(0xffffffffu, !(ps < kAttendLimit));
+    if (slow) fetch();               // rare: the scores are still in TMEM
+  }
+  if (slow) {
+    float top = -INFINITY;
+    const bool docs = edge && r.docs != nullptr;
+    const int id = docs ? r.docs[i] : 0;
+#pragma unroll
+    for (int e = 0; e < 64; ++e) {
+      const int j = j0 + e;
+      float z = v[e] * lin;
+      if (BIAS) z = fmaf(-r.slope2, fabsf((float)(i - j)), z);
+      if (edge) {
+        bool ok = j < r.t && (j <= i || j < r.prefix);
+        if (docs) ok = ok && id >= 0 && r.docs[min(j, r.t - 1)] == id;
+        z = ok ? z : -INFINITY;
+      }
+      v[e] = z;
+      top = fmaxf(top, z);
+    }
+    const float now = fmaxf(ref, top);
+    if (__any_sync(0xffffffffu, now != ref)) {
+      const bool fresh = __all_sync(0xffffffffu, ref == -INFINITY);        // nothing accumulated yet
+      const float f = fast_exp2(ref - (now == -INFINITY ? 0.f : now));
+      if (!fresh) {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          float o[16];
+          tmem_ld16(tO + 16 * c, o);
+          tmem_ld_wait16(o);
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
+          tmem_st16(tO + 16 * c, w);
+        }
+      }
+      s *= f;
+      ref = now;
+    }
+    exponentials(1.f, ref == -INFINITY ? 0.f : -ref, 0.f);
+  }
+  s += ps;
+  tmem_st16(tS, pw);
+  tmem_st16(tS + 16, pw + 16);
+  tmem_st_wait();
+}
+
+// grid = batch * heads * ceil(t / (128 NT)), last queries (the longest rows) first.
+template <int D, int NT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT == 1 ? 2 : 1) attend_forward_kernel(
+    const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+    const __grid_constant__ attend::Args a) {
+  using F = AttendForward<D, NT>;
+  constexpr int W = kForm<D>, R = F::kRing;
+  constexpr uint32_t TB = F::kTile, HB = F::kHalf, HSub = kTileBytes / 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  const uint32_t sQ = smem_u32(smem), sK = sQ + NT * TB, sV = sK + R * HB;
+  float2* sStat = reinterpret_cast<float2*>(smem + F::kOperands);
+  int* sFlag = reinterpret_cast<int*>(smem + F::kOperands + F::kStats);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::kOperands + F::kStats + F::kFlags);
+  const uint32_t qfull = smem_u32(bars), kfull = qfull + 8, kfree = kfull + 8 * R, sdone = kfree + 8 * R, pready = sdone + 16 * NT;
+  Ctl* ctl = reinterpret_cast<Ctl*>(bars + 1 + 2 * R + 4 * NT);
+  __shared__ int s_range[2];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
+  const int warp_u = uniform_warp();
+  const uint32_t lead = elect_one();
+  const int heads = a.batch * a.heads, blocks = (a.t + NT * kTileRows - 1) / (NT * kTileRows);
+  const int n = (int)(blockIdx.x % heads), ib = (blocks - 1 - (int)(blockIdx.x / heads)) * NT;
+  const int b = n / a.heads, h = n % a.heads, nk = b * a.kv_heads + h / (a.heads / a.kv_heads);
+  const Row r = attend::make_row(a, b, h);
+  const float lin = CAP ? r.cap2 : r.pre, pre = CAP ? a.scale / a.cap : 0.f;
+  Docs dq[NT];
+#pragma unroll
+  for (int x = 0; x < NT; ++x) {
+    const int i0 = (ib + x) * kTileRows;
+    dq[x] = r.ranges != nullptr && i0 < r.t ? docs_of(r, i0, i0 + kTileRows - 1) : Docs{INT_MAX, -1, -1};
+  }
+  auto state = [&](int x, int hh) {                     // of query tile x and half tile hh
+    const int i0 = (ib + x) * kTileRows, j0 = hh * 64;
+    if (i0 >= r.t) return 0;
+    const Docs dj = r.ranges != nullptr ? docs_of(r, j0, j0 + 63) : Docs{INT_MAX, -1, -1};
+    return pair_state<BIAS>(r, i0, i0 + kTileRows - 1, dq[x], j0, j0 + 63, dj);
+  };
+
+  if (tid == 0) {
+    ctl->abort = 0;
+    s_range[0] = INT_MAX;
+    s_range[1] = 0;
+    for (int x = 0; x < 1 + 2 * R + 2 * NT; ++x) mbar_init(qfull + 8 * x, 1);        // qfull, kfull, kfree, sdone
+    for (int x = 0; x < 2 * NT; ++x) mbar_init(pready + 8 * x, 4);
+    fence_barrier_init();
+  }
+  for (int x = tid; x < NT * 128; x += F::kThreads) sFlag[x] = 0;
+  __syncwarp();
+  if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
+  __syncthreads();
+  // half tiles [h0, h1) that any of the CTA's queries sees
+  {
+    const int i1 = min(r.t, (ib + NT) * kTileRows) - 1, top = (attend::key_end(r, i1) + 63) / 64;
+    if (r.ranges == nullptr) {
+      if (tid == 0) { s_range[0] = 0; s_range[1] = top; }
+    } else {
+      for (int hh = tid; hh < top; hh += F::kThreads) {
+        bool any = false;
+#pragma unroll
+        for (int x = 0; x < NT; ++x) any = any || state(x, hh) != 0;
+        if (any) { atomicMin(&s_range[0], hh); atomicMax(&s_range[1], hh + 1); }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(ctl->tmem);
+  const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0;
+
+  if (warp_u == 8 * NT) {
+    // ------------------------------------------------------------ the issuing warp
+    constexpr uint32_t id_s = instr_desc(128, 64, 0, 0), id_p = instr_desc(128, D, 0, 1);
+    const Desc dQ = make_desc(sQ, 16, 1024), dK = make_desc(sK, 16, 1024), dV = make_desc(sV, HSub, 1024);
+    auto load_keys = [&](int e) {
+      const int st = e % R;
+      if (!lead) return;
+      mbar_expect_tx(kfull + 8 * st, 2 * HB);
+      tma_load_rows<W>(sK + HB * st, &map_k, (h0 + e) * 64, nk, kfull + 8 * st, HSub);
+      tma_load_rows<W>(sV + HB * st, &map_v, (h0 + e) * 64, nk, kfull + 8 * st, HSub);
+    };
+    const int tiles = NT == 2 && (ib + 1) * kTileRows < r.t ? 2 : 1;
+    if (nh > 0) {
+      if (lead) {
+        mbar_expect_tx(qfull, tiles * TB);
+        for (int x = 0; x < tiles; ++x) tma_load_rows<W>(sQ + TB * x, &map_q, (ib + x) * kTileRows, n, qfull);
+      }
+      for (int e = 0; e < R && e < nh; ++e) load_keys(e);
+      mbar_wait_warp(qfull, 0, ctl, &g_attend_status, kErrWaitTma);
+      uint32_t pending = 0, flip = 0;                    // warpgroups with a P~ to come, the parity of the next
+      for (int e = 0; e < nh + 2; ++e) {
+        if (e < nh) mbar_wait_warp(kfull + 8 * (e % R), (e / R) & 1, ctl, &g_attend_status, kErrWaitTma);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          const int w = 2 * x + (e & 1);
+          const uint32_t tS = tmem + F::kWgCols * w;
+          if (pending >> w & 1) {                        // of half tile e - 2
+            mbar_wait_warp(pready + 8 * w, flip >> w & 1, ctl, &g_attend_status, kErrWaitTile);
+            flip ^= 1u << w;
+            pending &= ~(1u << w);
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)               // 16 keys per instruction: 16 rows of 128 B = 128 units
+              mma_ts(lead, tS + 64, tS + 8 * kk, dV, (HB >> 4) * ((e - 2) % R) + 128 * kk, id_p, 1);
+          }
+          if (e < nh && uniform(state(x, h0 + e)) != 0) {
+            tc_fence_after();
+            mma_scores_wide<W>(lead, tS, Desc{dQ.lo + (TB >> 4) * x, dQ.hi}, kTileBytes, Desc{dK.lo + (HB >> 4) * (e % R), dK.hi},
+                               HSub, id_s);
+            mma_commit(lead, sdone + 8 * w);             // the scores, and every product in front of them
+            pending |= 1u << w;
+          }
+        }
+        if (e >= 2) mma_commit(lead, kfree + 8 * ((e - 2) % R));
+        // half tile e - 3, whose products were issued one round ago, makes room for e - 3 + R
+        if (e >= 3 && e - 3 + R < nh) {
+          mbar_wait_warp(kfree + 8 * ((e - 3) % R), ((e - 3) / R) & 1, ctl, &g_attend_status, kErrWaitMma);
+          load_keys(e - 3 + R);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 2 * NT; ++w) mma_commit(lead, sdone + 8 * w);              // the last products
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ the compute warps: lane = query
+    const uint32_t tS = tmem + F::kWgCols * wg + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 64;
+    {
+      uint32_t z[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) z[c] = 0u;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) tmem_st16(tO + 16 * c, z);
+      tmem_st_wait();
+    }
+    const int tile = NT == 2 ? wg >> 1 : 0, half = wg & 1, i = (ib + tile) * kTileRows + row, is = min(i, r.t - 1);
+    float ref = -INFINITY, s = 0.f;
+    int turn = 0;
+    for (int e = half; e < nh; e += 2) {
+      const int what = (int)uniform(state(tile, h0 + e));
+      if (what == 0) continue;
+      mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
+      ++turn;
+      tc_fence_after();
+      forward_step<D, CAP, BIAS>(tS, tO, r, lin, pre, (h0 + e) * 64, is, what == 1, ref, s);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pready + 8 * wg);
+    }
+    if (nh > 0) mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
+    tc_fence_after();
+    // every product has read the ring, which the merge goes over
+    asm volatile("bar.sync 1, %0;" ::"n"(256 * NT) : "memory");
+    // Each of a tile's two warpgroups finishes half of the features: it hands the other half of its accumulator over.
+    constexpr int kPart = D / 2;
+    float* sX = reinterpret_cast<float*>(smem + NT * TB) + tile * 128 * D;           // [2][128][kPart]
+    float2* stat = sStat + 256 * tile;
+    stat[half * 128 + row] = make_float2(ref, s);
+    float* give = sX + ((1 - half) * 128 + row) * kPart;
+    __syncwarp();
+#pragma unroll
+    for (int c0 = 0; c0 < kPart; c0 += 32) {
+      float o[32];
+      tmem_ld32(tO + kPart * (1 - half) + c0, o);
+      tmem_ld_wait(o);
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        reinterpret_cast<float4*>(give + c0)[c ^ (row & 7)] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+    }
+    auto meet = [tile] {
+      if (NT == 1 || tile == 0) asm volatile("bar.sync 2, 256;" ::: "memory");
+      else asm volatile("bar.sync 3, 256;" ::: "memory");
+    };
+    meet();
+    const float2 other = stat[(1 - half) * 128 + row];
+    const float m = fmaxf(ref, other.x), base = m == -INFINITY ? 0.f : m;
+    const float f_own = fast_exp2(ref - base), f_oth = fast_exp2(other.x - base);
+    const float den = s * f_own + other.y * f_oth, inv = den == 0.f ? 0.f : 1.f / den;
+    __syncwarp();
+    const float a_own = f_own * inv, a_oth = f_oth * inv;
+    const float* take = sX + (half * 128 + row) * kPart;
+    bool bad = false;
+#pragma unroll
+    for (int c0 = 0; c0 < kPart; c0 += 32) {
+      float o[32];
+      __syncwarp();
+      tmem_ld32(tO + kPart * half + c0, o);
+      tmem_ld_wait(o);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float4 x = reinterpret_cast<const float4*>(take + c0)[c ^ (row & 7)];
+        o[4 * c] = o[4 * c] * a_own + x.x * a_oth;
+        o[4 * c + 1] = o[4 * c + 1] * a_own + x.y * a_oth;
+        o[4 * c + 2] = o[4 * c + 2] * a_own + x.z * a_oth;
+        o[4 * c + 3] = o[4 * c + 3] * a_own + x.w * a_oth;
+      }
+      float sum = 0.f;                                    // not finite if any of them is not
+#pragma unroll
+      for (int c = 0; c < 32; ++c) sum = fmaf(o[c], 0.f, sum);
+      bad = bad || sum != 0.f;
+      if (i < r.t) {
+        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + ((int64_t)n * a.t + i) * D + kPart * half + c0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          dst[c] = make_uint4(pack_pair(o[8 * c], o[8 * c + 1]), pack_pair(o[8 * c + 2], o[8 * c + 3]),
+                              pack_pair(o[8 * c + 4], o[8 * c + 5]), pack_pair(o[8 * c + 6], o[8 * c + 7]));
+      }
+    }
+    if (half == 0 && i < r.t && a.lse != nullptr) a.lse[(int64_t)n * a.t + i] = den == 0.f ? INFINITY : m + log2f(den);
+    if (bad && i < r.t) sFlag[tile * 128 + row] = 1;
+    meet();
+    // (both warpgroups have written their halves; a warp's rows are its own lanes', every other one of them)
+    unsigned again = __ballot_sync(0xffffffffu, sFlag[tile * 128 + row] != 0) & (half ? 0xaaaaaaaau : 0x55555555u);
+    for (; again; again &= again - 1)
+      attend::redo_forward_row<__nv_bfloat16, D>(a, b, h, (ib + tile) * kTileRows + (row & 96) + __ffs(again) - 1);
+  }
+  drain_if_aborted(ctl);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_free(tmem, F::kTmem);
+}
+
+// ---- backward ------------------------------------------------------------------------------------------
+// STAY 0: queries stay (dq), 1: keys stay (dk, dv).  Staying tile: [Q, dout] or [K, V], rows of 128; passing half tiles: [K, V] or
+// [Q, dout], rows of 64, with the passing queries' (lse, delta).
+template <int D, int STAY> struct AttendBackward {
+  static constexpr int kWg = D == 128 && STAY == 1 ? 2 : 3;
+  static constexpr int kThreads = 128 * kWg + 64;
+  static constexpr int kRing = D == 64 ? 6 : STAY == 1 ? 4 : 5;         // one more than are in work, at least
+  static constexpr uint32_t kTile = Rows<kForm<D>>::kBytes, kHalf = kTile / 2;
+  static constexpr int kAcc = STAY == 1 ? 2 * D : D;                     // accumulator columns
+  static_assert(kWg * 128 + kAcc <= 512, "the warpgroups' scores and the accumulators fit TMEM");
+  // staying tiles | passing tiles [ring] x 2 | (lse, delta) [ring][64] | flags [128] | barriers + control
+  static constexpr int kOperands = (int)(2 * kTile + 2 * kRing * kHalf);
+  static constexpr int kStats = STAY == 1 ? kRing * 512 : 0;
+  static constexpr int kBytes = kOperands + kStats + 512 + 256 + 1024;
+};
+
+// Bytes of global memory into shared memory, both on 16-byte boundaries.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
+}
+
+// A warpgroup's step over 64 columns: S at tS, dout . v at tS + 64.  P (keys stay) as bf16 over the scores and dS over the
+// others, both as A operands.  x0: the first passing token, y: the lane's own; st: (lse, delta) of the passing queries.
+template <int STAY, bool CAP, bool BIAS>
+__device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float lin, float pre, int x0, int y, bool edge, float2 own,
+                                              const float4* st) {
+  const bool docs = edge && r.docs != nullptr;
+  const int id = docs ? r.docs[y] : 0;
+#pragma unroll
+  for (int c0 = 0; c0 < 64; c0 += 32) {
+    float v[32], g[32];
+    tmem_ld32(tS + c0, v);
+    tmem_ld32(tS + 64 + c0, g);
+    tmem_ld_wait(v);
+    tmem_ld_wait(g);
+    if (CAP) cap_scores<32>(v, pre);
+    uint32_t pw[16], gw[16];
+    const float2 mm = make_float2(lin, lin);
+    // the distance's term of column e: first + step * e (one sign throughout, except in masked tiles)
+    const float step = STAY == 1 ? -r.slope2 : r.slope2;
+    const float first = STAY == 1 ? r.slope2 * (float)(y - x0 - c0) : r.slope2 * (float)(x0 + c0 - y);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      float2 off, delta;                                  // -lse (and the distance's term), -delta
+      if (STAY == 1) {
+        const float4 x = st[(c0 + e) >> 1];
+        off = make_float2(-x.x, -x.z);
+        delta = make_float2(-x.y, -x.w);
+      } else {
+        off = make_float2(-own.x, -own.x);
+        delta = make_float2(-own.y, -own.y);
+      }
+      if (BIAS) {
+        float2 far = fma2(make_float2(step, step), make_float2((float)e, (float)(e + 1)), make_float2(first, first));
+        if (edge) far = make_float2(-fabsf(far.x), -fabsf(far.y));
+        off = add2(off, far);
+      }
+      float2 z = fma2(make_float2(v[e], v[e + 1]), mm, off);
+      float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+      float2 d = add2(make_float2(g[e], g[e + 1]), delta);
+      d = mul2(p, d);
+      if (CAP) {
+        const float2 t = make_float2(v[e], v[e + 1]), minus = make_float2(-t.x, -t.y);
+        d = mul2(d, fma2(minus, t, make_float2(1.f, 1.f)));
+      }
+      if (edge) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int x = x0 + c0 + e + k, i = STAY == 1 ? x : y, j = STAY == 1 ? y : x;
+          bool ok = x < r.t && (j <= i || j < r.prefix);
+          if (docs) ok = ok && id >= 0 && r.docs[min(x, r.t - 1)] == id;
+          if (!ok) (k ? p.y : p.x) = 0.f, (k ? d.y : d.x) = 0.f;
+        }
+      }
+      if (STAY == 1) pw[e >> 1] = pack_pair(p.x, p.y);
+      gw[e >> 1] = pack_pair(d.x, d.y);
+    }
+    if (STAY == 1) tmem_st16(tS + c0 / 2, pw);
+    tmem_st16(tS + 64 + c0 / 2, gw);
+  }
+  tmem_st_wait();
+}
+
+// grid = rows * ceil(t / 128): dq: batch * heads rows, last queries first; dk, dv: batch * kv_heads rows, first keys first.
+// map_a, map_b: Q and dout (batch * heads rows); map_c, map_d: K and V (batch * kv_heads rows), boxes of 64 rows all.
+// stats: (lse, delta) of every query, padded to whole half tiles with (+inf, 0): (batch * heads, 64 ceil(t / 64)).
+template <int D, int STAY, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_backward_kernel(
+    const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
+    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ attend::Args a, const float2* __restrict__ stats) {
+  using F = AttendBackward<D, STAY>;
+  constexpr int W = kForm<D>, R = F::kRing, NW = F::kWg;
+  constexpr uint32_t TB = F::kTile, HB = F::kHalf, HSub = kTileBytes / 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  const uint32_t sA = smem_u32(smem), sB = sA + 2 * TB, sC = sB + R * HB, sStat = sC + R * HB;
+  const float4* stat = reinterpret_cast<const float4*>(smem + F::kOperands);
+  int* sFlag = reinterpret_cast<int*>(smem + F::kOperands + F::kStats);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::kOperands + F::kStats + 512);
+  const uint32_t afull = smem_u32(bars), bfull = afull + 8, bfree = bfull + 8 * R, sdone = bfree + 8 * R, alldone = sdone + 8 * NW,
+                 pready = alldone + 8;
+  Ctl* ctl = reinterpret_cast<Ctl*>(bars + 2 + 2 * R + 2 * NW);
+  __shared__ int s_range[2];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
+  const int warp_u = uniform_warp();
+  const uint32_t lead = elect_one();
+  const int group = a.heads / a.kv_heads, rows = a.batch * (STAY == 1 ? a.kv_heads : a.heads);
+  const int tiles = (a.t + kTileRows - 1) / kTileRows, padded = (a.t + 63) / 64 * 64;
+  const int n = (int)(blockIdx.x % rows), block = (int)(blockIdx.x / rows);
+  const int y0 = (STAY == 1 ? block : tiles - 1 - block) * kTileRows, y1 = min(y0 + kTileRows, a.t) - 1;
+  const int b = n / (STAY == 1 ? a.kv_heads : a.heads), head = n % (STAY == 1 ? a.kv_heads : a.heads);
+  const int passes = STAY == 1 ? group : 1;                      // heads whose queries pass
+  Row r = attend::make_row(a, b, STAY == 1 ? head * group : head);
+  const float lin = CAP ? r.cap2 : r.pre, pre = CAP ? a.scale / a.cap : 0.f;
+  const Docs dy = r.ranges != nullptr ? docs_of(r, y0, y1) : Docs{INT_MAX, -1, -1};
+  auto state = [&](int hh) {                                     // of the tile and passing half tile hh
+    const int x0 = hh * 64;
+    const Docs dx = r.ranges != nullptr ? docs_of(r, x0, x0 + 63) : Docs{INT_MAX, -1, -1};
+    return STAY == 1 ? pair_state<BIAS>(r, x0, x0 + 63, dx, y0, y1, dy) : pair_state<BIAS>(r, y0, y1, dy, x0, x0 + 63, dx);
+  };
+
+  if (tid == 0) {
+    ctl->abort = 0;
+    s_range[0] = INT_MAX;
+    s_range[1] = 0;
+    for (int x = 0; x < 2 + 2 * R + NW; ++x) mbar_init(afull + 8 * x, 1);        // afull, bfull, bfree, sdone, alldone
+    for (int x = 0; x < NW; ++x) mbar_init(pready + 8 * x, 4);
+    fence_barrier_init();
+  }
+  if (tid < 128) sFlag[tid] = 0;
+  __syncwarp();
+  if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), 512);
+  __syncthreads();
+  {
+    // passing half tiles [h0, h1) of which any sees the tile (or is seen by it)
+    const int lo = STAY == 1 ? attend::first_query(r, y0) / 64 : 0, hi = STAY == 1 ? padded / 64 : (attend::key_end(r, y1) + 63) / 64;
+    if (r.ranges == nullptr) {
+      if (tid == 0) { s_range[0] = lo; s_range[1] = hi; }
+    } else {
+      for (int hh = lo + tid; hh < hi; hh += F::kThreads)
+        if (state(hh) != 0) { atomicMin(&s_range[0], hh); atomicMax(&s_range[1], hh + 1); }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(ctl->tmem), tAcc = tmem + 128 * NW;
+  const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0, ne = nh * passes;
+
+  if (warp_u == 4 * NW) {
+    // ------------------------------------------------------------ the warp that issues MMAs
+    constexpr uint32_t id_s = instr_desc(128, 64, 0, 0), id_a = instr_desc(128, D, 0, 1);
+    const Desc dA = make_desc(sA, 16, 1024), dB = make_desc(sB, 16, 1024), dC = make_desc(sC, 16, 1024);
+    const Desc dBm = make_desc(sB, HSub, 1024), dCm = make_desc(sC, HSub, 1024);
+    if (ne > 0) {
+      mbar_wait_warp(afull, 0, ctl, &g_attend_status, kErrWaitTma);
+      uint32_t pending = 0, flip = 0, started = 0;         // warpgroups with a dS to come, the parity of the next
+      for (int e = 0; e < ne + NW; ++e) {
+        const int w = e % NW;
+        const uint32_t tS = tmem + 128 * w;
+        if (pending >> w & 1) {                            // of half tile e - NW
+          const int st = (e - NW) % R;
+          mbar_wait_warp(pready + 8 * w, flip >> w & 1, ctl, &g_attend_status, kErrWaitTile);
+          flip ^= 1u << w;
+          pending &= ~(1u << w);
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)                   // dS times the passing queries (or keys)
+            mma_ts(lead, tAcc, tS + 64 + 8 * kk, dBm, (HB >> 4) * st + 128 * kk, id_a, started | (kk > 0));
+          if (STAY == 1) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)                 // P times their dout
+              mma_ts(lead, tAcc + D, tS + 8 * kk, dCm, (HB >> 4) * st + 128 * kk, id_a, started | (kk > 0));
+          }
+          started = 1;
+        }
+        if (e >= NW) mma_commit(lead, bfree + 8 * ((e - NW) % R));
+        if (e < ne) {
+          mbar_wait_warp(bfull + 8 * (e % R), (e / R) & 1, ctl, &g_attend_status, kErrWaitTma);
+          if (uniform(state(h0 + e % nh)) != 0) {
+            tc_fence_after();
+            mma_scores_wide<W>(lead, tS, dA, kTileBytes, Desc{dB.lo + (HB >> 4) * (e % R), dB.hi}, HSub, id_s);
+            mma_scores_wide<W>(lead, tS + 64, Desc{dA.lo + (TB >> 4), dA.hi}, kTileBytes, Desc{dC.lo + (HB >> 4) * (e % R), dC.hi}, HSub,
+                               id_s);
+            mma_commit(lead, sdone + 8 * w);
+            pending |= 1u << w;
+          }
+        }
+      }
+      mma_commit(lead, alldone);
+    }
+    __syncwarp();
+  } else if (warp_u == 4 * NW + 1) {
+    // ------------------------------------------------------------ the warp that issues copies
+    const int nx = STAY == 1 ? b * a.heads + head * group : b * a.kv_heads + head / group;      // the passing rows, the first of them
+    if (ne > 0 && lead) {
+      mbar_expect_tx(afull, 2 * TB);
+      // (two boxes of 64 rows for each sub-tile: a box behind the last row reads zeros)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          tma_load_rows<W>(sA + TB * x + HSub * half, STAY == 1 ? (x ? &map_v : &map_k) : (x ? &map_do : &map_q), y0 + 64 * half, n, afull,
+                           kTileBytes);
+    }
+    __syncwarp();
+    for (int e = 0; e < ne; ++e) {
+      const int st = e % R, hh = h0 + e % nh, m = nx + e / nh;
+      if (e >= R) mbar_wait_warp(bfree + 8 * st, (e / R - 1) & 1, ctl, &g_attend_status, kErrWaitMma);
+      if (lead) {
+        mbar_expect_tx(bfull + 8 * st, 2 * HB + (STAY == 1 ? 512 : 0));
+        tma_load_rows<W>(sB + HB * st, STAY == 1 ? &map_q : &map_k, hh * 64, m, bfull + 8 * st, HSub);
+        tma_load_rows<W>(sC + HB * st, STAY == 1 ? &map_do : &map_v, hh * 64, m, bfull + 8 * st, HSub);
+        if (STAY == 1) bulk_load(sStat + 512 * st, stats + (int64_t)m * padded + hh * 64, 512, bfull + 8 * st);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ the compute warps: lane = the staying query or key
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + 128 * wg + lanes;
+    const int y = y0 + row, ys = min(y, a.t - 1);
+    float2 own = make_float2(0.f, 0.f);
+    if (STAY == 0) own = y < a.t ? stats[(int64_t)n * padded + y] : make_float2(INFINITY, 0.f);
+    int turn = 0;
+    for (int e = wg; e < ne; e += NW) {
+      if (STAY == 1 && BIAS) r.slope2 = a.slopes[head * group + e / nh] * kLog2e;
+      const int hh = h0 + (passes == 1 ? e : e % nh), what = (int)uniform(state(hh));
+      if (what == 0) continue;
+      mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
+      ++turn;
+      tc_fence_after();
+      backward_step<STAY, CAP, BIAS>(tS, r, lin, pre, hh * 64, ys, what == 1, own, stat + 32 * (e % R));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pready + 8 * wg);
+    }
+    if (ne > 0) mbar_wait_warp(alldone, 0, ctl, &g_attend_status, kErrWaitMma);
+    tc_fence_after();
+    bool bad = false;
+    for (int c0 = 32 * wg; c0 < F::kAcc; c0 += 32 * NW) {
+      float o[32];
+      __syncwarp();
+      tmem_ld32(tAcc + lanes + c0, o);
+      tmem_ld_wait(o);
+      const bool second = STAY == 1 && c0 >= D;            // dv
+      const float f = second ? 1.f : a.scale;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        o[c] = ne == 0 ? 0.f : o[c] * f;
+        sum = fmaf(o[c], 0.f, sum);
+      }
+      bad = bad || sum != 0.f;
+      if (y < a.t) {
+        __nv_bfloat16* base = reinterpret_cast<__nv_bfloat16*>(STAY == 0 ? a.dq : second ? a.dv : a.dk);
+        uint4* dst = reinterpret_cast<uint4*>(base + ((int64_t)n * a.t + y) * D + (second ? c0 - D : c0));
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          dst[c] = make_uint4(pack_pair(o[8 * c], o[8 * c + 1]), pack_pair(o[8 * c + 2], o[8 * c + 3]),
+                              pack_pair(o[8 * c + 4], o[8 * c + 5]), pack_pair(o[8 * c + 6], o[8 * c + 7]));
+      }
+    }
+    if (bad && y < a.t) sFlag[row] = 1;
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * NW) : "memory");
+    // rows that are not finite, each by one warp: rows and warps are told apart by their number modulo the warpgroups
+    unsigned again = __ballot_sync(0xffffffffu, sFlag[row] != 0 && row % NW == wg);
+    for (; again; again &= again - 1) {
+      const int z = y0 + (row & 96) + __ffs(again) - 1;
+      if (STAY == 0) attend::redo_dq_row<__nv_bfloat16, D>(a, b, head, z);
+      else attend::redo_dkv_row<__nv_bfloat16, D>(a, b, head, z);
+    }
+  }
+  drain_if_aborted(ctl);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_free(tmem, 512);
+}
+
+// (lse, delta_i = dout_i . out_i) of every query, padded.  D / 8 lanes a row, 16 bytes each.
+template <int D>
+__global__ void __launch_bounds__(256) attend_stats_kernel(attend::Args a, float2* __restrict__ stats) {
+  constexpr int L = D / 8;
+  const int padded = (a.t + 63) / 64 * 64;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L, n = at / padded;
+  const int i = (int)(at % padded), u = threadIdx.x % L;
+  const bool real = n < (int64_t)a.batch * a.heads && i < a.t;
+  float s = 0.f;
+  if (real) {
+    const int64_t x = (n * a.t + i) * L + u;
+    const uint4 g = reinterpret_cast<const uint4*>(a.dout)[x], o = reinterpret_cast<const uint4*>(a.out)[x];
+    const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(&g);
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(to_f32(p[e]), to_f32(q[e]), s);
+  }
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (u == 0 && n < (int64_t)a.batch * a.heads) {
+    stats[at] = real ? make_float2(a.lse[n * a.t + i], s) : make_float2(INFINITY, 0.f);
+    if (real) a.delta[n * a.t + i] = s;
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                CUtensorMapFloatOOBfill);
+inline EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeTiled)p;
+  }();
+  return fn;
+}
+// (n, t, d) bf16 rows as boxes {64 features, box rows, 1}, 128-byte swizzle; rows past t read as zero.  True: encoded.
+inline bool attend_map(CUtensorMap* map, const void* base, int64_t n, int64_t t, int d, int box) {
+  // the encoder wants a current context, which a thread that has only selected a device (one of autograd's) need not have yet
+  static thread_local bool bound = false;
+  if (!bound) {
+    cudaFree(nullptr);
+    bound = true;
+  }
+  EncodeTiled fn = encode_tiled();
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)t, (cuuint64_t)n};
+  const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)t * d * 2};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, boxes, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace tc
+}  // namespace dil

@@ -129,12 +129,12 @@ class _SoftmaxAttention(torch.autograd.Function):
         lib = _lib.load()
         dout = aligned(dout)
         dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
-        delta = torch.empty_like(lse)
+        scratch = torch.empty(lib.dilution_attend_scratch_bytes(batch, heads, seq), device=q.device, dtype=torch.uint8)
         with on_device(q.device):
             _lib.check(lib.dilution_attend_backward(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _CODE[q.dtype], batch, heads, kv_heads, seq, dim, 1.0 / math.sqrt(dim),
                 ctx.softcap, K._ptr(slopes), K._ptr(documents), K._ptr(prefix), K._ptr(ranges), out.data_ptr(), lse.data_ptr(),
-                dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), K._stream(q.device)),
+                dout.data_ptr(), scratch.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), K._stream(q.device)),
                 "dilution_attend_backward")
         return dq, dk, dv, None, None, None, None
 
