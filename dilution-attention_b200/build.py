@@ -25,7 +25,7 @@ NVCC_FLAGS = [
     "-Xptxas=-v",
     "-Xcompiler", "-fPIC",
 ]
-UNITS = ("abi.cu", "operators.cu")     # one object each, next to its source
+UNITS = ("abi.cu", "operators.cu", "trees.cu")     # one object each, next to its source
 
 
 def _includes(path, seen=None):

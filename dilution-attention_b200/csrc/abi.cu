@@ -506,7 +506,7 @@ int dilution_device_status(void) {
 #ifdef DILUTION_TENSOR_PATH
   int v = 0;
   if (dil::tc::read_status(&v) != 0) return fail(DILUTION_ERR_CUDA, "dilution_device_status: could not read the status word");
-  if (v == 0 && dil::operators_read_status(&v) != 0)
+  if ((v == 0 && dil::operators_read_status(&v) != 0) || (v == 0 && dil::trees_read_status(&v) != 0))
     return fail(DILUTION_ERR_CUDA, "dilution_device_status: could not read the status word");
   if (v != 0) return fail(DILUTION_ERR_DEVICE, "a kernel gave up a bounded wait (code %d)", v);
 #endif

@@ -1,5 +1,4 @@
-// extern "C" entry points of the operators around the attention layers: masked softmax attention, draft trees over a cache,
-// eviction.  Argument validation, kernel selection and launches; declarations in include/dilution_b200.h.
+// extern "C" entry points of masked softmax attention and of eviction.  Argument validation, kernel selection and launches; declarations in include/dilution_b200.h.
 
 #include <algorithm>
 #include <cstdint>
@@ -9,56 +8,13 @@
 #include "abi_internal.h"
 #include "attend_simt.cuh"
 #include "evict_kernels.cuh"
-#include "once_per_device.cuh"
 #include "tc_attend.cuh"
-#include "tree_simt.cuh"
 
 namespace dil {
 
-int operators_read_status(int* code) {
-  int v = 0;
-  if (cudaDeviceSynchronize() != cudaSuccess) return 3;
-  if (cudaMemcpyFromSymbol(&v, tc::g_attend_status, sizeof(int)) != cudaSuccess) return 3;
-  if (v != 0) {
-    const int zero = 0;
-    cudaMemcpyToSymbol(tc::g_attend_status, &zero, sizeof(int));
-  }
-  *code = v;
-  return 0;
-}
+int operators_read_status(int* code) { return read_status_word(tc::g_attend_status, code); }
 
 namespace {
-
-bool valid_d(int d) { return d == 16 || d == 32 || d == 64 || d == 128; }
-bool misaligned(std::initializer_list<const void*> ps) {
-  uintptr_t x = 0;
-  for (const void* p : ps) x |= (uintptr_t)p;
-  return x & 15;
-}
-
-template <typename K> int opt_in(K kernel, int bytes) {
-  static OncePerDevice done;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
-  if (bytes <= 48 * 1024 || done.done((const void*)kernel, dev)) return DILUTION_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return abi_fail(DILUTION_ERR_CUDA, "cudaFuncSetAttribute(%d): %s", bytes, cudaGetErrorString(e));
-  done.set((const void*)kernel, dev);
-  return DILUTION_OK;
-}
-
-// f(T(), integral_constant<int, D>()) for the element type and head size.
-template <typename T, typename F> int with_d(int d, F f) {
-  switch (d) {
-    case 16: return f(T(), std::integral_constant<int, 16>());
-    case 32: return f(T(), std::integral_constant<int, 32>());
-    case 64: return f(T(), std::integral_constant<int, 64>());
-    default: return f(T(), std::integral_constant<int, 128>());
-  }
-}
-template <typename F> int with_type(int dtype, int d, F f) {
-  return dtype == DILUTION_F32 ? with_d<float>(d, f) : with_d<__nv_bfloat16>(d, f);
-}
 
 // ---- masked softmax attention ------------------------------------------------------------------
 int64_t doc_spans(int64_t t) { return (t + attend::kSpan - 1) / attend::kSpan; }
@@ -128,8 +84,8 @@ struct AttendMaps {
 };
 int attend_maps(AttendMaps& m, const attend::Args& a, int d, int q_box, int k_box) {
   const int64_t nq = (int64_t)a.batch * a.heads, nk = (int64_t)a.batch * a.kv_heads;
-  if (!tc::attend_map(&m.q, a.q, nq, a.t, d, q_box) || !tc::attend_map(&m.k, a.k, nk, a.t, d, k_box) ||
-      !tc::attend_map(&m.v, a.v, nk, a.t, d, k_box) || (a.dout && !tc::attend_map(&m.dout, a.dout, nq, a.t, d, q_box)))
+  if (!tc::tile_map(&m.q, a.q, nq, a.t, d, q_box) || !tc::tile_map(&m.k, a.k, nk, a.t, d, k_box) ||
+      !tc::tile_map(&m.v, a.v, nk, a.t, d, k_box) || (a.dout && !tc::tile_map(&m.dout, a.dout, nq, a.t, d, q_box)))
     return abi_fail(DILUTION_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   return DILUTION_OK;
 }
@@ -178,7 +134,7 @@ template <int D> int tc_backward(const attend::Args& a, float2* stats, cudaStrea
   return tc_backward_half<D, 0>(a, m, stats, st);
 }
 
-bool on_tensor_cores(int dtype, int d) { return dtype == DILUTION_BF16 && (d == 64 || d == 128); }
+template <typename T, int D> constexpr bool kOnTensorCores = std::is_same<T, __nv_bfloat16>::value && (D == 64 || D == 128);
 
 // delta (batch * heads, t) fp32, then (lse, delta) padded to half tiles.
 size_t delta_bytes(int64_t batch, int64_t heads, int64_t t) { return (size_t)((batch * heads * t * 4 + 255) / 256 * 256); }
@@ -207,109 +163,6 @@ attend::Args attend_args(const void* q, const void* k, const void* v, int64_t ba
   return a;
 }
 
-// ---- draft trees -----------------------------------------------------------------------------------
-// Parts that a key head's keys are cut into: enough blocks for four on every SM, of 256 keys at least.
-int tree_chunks(int64_t blocks, int64_t keys) {
-  const int64_t want = (148 * 4 + blocks - 1) / std::max<int64_t>(blocks, 1), most = (keys + 255) / 256;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
-}
-int tree_row_blocks(int rows) { return rows <= 16 ? 1 : (rows + 63) / 64; }
-
-struct TreeScratch {
-  size_t part, psum, pout, bytes;
-};
-TreeScratch tree_scratch(int64_t heads, int64_t rows, int64_t chunks, int d) {
-  TreeScratch s;
-  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t n = (size_t)(heads * rows * chunks);
-  s.part = 0;
-  s.psum = up(n * sizeof(float2));
-  s.pout = s.psum + up(n * sizeof(float));
-  s.bytes = s.pout + n * d * sizeof(float);
-  return s;
-}
-int64_t tree_keys(const tree::Args& a) { return (a.pos_dev ? a.capacity : a.len) + a.nodes; }
-
-int check_tree(const char* fn, const tree::Args& a, int64_t length, int dtype, int d) {
-  if (dtype != DILUTION_F32 && dtype != DILUTION_BF16)
-    return abi_fail(DILUTION_ERR_ARG, "%s: dtype must be DILUTION_F32 or DILUTION_BF16", fn);
-  if (!valid_d(d)) return abi_fail(DILUTION_ERR_UNSUPPORTED, "%s: head_dim %d not in {16, 32, 64, 128}", fn, d);
-  if (a.batch < 1 || a.kv_heads < 1 || a.group < 1 || (int64_t)a.batch * a.kv_heads > 65535 || a.group > 1024)
-    return abi_fail(DILUTION_ERR_ARG, "%s: batch * kv_heads must be in [1, 65535] and the heads of a group in [1, 1024]", fn);
-  if (a.nodes < 1 || a.nodes > tree::kMaxNodes)
-    return abi_fail(DILUTION_ERR_ARG, "%s: a tree has 1 to %d nodes, not %d", fn, tree::kMaxNodes, a.nodes);
-  if (a.capacity < 1 || a.capacity > (1 << 30) || length < 0 || length > a.capacity)
-    return abi_fail(DILUTION_ERR_ARG, "%s: length %lld outside cache capacity %lld", fn, (long long)length, (long long)a.capacity);
-  if (!(a.cap >= 0.f) || a.cap > 3e38f || !(a.scale > 0.f))
-    return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap finite, 0 for none", fn);
-  if (!a.q || !a.kn || !a.vn || !a.kc || !a.vc || !a.parents || !a.lse) return abi_fail(DILUTION_ERR_ARG, "%s: null pointer", fn);
-  if (misaligned({a.q, a.kn, a.vn, a.kc, a.vc}))
-    return abi_fail(DILUTION_ERR_ARG, "%s: q, drafted keys and values and caches must be 16-byte aligned", fn);
-  return DILUTION_OK;
-}
-
-tree::Args tree_args(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache,
-                     const int* parents, int64_t parent_stride, int64_t batch, int64_t kv_heads, int group, int nodes,
-                     int64_t capacity, int64_t length, const int* length_dev, float scale, float* lse) {
-  tree::Args a{};
-  a.q = q;
-  a.kn = k_new;
-  a.vn = v_new;
-  a.kc = k_cache;
-  a.vc = v_cache;
-  a.parents = parents;
-  a.parent_stride = parent_stride;
-  a.pos_dev = length_dev;
-  a.lse = lse;
-  a.capacity = capacity;
-  a.len = (int)std::min<int64_t>(length, INT_MAX);
-  a.batch = batch > INT_MAX || batch < 0 ? -1 : (int)batch;
-  a.kv_heads = kv_heads > INT_MAX || kv_heads < 0 ? -1 : (int)kv_heads;
-  a.group = group;
-  a.nodes = nodes;
-  a.scale = scale;
-  return a;
-}
-
-void place_scratch(tree::Args& a, void* scratch, int rows, int d) {
-  const TreeScratch s = tree_scratch((int64_t)a.batch * a.kv_heads, rows, a.chunks, d);
-  char* p = (char*)scratch;
-  a.part = (float2*)(p + s.part);
-  a.psum = (float*)(p + s.psum);
-  a.pout = (float*)(p + s.pout);
-}
-
-template <typename T, int D, int RI, bool OUT> int simt_softmax(const tree::Args& a, cudaStream_t st) {
-  constexpr int smem = sizeof(tree::Smem<D, RI>);
-  if (int rc = opt_in(tree::simt_softmax_kernel<T, D, RI, OUT>, smem)) return rc;
-  LaunchMark mark(OUT ? "tree_softmax" : "tree_stats", st);
-  const dim3 grid(a.chunks, (a.group * a.nodes + 16 * RI - 1) / (16 * RI), a.batch * a.kv_heads);
-  tree::simt_softmax_kernel<T, D, RI, OUT><<<grid, tree::kThreads, smem, st>>>(a);
-  return abi_check_launch("tree_softmax");
-}
-template <typename T, int D, int RI> int simt_dilute(const tree::Args& a, cudaStream_t st) {
-  constexpr int smem = sizeof(tree::Smem<D, RI>);
-  if (int rc = opt_in(tree::simt_dilute_kernel<T, D, RI>, smem)) return rc;
-  LaunchMark mark("tree_dilute", st);
-  tree::simt_dilute_kernel<T, D, RI><<<dim3(a.chunks, 1, a.batch * a.kv_heads), tree::kThreads, smem, st>>>(a);
-  return abi_check_launch("tree_dilute");
-}
-template <typename T, int D, int RI> int simt_advance(const tree::Args& a, const tree::Accept& c, cudaStream_t st) {
-  constexpr int smem = sizeof(tree::Smem<D, RI>);
-  if (int rc = opt_in(tree::simt_advance_kernel<T, D, RI>, smem)) return rc;
-  LaunchMark mark("tree_advance", st);
-  const int64_t tiles = ((a.pos_dev ? a.capacity : a.len) + c.accepted + tree::kKeys - 1) / tree::kKeys;
-  tree::simt_advance_kernel<T, D, RI>
-      <<<dim3((unsigned)std::min<int64_t>(tiles, a.chunks), 1, a.batch * a.kv_heads), tree::kThreads, smem, st>>>(a, c);
-  return abi_check_launch("tree_advance");
-}
-
-template <typename T, bool DILUTE> int join(const tree::Args& a, int d, cudaStream_t st) {
-  LaunchMark mark("tree_join", st);
-  tree::join_kernel<T, DILUTE><<<(unsigned)((int64_t)a.batch * a.kv_heads * a.group * a.nodes), d, 0, st>>>(a, d);
-  return abi_check_launch("tree_join");
-}
-
 }  // namespace
 }  // namespace dil
 
@@ -332,11 +185,11 @@ int dilution_attend_forward(const void* q, const void* k, const void* v, int dty
   if (int rc = check_attend("dilution_attend_forward", a, dtype, d)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = launch_ranges(a, st)) return rc;
-  if (on_tensor_cores(dtype, d)) {
-    if (d == 128) return tc_forward<128, 1>(a, st);
-    return (int64_t)a.batch * a.heads * ((a.t + 255) / 256) >= 148 ? tc_forward<64, 2>(a, st) : tc_forward<64, 1>(a, st);
-  }
-  return with_type(dtype, d, [&](auto type, auto dim) { return simt_forward<decltype(type), dim()>(a, st); });
+  return with_type(dtype, d, [&](auto type, auto dim) {
+    if constexpr (!kOnTensorCores<decltype(type), dim()>) return simt_forward<decltype(type), dim()>(a, st);
+    else if constexpr (dim() == 128) return tc_forward<128, 1>(a, st);
+    else return a.docs == nullptr && a.t >= 2048 ? tc_forward<64, 2>(a, st) : tc_forward<64, 1>(a, st);
+  });
 }
 
 int dilution_attend_backward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
@@ -353,97 +206,10 @@ int dilution_attend_backward(const void* q, const void* k, const void* v, int dt
   if (int rc = check_attend("dilution_attend_backward", a, dtype, d)) return rc;
   if (!lse || !dout || !scratch || !dq || !dk || !dv || misaligned({scratch})) return abi_fail(DILUTION_ERR_ARG, "dilution_attend_backward: null or misaligned pointer");
   cudaStream_t st = (cudaStream_t)stream;
-  if (on_tensor_cores(dtype, d)) {
-    float2* stats = (float2*)((char*)scratch + delta_bytes(batch, heads, t));
-    return d == 128 ? tc_backward<128>(a, stats, st) : tc_backward<64>(a, stats, st);
-  }
-  return with_type(dtype, d, [&](auto type, auto dim) { return simt_backward<decltype(type), dim()>(a, st); });
-}
-
-size_t dilution_tree_scratch_bytes(int64_t batch, int64_t kv_heads, int group, int nodes, int64_t length, int d) {
-  if (batch < 1 || kv_heads < 1 || group < 1 || nodes < 1 || length < 0 || d < 1) return 0;
-  const int rows = group * nodes;
-  return tree_scratch(batch * kv_heads, rows, tree_chunks(batch * kv_heads * tree_row_blocks(rows), length + nodes), d).bytes;
-}
-
-int dilution_tree_softmax(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache, int dtype,
-                          int64_t batch, int64_t kv_heads, int group, int nodes, int64_t capacity, int64_t length,
-                          const int* length_dev, int d, float scale, float cap, const float* slopes, const int* parents,
-                          int64_t parent_stride, float* lse, void* out, void* scratch, void* stream) {
-  tree::Args a = tree_args(q, k_new, v_new, k_cache, v_cache, parents, parent_stride, batch, kv_heads, group, nodes, capacity,
-                           length, length_dev, scale, lse);
-  a.cap = cap;
-  a.slopes = slopes;
-  a.out = out;
-  if (int rc = check_tree("dilution_tree_softmax", a, length, dtype, d)) return rc;
-  if (!out || !scratch || misaligned({scratch})) return abi_fail(DILUTION_ERR_ARG, "dilution_tree_softmax: null or misaligned pointer");
-  const int rows = group * nodes;
-  a.chunks = tree_chunks((int64_t)a.batch * a.kv_heads * tree_row_blocks(rows), tree_keys(a));
-  place_scratch(a, scratch, rows, d);
-  cudaStream_t st = (cudaStream_t)stream;
   return with_type(dtype, d, [&](auto type, auto dim) {
-    using T = decltype(type);
-    if (int rc = rows <= 16 ? simt_softmax<T, dim(), 1, true>(a, st) : simt_softmax<T, dim(), 4, true>(a, st)) return rc;
-    return join<T, false>(a, d, st);
-  });
-}
-
-int dilution_tree_dilute(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache, int dtype,
-                         int64_t batch, int64_t heads, int nodes, int64_t capacity, int64_t length, const int* length_dev, int d,
-                         float scale, float eps, const float* committed, const int* parents, int64_t parent_stride, float* lse,
-                         void* out, void* scratch, void* stream) {
-  tree::Args a = tree_args(q, k_new, v_new, k_cache, v_cache, parents, parent_stride, batch, heads, 1, nodes, capacity, length,
-                           length_dev, scale, lse);
-  a.committed = committed;
-  a.out = out;
-  a.eps = eps;
-  if (int rc = check_tree("dilution_tree_dilute", a, length, dtype, d)) return rc;
-  if (!out || !committed || !scratch || misaligned({scratch}))
-    return abi_fail(DILUTION_ERR_ARG, "dilution_tree_dilute: null or misaligned pointer");
-  a.chunks = tree_chunks((int64_t)a.batch * a.kv_heads, tree_keys(a));
-  place_scratch(a, scratch, nodes, d);
-  cudaStream_t st = (cudaStream_t)stream;
-  return with_type(dtype, d, [&](auto type, auto dim) {
-    using T = decltype(type);
-    if (int rc = nodes <= 16 ? simt_softmax<T, dim(), 1, false>(a, st) : simt_softmax<T, dim(), 4, false>(a, st)) return rc;
-    {
-      LaunchMark mark("tree_join_stats", st);
-      const int64_t all = (int64_t)a.batch * a.kv_heads * nodes;
-      tree::join_stats_kernel<<<(unsigned)((all + 7) / 8), 256, 0, st>>>(a);
-      if (int rc = abi_check_launch("tree_join_stats")) return rc;
-    }
-    if (int rc = nodes <= 16 ? simt_dilute<T, dim(), 1>(a, st) : simt_dilute<T, dim(), 4>(a, st)) return rc;
-    return join<T, true>(a, d, st);
-  });
-}
-
-int dilution_tree_accept(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, int dtype,
-                         int64_t batch, int64_t kv_heads, int group, int nodes, int64_t capacity, int64_t length,
-                         const int* length_dev, int d, float scale, float cap, const float* slopes, const int* parents,
-                         int64_t parent_stride, const float* lse, const int* path, int64_t path_stride, int accepted,
-                         const float* committed, float* advanced, void* stream) {
-  tree::Args a = tree_args(q, k_new, v_new, k_cache, v_cache, parents, parent_stride, batch, kv_heads, group, nodes, capacity,
-                           length, length_dev, scale, const_cast<float*>(lse));
-  a.cap = cap;
-  a.slopes = slopes;
-  a.committed = committed;
-  if (int rc = check_tree("dilution_tree_accept", a, length, dtype, d)) return rc;
-  if (!path || (committed == nullptr) != (advanced == nullptr)) return abi_fail(DILUTION_ERR_ARG, "dilution_tree_accept: null pointer");
-  if (accepted < 1 || accepted > nodes || (!length_dev && length + accepted > capacity))
-    return abi_fail(DILUTION_ERR_ARG, "dilution_tree_accept: %d accepted nodes of %d behind %lld keys of %lld", accepted, nodes,
-                    (long long)length, (long long)capacity);
-  const tree::Accept c{path, path_stride, accepted, advanced, k_cache, v_cache};
-  a.chunks = tree_chunks((int64_t)a.batch * a.kv_heads, tree_keys(a));
-  cudaStream_t st = (cudaStream_t)stream;
-  return with_type(dtype, d, [&](auto type, auto dim) {
-    using T = decltype(type);
-    if (advanced)
-      if (int rc = group * accepted <= 16 ? simt_advance<T, dim(), 1>(a, c, st) : simt_advance<T, dim(), 4>(a, c, st)) return rc;
-    LaunchMark mark("tree_append", st);
-    const int row_bytes = d * (int)sizeof(T);
-    const int64_t threads = (int64_t)a.batch * a.kv_heads * accepted * (row_bytes / 16);
-    tree::append_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a, c, row_bytes);
-    return abi_check_launch("tree_append");
+    if constexpr (kOnTensorCores<decltype(type), dim()>)
+      return tc_backward<dim()>(a, (float2*)((char*)scratch + delta_bytes(batch, heads, t)), st);
+    else return simt_backward<decltype(type), dim()>(a, st);
   });
 }
 

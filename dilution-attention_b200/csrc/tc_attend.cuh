@@ -17,7 +17,7 @@
 #pragma once
 
 #include "attend_common.cuh"
-#include "tc_common.cuh"
+#include "tc_score.cuh"
 
 namespace dil {
 namespace tc {
@@ -25,15 +25,6 @@ namespace tc {
 __device__ int g_attend_status = 0;        // first bounded wait that ran out (0 = none)
 
 using attend::Row;
-
-__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-// Head sizes: D / 64 sub-tiles of 64 features (tc_common.cuh).
-template <int D> constexpr int kForm = D == 128 ? kWide128 : kNarrow;
 
 // ---- which pairs of tiles ------------------------------------------------------------------------
 struct Docs {
@@ -65,41 +56,6 @@ __device__ __forceinline__ int pair_state(const Row& r, int i0, int i1, const Do
   return j1 <= i0 || j1 < r.prefix ? 2 : 1;
 }
 
-// ---- scores ----------------------------------------------------------------------------------------
-// tanh of two values, |x| <= 1: x + x^3 P(x^2) with a least-maximum fit of degree 5, 1.6e-7 relative.  Nine packed instructions,
-// where the two special-function operations of a value take 16 cycles of a warp's quarter.
-__device__ __forceinline__ float2 tanh_poly2(float2 x) {
-  auto both = [](float c) { return make_float2(c, c); };
-  const float2 y = mul2(x, x);
-  float2 p = fma2(y, both(0.0010702026775106788f), both(-0.006294633727520704f));
-  p = fma2(p, y, both(0.02039860375225544f));
-  p = fma2(p, y, both(-0.053518135100603104f));
-  p = fma2(p, y, both(0.133268341422081f));
-  p = fma2(p, y, both(-0.3333301842212677f));
-  p = mul2(p, y);
-  return fma2(x, p, x);
-}
-// v = tanh(v * pre) of N products q . k.  pre: scale / cap.
-template <int N> __device__ __forceinline__ void cap_scores(float* v, float pre) {
-  float top = 0.f;
-#pragma unroll
-  for (int e = 0; e < N; e += 2) top = fmaxf(top, fmaxf(fabsf(v[e]), fabsf(v[e + 1])));
-  // (fmaxf passes over a NaN, which comes through either form)
-  if (__any_sync(0xffffffffu, top * pre > 1.f)) {
-    const float twice = pre * 2.f * kLog2e;
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = fmaf(-2.f, fast_rcp(1.f + fast_exp2(v[e] * twice)), 1.f);
-  } else {
-    const float2 pp = make_float2(pre, pre);
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-      const float2 t = tanh_poly2(mul2(make_float2(v[e], v[e + 1]), pp));
-      v[e] = t.x;
-      v[e + 1] = t.y;
-    }
-  }
-}
-
 // ---- forward -----------------------------------------------------------------------------------------
 template <int D, int NT> struct AttendForward {
   static constexpr int kThreads = 256 * NT + 32;
@@ -117,6 +73,49 @@ template <int D, int NT> struct AttendForward {
 
 constexpr float kAttendLimit = 1099511627776.f;      // 2^40: a half tile whose P~ sum to more moves the reference
 
+// Bits of 64 tokens x0 .. that have the lane's document id, which may differ from lane to lane (a negative one: none).  Each lane
+// brings two of the tokens' ids; lanes of one id are served together.
+__device__ __forceinline__ uint2 document_bits(const Row& r, int x0, int id) {
+  const int lane = threadIdx.x & 31, k0 = r.docs[min(x0 + lane, r.t - 1)], k1 = r.docs[min(x0 + 32 + lane, r.t - 1)];
+  uint2 bits = make_uint2(0, 0);
+  for (unsigned todo = __ballot_sync(0xffffffffu, id >= 0); todo;) {
+    const int want = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
+    const uint2 same = make_uint2(__ballot_sync(0xffffffffu, k0 == want), __ballot_sync(0xffffffffu, k1 == want));
+    if (id == want) bits = same;
+    todo &= ~__ballot_sync(0xffffffffu, id == want);
+  }
+  return bits;
+}
+// The lowest n of 64 bits.
+__device__ __forceinline__ uint2 low_bits(int n) {
+  return make_uint2(n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1, n >= 64 ? ~0u : n <= 32 ? 0u : (1u << (n - 32)) - 1);
+}
+__device__ __forceinline__ bool bit_of(const uint2& m, int e) { return (e < 32 ? m.x >> e : m.y >> (e - 32)) & 1; }
+// Which of the keys j0 .. query i sees, and which of the queries i0 .. see key j.
+__device__ __forceinline__ uint2 key_bits(const Row& r, int i, int j0) {
+  uint2 m = low_bits(min(max(i + 1, r.prefix), r.t) - j0);
+  if (r.docs != nullptr) {
+    const uint2 d = document_bits(r, j0, r.docs[i]);
+    m.x &= d.x;
+    m.y &= d.y;
+  }
+  return m;
+}
+__device__ __forceinline__ uint2 query_bits(const Row& r, int i0, int j) {
+  uint2 m = low_bits(r.t - i0);
+  if (j >= r.prefix) {
+    const uint2 x = low_bits(j - i0);
+    m.x &= ~x.x;
+    m.y &= ~x.y;
+  }
+  if (r.docs != nullptr) {
+    const uint2 d = document_bits(r, i0, r.docs[j]);
+    m.x &= d.x;
+    m.y &= d.y;
+  }
+  return m;
+}
+
 // A warpgroup's step over the 64 scores of keys j0 .. at tS: P~ = 2^(z - reference) as bf16 over the scores, their sum
 // into s.  The reference is the maximum of the first half tile that a row sees and moves where a later one's P~ sum to more
 // than 2^40; only then is the accumulator rescaled.  bf16 has the range of fp32: P~ below that limit keeps 8 bits.
@@ -126,25 +125,39 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
   float v[64];
   uint32_t pw[32];
   float ps;
+  bool some = true;                  // the row sees any of the keys
+  // the scores as z = mul v + add + step e, masked ones -inf
   auto fetch = [&]() {
     tmem_ld32(tS, v);
     tmem_ld32(tS + 32, v + 32);
     tmem_ld_wait(v);
     tmem_ld_wait(v + 32);
     if (CAP) cap_scores<64>(v, pre);
+    if (edge) {
+      const uint2 m = key_bits(r, i, j0);
+      some = (m.x | m.y) != 0;
+      if (BIAS) {                    // distances of both signs
+        const float far = (float)(i - j0);
+#pragma unroll
+        for (int e = 0; e < 64; ++e) v[e] = fmaf(v[e], lin, -r.slope2 * fabsf(far - (float)e));
+      }
+#pragma unroll
+      for (int e = 0; e < 64; ++e) v[e] = bit_of(m, e) ? v[e] : -INFINITY;
+    }
   };
-  // P~ of scores mul * v + add + step * e
+  const float mul = BIAS && edge ? 1.f : lin, step = BIAS && !edge ? r.slope2 : 0.f;
+  const float add = BIAS && !edge ? r.slope2 * (float)(j0 - i) : 0.f;
   auto exponentials = [&](float mul, float add, float step) {
-    const float2 mm = make_float2(mul, mul);
+    const float2 mm = make_float2(mul, mul), four = make_float2(4.f * step, 4.f * step);
     float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+    float2 o0 = make_float2(add, BIAS ? add + step : add), o1 = BIAS ? make_float2(add + 2.f * step, add + 3.f * step) : o0;
 #pragma unroll
     for (int e = 0; e < 64; e += 4) {
-      float2 o0 = make_float2(add, add), o1 = o0;
-      if (BIAS) {
-        o0 = fma2(make_float2(step, step), make_float2((float)e, (float)(e + 1)), o0);
-        o1 = fma2(make_float2(step, step), make_float2((float)(e + 2), (float)(e + 3)), o1);
-      }
       const float2 z0 = fma2(make_float2(v[e], v[e + 1]), mm, o0), z1 = fma2(make_float2(v[e + 2], v[e + 3]), mm, o1);
+      if (BIAS) {
+        o0 = add2(o0, four);
+        o1 = add2(o1, four);
+      }
       const float2 p0 = make_float2(fast_exp2(z0.x), fast_exp2(z0.y)), p1 = make_float2(fast_exp2(z1.x), fast_exp2(z1.y));
       a0 = add2(a0, p0);
       a1 = add2(a1, p1);
@@ -155,28 +168,18 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
     ps = a.x + a.y;
   };
   fetch();
-  bool slow = edge || __any_sync(0xffffffffu, ref == -INFINITY);
+  bool slow = __any_sync(0xffffffffu, ref == -INFINITY && some);
   if (!slow) {
-    exponentials(lin, (BIAS ? r.slope2 * (float)(j0 - i) : 0.f) - ref, r.slope2);
+    exponentials(mul, ref == -INFINITY ? 0.f : add - ref, step);
     slow = __any_sync(0xffffffffu, !(ps < kAttendLimit));
     if (slow) fetch();               // rare: the scores are still in TMEM
   }
   if (slow) {
     float top = -INFINITY;
-    const bool docs = edge && r.docs != nullptr;
-    const int id = docs ? r.docs[i] : 0;
 #pragma unroll
     for (int e = 0; e < 64; ++e) {
-      const int j = j0 + e;
-      float z = v[e] * lin;
-      if (BIAS) z = fmaf(-r.slope2, fabsf((float)(i - j)), z);
-      if (edge) {
-        bool ok = j < r.t && (j <= i || j < r.prefix);
-        if (docs) ok = ok && id >= 0 && r.docs[min(j, r.t - 1)] == id;
-        z = ok ? z : -INFINITY;
-      }
-      v[e] = z;
-      top = fmaxf(top, z);
+      v[e] = fmaf(v[e], mul, BIAS ? fmaf(step, (float)e, add) : 0.f);
+      top = fmaxf(top, v[e]);
     }
     const float now = fmaxf(ref, top);
     if (__any_sync(0xffffffffu, now != ref)) {
@@ -456,8 +459,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 template <int STAY, bool CAP, bool BIAS>
 __device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float lin, float pre, int x0, int y, bool edge, float2 own,
                                               const float4* st) {
-  const bool docs = edge && r.docs != nullptr;
-  const int id = docs ? r.docs[y] : 0;
+  uint2 bits = make_uint2(0, 0);
+  if (edge) bits = STAY == 1 ? query_bits(r, x0, y) : key_bits(r, y, x0);
 #pragma unroll
   for (int c0 = 0; c0 < 64; c0 += 32) {
     float v[32], g[32];
@@ -471,6 +474,7 @@ __device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float l
     // the distance's term of column e: first + step * e (one sign throughout, except in masked tiles)
     const float step = STAY == 1 ? -r.slope2 : r.slope2;
     const float first = STAY == 1 ? r.slope2 * (float)(y - x0 - c0) : r.slope2 * (float)(x0 + c0 - y);
+    float2 far = make_float2(first, first + step);
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
       float2 off, delta;                                  // -lse (and the distance's term), -delta
@@ -483,9 +487,8 @@ __device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float l
         delta = make_float2(-own.y, -own.y);
       }
       if (BIAS) {
-        float2 far = fma2(make_float2(step, step), make_float2((float)e, (float)(e + 1)), make_float2(first, first));
-        if (edge) far = make_float2(-fabsf(far.x), -fabsf(far.y));
-        off = add2(off, far);
+        off = add2(off, edge ? make_float2(-fabsf(far.x), -fabsf(far.y)) : far);
+        far = add2(far, make_float2(2.f * step, 2.f * step));
       }
       float2 z = fma2(make_float2(v[e], v[e + 1]), mm, off);
       float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
@@ -496,13 +499,8 @@ __device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float l
         d = mul2(d, fma2(minus, t, make_float2(1.f, 1.f)));
       }
       if (edge) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int x = x0 + c0 + e + k, i = STAY == 1 ? x : y, j = STAY == 1 ? y : x;
-          bool ok = x < r.t && (j <= i || j < r.prefix);
-          if (docs) ok = ok && id >= 0 && r.docs[min(x, r.t - 1)] == id;
-          if (!ok) (k ? p.y : p.x) = 0.f, (k ? d.y : d.x) = 0.f;
-        }
+        if (!bit_of(bits, c0 + e)) p.x = d.x = 0.f;
+        if (!bit_of(bits, c0 + e + 1)) p.y = d.y = 0.f;
       }
       if (STAY == 1) pw[e >> 1] = pack_pair(p.x, p.y);
       gw[e >> 1] = pack_pair(d.x, d.y);
@@ -732,37 +730,6 @@ __global__ void __launch_bounds__(256) attend_stats_kernel(attend::Args a, float
     stats[at] = real ? make_float2(a.lse[n * a.t + i], s) : make_float2(INFINITY, 0.f);
     if (real) a.delta[n * a.t + i] = s;
   }
-}
-
-// ---- launches ------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                CUtensorMapFloatOOBfill);
-inline EncodeTiled encode_tiled() {
-  static EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return (EncodeTiled)p;
-  }();
-  return fn;
-}
-// (n, t, d) bf16 rows as boxes {64 features, box rows, 1}, 128-byte swizzle; rows past t read as zero.  True: encoded.
-inline bool attend_map(CUtensorMap* map, const void* base, int64_t n, int64_t t, int d, int box) {
-  // the encoder wants a current context, which a thread that has only selected a device (one of autograd's) need not have yet
-  static thread_local bool bound = false;
-  if (!bound) {
-    cudaFree(nullptr);
-    bound = true;
-  }
-  EncodeTiled fn = encode_tiled();
-  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)t, (cuuint64_t)n};
-  const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)t * d * 2};
-  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
-  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, boxes, ones,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace tc

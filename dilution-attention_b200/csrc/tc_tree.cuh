@@ -1,0 +1,587 @@
+// Tree steps over a bf16 cache with heads of 64 and 128, on the tensor cores.  All nodes see all cached keys, so the kernels
+// that stream the cache know no mask but its end; the nodes' own keys (64 at most) are joined in afterwards with fp32 FMAs.
+//
+//   scan_kernel : scores S = Q K^T, lane = row of the key head; online softmax, and P V if asked for.  Rows are few, lanes are
+//                 128: up to 32 (64) rows are laid out four times (twice), each time against another quarter (half) of a tile's
+//                 keys.  That is a product with a block-diagonal Q: the quarters' operands are one buffer with zeros around the
+//                 rows, read from another offset, and each warp's P~ goes to columns of its own that are zero in other
+//                 lanes.  The tensor pipe has the time (the cache's bytes are the bound), the special-function unit has not.
+//   sweep_kernel: S^T = K Q^T, lane = key, for what belongs to keys: a thread walks the tree in the nodes' order with its
+//                 key's demand (a node's demand is its parent's demand and bid; a parent further back is found in the TMEM
+//                 column that its score came from), and out^T += V^T share; or it adds the accepted nodes' bids.
+// A chunk of a key head's keys per CTA; one warp issues copies, one MMAs, two warpgroups take tiles in turn.
+#pragma once
+
+#include "tc_score.cuh"
+#include "tree_common.cuh"
+
+namespace dil {
+namespace tc {
+
+__device__ int g_tree_status = 0;          // first bounded wait that ran out (0 = none)
+
+// 16 bytes c of row `row` of a [rows][64] bf16 tile under the 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int row, int c) { return (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)); }
+
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
+}
+
+// A cache's tile whose last rows lie behind its end (a length that only the device knows: the copy could not leave them out).
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int rows, int from, int subs) {
+  for (int s = 0; s < subs; ++s)
+    for (int x = from * 8 + (int)(threadIdx.x & 31); x < rows * 8; x += 32)
+      reinterpret_cast<uint4*>(tile + s * rows * 128)[x] = make_uint4(0, 0, 0, 0);
+}
+
+// Barriers of a CTA that streams a cache: full[R], free[R], sdone[2], alldone, pready[2].
+template <int R> struct StreamBars {
+  uint32_t full, free, sdone, alldone, pready;
+  Ctl* ctl;
+  __device__ __forceinline__ StreamBars(uint64_t* b) {
+    full = smem_u32(b);
+    free = full + 8 * R;
+    sdone = free + 8 * R;
+    alldone = sdone + 16;
+    pready = alldone + 8;
+    ctl = reinterpret_cast<Ctl*>(b + 2 * R + 5);
+  }
+  __device__ __forceinline__ void init() const {
+    ctl->abort = 0;
+    for (int x = 0; x < 2 * R + 3; ++x) mbar_init(full + 8 * x, 1);
+    for (int x = 0; x < 2; ++x) mbar_init(pready + 8 * x, 4);
+    fence_barrier_init();
+  }
+};
+
+// The warp that copies tiles [e0, e0 + ne) of KT keys, K and (if V) values behind them, into the ring.
+template <int D, int KT, int R, bool V>
+__device__ __forceinline__ void stream_tiles(const StreamBars<R>& bars, const CUtensorMap* map_k, const CUtensorMap* map_v, uint32_t ring,
+                                             int first, int ne, int nk, uint32_t lead) {
+  constexpr uint32_t kOne = KT * D * 2, kStage = V ? 2 * kOne : kOne;
+  for (int e = 0; e < ne; ++e) {
+    const int st = e % R;
+    if (e >= R) mbar_wait_warp(bars.free + 8 * st, (e / R - 1) & 1, bars.ctl, &g_tree_status, kErrWaitMma);
+    if (lead) {
+      mbar_expect_tx(bars.full + 8 * st, kStage);
+#pragma unroll
+      for (int x = 0; x < KT / 64; ++x) {
+        tma_load_rows<kForm<D>>(ring + kStage * st + 8192 * x, map_k, (first + e) * KT + 64 * x, nk, bars.full + 8 * st, KT * 128);
+        if (V) tma_load_rows<kForm<D>>(ring + kStage * st + kOne + 8192 * x, map_v, (first + e) * KT + 64 * x, nk, bars.full + 8 * st, KT * 128);
+      }
+    }
+    __syncwarp();
+  }
+}
+
+// ---- scan ----------------------------------------------------------------------------------------------
+template <int D, int G, bool OUT> struct Scan {
+  static constexpr int kRows = 128 / G, kCols = G == 4 ? 32 : 64, kKeys = kCols * G;
+  static constexpr int kThreads = 320;
+  static constexpr uint32_t kOne = kKeys * D * 2, kStage = OUT ? 2 * kOne : kOne;
+  static constexpr int kRing = (int)(131072 / kStage) < 8 ? (int)(131072 / kStage) : 8;
+  static constexpr int kBufRows = (G - 1) * kRows + 128;                   // zeros, the rows, zeros
+  static constexpr uint32_t kBufSub = kBufRows * 128;
+  static constexpr int kBuf = (int)kBufSub * (D / 64), kRingBytes = (int)kStage * kRing;
+  static constexpr int kBytes = kBuf + kRingBytes + 2048 + 256 + 1024;
+  static constexpr int kWgCols = 128 + (OUT ? D : 0), kTmem = OUT ? 512 : 256;
+  static_assert(2 * kWgCols <= kTmem, "the warpgroups' columns fit the allocation");
+  static_assert(!OUT || 256 * D * 4 <= kRingBytes, "the merge area fits the ring");
+  static_assert(kRing >= 2 && kBytes <= 232448, "shared memory");
+};
+
+// One warpgroup's step: kCols scores of a lane at tS, its P~ (OUT) to tP.
+template <int D, int N, bool OUT>
+__device__ __forceinline__ void scan_step(uint32_t tS, uint32_t tP, uint32_t tO, float lin, float pre, bool cap, float slope2, float far, int valid,
+                                          float& ref, float& s) {
+  float v[N];
+  uint32_t pw[N / 2];
+  float ps;
+  auto fetch = [&]() {
+    tmem_ld32(tS, v);
+    if (N == 64) tmem_ld32(tS + 32, v + (N - 32));
+    tmem_ld_wait(v);
+    if (N == 64) tmem_ld_wait(v + (N - 32));
+    if (cap) cap_scores<N>(v, pre);
+    if (valid < N) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = e < valid ? v[e] : -INFINITY;
+    }
+  };
+  // z = mul v + add + step e (the distance shrinks with the key's position)
+  auto exponentials = [&](float mul, float add, float step) {
+    const float2 mm = make_float2(mul, mul), four = make_float2(4.f * step, 4.f * step);
+    float2 o0 = make_float2(add, add + step), o1 = make_float2(add + 2.f * step, add + 3.f * step);
+    float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const float2 z0 = fma2(make_float2(v[e], v[e + 1]), mm, o0), z1 = fma2(make_float2(v[e + 2], v[e + 3]), mm, o1);
+      o0 = add2(o0, four);
+      o1 = add2(o1, four);
+      const float2 p0 = make_float2(fast_exp2(z0.x), fast_exp2(z0.y)), p1 = make_float2(fast_exp2(z1.x), fast_exp2(z1.y));
+      a0 = add2(a0, p0);
+      a1 = add2(a1, p1);
+      if (OUT) {
+        pw[e >> 1] = pack_pair(p0.x, p0.y);
+        pw[(e >> 1) + 1] = pack_pair(p1.x, p1.y);
+      }
+    }
+    const float2 a = add2(a0, a1);
+    ps = a.x + a.y;
+  };
+  const float add = -slope2 * far;
+  fetch();
+  bool slow = __any_sync(0xffffffffu, ref == -INFINITY && valid > 0);
+  if (!slow) {
+    exponentials(lin, ref == -INFINITY ? 0.f : add - ref, slope2);
+    slow = __any_sync(0xffffffffu, !(ps < 1099511627776.f));       // 2^40
+    if (slow) fetch();               // rare: the scores are still in TMEM
+  }
+  if (slow) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      v[e] = fmaf(v[e], lin, fmaf(slope2, (float)e, add));
+      top = fmaxf(top, v[e]);
+    }
+    const float now = fmaxf(ref, top);
+    if (__any_sync(0xffffffffu, now != ref)) {
+      const bool fresh = __all_sync(0xffffffffu, ref == -INFINITY);
+      const float f = fast_exp2(ref - (now == -INFINITY ? 0.f : now));
+      if (OUT && !fresh) {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          float o[16];
+          tmem_ld16(tO + 16 * c, o);
+          tmem_ld_wait16(o);
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
+          tmem_st16(tO + 16 * c, w);
+        }
+      }
+      s *= f;
+      ref = now;
+    }
+    exponentials(1.f, ref == -INFINITY ? 0.f : -ref, 0.f);
+  }
+  s += ps;
+  if (OUT) {
+    tmem_st16(tP, pw);
+    if (N == 64) tmem_st16(tP + 16, pw + (N / 2 - 16));
+    tmem_st_wait();
+  }
+}
+
+// grid = (chunks, ceil(rows / 128) or 1, batch * kv_heads)
+template <int D, int G, bool OUT>
+__global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                      const __grid_constant__ tree::Args a) {
+  using F = Scan<D, G, OUT>;
+  constexpr int R = F::kRing, KT = F::kKeys, NC = F::kCols, SUB = D / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  const uint32_t sQ = smem_u32(smem), ring = sQ + F::kBuf;
+  float2* sStat = reinterpret_cast<float2*>(smem + F::kBuf + F::kRingBytes);              // [2][128]
+  const StreamBars<R> bars(reinterpret_cast<uint64_t*>(smem + F::kBuf + F::kRingBytes + 2048));
+  Ctl* ctl = bars.ctl;
+  __shared__ tree::Lineage lineage;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
+  const int warp_u = uniform_warp();
+  const uint32_t lead = elect_one();
+  const int nk = blockIdx.z, b = nk / a.kv_heads, hk = nk % a.kv_heads, rows = a.group * a.nodes, r0 = blockIdx.y * 128;
+  const int len = (int)uniform(tree::cache_len(a.pos_dev, a.len, a.capacity));
+  const int2 keys = tree::chunk_keys(len, a.chunks, blockIdx.x, KT);
+  const int first = keys.x / KT, ne = (keys.y - keys.x + KT - 1) / KT;
+
+  if (tid == 0) bars.init();
+  // the rows between zeros
+  for (int x = tid; x < F::kBufRows * 8 * SUB; x += F::kThreads) {
+    const int sub = x / (F::kBufRows * 8), br = x / 8 % F::kBufRows, c = x % 8, r = r0 + br - (G - 1) * F::kRows;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (r >= r0 && r < min(rows, r0 + F::kRows))
+      w = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((int64_t)nk * rows + r) * D + 64 * sub + 8 * c);
+    *reinterpret_cast<uint4*>(smem + sub * F::kBufSub + swizzled(br, c)) = w;
+  }
+  fence_async_smem();
+  if (a.slopes != nullptr) tree::make_lineage(&lineage, a.parents + b * a.parent_stride, a.nodes);
+  __syncwarp();
+  if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(ctl->tmem);
+
+  if (warp_u == 8) {
+    // ------------------------------------------------------------ the warp that issues MMAs
+    constexpr uint32_t id_s = instr_desc(128, NC, 0, 0), id_p = instr_desc(128, D, 0, 1);
+    const Desc dQ = make_desc(sQ, 16, 1024), dK = make_desc(ring, 16, 1024), dV = make_desc(ring + F::kOne, KT * 128, 1024);
+    // what the compute warps clear (their P~ columns and accumulators) is clear before the first product
+    asm volatile("bar.sync 4, 288;" ::: "memory");
+    tc_fence_after();
+    for (int e = 0; e < ne + 2; ++e) {
+      const int w = e & 1;
+      const uint32_t tS = tmem + F::kWgCols * w;
+      if (e >= 2) {
+        mbar_wait_warp(bars.pready + 8 * w, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitTile);
+        tc_fence_after();
+        if (OUT) {
+          const int st = (e - 2) % R;
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int kk = 0; kk < NC / 16; ++kk)               // 16 keys per instruction: 16 rows of 128 B = 128 units
+              mma_ts(lead, tS + 128, tS + 64 + (NC / 2) * g + 8 * kk, dV, (F::kStage >> 4) * st + 8 * NC * g + 128 * kk, id_p, 1);
+          mma_commit(lead, bars.free + 8 * st);
+        }
+      }
+      if (e < ne) {
+        const int st = e % R, from = len - (first + e) * KT;
+        mbar_wait_warp(bars.full + 8 * st, (e / R) & 1, ctl, &g_tree_status, kErrWaitTma);
+        if (from < KT) {
+          zero_rows(smem + F::kBuf + F::kStage * st, KT, from, SUB);
+          if (OUT) zero_rows(smem + F::kBuf + F::kStage * st + F::kOne, KT, from, SUB);
+          fence_async_smem();
+          __syncwarp();
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int s = 0; s < SUB; ++s)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(lead, tS, dQ, (F::kBufSub >> 4) * s + 8 * F::kRows * (G - 1 - g) + 2 * kk, dK,
+                     (F::kStage >> 4) * st + 8 * KT * s + 8 * NC * g + 2 * kk, id_s, g > 0 || s > 0 || kk > 0);
+        mma_commit(lead, bars.sdone + 8 * w);
+        if (!OUT) mma_commit(lead, bars.free + 8 * st);
+      }
+    }
+    mma_commit(lead, bars.alldone);
+    __syncwarp();
+  } else if (warp_u == 9) {
+    stream_tiles<D, KT, R, OUT>(bars, &map_k, &map_v, ring, first, ne, nk, lead);
+  } else {
+    // ------------------------------------------------------------ the compute warps: lane = row of a group
+    const uint32_t tS = tmem + F::kWgCols * wg + ((uint32_t)((warp & 3) * 32) << 16), tP = tS + 64, tO = tS + 128;
+    const int g = row / F::kRows, x = row % F::kRows, r = r0 + x, rs = min(r, rows - 1);
+    if (OUT) {
+      uint32_t z[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) z[c] = 0u;
+#pragma unroll
+      for (int c = 0; c < 4 + D / 16; ++c) tmem_st16(tP + 16 * c, z);
+      tmem_st_wait();
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 4, 288;" ::: "memory");
+    const bool cap = a.cap > 0.f;
+    const float lin = cap ? a.cap * kLog2e : a.scale * kLog2e, pre = cap ? a.scale / a.cap : 0.f;
+    float slope2 = 0.f;
+    int at = len;
+    if (a.slopes != nullptr) {
+      slope2 = a.slopes[hk * a.group + rs / a.nodes] * kLog2e;
+      at += lineage.depth[rs % a.nodes];
+    }
+    float ref = -INFINITY, s = 0.f;
+    for (int e = wg; e < ne; e += 2) {
+      const int j0 = (first + e) * KT + NC * g;
+      mbar_wait_warp(bars.sdone + 8 * wg, (e >> 1) & 1, ctl, &g_tree_status, kErrWaitMma);
+      tc_fence_after();
+      scan_step<D, NC, OUT>(tS, tP + (NC / 2) * g, tO, lin, pre, cap, slope2, (float)(at - j0), len - j0, ref, s);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars.pready + 8 * wg);
+    }
+    // rows that are laid out several times, and the two warpgroups' keys, are one row
+    sStat[wg * 128 + row] = make_float2(ref, s);
+    float* sO = reinterpret_cast<float*>(smem + F::kBuf);           // [2][128][D], over the ring
+    if (OUT) {
+      mbar_wait_warp(bars.alldone, 0, ctl, &g_tree_status, kErrWaitMma);
+      tc_fence_after();
+      __syncwarp();
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        float o[32];
+        tmem_ld32(tO + c0, o);
+        tmem_ld_wait(o);
+        float4* dst = reinterpret_cast<float4*>(sO + (wg * 128 + row) * D + c0);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) dst[c ^ (row & 7)] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+      }
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    constexpr int kUnits = OUT ? D / 4 : 1;
+    const int64_t base = ((int64_t)nk * a.chunks + blockIdx.x) * rows;
+    for (int y = tid; y < F::kRows * kUnits; y += 256) {
+      const int xr = y / kUnits, c = y % kUnits;
+      if (r0 + xr >= rows) break;
+      float m = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int p = 0; p < 2 * G; ++p) m = fmaxf(m, sStat[(p / G) * 128 + (p % G) * F::kRows + xr].x);
+      const float from = m == -INFINITY ? 0.f : m;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int p = 0; p < 2 * G; ++p) {
+        const int lane_row = (p / G) * 128 + (p % G) * F::kRows + xr;
+        const float2 st = sStat[lane_row];
+        const float f = fast_exp2(st.x - from);
+        sum = fmaf(st.y, f, sum);
+        if (OUT) {
+          const float4 z = reinterpret_cast<const float4*>(sO + lane_row * D)[(c & ~7) | ((c & 7) ^ (lane_row & 7))];
+          o.x = fmaf(z.x, f, o.x);
+          o.y = fmaf(z.y, f, o.y);
+          o.z = fmaf(z.z, f, o.z);
+          o.w = fmaf(z.w, f, o.w);
+        }
+      }
+      if (c == 0) a.part[base + r0 + xr] = make_float2(m, sum);
+      if (OUT) reinterpret_cast<float4*>(a.pout + (base + r0 + xr) * D)[c] = o;
+    }
+  }
+  drain_if_aborted(ctl);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_free(tmem, F::kTmem);
+}
+
+// ---- sweep ---------------------------------------------------------------------------------------------
+// What the thread of a key has to know of a row.
+struct NodeStep {
+  float lse;
+  int up;              // -1: the cached demand; -2: the node in front; otherwise the parent, whose column is read
+  int keep;            // a later node reads this one's column
+  float slope2;        // of an accepted row, and its position
+};
+
+template <int D, int N, bool DILUTE> struct Sweep {
+  static constexpr int kKeys = 128, kThreads = 320;
+  static constexpr uint32_t kOne = 128 * D * 2, kStage = DILUTE ? 2 * kOne : kOne;
+  static constexpr int kRing = (int)(131072 / kStage) < 8 ? (int)(131072 / kStage) : 8;
+  static constexpr uint32_t kQSub = N * 128;
+  static constexpr int kQ = N * 128 * (D / 64), kRingBytes = (int)kStage * kRing;
+  // Q | ring | share [2][128][64] | ones [2][16][64] | node steps and positions | barriers + control
+  static constexpr int kShare = DILUTE ? 2 * 16384 : 0, kOnes = DILUTE ? 4096 : 0;
+  static constexpr int kBytes = (kQ + 1023) / 1024 * 1024 + kRingBytes + kShare + kOnes + 64 * 16 + 256 + 256 + 1024;
+  static constexpr int kTmem = 256;                                          // S^T 2 x 64, out^T 64, sums 64
+  static_assert(kRing >= 2 && kBytes <= 232448, "shared memory");
+};
+
+// DILUTE: shares of the nodes and their part of share V.  Otherwise: advanced = committed + the bids of the accepted rows.
+// grid = (chunks, 1, batch * kv_heads); N >= rows
+template <int D, int N, bool DILUTE>
+__global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                       const __grid_constant__ tree::Args a, const __grid_constant__ tree::Accept acc) {
+  using F = Sweep<D, N, DILUTE>;
+  constexpr int R = F::kRing, KT = 128, SUB = D / 64, kQ = (F::kQ + 1023) / 1024 * 1024;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint8_t *pShare = smem + kQ + F::kRingBytes, *pOnes = pShare + F::kShare;
+  const uint32_t sQ = smem_u32(smem), ring = sQ + kQ, sShare = smem_u32(pShare), sOnes = smem_u32(pOnes);
+  NodeStep* step = reinterpret_cast<NodeStep*>(pOnes + F::kOnes);
+  int* place = reinterpret_cast<int*>(step + 64);                                        // positions of accepted rows
+  const StreamBars<R> bars(reinterpret_cast<uint64_t*>(place + 64));
+  Ctl* ctl = bars.ctl;
+  __shared__ tree::Lineage lineage;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
+  const int warp_u = uniform_warp();
+  const uint32_t lead = elect_one();
+  const int nk = blockIdx.z, b = nk / a.kv_heads, hk = nk % a.kv_heads;
+  const int rows = DILUTE ? a.nodes : a.group * acc.accepted;
+  const int len = (int)uniform(tree::cache_len(a.pos_dev, a.len, a.capacity));
+  const int2 keys = tree::chunk_keys(len, a.chunks, blockIdx.x, KT);
+  const int first = keys.x / KT, ne = (keys.y - keys.x + KT - 1) / KT;
+
+  if (tid == 0) bars.init();
+  tree::make_lineage(&lineage, a.parents + b * a.parent_stride, a.nodes);
+  // row r of the sweep is row q_row(r) of the key head's queries
+  auto q_row = [&](int r) { return DILUTE ? r : r / acc.accepted * a.nodes + tree::path_node(a, acc, b, r % acc.accepted); };
+  if (tid < N) {
+    NodeStep s{0.f, -1, 0, 0.f};
+    int at = 0;
+    if (tid < rows) {
+      const int q = q_row(tid);
+      s.lse = a.lse[((int64_t)nk * a.group) * a.nodes + q];
+      if (DILUTE) {
+        const int up = lineage.parent[tid];
+        s.up = up >= 0 && up == tid - 1 ? -2 : up;
+        for (int y = tid + 2; y < a.nodes; ++y) s.keep |= lineage.parent[y] == tid;
+      } else {
+        s.slope2 = a.slopes != nullptr ? a.slopes[hk * a.group + q / a.nodes] * kLog2e : 0.f;
+        at = lineage.depth[q % a.nodes];
+      }
+    }
+    step[tid] = s;
+    place[tid] = len + at;
+  }
+  for (int x = tid; x < N * 8 * SUB; x += F::kThreads) {
+    const int sub = x / (N * 8), r = x / 8 % N, c = x % 8;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (r < rows)
+      w = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((int64_t)nk * a.group * a.nodes + q_row(r)) * D +
+                                          64 * sub + 8 * c);
+    *reinterpret_cast<uint4*>(smem + sub * F::kQSub + swizzled(r, c)) = w;
+  }
+  if (DILUTE) {
+    // shares of nodes behind the last stay zero; ones: column 0 of both groups of 64
+    for (int x = tid; x < F::kShare / 16; x += F::kThreads) reinterpret_cast<uint4*>(pShare)[x] = make_uint4(0, 0, 0, 0);
+    for (int x = tid; x < 256; x += F::kThreads)
+      *reinterpret_cast<uint4*>(pOnes + (x >> 7) * 2048 + swizzled((x >> 3) & 15, x & 7)) = make_uint4((x & 7) == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);
+  }
+  fence_async_smem();
+  __syncwarp();
+  if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(ctl->tmem);
+
+  if (warp_u == 8) {
+    // ------------------------------------------------------------ the warp that issues MMAs
+    constexpr uint32_t id_s = instr_desc(128, N, 0, 0), id_o = instr_desc(128, N, 1, 1);
+    const Desc dK = make_desc(ring, 16, 1024), dQ = make_desc(sQ, 16, 1024);
+    const Desc dOnes = make_desc(sOnes, 2048, 1024);
+    for (int e = 0; e < ne + 2; ++e) {
+      const int w = e & 1;
+      const uint32_t tS = tmem + 64 * w;
+      if (e >= 2) {
+        mbar_wait_warp(bars.pready + 8 * w, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitTile);
+        tc_fence_after();
+        if (DILUTE) {
+          const int st = (e - 2) % R;
+          const uint32_t v = ring + F::kStage * st + F::kOne;
+          const Desc dP = make_desc(sShare + 16384 * w, 16384, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            // heads of 64: the second 64 rows of A are the ones, out^T has the sums in row 64
+            const uint32_t at = v + 2048 * kk;
+            mma_ss(lead, tmem + 128, make_desc(at, D == 64 ? sOnes - at : KT * 128, 1024), 0, dP, 128 * kk, id_o, e > 2 || kk > 0);
+            if (D == 128) mma_ss(lead, tmem + 192, dOnes, 0, dP, 128 * kk, id_o, e > 2 || kk > 0);
+          }
+          mma_commit(lead, bars.free + 8 * st);
+        }
+      }
+      if (e < ne) {
+        const int st = e % R, from = len - (first + e) * KT;
+        mbar_wait_warp(bars.full + 8 * st, (e / R) & 1, ctl, &g_tree_status, kErrWaitTma);
+        if (from < KT) {
+          zero_rows(smem + kQ + F::kStage * st, KT, from, SUB);
+          if (DILUTE) zero_rows(smem + kQ + F::kStage * st + F::kOne, KT, from, SUB);
+          fence_async_smem();
+          __syncwarp();
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(lead, tS, dK, (F::kStage >> 4) * st + 8 * KT * s + 2 * kk, dQ, (F::kQSub >> 4) * s + 2 * kk, id_s, s > 0 || kk > 0);
+        mma_commit(lead, bars.sdone + 8 * w);
+        if (!DILUTE) mma_commit(lead, bars.free + 8 * st);
+      }
+    }
+    mma_commit(lead, bars.alldone);
+    __syncwarp();
+  } else if (warp_u == 9) {
+    stream_tiles<D, KT, R, DILUTE>(bars, &map_k, &map_v, ring, first, ne, nk, lead);
+  } else {
+    // ------------------------------------------------------------ the compute warps: lane = key
+    const uint32_t tS = tmem + 64 * wg + ((uint32_t)((warp & 3) * 32) << 16);
+    const bool cap = a.cap > 0.f;
+    const float lin = cap ? a.cap * kLog2e : a.scale * kLog2e, pre = cap ? a.scale / a.cap : 0.f;
+    for (int e = wg; e < ne; e += 2) {
+      const int j = (first + e) * KT + row;
+      const bool live = j < len;
+      const int64_t at = (int64_t)nk * a.capacity + j;
+      const float base = live ? a.committed[at] : 0.f;
+      mbar_wait_warp(bars.sdone + 8 * wg, (e >> 1) & 1, ctl, &g_tree_status, kErrWaitMma);
+      tc_fence_after();
+      float last = base, total = base;
+#pragma unroll
+      for (int c0 = 0; c0 < N; c0 += 16) {
+        if (c0 >= rows) break;
+        float v[16];
+        __syncwarp();
+        tmem_ld16(tS + c0, v);
+        tmem_ld_wait16(v);
+        if (DILUTE) {
+          uint32_t w[8];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const NodeStep s = step[c0 + y];
+            float p = fast_exp2(fmaf(v[y], lin, -s.lse));
+            if (!live || c0 + y >= rows) p = 0.f;
+            float had = last;
+            if (s.up != -2) {
+              had = base;
+              if (s.up >= 0) {
+                tmem_st_wait();
+                tmem_ld1(tS + s.up, &had);
+                tmem_ld_wait1(&had);
+              }
+            }
+            last = had + p;
+            if (s.keep) tmem_st1(tS + c0 + y, last);
+            const float share = p * fast_rcp(last + a.eps);
+            // (a demand or a bid that is no number goes on to the output)
+            v[y] = p == 0.f ? 0.f : share;
+          }
+#pragma unroll
+          for (int y = 0; y < 8; ++y) w[y] = pack_pair(v[2 * y], v[2 * y + 1]);
+          uint8_t* dst = pShare + 16384 * wg;
+          *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+          if (cap) cap_scores<16>(v, pre);
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const NodeStep s = step[c0 + y];
+            const float z = fmaf(v[y], lin, -s.lse - s.slope2 * (float)(place[c0 + y] - j));
+            if (c0 + y < rows) total += fast_exp2(z);
+          }
+        }
+      }
+      if (DILUTE) {
+        tmem_st_wait();
+        fence_async_smem();
+      } else if (live) {
+        acc.advanced[at] = total;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars.pready + 8 * wg);
+    }
+    mbar_wait_warp(bars.alldone, 0, ctl, &g_tree_status, kErrWaitMma);
+    tc_fence_after();
+    if (DILUTE && wg == 0) {
+      // out^T: lane = feature.  Chunks without keys have no product to read.
+      const int64_t first_row = ((int64_t)nk * a.chunks + blockIdx.x) * rows;
+#pragma unroll
+      for (int c0 = 0; c0 < N; c0 += 16) {
+        float o[16], t[16];
+        __syncwarp();
+        tmem_ld16(tS + 128 + c0, o);
+        tmem_ld_wait16(o);
+        if (D == 128) {
+          tmem_ld16(tS + 192 + c0, t);
+          tmem_ld_wait16(t);
+        }
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+          if (c0 + y >= rows) break;
+          if (row < D) a.pout[(first_row + c0 + y) * D + row] = ne > 0 ? o[y] : 0.f;
+          if (row == (D == 64 ? 64 : 0)) a.psum[first_row + c0 + y] = ne > 0 ? (D == 64 ? o[y] : t[y]) : 0.f;
+        }
+      }
+    }
+  }
+  drain_if_aborted(ctl);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_free(tmem, F::kTmem);
+}
+
+}  // namespace tc
+}  // namespace dil

@@ -93,5 +93,20 @@ __device__ __forceinline__ float score(float dot, float scale, float cap, float 
   return fmaf(-slope2, far, z);
 }
 
+// The accepted branch: what tree_accept writes.  path: (batch or 1, accepted) nodes.
+struct Accept {
+  const int* path;
+  int64_t path_stride;
+  int accepted;
+  float* advanced;         // (batch, kv_heads, capacity), or null: no demand is kept
+  void* kc;
+  void* vc;
+};
+
+// The node of place x of the path, held inside the tree.
+__device__ __forceinline__ int path_node(const Args& a, const Accept& c, int b, int x) {
+  return min(max(c.path[b * c.path_stride + x], 0), a.nodes - 1);
+}
+
 }  // namespace tree
 }  // namespace dil

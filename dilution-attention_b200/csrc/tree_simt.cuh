@@ -306,21 +306,6 @@ __global__ void __launch_bounds__(kThreads) simt_dilute_kernel(Args a) {
   }
 }
 
-// The accepted branch: what tree_accept writes.  path: (batch or 1, accepted) nodes.
-struct Accept {
-  const int* path;
-  int64_t path_stride;
-  int accepted;
-  float* advanced;         // (batch, kv_heads, capacity), or null: no demand is kept
-  void* kc;
-  void* vc;
-};
-
-// The node of place x of the path, held inside the tree.
-__device__ __forceinline__ int path_node(const Args& a, const Accept& c, int b, int x) {
-  return min(max(c.path[b * c.path_stride + x], 0), a.nodes - 1);
-}
-
 // advanced_j = committed_j + the bids of the accepted nodes (of all heads that share the key head), for cached keys; the
 // bids of one another for the accepted nodes' own keys.  grid = (blocks of tiles, 1, batch * kv_heads)
 template <typename T, int D, int RI>

@@ -1,0 +1,326 @@
+// extern "C" entry points of draft trees over a cache.  Argument validation, kernel selection and launches; declarations in
+// include/dilution_b200.h.
+
+#include <algorithm>
+#include <climits>
+
+#include "abi_internal.h"
+#include "tc_tree.cuh"
+#include "tree_join.cuh"
+#include "tree_simt.cuh"
+
+namespace dil {
+
+int trees_read_status(int* code) { return read_status_word(tc::g_tree_status, code); }
+
+namespace {
+
+// Parts that a key head's keys are cut into.  fp32 FMAs: enough blocks for four on every SM, of 256 keys at least.
+int simt_chunks(int64_t blocks, int64_t keys) {
+  const int64_t want = (148 * 4 + blocks - 1) / std::max<int64_t>(blocks, 1), most = (keys + 255) / 256;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
+}
+// Tensor cores: one block per SM, so as many parts as make the fewest rounds of tiles of 128 keys, where a block's start and
+// end take as long as about four tiles.
+int tc_chunks(int64_t blocks, int64_t keys) {
+  const int64_t tiles = std::max<int64_t>(1, (keys + 127) / 128);
+  int64_t best = 0;
+  int chunks = 1;
+  for (int64_t c = 1; c <= std::min<int64_t>(tiles, 148); ++c) {
+    const int64_t cost = (blocks * c + 147) / 148 * ((tiles + c - 1) / c + 4);
+    if (c == 1 || cost < best) {
+      best = cost;
+      chunks = (int)c;
+    }
+  }
+  return chunks;
+}
+int row_blocks(int rows, int of) { return (rows + of - 1) / of; }
+int simt_row_blocks(int rows) { return rows <= 16 ? 1 : row_blocks(rows, 64); }
+
+template <typename T, int D> constexpr bool kOnTensorCores = std::is_same<T, __nv_bfloat16>::value && (D == 64 || D == 128);
+
+struct TreeScratch {
+  size_t part, psum, shares, pout, bytes;
+};
+TreeScratch tree_scratch(int64_t heads, int group, int nodes, int64_t chunks, int d) {
+  TreeScratch s;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t n = (size_t)heads * group * nodes * chunks;
+  s.part = 0;
+  s.psum = up(n * sizeof(float2));
+  s.shares = s.psum + up(n * sizeof(float));
+  s.pout = s.shares + up((size_t)heads * nodes * nodes * sizeof(float));
+  s.bytes = s.pout + n * d * sizeof(float);
+  return s;
+}
+int64_t tree_keys(const tree::Args& a) { return (a.pos_dev ? a.capacity : a.len) + a.nodes; }
+
+int check_tree(const char* fn, const tree::Args& a, int64_t length, int dtype, int d) {
+  if (dtype != DILUTION_F32 && dtype != DILUTION_BF16)
+    return abi_fail(DILUTION_ERR_ARG, "%s: dtype must be DILUTION_F32 or DILUTION_BF16", fn);
+  if (!valid_d(d)) return abi_fail(DILUTION_ERR_UNSUPPORTED, "%s: head_dim %d not in {16, 32, 64, 128}", fn, d);
+  if (a.batch < 1 || a.kv_heads < 1 || a.group < 1 || (int64_t)a.batch * a.kv_heads > 65535 || a.group > 1024)
+    return abi_fail(DILUTION_ERR_ARG, "%s: batch * kv_heads must be in [1, 65535] and the heads of a group in [1, 1024]", fn);
+  if (a.nodes < 1 || a.nodes > tree::kMaxNodes)
+    return abi_fail(DILUTION_ERR_ARG, "%s: a tree has 1 to %d nodes, not %d", fn, tree::kMaxNodes, a.nodes);
+  if (a.capacity < 1 || a.capacity > (1 << 30) || length < 0 || length > a.capacity)
+    return abi_fail(DILUTION_ERR_ARG, "%s: length %lld outside cache capacity %lld", fn, (long long)length, (long long)a.capacity);
+  if (!(a.cap >= 0.f) || a.cap > 3e38f || !(a.scale > 0.f))
+    return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap finite, 0 for none", fn);
+  if (!a.q || !a.kn || !a.vn || !a.kc || !a.vc || !a.parents || !a.lse) return abi_fail(DILUTION_ERR_ARG, "%s: null pointer", fn);
+  if (misaligned({a.q, a.kn, a.vn, a.kc, a.vc}))
+    return abi_fail(DILUTION_ERR_ARG, "%s: q, drafted keys and values and caches must be 16-byte aligned", fn);
+  return DILUTION_OK;
+}
+
+tree::Args tree_args(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache,
+                     const int* parents, int64_t parent_stride, int64_t batch, int64_t kv_heads, int group, int nodes,
+                     int64_t capacity, int64_t length, const int* length_dev, float scale, float* lse) {
+  tree::Args a{};
+  a.q = q;
+  a.kn = k_new;
+  a.vn = v_new;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.parents = parents;
+  a.parent_stride = parent_stride;
+  a.pos_dev = length_dev;
+  a.lse = lse;
+  a.capacity = capacity;
+  a.len = (int)std::min<int64_t>(length, INT_MAX);
+  a.batch = batch > INT_MAX || batch < 0 ? -1 : (int)batch;
+  a.kv_heads = kv_heads > INT_MAX || kv_heads < 0 ? -1 : (int)kv_heads;
+  a.group = group;
+  a.nodes = nodes;
+  a.scale = scale;
+  return a;
+}
+
+float* place_scratch(tree::Args& a, void* scratch, int d) {
+  const TreeScratch s = tree_scratch((int64_t)a.batch * a.kv_heads, a.group, a.nodes, a.chunks, d);
+  char* p = (char*)scratch;
+  a.part = (float2*)(p + s.part);
+  a.psum = (float*)(p + s.psum);
+  a.pout = (float*)(p + s.pout);
+  return (float*)(p + s.shares);
+}
+
+template <typename T, int D, int RI, bool OUT> int simt_softmax(const tree::Args& a, cudaStream_t st) {
+  constexpr int smem = sizeof(tree::Smem<D, RI>);
+  if (int rc = opt_in(tree::simt_softmax_kernel<T, D, RI, OUT>, smem)) return rc;
+  LaunchMark mark(OUT ? "tree_softmax" : "tree_stats", st);
+  const dim3 grid(a.chunks, (a.group * a.nodes + 16 * RI - 1) / (16 * RI), a.batch * a.kv_heads);
+  tree::simt_softmax_kernel<T, D, RI, OUT><<<grid, tree::kThreads, smem, st>>>(a);
+  return abi_check_launch("tree_softmax");
+}
+template <typename T, int D, int RI> int simt_dilute(const tree::Args& a, cudaStream_t st) {
+  constexpr int smem = sizeof(tree::Smem<D, RI>);
+  if (int rc = opt_in(tree::simt_dilute_kernel<T, D, RI>, smem)) return rc;
+  LaunchMark mark("tree_dilute", st);
+  tree::simt_dilute_kernel<T, D, RI><<<dim3(a.chunks, 1, a.batch * a.kv_heads), tree::kThreads, smem, st>>>(a);
+  return abi_check_launch("tree_dilute");
+}
+template <typename T, int D, int RI> int simt_advance(const tree::Args& a, const tree::Accept& c, cudaStream_t st) {
+  constexpr int smem = sizeof(tree::Smem<D, RI>);
+  if (int rc = opt_in(tree::simt_advance_kernel<T, D, RI>, smem)) return rc;
+  LaunchMark mark("tree_advance", st);
+  const int64_t tiles = ((a.pos_dev ? a.capacity : a.len) + c.accepted + tree::kKeys - 1) / tree::kKeys;
+  tree::simt_advance_kernel<T, D, RI>
+      <<<dim3((unsigned)std::min<int64_t>(tiles, a.chunks), 1, a.batch * a.kv_heads), tree::kThreads, smem, st>>>(a, c);
+  return abi_check_launch("tree_advance");
+}
+
+template <typename T, bool DILUTE> int join(const tree::Args& a, int d, cudaStream_t st) {
+  LaunchMark mark("tree_join", st);
+  tree::join_kernel<T, DILUTE><<<(unsigned)((int64_t)a.batch * a.kv_heads * a.group * a.nodes), d, 0, st>>>(a, d);
+  return abi_check_launch("tree_join");
+}
+
+// ---- tensor cores
+int cache_maps(CUtensorMap* k, CUtensorMap* v, const tree::Args& a, int d) {
+  const int64_t n = (int64_t)a.batch * a.kv_heads;
+  if (!tc::tile_map(k, a.kc, n, a.capacity, d, 64) || !tc::tile_map(v, a.vc, n, a.capacity, d, 64))
+    return abi_fail(DILUTION_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  return DILUTION_OK;
+}
+
+template <int D, int G, bool OUT> int tc_scan_rows(const tree::Args& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  using F = tc::Scan<D, G, OUT>;
+  if (int rc = opt_in(tc::scan_kernel<D, G, OUT>, F::kBytes)) return rc;
+  LaunchMark mark(OUT ? "tree_softmax" : "tree_stats", st);
+  const dim3 grid(a.chunks, G == 1 ? row_blocks(a.group * a.nodes, 128) : 1, a.batch * a.kv_heads);
+  tc::scan_kernel<D, G, OUT><<<grid, F::kThreads, F::kBytes, st>>>(k, v, a);
+  return abi_check_launch("tree_scan");
+}
+template <int D, bool OUT> int tc_scan(const tree::Args& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  const int rows = a.group * a.nodes;
+  if (rows <= 32) return tc_scan_rows<D, 4, OUT>(a, k, v, st);
+  if (rows <= 64) return tc_scan_rows<D, 2, OUT>(a, k, v, st);
+  if constexpr (OUT) return tc_scan_rows<D, 1, OUT>(a, k, v, st);
+  return DILUTION_OK;            // (a dilution layer's rows are its nodes, 64 at most)
+}
+template <int D, int N, bool DILUTE>
+int tc_sweep_rows(const tree::Args& a, const tree::Accept& c, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  using F = tc::Sweep<D, N, DILUTE>;
+  if (int rc = opt_in(tc::sweep_kernel<D, N, DILUTE>, F::kBytes)) return rc;
+  LaunchMark mark(DILUTE ? "tree_dilute" : "tree_advance", st);
+  tc::sweep_kernel<D, N, DILUTE><<<dim3(a.chunks, 1, a.batch * a.kv_heads), F::kThreads, F::kBytes, st>>>(k, v, a, c);
+  return abi_check_launch("tree_sweep");
+}
+template <int D, bool DILUTE>
+int tc_sweep(const tree::Args& a, const tree::Accept& c, int rows, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  if (rows <= 16) return tc_sweep_rows<D, 16, DILUTE>(a, c, k, v, st);
+  if (rows <= 32) return tc_sweep_rows<D, 32, DILUTE>(a, c, k, v, st);
+  return tc_sweep_rows<D, 64, DILUTE>(a, c, k, v, st);
+}
+
+template <int D> int tc_softmax(tree::Args a, void* scratch, cudaStream_t st) {
+  CUtensorMap k, v;
+  if (int rc = cache_maps(&k, &v, a, D)) return rc;
+  const int rows = a.group * a.nodes;
+  a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads * row_blocks(rows, 128), tree_keys(a));
+  place_scratch(a, scratch, D);
+  if (int rc = tc_scan<D, true>(a, k, v, st)) return rc;
+  LaunchMark mark("tree_join", st);
+  tree::join_softmax_kernel<D><<<(unsigned)((int64_t)a.batch * a.kv_heads * rows), D, 0, st>>>(a);
+  return abi_check_launch("tree_join");
+}
+
+template <int D> int tc_dilute(tree::Args a, void* scratch, cudaStream_t st) {
+  CUtensorMap k, v;
+  if (int rc = cache_maps(&k, &v, a, D)) return rc;
+  const int64_t heads = (int64_t)a.batch * a.kv_heads;
+  a.chunks = tc_chunks(heads, tree_keys(a));
+  float* shares = place_scratch(a, scratch, D);
+  if (int rc = tc_scan<D, false>(a, k, v, st)) return rc;
+  {
+    LaunchMark mark("tree_join_bids", st);
+    const int smem = a.nodes * (a.nodes + 1) * 4;
+    if (int rc = opt_in(tree::join_bids_kernel<D>, 64 * 65 * 4, 36 * 1024)) return rc;
+    tree::join_bids_kernel<D><<<(unsigned)heads, 256, smem, st>>>(a, shares);
+    if (int rc = abi_check_launch("tree_join_bids")) return rc;
+  }
+  if (int rc = tc_sweep<D, true>(a, tree::Accept{}, a.nodes, k, v, st)) return rc;
+  LaunchMark mark("tree_join", st);
+  tree::join_dilute_kernel<D><<<(unsigned)(heads * a.nodes), D, 0, st>>>(a, shares);
+  return abi_check_launch("tree_join");
+}
+
+template <int D> int tc_accept(tree::Args a, const tree::Accept& c, cudaStream_t st) {
+  if (c.advanced) {
+    CUtensorMap k, v;
+    if (int rc = cache_maps(&k, &v, a, D)) return rc;
+    a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads, tree_keys(a));
+    if (int rc = tc_sweep<D, false>(a, c, a.group * c.accepted, k, v, st)) return rc;
+  }
+  LaunchMark mark("tree_append", st);
+  tree::accept_nodes_kernel<D><<<(unsigned)(a.batch * a.kv_heads), 256, 0, st>>>(a, c);
+  return abi_check_launch("tree_append");
+}
+
+}  // namespace
+}  // namespace dil
+
+using namespace dil;
+
+extern "C" {
+
+size_t dilution_tree_scratch_bytes(int64_t batch, int64_t kv_heads, int group, int nodes, int64_t length, int d) {
+  if (batch < 1 || kv_heads < 1 || group < 1 || nodes < 1 || length < 0 || d < 1) return 0;
+  const int64_t heads = batch * kv_heads, keys = length + nodes;
+  const int rows = group * nodes;
+  const int chunks = std::max(simt_chunks(heads * simt_row_blocks(rows), keys), tc_chunks(heads * row_blocks(rows, 128), keys));
+  return tree_scratch(heads, group, nodes, chunks, d).bytes;
+}
+
+int dilution_tree_softmax(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache, int dtype,
+                          int64_t batch, int64_t kv_heads, int group, int nodes, int64_t capacity, int64_t length,
+                          const int* length_dev, int d, float scale, float cap, const float* slopes, const int* parents,
+                          int64_t parent_stride, float* lse, void* out, void* scratch, void* stream) {
+  tree::Args a = tree_args(q, k_new, v_new, k_cache, v_cache, parents, parent_stride, batch, kv_heads, group, nodes, capacity,
+                           length, length_dev, scale, lse);
+  a.cap = cap;
+  a.slopes = slopes;
+  a.out = out;
+  if (int rc = check_tree("dilution_tree_softmax", a, length, dtype, d)) return rc;
+  if (!out || !scratch || misaligned({scratch})) return abi_fail(DILUTION_ERR_ARG, "dilution_tree_softmax: null or misaligned pointer");
+  const int rows = group * nodes;
+  cudaStream_t st = (cudaStream_t)stream;
+  return with_type(dtype, d, [&](auto type, auto dim) {
+    using T = decltype(type);
+    if constexpr (kOnTensorCores<T, dim()>) return tc_softmax<dim()>(a, scratch, st);
+    else {
+    a.chunks = simt_chunks((int64_t)a.batch * a.kv_heads * simt_row_blocks(rows), tree_keys(a));
+    place_scratch(a, scratch, d);
+    if (int rc = rows <= 16 ? simt_softmax<T, dim(), 1, true>(a, st) : simt_softmax<T, dim(), 4, true>(a, st)) return rc;
+    return join<T, false>(a, d, st);
+    }
+  });
+}
+
+int dilution_tree_dilute(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache, int dtype,
+                         int64_t batch, int64_t heads, int nodes, int64_t capacity, int64_t length, const int* length_dev, int d,
+                         float scale, float eps, const float* committed, const int* parents, int64_t parent_stride, float* lse,
+                         void* out, void* scratch, void* stream) {
+  tree::Args a = tree_args(q, k_new, v_new, k_cache, v_cache, parents, parent_stride, batch, heads, 1, nodes, capacity, length,
+                           length_dev, scale, lse);
+  a.committed = committed;
+  a.out = out;
+  a.eps = eps;
+  if (int rc = check_tree("dilution_tree_dilute", a, length, dtype, d)) return rc;
+  if (!out || !committed || !scratch || misaligned({scratch}))
+    return abi_fail(DILUTION_ERR_ARG, "dilution_tree_dilute: null or misaligned pointer");
+  cudaStream_t st = (cudaStream_t)stream;
+  return with_type(dtype, d, [&](auto type, auto dim) {
+    using T = decltype(type);
+    if constexpr (kOnTensorCores<T, dim()>) return tc_dilute<dim()>(a, scratch, st);
+    else {
+    a.chunks = simt_chunks((int64_t)a.batch * a.kv_heads * simt_row_blocks(nodes), tree_keys(a));
+    place_scratch(a, scratch, d);
+    if (int rc = nodes <= 16 ? simt_softmax<T, dim(), 1, false>(a, st) : simt_softmax<T, dim(), 4, false>(a, st)) return rc;
+    {
+      LaunchMark mark("tree_join_stats", st);
+      const int64_t all = (int64_t)a.batch * a.kv_heads * nodes;
+      tree::join_stats_kernel<<<(unsigned)((all + 7) / 8), 256, 0, st>>>(a);
+      if (int rc = abi_check_launch("tree_join_stats")) return rc;
+    }
+    if (int rc = nodes <= 16 ? simt_dilute<T, dim(), 1>(a, st) : simt_dilute<T, dim(), 4>(a, st)) return rc;
+    return join<T, true>(a, d, st);
+    }
+  });
+}
+
+int dilution_tree_accept(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, int dtype,
+                         int64_t batch, int64_t kv_heads, int group, int nodes, int64_t capacity, int64_t length,
+                         const int* length_dev, int d, float scale, float cap, const float* slopes, const int* parents,
+                         int64_t parent_stride, const float* lse, const int* path, int64_t path_stride, int accepted,
+                         const float* committed, float* advanced, void* stream) {
+  tree::Args a = tree_args(q, k_new, v_new, k_cache, v_cache, parents, parent_stride, batch, kv_heads, group, nodes, capacity,
+                           length, length_dev, scale, const_cast<float*>(lse));
+  a.cap = cap;
+  a.slopes = slopes;
+  a.committed = committed;
+  if (int rc = check_tree("dilution_tree_accept", a, length, dtype, d)) return rc;
+  if (!path || (committed == nullptr) != (advanced == nullptr)) return abi_fail(DILUTION_ERR_ARG, "dilution_tree_accept: null pointer");
+  if (accepted < 1 || accepted > nodes || (!length_dev && length + accepted > capacity))
+    return abi_fail(DILUTION_ERR_ARG, "dilution_tree_accept: %d accepted nodes of %d behind %lld keys of %lld", accepted, nodes,
+                    (long long)length, (long long)capacity);
+  const tree::Accept c{path, path_stride, accepted, advanced, k_cache, v_cache};
+  cudaStream_t st = (cudaStream_t)stream;
+  return with_type(dtype, d, [&](auto type, auto dim) {
+    using T = decltype(type);
+    if constexpr (kOnTensorCores<T, dim()>)
+      if (!advanced || group * accepted <= 64) return tc_accept<dim()>(a, c, st);
+    a.chunks = simt_chunks((int64_t)a.batch * a.kv_heads, tree_keys(a));
+    if (advanced)
+      if (int rc = group * accepted <= 16 ? simt_advance<T, dim(), 1>(a, c, st) : simt_advance<T, dim(), 4>(a, c, st)) return rc;
+    LaunchMark mark("tree_append", st);
+    const int row_bytes = d * (int)sizeof(T);
+    const int64_t threads = (int64_t)a.batch * a.kv_heads * accepted * (row_bytes / 16);
+    tree::append_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a, c, row_bytes);
+    return abi_check_launch("tree_append");
+  });
+}
+
+}  // extern "C"
