@@ -1,11 +1,12 @@
 // A cache's keys that were bid for least make room: of each (batch, head) row the first `sinks` keys, the last `recent`
 // and, of those between, the ones of the highest rank stay, in their order.
 //
-// select_kernel finds the rank of the last key that stays, digit by digit of its bits (11, 11 and 10), each from one
-// histogram of the row, and writes the positions that stay.  Ranks are compared as torch.sort does: NaN above every
-// number, -0 like 0, equal ones by position.  A row's keys are spread over the CTAs of a cluster, which hold them in
-// shared memory through the passes (rows too long for that read them again) and add up their histograms through
-// distributed shared memory.  gather_kernel then moves the rows, and is bound by the bytes it moves.
+// select_kernel finds the rank of the last key that stays, eight bits at a time, each from one histogram of the row, and
+// writes the positions that stay.  Ranks are compared as torch.sort does: NaN above every number, -0 like 0, equal ones by
+// position.  A row's keys are spread over the CTAs of a cluster, which hold them in shared memory through the passes (rows
+// too long for that read them again) and add up their histograms through distributed shared memory.  Where the clusters of
+// all rows fill the chip, a cluster moves its row's keys itself, so that one row's passes, which wait for one another, run
+// next to other rows' copies; few rows are moved by gather_kernel, on all SMs.  What bounds it are the bytes that are moved.
 #pragma once
 
 #include "common.cuh"
@@ -14,7 +15,8 @@ namespace dil {
 namespace evict {
 
 constexpr int kThreads = 512;
-constexpr int kBins = 2048;
+constexpr int kBins = 256;
+constexpr int kCopies = 8;               // of a histogram: ranks share their first bits, and lanes that add to one word take turns
 constexpr int kMaxHeld = 48 * 1024;      // keys of a CTA that fit its shared memory (192 KB)
 
 struct Args {
@@ -23,6 +25,15 @@ struct Args {
   int length, keep, recent, sinks, seg;
   int held;                  // a CTA's keys fit its shared memory
   int* index;                // (n, keep)
+  const uint4* k;            // (n, capacity, 2^shift) units of 16 bytes
+  const uint4* v;
+  const float* committed;    // (n, capacity), or null
+  int64_t capacity;
+  int new_capacity, shift;
+  int moves;                 // select_kernel moves the rows too
+  uint4* k_out;              // (n, new_capacity, 2^shift)
+  uint4* v_out;
+  float* committed_out;
 };
 
 // Bits that grow with the rank.
@@ -35,131 +46,174 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, int rank) 
   return __float_as_uint(ld_cluster(reinterpret_cast<const float*>(p), rank));
 }
 
-struct Shared {
-  uint32_t hist[kBins];
-  uint32_t warps[2][kThreads / 32];
-  uint32_t counts[2];          // this CTA's: keys that stay whatever the ties, keys at the threshold
-  uint32_t digit, need;
-};
-
-// Counts of a and b in front of the thread within the block, and the block's sums.  Two barriers.
-__device__ __forceinline__ void block_counts(Shared& s, bool a, bool b, uint32_t& before_a, uint32_t& before_b, uint32_t& all_a,
-                                             uint32_t& all_b) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t ma = __ballot_sync(0xffffffffu, a), mb = __ballot_sync(0xffffffffu, b), below = (1u << lane) - 1;
-  if (lane == 0) { s.warps[0][warp] = __popc(ma); s.warps[1][warp] = __popc(mb); }
-  __syncthreads();
-  before_a = __popc(ma & below);
-  before_b = __popc(mb & below);
-  all_a = all_b = 0;
+// Units [first, last) of a row's new places (2^shift units a key), N at a time a thread.
+template <int THREADS, int N> __device__ __forceinline__ void move_units(const Args& a, int64_t row, int first, int last) {
+  const int* index = a.index + row * a.keep;
+  const uint4 *k_in = a.k + (row * a.capacity << a.shift), *v_in = a.v + (row * a.capacity << a.shift);
+  const int64_t to = row * a.new_capacity;
+  const int low = (1 << a.shift) - 1;
+  auto position = [&](int at) {
+    const int place = at >> a.shift;
+    return at < last && place < a.keep ? __ldcg(index + place) : -1;
+  };
+  int src[N], next[N];               // (the next positions are under way while these rows are)
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    const uint32_t x = s.warps[0][w], y = s.warps[1][w];
-    if (w < warp) { before_a += x; before_b += y; }
-    all_a += x;
-    all_b += y;
+  for (int x = 0; x < N; ++x) next[x] = position(first + (int)threadIdx.x + x * THREADS);
+  for (int base = first + (int)threadIdx.x; base < last; base += N * THREADS) {
+    uint4 k[N], v[N];
+#pragma unroll
+    for (int x = 0; x < N; ++x) src[x] = next[x];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const int64_t from = ((int64_t)src[x] << a.shift) + (base + x * THREADS & low);
+      k[x] = v[x] = make_uint4(0, 0, 0, 0);
+      if (src[x] >= 0) {
+        k[x] = __ldcs(k_in + from);
+        v[x] = __ldcs(v_in + from);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < N; ++x) next[x] = position(base + (N + x) * THREADS);
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const int at = base + x * THREADS;
+      if (at >= last) break;
+      a.k_out[(to << a.shift) + at] = k[x];
+      a.v_out[(to << a.shift) + at] = v[x];
+      if ((at & low) == 0 && a.committed != nullptr)
+        a.committed_out[to + (at >> a.shift)] = src[x] >= 0 ? a.committed[row * a.capacity + src[x]] : 0.f;
+    }
   }
-  __syncthreads();
 }
 
+struct Shared {
+  uint32_t copies[kBins * kCopies];
+  uint32_t hist[2][kBins];     // the CTA's, two passes apart: the others may still read the last one
+  uint32_t warps[2][kThreads / 32];
+  uint32_t counts[2];          // this CTA's: keys that stay whatever the ties, keys at the threshold
+  uint32_t digit, need, whole;
+};
+
 // grid = clusters of `ranks` CTAs, one per row.
-__global__ void __launch_bounds__(kThreads) select_kernel(Args a, int ranks) {
-  extern __shared__ uint32_t held[];
+__global__ void __launch_bounds__(kThreads, 4) select_kernel(Args a, int ranks) {
+  extern __shared__ uint4 held4[];
   __shared__ Shared s;
-  const int tid = threadIdx.x, rank = blockIdx.x % ranks;
+  uint32_t* held = reinterpret_cast<uint32_t*>(held4);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % ranks;
   const int64_t n = blockIdx.x / ranks;
   const float* scores = a.scores + n * a.score_stride;
-  const int i0 = min(a.length, rank * a.seg), i1 = min(a.length, i0 + a.seg);
-  const int c0 = a.sinks, c1 = a.length - a.recent;                 // the keys that have to prove themselves
+  const int i0 = min(a.length, rank * a.seg), i1 = min(a.length, i0 + a.seg), count = i1 - i0;
+  const int c0 = a.sinks - i0, c1 = a.length - a.recent - i0;       // the keys that have to prove themselves, from i0 on
   if (a.held) {
-    for (int i = i0 + tid; i < i1; i += kThreads) held[i - i0] = rank_bits(scores[i]);
+    for (int i = tid; i < count; i += kThreads) held[i] = rank_bits(scores[i0 + i]);
     __syncthreads();
   }
-  auto bits = [&](int i) { return a.held ? held[i - i0] : rank_bits(scores[i]); };
+  auto bits = [&](int i) { return a.held ? held[i] : rank_bits(scores[i0 + i]); };
   uint32_t need = a.keep - a.sinks - a.recent, prefix = 0, mask = 0;
   if (need > 0) {
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-      for (int x = tid; x < kBins; x += kThreads) s.hist[x] = 0;
+    for (int pass = 0; pass < 4; ++pass) {
+      const int shift = 24 - 8 * pass;
+      for (int x = tid; x < kBins * kCopies / 4; x += kThreads) reinterpret_cast<uint4*>(s.copies)[x] = make_uint4(0, 0, 0, 0);
       __syncthreads();
-      const int lo = max(i0, c0), hi = min(i1, c1);
-      for (int base = lo; base < hi; base += kThreads) {
-        const int i = base + tid;
-        int d = -1;
-        if (i < hi) {
-          const uint32_t u = bits(i);
-          if ((u & mask) == prefix) d = (u >> shift) & (bins - 1);
+      uint32_t* mine = s.copies + (tid & (kCopies - 1));
+      const int lo = max(0, c0), hi = min(count, c1);
+      auto add = [&](uint32_t u) {
+        if ((u & mask) == prefix) atomicAdd(mine + (u >> shift & 255u) * kCopies, 1u);
+      };
+      if (a.held) {                  // four at a time; the first and the last four may be cut
+        const int q0 = (lo + 3) / 4, q1 = max(q0, hi / 4);
+        for (int q = q0 + tid; q < q1; q += kThreads) {
+          const uint4 u = held4[q];
+          add(u.x);
+          add(u.y);
+          add(u.z);
+          add(u.w);
         }
-        // a warp of one digit (fresh keys are alike) adds once
-        if (__all_sync(0xffffffffu, d == __shfl_sync(0xffffffffu, d, 0))) {
-          if ((tid & 31) == 0 && d >= 0) atomicAdd(&s.hist[d], 32u);
-        } else if (d >= 0) {
-          atomicAdd(&s.hist[d], 1u);
-        }
+        const int edge = tid < 4 ? lo + tid : 4 * q1 + tid - 4;
+        if (tid < 8 && edge >= lo && edge < hi && (tid < 4 ? edge < 4 * q0 : true)) add(held[edge]);
+      } else {
+        for (int i = lo + tid; i < hi; i += kThreads) add(bits(i));
+      }
+      __syncthreads();
+      if (tid < kBins) {
+        const uint4 x = reinterpret_cast<const uint4*>(s.copies)[2 * tid], y = reinterpret_cast<const uint4*>(s.copies)[2 * tid + 1];
+        s.hist[pass & 1][tid] = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
       }
       if (ranks > 1) cluster_sync(); else __syncthreads();
-      // thread t holds bins from the top: 4 t .. 4 t + 3 below the last
-      uint32_t c[kBins / kThreads], sum = 0;
+      // thread t < 256 holds bin 255 - t of the whole row
+      uint32_t sum = 0;
+      if (tid < kBins) {
+        const uint32_t* bin = &s.hist[pass & 1][kBins - 1 - tid];
+        if (ranks > 1) {
+          uint32_t x[8];             // (all under way at once)
 #pragma unroll
-      for (int x = 0; x < kBins / kThreads; ++x) {
-        const int bin = kBins - 1 - (tid * (kBins / kThreads) + x);
-        c[x] = 0;
-        if (ranks > 1)
-          for (int y = 0; y < ranks; ++y) c[x] += ld_cluster_u32(&s.hist[bin], y);
-        else c[x] = s.hist[bin];
-        sum += c[x];
+          for (int y = 0; y < 8; ++y) x[y] = y < ranks ? ld_cluster_u32(bin, y) : 0u;
+#pragma unroll
+          for (int y = 0; y < 8; ++y) sum += x[y];
+        } else {
+          sum = *bin;
+        }
       }
       uint32_t inc = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
-        if ((tid & 31) >= o) inc += y;
+        if (lane >= o) inc += y;
       }
-      if ((tid & 31) == 31) s.warps[0][tid >> 5] = inc;
+      if (lane == 31) s.warps[0][warp] = inc;
       __syncthreads();
-      uint32_t before = inc - sum;
-      for (int w = 0; w < tid >> 5; ++w) before += s.warps[0][w];
-      if (before < need && need <= before + sum) {
+      if (tid < kBins) {
+        uint32_t before = inc - sum;
 #pragma unroll
-        for (int x = 0; x < kBins / kThreads; ++x) {
-          if (before < need && need <= before + c[x]) {
-            s.digit = kBins - 1 - (tid * (kBins / kThreads) + x);
-            s.need = need - before;
-          }
-          before += c[x];
+        for (int w = 0; w < kBins / 32; ++w) before += w < warp ? s.warps[0][w] : 0u;
+        if (before < need && need <= before + sum) {
+          s.digit = kBins - 1 - tid;
+          s.need = need - before;
+          s.whole = need == before + sum;
         }
       }
-      if (ranks > 1) cluster_sync(); else __syncthreads();         // (the others have read this CTA's histogram too)
-      prefix |= s.digit << shift;
-      mask |= (uint32_t)(bins - 1) << shift;
-      need = s.need;
       __syncthreads();
+      prefix |= s.digit << shift;
+      mask |= 255u << shift;
+      need = s.need;
+      if (s.whole) break;              // every key of these bits stays: the others need not be told apart
     }
   }
-  // prefix is now the rank of the last key that stays, need how many of that rank do
+  // prefix has the bits of the last key that stays, need is how many of those bits do
   auto state = [&](int i, bool& above, bool& equal) {
     above = equal = false;
-    if (i >= i1) return;
+    if (i >= count) return;
     if (i < c0 || i >= c1) { above = true; return; }
-    const uint32_t u = bits(i);
-    above = need > 0 && u > prefix;
-    equal = need > 0 && u == prefix;
+    if (need == 0) return;
+    const uint32_t u = bits(i) & mask;
+    above = u > prefix;
+    equal = u == prefix;
   };
-  uint32_t above_before = 0, equal_before = 0;
+  // a warp has a stretch of its own: counts of the warps, then of the CTAs, then each walks through its stretch again
+  constexpr int kWarps = kThreads / 32;
+  const int per = ((count + kWarps - 1) / kWarps + 31) / 32 * 32, w0 = min(count, warp * per), w1 = min(count, w0 + per);
+  uint32_t na = 0, ne = 0;
+  for (int i = w0 + lane; i < w1; i += 32) {
+    bool above, equal;
+    state(i, above, equal);
+    na += above;
+    ne += equal;
+  }
+  na = __reduce_add_sync(0xffffffffu, na);
+  ne = __reduce_add_sync(0xffffffffu, ne);
+  if (lane == 0) { s.warps[0][warp] = na; s.warps[1][warp] = ne; }
+  __syncthreads();
+  uint32_t above_before = 0, equal_before = 0, all_above = 0, all_equal = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const uint32_t x = s.warps[0][w], y = s.warps[1][w];
+    if (w < warp) { above_before += x; equal_before += y; }
+    all_above += x;
+    all_equal += y;
+  }
   if (ranks > 1) {
-    uint32_t na = 0, ne = 0;
-    for (int i = i0 + tid; i < i1; i += kThreads) {
-      bool above, equal;
-      state(i, above, equal);
-      na += above;
-      ne += equal;
-    }
-    na = __reduce_add_sync(0xffffffffu, na);
-    ne = __reduce_add_sync(0xffffffffu, ne);
-    if (tid < 2) s.counts[tid] = 0;
-    __syncthreads();
-    if ((tid & 31) == 0) { atomicAdd(&s.counts[0], na); atomicAdd(&s.counts[1], ne); }
+    if (tid == 0) { s.counts[0] = all_above; s.counts[1] = all_equal; }
     cluster_sync();
     for (int y = 0; y < rank; ++y) {
       above_before += ld_cluster_u32(&s.counts[0], y);
@@ -167,42 +221,26 @@ __global__ void __launch_bounds__(kThreads) select_kernel(Args a, int ranks) {
     }
   }
   int* index = a.index + n * a.keep;
-  for (int base = i0; base < i1; base += kThreads) {
+  const uint32_t below = (1u << lane) - 1;
+  for (int base = w0; base < w1; base += 32) {
     bool above, equal;
-    uint32_t xa, xe, ta, te;
-    state(base + tid, above, equal);
-    block_counts(s, above, equal, xa, xe, ta, te);
-    xa += above_before;
-    xe += equal_before;
-    const uint32_t at = xa + min(xe, need);
-    if ((above || (equal && xe < need)) && at < (uint32_t)a.keep) index[at] = base + tid;
-    above_before += ta;
-    equal_before += te;
+    state(base + lane < w1 ? base + lane : count, above, equal);
+    const uint32_t ma = __ballot_sync(0xffffffffu, above), me = __ballot_sync(0xffffffffu, equal);
+    const uint32_t xe = equal_before + __popc(me & below), at = above_before + __popc(ma & below) + min(xe, need);
+    if ((above || (equal && xe < need)) && at < (uint32_t)a.keep) index[at] = i0 + base + lane;
+    above_before += __popc(ma);
+    equal_before += __popc(me);
   }
-  if (ranks > 1) cluster_sync();        // no CTA leaves while another may read its counts
+  if (ranks > 1) cluster_sync(); else __syncthreads();        // (and no CTA leaves while another may read its counts)
+  if (!a.moves) return;
+  const int units = a.new_capacity << a.shift, part = (units + ranks - 1) / ranks;
+  move_units<kThreads, 1>(a, n, min(units, rank * part), min(units, (rank + 1) * part));
 }
 
-// Rows of k and v (16 bytes a thread) and their demand; zeros behind the last that stays.
-__global__ void __launch_bounds__(256) gather_kernel(const uint4* __restrict__ k, const uint4* __restrict__ v,
-                                                     const float* __restrict__ committed, const int* __restrict__ index,
-                                                     int64_t n, int64_t capacity, int keep, int64_t new_capacity, int per,
-                                                     uint4* __restrict__ k_out, uint4* __restrict__ v_out,
-                                                     float* __restrict__ committed_out) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, place = at / per, row = place / new_capacity;
-  if (row >= n) return;
-  const int u = (int)(at % per);
-  const int64_t x = place % new_capacity;
-  uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  float c = 0.f;
-  if (x < keep) {
-    const int64_t src = row * capacity + index[row * keep + x];
-    kx = k[src * per + u];
-    vx = v[src * per + u];
-    if (u == 0 && committed != nullptr) c = committed[src];
-  }
-  k_out[at] = kx;
-  v_out[at] = vx;
-  if (u == 0 && committed != nullptr) committed_out[place] = c;
+// Rows of k and v and their demand; zeros behind the last that stays.  Four units of 16 bytes of each a thread.
+__global__ void __launch_bounds__(256) gather_kernel(Args a) {
+  const int units = a.new_capacity << a.shift, blocks = (units + 1023) / 1024, first = (int)(blockIdx.x % blocks) * 1024;
+  move_units<256, 4>(a, blockIdx.x / blocks, first, min(units, first + 1024));
 }
 
 }  // namespace evict

@@ -225,29 +225,38 @@ int dilution_evict(const void* k_cache, const void* v_cache, const float* commit
     return abi_fail(DILUTION_ERR_ARG, "dilution_evict: keep %lld of %lld keys with %lld recent and %lld first ones", (long long)keep,
                     (long long)length, (long long)recent, (long long)sinks);
   const int per = d * (dtype == DILUTION_F32 ? 4 : 2) / 16;
-  if (new_capacity < keep || new_capacity > (1 << 30) || n * new_capacity * per / 256 >= (int64_t)1 << 31)
+  if (new_capacity < keep || new_capacity > (1 << 25) || n * (new_capacity * per / 1024 + 1) >= (int64_t)1 << 31)
     return abi_fail(DILUTION_ERR_ARG, "dilution_evict: new capacity %lld", (long long)new_capacity);
   if (!k_cache || !v_cache || !scores || !k_out || !v_out || !index || (committed == nullptr) != (committed_out == nullptr))
     return abi_fail(DILUTION_ERR_ARG, "dilution_evict: null pointer");
   if (misaligned({k_cache, v_cache, k_out, v_out})) return abi_fail(DILUTION_ERR_ARG, "dilution_evict: caches must be 16-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
+  // CTAs of a row: until all SMs have one or a CTA has 256 keys, and until a CTA has 8192 keys
+  int ranks = 1;
+  while (ranks < 8 && n * ranks < 148 && length / (2 * ranks) >= 256) ranks *= 2;
+  while (ranks < 8 && (length + ranks - 1) / ranks > 8192) ranks *= 2;
+  evict::Args a{};
+  a.scores = scores;
+  a.score_stride = score_stride;
+  a.length = (int)length;
+  a.keep = (int)keep;
+  a.recent = (int)recent;
+  a.sinks = (int)sinks;
+  a.seg = (int)((length + ranks - 1) / ranks);
+  a.held = a.seg <= evict::kMaxHeld;
+  a.index = index;
+  a.k = (const uint4*)k_cache;
+  a.v = (const uint4*)v_cache;
+  a.committed = committed;
+  a.capacity = capacity;
+  a.new_capacity = (int)new_capacity;
+  while (1 << a.shift < per) ++a.shift;
+  a.moves = n * ranks >= 148;
+  a.k_out = (uint4*)k_out;
+  a.v_out = (uint4*)v_out;
+  a.committed_out = committed_out;
+  if (int rc = opt_in(evict::select_kernel, evict::kMaxHeld * 4)) return rc;
   {
-    // CTAs of a row: until all SMs have one, or a CTA has 1024 keys
-    int ranks = 1;
-    while (ranks < 8 && n * ranks < 148 && length / (2 * ranks) >= 1024) ranks *= 2;
-    while (ranks < 8 && (length + ranks - 1) / ranks > 8192) ranks *= 2;
-    evict::Args a;
-    a.scores = scores;
-    a.score_stride = score_stride;
-    a.length = (int)length;
-    a.keep = (int)keep;
-    a.recent = (int)recent;
-    a.sinks = (int)sinks;
-    a.seg = (int)((length + ranks - 1) / ranks);
-    a.held = a.seg <= evict::kMaxHeld;
-    a.index = index;
-    const int smem = a.held ? a.seg * 4 : 0;
-    if (int rc = opt_in(evict::select_kernel, evict::kMaxHeld * 4)) return rc;
     LaunchMark mark("evict_select", st);
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
@@ -256,18 +265,17 @@ int dilution_evict(const void* k_cache, const void* v_cache, const float* commit
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(n * ranks));
     cfg.blockDim = dim3(evict::kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = a.held ? (a.seg + 3) / 4 * 16 : 0;
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, evict::select_kernel, a, ranks);
     if (e != cudaSuccess) return abi_fail(DILUTION_ERR_CUDA, "evict_select: %s", cudaGetErrorString(e));
   }
+  if (a.moves) return DILUTION_OK;
   LaunchMark mark("evict_gather", st);
-  const int64_t threads = n * new_capacity * per;
-  evict::gather_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(
-      (const uint4*)k_cache, (const uint4*)v_cache, committed, index, n, capacity, (int)keep, new_capacity, per, (uint4*)k_out,
-      (uint4*)v_out, committed_out);
+  const int64_t blocks = n * ((new_capacity * per + 1023) / 1024);
+  evict::gather_kernel<<<(unsigned)blocks, 256, 0, st>>>(a);
   return abi_check_launch("evict_gather");
 }
 

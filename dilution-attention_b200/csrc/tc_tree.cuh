@@ -34,60 +34,79 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int rows, int from, int
       reinterpret_cast<uint4*>(tile + s * rows * 128)[x] = make_uint4(0, 0, 0, 0);
 }
 
-// Barriers of a CTA that streams a cache: full[R], free[R], sdone[2], alldone, pready[2].
-template <int R> struct StreamBars {
-  uint32_t full, free, sdone, alldone, pready;
+// Barriers of a CTA that streams a cache, keys through RK stages and values through RV, and scores it into NB buffers.  Keys
+// are let go once they are scored, values by the product, which comes up to NB - 1 tiles later.  A buffer's scores are there
+// (sdone) and have been used (ready); the last product of a warpgroup's values is through (used), and all are (alldone).
+template <int RK, int RV, int NB> struct StreamBars {
+  static_assert(NB <= RV + 1, "the copies of a tile's values never wait for a later tile's scores");
+  uint32_t kfull, kfree, vfull, vfree, sdone, used, alldone, ready;
   Ctl* ctl;
+  static constexpr int kBytes = 8 * (2 * RK + 2 * RV + 2 * NB + 3) + 16;
   __device__ __forceinline__ StreamBars(uint64_t* b) {
-    full = smem_u32(b);
-    free = full + 8 * R;
-    sdone = free + 8 * R;
-    alldone = sdone + 16;
-    pready = alldone + 8;
-    ctl = reinterpret_cast<Ctl*>(b + 2 * R + 5);
+    kfull = smem_u32(b);
+    kfree = kfull + 8 * RK;
+    vfull = kfree + 8 * RK;
+    vfree = vfull + 8 * RV;
+    sdone = vfree + 8 * RV;
+    used = sdone + 8 * NB;
+    alldone = used + 16;
+    ready = alldone + 8;
+    ctl = reinterpret_cast<Ctl*>(b + 2 * RK + 2 * RV + 2 * NB + 3);
   }
   __device__ __forceinline__ void init() const {
     ctl->abort = 0;
-    for (int x = 0; x < 2 * R + 3; ++x) mbar_init(full + 8 * x, 1);
-    for (int x = 0; x < 2; ++x) mbar_init(pready + 8 * x, 4);
+    for (int x = 0; x < 2 * RK + 2 * RV + NB + 3; ++x) mbar_init(kfull + 8 * x, 1);
+    for (int x = 0; x < NB; ++x) mbar_init(ready + 8 * x, 4);
     fence_barrier_init();
   }
 };
 
-// The warp that copies tiles [e0, e0 + ne) of KT keys, K and (if V) values behind them, into the ring.
-template <int D, int KT, int R, bool V>
-__device__ __forceinline__ void stream_tiles(const StreamBars<R>& bars, const CUtensorMap* map_k, const CUtensorMap* map_v, uint32_t ring,
-                                             int first, int ne, int nk, uint32_t lead) {
-  constexpr uint32_t kOne = KT * D * 2, kStage = V ? 2 * kOne : kOne;
-  for (int e = 0; e < ne; ++e) {
-    const int st = e % R;
-    if (e >= R) mbar_wait_warp(bars.free + 8 * st, (e / R - 1) & 1, bars.ctl, &g_tree_status, kErrWaitMma);
+// The warp that copies tiles [first, first + ne) of KT keys and (if V) their values.
+template <int D, int KT, int RK, int RV, int NB, bool V>
+__device__ __forceinline__ void stream_tiles(const StreamBars<RK, RV, NB>& bars, const CUtensorMap* map_k, const CUtensorMap* map_v,
+                                             uint32_t ring_k, uint32_t ring_v, int first, int ne, int nk, uint32_t lead) {
+  constexpr uint32_t kOne = KT * D * 2;
+  auto copy = [&](const CUtensorMap* map, uint32_t dst, int e, uint32_t bar) {
     if (lead) {
-      mbar_expect_tx(bars.full + 8 * st, kStage);
+      mbar_expect_tx(bar, kOne);
 #pragma unroll
-      for (int x = 0; x < KT / 64; ++x) {
-        tma_load_rows<kForm<D>>(ring + kStage * st + 8192 * x, map_k, (first + e) * KT + 64 * x, nk, bars.full + 8 * st, KT * 128);
-        if (V) tma_load_rows<kForm<D>>(ring + kStage * st + kOne + 8192 * x, map_v, (first + e) * KT + 64 * x, nk, bars.full + 8 * st, KT * 128);
-      }
+      for (int x = 0; x < KT / 64; ++x) tma_load_rows<kForm<D>>(dst + 8192 * x, map, (first + e) * KT + 64 * x, nk, bar, KT * 128);
     }
     __syncwarp();
+  };
+  for (int e = 0; e < ne; ++e) {
+    const int k = e % RK, v = e % RV;
+    if (e >= RK) mbar_wait_warp(bars.kfree + 8 * k, (e / RK - 1) & 1, bars.ctl, &g_tree_status, kErrWaitMma);
+    copy(map_k, ring_k + kOne * k, e, bars.kfull + 8 * k);
+    if (V) {
+      if (e >= RV) mbar_wait_warp(bars.vfree + 8 * v, (e / RV - 1) & 1, bars.ctl, &g_tree_status, kErrWaitMma);
+      copy(map_v, ring_v + kOne * v, e, bars.vfull + 8 * v);
+    }
   }
 }
 
 // ---- scan ----------------------------------------------------------------------------------------------
+// Registers, TMEM and shared memory of two CTAs on an SM: the start and the end of one overlap the other's tiles.
+constexpr int ctas_per_sm(int bytes, int tmem) { return 2 * (bytes + 2304) <= 233472 && 2 * tmem <= 512 ? 2 : 1; }
+
 template <int D, int G, bool OUT> struct Scan {
-  static constexpr int kRows = 128 / G, kCols = G == 4 ? 32 : 64, kKeys = kCols * G;
-  static constexpr int kThreads = 320;
-  static constexpr uint32_t kOne = kKeys * D * 2, kStage = OUT ? 2 * kOne : kOne;
-  static constexpr int kRing = (int)(131072 / kStage) < 8 ? (int)(131072 / kStage) : 8;
+  static constexpr int kRows = 128 / G, kCols = G == 1 ? 64 : 32, kKeys = kCols * G;
+  static constexpr int kWg = OUT && D == 64 ? 1 : 2;                       // warpgroups, which take tiles in turn
+  static constexpr int kThreads = 128 * kWg + 64;
+  static constexpr uint32_t kOne = kKeys * D * 2;
+  static constexpr int kSpace = D == 64 ? 65536 : 131072, kStages = (int)(kSpace / kOne) < 8 ? (int)(kSpace / kOne) : 8;
+  static constexpr int kK = OUT ? kStages / 2 : kStages, kV = OUT ? kStages / 2 : 4;
   static constexpr int kBufRows = (G - 1) * kRows + 128;                   // zeros, the rows, zeros
   static constexpr uint32_t kBufSub = kBufRows * 128;
-  static constexpr int kBuf = (int)kBufSub * (D / 64), kRingBytes = (int)kStage * kRing;
-  static constexpr int kBytes = kBuf + kRingBytes + 2048 + 256 + 1024;
-  static constexpr int kWgCols = 128 + (OUT ? D : 0), kTmem = OUT ? 512 : 256;
-  static_assert(2 * kWgCols <= kTmem, "the warpgroups' columns fit the allocation");
-  static_assert(!OUT || 256 * D * 4 <= kRingBytes, "the merge area fits the ring");
-  static_assert(kRing >= 2 && kBytes <= 232448, "shared memory");
+  static constexpr int kBuf = (int)kBufSub * (D / 64), kRingBytes = (int)kOne * kStages;
+  static constexpr int kBytes = kBuf + kRingBytes + 2048 + 512 + 1024;
+  // score buffers (tiles are scored ahead of the arithmetic), then P~ and the accumulator of each warpgroup
+  static constexpr int kWgCols = OUT ? 64 + D : 0, kBuffers = OUT ? 2 : 4;
+  static constexpr int kCols32 = kBuffers * kCols + kWg * kWgCols, kTmem = kCols32 <= 256 ? 256 : 512;
+  static constexpr int kPerSm = ctas_per_sm(kBytes, kTmem);
+  static_assert(kCols32 <= 512 && StreamBars<kK, kV, kBuffers>::kBytes <= 512, "score buffers");
+  static_assert(!OUT || kWg * 128 * D * 4 <= kRingBytes, "the merge area fits the ring");
+  static_assert(kK >= 2 && kBytes <= 231000, "shared memory");
 };
 
 // One warpgroup's step: kCols scores of a lane at tS, its P~ (OUT) to tP.
@@ -175,15 +194,15 @@ __device__ __forceinline__ void scan_step(uint32_t tS, uint32_t tP, uint32_t tO,
 
 // grid = (chunks, ceil(rows / 128) or 1, batch * kv_heads)
 template <int D, int G, bool OUT>
-__global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kPerSm) scan_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                       const __grid_constant__ tree::Args a) {
   using F = Scan<D, G, OUT>;
-  constexpr int R = F::kRing, KT = F::kKeys, NC = F::kCols, SUB = D / 64;
+  constexpr int RK = F::kK, RV = F::kV, NB = F::kBuffers, NW = F::kWg, KT = F::kKeys, NC = F::kCols, SUB = D / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
-  const uint32_t sQ = smem_u32(smem), ring = sQ + F::kBuf;
+  const uint32_t sQ = smem_u32(smem), ring_k = sQ + F::kBuf, ring_v = ring_k + F::kOne * RK;
   float2* sStat = reinterpret_cast<float2*>(smem + F::kBuf + F::kRingBytes);              // [2][128]
-  const StreamBars<R> bars(reinterpret_cast<uint64_t*>(smem + F::kBuf + F::kRingBytes + 2048));
+  const StreamBars<RK, RV, NB> bars(reinterpret_cast<uint64_t*>(smem + F::kBuf + F::kRingBytes + 2048));
   Ctl* ctl = bars.ctl;
   __shared__ tree::Lineage lineage;
 
@@ -213,35 +232,20 @@ __global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CU
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem);
 
-  if (warp_u == 8) {
+  if (warp_u == 4 * NW) {
     // ------------------------------------------------------------ the warp that issues MMAs
     constexpr uint32_t id_s = instr_desc(128, NC, 0, 0), id_p = instr_desc(128, D, 0, 1);
-    const Desc dQ = make_desc(sQ, 16, 1024), dK = make_desc(ring, 16, 1024), dV = make_desc(ring + F::kOne, KT * 128, 1024);
+    const Desc dQ = make_desc(sQ, 16, 1024), dK = make_desc(ring_k, 16, 1024), dV = make_desc(ring_v, KT * 128, 1024);
     // what the compute warps clear (their P~ columns and accumulators) is clear before the first product
-    asm volatile("bar.sync 4, 288;" ::: "memory");
+    asm volatile("bar.sync 4, %0;" ::"n"(128 * NW + 32) : "memory");
     tc_fence_after();
-    for (int e = 0; e < ne + 2; ++e) {
-      const int w = e & 1;
-      const uint32_t tS = tmem + F::kWgCols * w;
-      if (e >= 2) {
-        mbar_wait_warp(bars.pready + 8 * w, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitTile);
-        tc_fence_after();
-        if (OUT) {
-          const int st = (e - 2) % R;
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int kk = 0; kk < NC / 16; ++kk)               // 16 keys per instruction: 16 rows of 128 B = 128 units
-              mma_ts(lead, tS + 128, tS + 64 + (NC / 2) * g + 8 * kk, dV, (F::kStage >> 4) * st + 8 * NC * g + 128 * kk, id_p, 1);
-          mma_commit(lead, bars.free + 8 * st);
-        }
-      }
+    for (int e = 0; e < ne + NB - 1; ++e) {
       if (e < ne) {
-        const int st = e % R, from = len - (first + e) * KT;
-        mbar_wait_warp(bars.full + 8 * st, (e / R) & 1, ctl, &g_tree_status, kErrWaitTma);
+        const int st = e % RK, from = len - (first + e) * KT;
+        const uint32_t tS = tmem + NC * (e % NB);
+        mbar_wait_warp(bars.kfull + 8 * st, (e / RK) & 1, ctl, &g_tree_status, kErrWaitTma);
         if (from < KT) {
-          zero_rows(smem + F::kBuf + F::kStage * st, KT, from, SUB);
-          if (OUT) zero_rows(smem + F::kBuf + F::kStage * st + F::kOne, KT, from, SUB);
+          zero_rows(smem + F::kBuf + F::kOne * st, KT, from, SUB);
           fence_async_smem();
           __syncwarp();
         }
@@ -253,18 +257,41 @@ __global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CU
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               mma_ss(lead, tS, dQ, (F::kBufSub >> 4) * s + 8 * F::kRows * (G - 1 - g) + 2 * kk, dK,
-                     (F::kStage >> 4) * st + 8 * KT * s + 8 * NC * g + 2 * kk, id_s, g > 0 || s > 0 || kk > 0);
-        mma_commit(lead, bars.sdone + 8 * w);
-        if (!OUT) mma_commit(lead, bars.free + 8 * st);
+                     (F::kOne >> 4) * st + 8 * KT * s + 8 * NC * g + 2 * kk, id_s, g > 0 || s > 0 || kk > 0);
+        mma_commit(lead, bars.sdone + 8 * (e % NB));
+        mma_commit(lead, bars.kfree + 8 * st);
+      }
+      if (e >= NB - 1) {                                         // tile e - NB + 1 has been read: its buffer is next
+        const int y = e - NB + 1, w = y % NW, st = y % RV;
+        mbar_wait_warp(bars.ready + 8 * (y % NB), (y / NB) & 1, ctl, &g_tree_status, kErrWaitTile);
+        tc_fence_after();
+        if (OUT) {
+          mbar_wait_warp(bars.vfull + 8 * st, (y / RV) & 1, ctl, &g_tree_status, kErrWaitTma);
+          const int from = len - (first + y) * KT;
+          if (from < KT) {
+            zero_rows(smem + F::kBuf + F::kOne * (RK + st), KT, from, SUB);
+            fence_async_smem();
+            __syncwarp();
+          }
+          tc_fence_after();
+          const uint32_t tP = tmem + NC * NB + F::kWgCols * w;
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int kk = 0; kk < NC / 16; ++kk)               // 16 keys per instruction: 16 rows of 128 B = 128 units
+              mma_ts(lead, tP + 64, tP + (NC / 2) * g + 8 * kk, dV, (F::kOne >> 4) * st + 8 * NC * g + 128 * kk, id_p, 1);
+          mma_commit(lead, bars.vfree + 8 * st);
+          mma_commit(lead, bars.used + 8 * w);
+        }
       }
     }
     mma_commit(lead, bars.alldone);
     __syncwarp();
-  } else if (warp_u == 9) {
-    stream_tiles<D, KT, R, OUT>(bars, &map_k, &map_v, ring, first, ne, nk, lead);
+  } else if (warp_u == 4 * NW + 1) {
+    stream_tiles<D, KT, RK, RV, NB, OUT>(bars, &map_k, &map_v, ring_k, ring_v, first, ne, nk, lead);
   } else {
     // ------------------------------------------------------------ the compute warps: lane = row of a group
-    const uint32_t tS = tmem + F::kWgCols * wg + ((uint32_t)((warp & 3) * 32) << 16), tP = tS + 64, tO = tS + 128;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tP = tmem + NC * NB + F::kWgCols * wg + lanes, tO = tP + 64;
     const int g = row / F::kRows, x = row % F::kRows, r = r0 + x, rs = min(r, rows - 1);
     if (OUT) {
       uint32_t z[16];
@@ -275,7 +302,7 @@ __global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CU
       tmem_st_wait();
     }
     tc_fence_before();
-    asm volatile("bar.sync 4, 288;" ::: "memory");
+    asm volatile("bar.sync 4, %0;" ::"n"(128 * NW + 32) : "memory");
     const bool cap = a.cap > 0.f;
     const float lin = cap ? a.cap * kLog2e : a.scale * kLog2e, pre = cap ? a.scale / a.cap : 0.f;
     float slope2 = 0.f;
@@ -285,18 +312,20 @@ __global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CU
       at += lineage.depth[rs % a.nodes];
     }
     float ref = -INFINITY, s = 0.f;
-    for (int e = wg; e < ne; e += 2) {
+    for (int e = wg; e < ne; e += NW) {
       const int j0 = (first + e) * KT + NC * g;
-      mbar_wait_warp(bars.sdone + 8 * wg, (e >> 1) & 1, ctl, &g_tree_status, kErrWaitMma);
+      mbar_wait_warp(bars.sdone + 8 * (e % NB), (e / NB) & 1, ctl, &g_tree_status, kErrWaitMma);
+      // the product of the warpgroup's last tile has read its P~
+      if (OUT && e >= NW) mbar_wait_warp(bars.used + 8 * wg, (e / NW - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
       tc_fence_after();
-      scan_step<D, NC, OUT>(tS, tP + (NC / 2) * g, tO, lin, pre, cap, slope2, (float)(at - j0), len - j0, ref, s);
+      scan_step<D, NC, OUT>(tmem + NC * (e % NB) + lanes, tP + (NC / 2) * g, tO, lin, pre, cap, slope2, (float)(at - j0), len - j0, ref, s);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars.pready + 8 * wg);
+      if (lane == 0) mbar_arrive(bars.ready + 8 * (e % NB));
     }
-    // rows that are laid out several times, and the two warpgroups' keys, are one row
+    // rows that are laid out several times, and the warpgroups' keys, are one row
     sStat[wg * 128 + row] = make_float2(ref, s);
-    float* sO = reinterpret_cast<float*>(smem + F::kBuf);           // [2][128][D], over the ring
+    float* sO = reinterpret_cast<float*>(smem + F::kBuf);           // [NW][128][D], over the ring
     if (OUT) {
       mbar_wait_warp(bars.alldone, 0, ctl, &g_tree_status, kErrWaitMma);
       tc_fence_after();
@@ -311,19 +340,19 @@ __global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CU
         for (int c = 0; c < 8; ++c) dst[c ^ (row & 7)] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
       }
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * NW) : "memory");
     constexpr int kUnits = OUT ? D / 4 : 1;
     const int64_t base = ((int64_t)nk * a.chunks + blockIdx.x) * rows;
-    for (int y = tid; y < F::kRows * kUnits; y += 256) {
+    for (int y = tid; y < F::kRows * kUnits; y += 128 * NW) {
       const int xr = y / kUnits, c = y % kUnits;
       if (r0 + xr >= rows) break;
       float m = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int p = 0; p < 2 * G; ++p) m = fmaxf(m, sStat[(p / G) * 128 + (p % G) * F::kRows + xr].x);
+      for (int p = 0; p < NW * G; ++p) m = fmaxf(m, sStat[(p / G) * 128 + (p % G) * F::kRows + xr].x);
       const float from = m == -INFINITY ? 0.f : m;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int p = 0; p < 2 * G; ++p) {
+      for (int p = 0; p < NW * G; ++p) {
         const int lane_row = (p / G) * 128 + (p % G) * F::kRows + xr;
         const float2 st = sStat[lane_row];
         const float f = fast_exp2(st.x - from);
@@ -350,38 +379,41 @@ __global__ void __launch_bounds__(320, 1) scan_kernel(const __grid_constant__ CU
 // What the thread of a key has to know of a row.
 struct NodeStep {
   float lse;
-  int up;              // -1: the cached demand; -2: the node in front; otherwise the parent, whose column is read
-  int keep;            // a later node reads this one's column
-  float slope2;        // of an accepted row, and its position
+  int up;              // the parent, or -1
+  int at;              // an accepted row's position, and the slope of its head
+  float slope2;
 };
 
 template <int D, int N, bool DILUTE> struct Sweep {
   static constexpr int kKeys = 128, kThreads = 320;
-  static constexpr uint32_t kOne = 128 * D * 2, kStage = DILUTE ? 2 * kOne : kOne;
-  static constexpr int kRing = (int)(131072 / kStage) < 8 ? (int)(131072 / kStage) : 8;
+  static constexpr uint32_t kOne = 128 * D * 2;
+  static constexpr int kSpace = D == 64 || !DILUTE ? 65536 : 131072, kStages = (int)(kSpace / kOne);
+  static constexpr int kK = DILUTE ? kStages / 2 : kStages, kV = DILUTE ? kStages / 2 : 4;
   static constexpr uint32_t kQSub = N * 128;
-  static constexpr int kQ = N * 128 * (D / 64), kRingBytes = (int)kStage * kRing;
+  static constexpr int kQ = N * 128 * (D / 64), kRingBytes = (int)kOne * kStages;
   // Q | ring | share [2][128][64] | ones [2][16][64] | node steps and positions | barriers + control
   static constexpr int kShare = DILUTE ? 2 * 16384 : 0, kOnes = DILUTE ? 4096 : 0;
-  static constexpr int kBytes = (kQ + 1023) / 1024 * 1024 + kRingBytes + kShare + kOnes + 64 * 16 + 256 + 256 + 1024;
-  static constexpr int kTmem = 256;                                          // S^T 2 x 64, out^T 64, sums 64
-  static_assert(kRing >= 2 && kBytes <= 232448, "shared memory");
+  static constexpr int kBytes = (kQ + 1023) / 1024 * 1024 + kRingBytes + kShare + kOnes + 64 * 16 + 256 + 512 + 1024;
+  static constexpr int kBuffers = DILUTE ? 2 : 4, kTmem = 256;             // S^T [buffers] x 64, out^T 64, sums 64
+  static constexpr int kPerSm = ctas_per_sm(kBytes, kTmem);
+  static_assert(kK >= 2 && kBytes <= 231000, "shared memory");
 };
 
 // DILUTE: shares of the nodes and their part of share V.  Otherwise: advanced = committed + the bids of the accepted rows.
 // grid = (chunks, 1, batch * kv_heads); N >= rows
 template <int D, int N, bool DILUTE>
-__global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                        const __grid_constant__ tree::Args a, const __grid_constant__ tree::Accept acc) {
   using F = Sweep<D, N, DILUTE>;
-  constexpr int R = F::kRing, KT = 128, SUB = D / 64, kQ = (F::kQ + 1023) / 1024 * 1024;
+  constexpr int RK = F::kK, RV = F::kV, NB = F::kBuffers, KT = 128, SUB = D / 64, kQ = (F::kQ + 1023) / 1024 * 1024;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint8_t *pShare = smem + kQ + F::kRingBytes, *pOnes = pShare + F::kShare;
-  const uint32_t sQ = smem_u32(smem), ring = sQ + kQ, sShare = smem_u32(pShare), sOnes = smem_u32(pOnes);
+  const uint32_t sQ = smem_u32(smem), ring_k = sQ + kQ, ring_v = ring_k + F::kOne * RK, sShare = smem_u32(pShare), sOnes = smem_u32(pOnes);
   NodeStep* step = reinterpret_cast<NodeStep*>(pOnes + F::kOnes);
-  int* place = reinterpret_cast<int*>(step + 64);                                        // positions of accepted rows
-  const StreamBars<R> bars(reinterpret_cast<uint64_t*>(place + 64));
+  uint64_t* walk = reinterpret_cast<uint64_t*>(step + 64);      // bits of the nodes that do not follow the one in front, and of
+                                                                // those whose demand a later node starts from
+  const StreamBars<RK, RV, NB> bars(walk + 32);
   Ctl* ctl = bars.ctl;
   __shared__ tree::Lineage lineage;
 
@@ -400,21 +432,25 @@ __global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ C
   auto q_row = [&](int r) { return DILUTE ? r : r / acc.accepted * a.nodes + tree::path_node(a, acc, b, r % acc.accepted); };
   if (tid < N) {
     NodeStep s{0.f, -1, 0, 0.f};
-    int at = 0;
+    bool jump = false, keep = false;
     if (tid < rows) {
       const int q = q_row(tid);
       s.lse = a.lse[((int64_t)nk * a.group) * a.nodes + q];
       if (DILUTE) {
-        const int up = lineage.parent[tid];
-        s.up = up >= 0 && up == tid - 1 ? -2 : up;
-        for (int y = tid + 2; y < a.nodes; ++y) s.keep |= lineage.parent[y] == tid;
+        s.up = lineage.parent[tid];
+        jump = s.up < 0 || s.up != tid - 1;
+        for (int y = tid + 2; y < a.nodes; ++y) keep = keep || lineage.parent[y] == tid;
       } else {
         s.slope2 = a.slopes != nullptr ? a.slopes[hk * a.group + q / a.nodes] * kLog2e : 0.f;
-        at = lineage.depth[q % a.nodes];
+        s.at = len + lineage.depth[q % a.nodes];
       }
     }
     step[tid] = s;
-    place[tid] = len + at;
+    const unsigned active = N < 32 ? (1u << N) - 1 : 0xffffffffu, j = __ballot_sync(active, jump), k = __ballot_sync(active, keep);
+    if (lane == 0) {
+      reinterpret_cast<uint32_t*>(walk)[warp] = j;
+      reinterpret_cast<uint32_t*>(walk)[2 + warp] = k;
+    }
   }
   for (int x = tid; x < N * 8 * SUB; x += F::kThreads) {
     const int sub = x / (N * 8), r = x / 8 % N, c = x % 8;
@@ -441,34 +477,15 @@ __global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ C
   if (warp_u == 8) {
     // ------------------------------------------------------------ the warp that issues MMAs
     constexpr uint32_t id_s = instr_desc(128, N, 0, 0), id_o = instr_desc(128, N, 1, 1);
-    const Desc dK = make_desc(ring, 16, 1024), dQ = make_desc(sQ, 16, 1024);
+    const Desc dK = make_desc(ring_k, 16, 1024), dQ = make_desc(sQ, 16, 1024);
     const Desc dOnes = make_desc(sOnes, 2048, 1024);
-    for (int e = 0; e < ne + 2; ++e) {
-      const int w = e & 1;
-      const uint32_t tS = tmem + 64 * w;
-      if (e >= 2) {
-        mbar_wait_warp(bars.pready + 8 * w, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitTile);
-        tc_fence_after();
-        if (DILUTE) {
-          const int st = (e - 2) % R;
-          const uint32_t v = ring + F::kStage * st + F::kOne;
-          const Desc dP = make_desc(sShare + 16384 * w, 16384, 1024);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            // heads of 64: the second 64 rows of A are the ones, out^T has the sums in row 64
-            const uint32_t at = v + 2048 * kk;
-            mma_ss(lead, tmem + 128, make_desc(at, D == 64 ? sOnes - at : KT * 128, 1024), 0, dP, 128 * kk, id_o, e > 2 || kk > 0);
-            if (D == 128) mma_ss(lead, tmem + 192, dOnes, 0, dP, 128 * kk, id_o, e > 2 || kk > 0);
-          }
-          mma_commit(lead, bars.free + 8 * st);
-        }
-      }
+    for (int e = 0; e < ne + NB - 1; ++e) {
       if (e < ne) {
-        const int st = e % R, from = len - (first + e) * KT;
-        mbar_wait_warp(bars.full + 8 * st, (e / R) & 1, ctl, &g_tree_status, kErrWaitTma);
+        const int st = e % RK, from = len - (first + e) * KT;
+        const uint32_t tS = tmem + 64 * (e % NB);
+        mbar_wait_warp(bars.kfull + 8 * st, (e / RK) & 1, ctl, &g_tree_status, kErrWaitTma);
         if (from < KT) {
-          zero_rows(smem + kQ + F::kStage * st, KT, from, SUB);
-          if (DILUTE) zero_rows(smem + kQ + F::kStage * st + F::kOne, KT, from, SUB);
+          zero_rows(smem + kQ + F::kOne * st, KT, from, SUB);
           fence_async_smem();
           __syncwarp();
         }
@@ -477,26 +494,56 @@ __global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ C
         for (int s = 0; s < SUB; ++s)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_ss(lead, tS, dK, (F::kStage >> 4) * st + 8 * KT * s + 2 * kk, dQ, (F::kQSub >> 4) * s + 2 * kk, id_s, s > 0 || kk > 0);
-        mma_commit(lead, bars.sdone + 8 * w);
-        if (!DILUTE) mma_commit(lead, bars.free + 8 * st);
+            mma_ss(lead, tS, dK, (F::kOne >> 4) * st + 8 * KT * s + 2 * kk, dQ, (F::kQSub >> 4) * s + 2 * kk, id_s, s > 0 || kk > 0);
+        mma_commit(lead, bars.sdone + 8 * (e % NB));
+        mma_commit(lead, bars.kfree + 8 * st);
+      }
+      if (e >= NB - 1) {
+        const int y = e - NB + 1, w = y & 1, st = y % RV;
+        mbar_wait_warp(bars.ready + 8 * (y % NB), (y / NB) & 1, ctl, &g_tree_status, kErrWaitTile);
+        tc_fence_after();
+        if (DILUTE) {
+          mbar_wait_warp(bars.vfull + 8 * st, (y / RV) & 1, ctl, &g_tree_status, kErrWaitTma);
+          const int from = len - (first + y) * KT;
+          if (from < KT) {
+            zero_rows(smem + kQ + F::kOne * (RK + st), KT, from, SUB);
+            fence_async_smem();
+            __syncwarp();
+          }
+          tc_fence_after();
+          const uint32_t v = ring_v + F::kOne * st;
+          const Desc dP = make_desc(sShare + 16384 * w, 16384, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            // heads of 64: the second 64 rows of A are the ones, out^T has the sums in row 64
+            const uint32_t at = v + 2048 * kk;
+            mma_ss(lead, tmem + 64 * NB, make_desc(at, D == 64 ? sOnes - at : KT * 128, 1024), 0, dP, 128 * kk, id_o, y > 0 || kk > 0);
+            if (D == 128) mma_ss(lead, tmem + 64 * NB + 64, dOnes, 0, dP, 128 * kk, id_o, y > 0 || kk > 0);
+          }
+          mma_commit(lead, bars.vfree + 8 * st);
+          mma_commit(lead, bars.used + 8 * w);
+        }
       }
     }
     mma_commit(lead, bars.alldone);
     __syncwarp();
   } else if (warp_u == 9) {
-    stream_tiles<D, KT, R, DILUTE>(bars, &map_k, &map_v, ring, first, ne, nk, lead);
+    stream_tiles<D, KT, RK, RV, NB, DILUTE>(bars, &map_k, &map_v, ring_k, ring_v, first, ne, nk, lead);
   } else {
     // ------------------------------------------------------------ the compute warps: lane = key
-    const uint32_t tS = tmem + 64 * wg + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const bool cap = a.cap > 0.f;
     const float lin = cap ? a.cap * kLog2e : a.scale * kLog2e, pre = cap ? a.scale / a.cap : 0.f;
+    const uint64_t jumps = walk[0], keeps = walk[1];
     for (int e = wg; e < ne; e += 2) {
       const int j = (first + e) * KT + row;
       const bool live = j < len;
       const int64_t at = (int64_t)nk * a.capacity + j;
       const float base = live ? a.committed[at] : 0.f;
-      mbar_wait_warp(bars.sdone + 8 * wg, (e >> 1) & 1, ctl, &g_tree_status, kErrWaitMma);
+      const uint32_t tS = tmem + 64 * (e % NB) + lanes;
+      mbar_wait_warp(bars.sdone + 8 * (e % NB), (e / NB) & 1, ctl, &g_tree_status, kErrWaitMma);
+      // the product of the warpgroup's last tile has read its shares
+      if (DILUTE && e >= 2) mbar_wait_warp(bars.used + 8 * wg, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
       tc_fence_after();
       float last = base, total = base;
 #pragma unroll
@@ -507,27 +554,29 @@ __global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ C
         tmem_ld16(tS + c0, v);
         tmem_ld_wait16(v);
         if (DILUTE) {
+          float d[16];
           uint32_t w[8];
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
-            const NodeStep s = step[c0 + y];
-            float p = fast_exp2(fmaf(v[y], lin, -s.lse));
-            if (!live || c0 + y >= rows) p = 0.f;
-            float had = last;
-            if (s.up != -2) {
-              had = base;
-              if (s.up >= 0) {
+            v[y] = fast_exp2(fmaf(v[y], lin, -step[c0 + y].lse));
+            if (!live || c0 + y >= rows) v[y] = 0.f;
+          }
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            if (jumps >> (c0 + y) & 1) {
+              const int up = step[c0 + y].up;
+              last = base;
+              if (up >= 0) {
                 tmem_st_wait();
-                tmem_ld1(tS + s.up, &had);
-                tmem_ld_wait1(&had);
+                tmem_ld1(tS + up, &last);
+                tmem_ld_wait1(&last);
               }
             }
-            last = had + p;
-            if (s.keep) tmem_st1(tS + c0 + y, last);
-            const float share = p * fast_rcp(last + a.eps);
-            // (a demand or a bid that is no number goes on to the output)
-            v[y] = p == 0.f ? 0.f : share;
+            d[y] = last = last + v[y];
+            if (keeps >> (c0 + y) & 1) tmem_st1(tS + c0 + y, last);
           }
+#pragma unroll
+          for (int y = 0; y < 16; ++y) v[y] *= fast_rcp(d[y] + a.eps);
 #pragma unroll
           for (int y = 0; y < 8; ++y) w[y] = pack_pair(v[2 * y], v[2 * y + 1]);
           uint8_t* dst = pShare + 16384 * wg;
@@ -538,7 +587,7 @@ __global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ C
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
             const NodeStep s = step[c0 + y];
-            const float z = fmaf(v[y], lin, -s.lse - s.slope2 * (float)(place[c0 + y] - j));
+            const float z = fmaf(v[y], lin, -s.lse - s.slope2 * (float)(s.at - j));
             if (c0 + y < rows) total += fast_exp2(z);
           }
         }
@@ -551,7 +600,7 @@ __global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ C
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars.pready + 8 * wg);
+      if (lane == 0) mbar_arrive(bars.ready + 8 * (e % NB));
     }
     mbar_wait_warp(bars.alldone, 0, ctl, &g_tree_status, kErrWaitMma);
     tc_fence_after();
@@ -562,10 +611,10 @@ __global__ void __launch_bounds__(320, 1) sweep_kernel(const __grid_constant__ C
       for (int c0 = 0; c0 < N; c0 += 16) {
         float o[16], t[16];
         __syncwarp();
-        tmem_ld16(tS + 128 + c0, o);
+        tmem_ld16(tmem + 64 * NB + lanes + c0, o);
         tmem_ld_wait16(o);
         if (D == 128) {
-          tmem_ld16(tS + 192 + c0, t);
+          tmem_ld16(tmem + 64 * NB + 64 + lanes + c0, t);
           tmem_ld_wait16(t);
         }
 #pragma unroll

@@ -20,14 +20,15 @@ int simt_chunks(int64_t blocks, int64_t keys) {
   const int64_t want = (148 * 4 + blocks - 1) / std::max<int64_t>(blocks, 1), most = (keys + 255) / 256;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
 }
-// Tensor cores: one block per SM, so as many parts as make the fewest rounds of tiles of 128 keys, where a block's start and
-// end take as long as about four tiles.
-int tc_chunks(int64_t blocks, int64_t keys) {
+// Tensor cores: as many parts as make the fewest rounds of tiles of 128 keys on the chip's SMs, where a block's start and end take as
+// long as about four tiles.
+int tc_chunks(int64_t blocks, int64_t keys, int per_sm) {
+  const int64_t slots = 148 * per_sm;
   const int64_t tiles = std::max<int64_t>(1, (keys + 127) / 128);
   int64_t best = 0;
   int chunks = 1;
-  for (int64_t c = 1; c <= std::min<int64_t>(tiles, 148); ++c) {
-    const int64_t cost = (blocks * c + 147) / 148 * ((tiles + c - 1) / c + 4);
+  for (int64_t c = 1; c <= std::min<int64_t>(tiles, 2 * 148); ++c) {
+    const int64_t cost = (blocks * c + slots - 1) / slots * ((tiles + c - 1) / c + 4);
     if (c == 1 || cost < best) {
       best = cost;
       chunks = (int)c;
@@ -179,7 +180,7 @@ template <int D> int tc_softmax(tree::Args a, void* scratch, cudaStream_t st) {
   CUtensorMap k, v;
   if (int rc = cache_maps(&k, &v, a, D)) return rc;
   const int rows = a.group * a.nodes;
-  a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads * row_blocks(rows, 128), tree_keys(a));
+  a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads * row_blocks(rows, 128), tree_keys(a), tc::Scan<D, 4, true>::kPerSm);
   place_scratch(a, scratch, D);
   if (int rc = tc_scan<D, true>(a, k, v, st)) return rc;
   LaunchMark mark("tree_join", st);
@@ -191,7 +192,7 @@ template <int D> int tc_dilute(tree::Args a, void* scratch, cudaStream_t st) {
   CUtensorMap k, v;
   if (int rc = cache_maps(&k, &v, a, D)) return rc;
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
-  a.chunks = tc_chunks(heads, tree_keys(a));
+  a.chunks = tc_chunks(heads, tree_keys(a), tc::Sweep<D, 64, true>::kPerSm);
   float* shares = place_scratch(a, scratch, D);
   if (int rc = tc_scan<D, false>(a, k, v, st)) return rc;
   {
@@ -211,7 +212,7 @@ template <int D> int tc_accept(tree::Args a, const tree::Accept& c, cudaStream_t
   if (c.advanced) {
     CUtensorMap k, v;
     if (int rc = cache_maps(&k, &v, a, D)) return rc;
-    a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads, tree_keys(a));
+    a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads, tree_keys(a), 2);
     if (int rc = tc_sweep<D, false>(a, c, a.group * c.accepted, k, v, st)) return rc;
   }
   LaunchMark mark("tree_append", st);
@@ -230,7 +231,7 @@ size_t dilution_tree_scratch_bytes(int64_t batch, int64_t kv_heads, int group, i
   if (batch < 1 || kv_heads < 1 || group < 1 || nodes < 1 || length < 0 || d < 1) return 0;
   const int64_t heads = batch * kv_heads, keys = length + nodes;
   const int rows = group * nodes;
-  const int chunks = std::max(simt_chunks(heads * simt_row_blocks(rows), keys), tc_chunks(heads * row_blocks(rows, 128), keys));
+  const int chunks = std::max(simt_chunks(heads * simt_row_blocks(rows), keys), std::max(tc_chunks(heads * row_blocks(rows, 128), keys, 1), tc_chunks(heads * row_blocks(rows, 128), keys, 2)));
   return tree_scratch(heads, group, nodes, chunks, d).bytes;
 }
 
