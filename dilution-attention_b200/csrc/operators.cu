@@ -188,7 +188,7 @@ int dilution_attend_forward(const void* q, const void* k, const void* v, int dty
   return with_type(dtype, d, [&](auto type, auto dim) {
     if constexpr (!kOnTensorCores<decltype(type), dim()>) return simt_forward<decltype(type), dim()>(a, st);
     else if constexpr (dim() == 128) return tc_forward<128, 1>(a, st);
-    else return a.docs == nullptr && a.t >= 2048 ? tc_forward<64, 2>(a, st) : tc_forward<64, 1>(a, st);
+    else return a.docs == nullptr && a.t >= 8192 ? tc_forward<64, 2>(a, st) : tc_forward<64, 1>(a, st);
   });
 }
 

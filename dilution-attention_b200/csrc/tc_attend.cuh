@@ -57,6 +57,25 @@ __device__ __forceinline__ int pair_state(const Row& r, int i0, int i1, const Do
 }
 
 // ---- forward -----------------------------------------------------------------------------------------
+// What pairs of tiles have to do is asked once per block and kept for this many half tiles from the first on: two bits each, of
+// 32 half tiles in a word: the warp that issues MMAs has to know in a few cycles, it is what all others wait for.
+constexpr int kStates = 4096;
+struct States {
+  uint32_t any[kStates / 32], masked[kStates / 32];
+};
+// Whole warps, 32 half tiles at a time; f: the state of a half tile, counted from the first.
+template <typename F> __device__ __forceinline__ void keep_states(States* s, int n, int warp, int warps, F f) {
+  const int lane = threadIdx.x & 31;
+  for (int e = 32 * warp; e < min(n, kStates); e += 32 * warps) {
+    const int what = e + lane < n ? f(e + lane) : 0;
+    const uint32_t any = __ballot_sync(0xffffffffu, what != 0), masked = __ballot_sync(0xffffffffu, what == 1);
+    if (lane == 0) {
+      s->any[e / 32] = any;
+      s->masked[e / 32] = masked;
+    }
+  }
+}
+
 template <int D, int NT> struct AttendForward {
   static constexpr int kThreads = 256 * NT + 32;
   static constexpr int kRing = D == 64 && NT == 1 ? 5 : D == 64 ? 8 : 5;           // half tiles of K and V
@@ -225,6 +244,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   const uint32_t qfull = smem_u32(bars), kfull = qfull + 8, kfree = kfull + 8 * R, sdone = kfree + 8 * R, pready = sdone + 16 * NT;
   Ctl* ctl = reinterpret_cast<Ctl*>(bars + 1 + 2 * R + 4 * NT);
   __shared__ int s_range[2];
+  __shared__ States s_state[NT];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
   const int warp_u = uniform_warp();
@@ -278,13 +298,15 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem);
   const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0;
+#pragma unroll
+  for (int x = 0; x < NT; ++x) keep_states(&s_state[x], nh, warp, F::kThreads / 32, [&](int e) { return state(x, h0 + e); });
+  __syncthreads();
 
   if (warp_u == 8 * NT) {
     // ------------------------------------------------------------ the issuing warp
     constexpr uint32_t id_s = instr_desc(128, 64, 0, 0), id_p = instr_desc(128, D, 0, 1);
     const Desc dQ = make_desc(sQ, 16, 1024), dK = make_desc(sK, 16, 1024), dV = make_desc(sV, HSub, 1024);
-    auto load_keys = [&](int e) {
-      const int st = e % R;
+    auto load_keys = [&](int e, int st) {
       if (!lead) return;
       mbar_expect_tx(kfull + 8 * st, 2 * HB);
       tma_load_rows<W>(sK + HB * st, &map_k, (h0 + e) * 64, nk, kfull + 8 * st, HSub);
@@ -296,11 +318,18 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
         mbar_expect_tx(qfull, tiles * TB);
         for (int x = 0; x < tiles; ++x) tma_load_rows<W>(sQ + TB * x, &map_q, (ib + x) * kTileRows, n, qfull);
       }
-      for (int e = 0; e < R && e < nh; ++e) load_keys(e);
+      for (int e = 0; e < R && e < nh; ++e) load_keys(e, e);
       mbar_wait_warp(qfull, 0, ctl, &g_attend_status, kErrWaitTma);
       uint32_t pending = 0, flip = 0;                    // warpgroups with a P~ to come, the parity of the next
+      // (counters in place of remainders: this warp's time between two products is what the others wait for)
+      int in = 0, out = 0, refill = 0;
+      uint32_t phase = 0, back = 0, word[NT];
       for (int e = 0; e < nh + 2; ++e) {
-        if (e < nh) mbar_wait_warp(kfull + 8 * (e % R), (e / R) & 1, ctl, &g_attend_status, kErrWaitTma);
+        if ((e & 31) == 0 && e < nh)
+#pragma unroll
+          for (int x = 0; x < NT; ++x)
+            word[x] = uniform(e < kStates ? s_state[x].any[e / 32] : __ballot_sync(0xffffffffu, e + lane < nh && state(x, h0 + e + lane) != 0));
+        if (e < nh) mbar_wait_warp(kfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
           const int w = 2 * x + (e & 1);
@@ -312,22 +341,29 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
             tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)               // 16 keys per instruction: 16 rows of 128 B = 128 units
-              mma_ts(lead, tS + 64, tS + 8 * kk, dV, (HB >> 4) * ((e - 2) % R) + 128 * kk, id_p, 1);
+              mma_ts(lead, tS + 64, tS + 8 * kk, dV, (HB >> 4) * out + 128 * kk, id_p, 1);
           }
-          if (e < nh && uniform(state(x, h0 + e)) != 0) {
+          if (e < nh && (word[x] >> (e & 31) & 1)) {
             tc_fence_after();
-            mma_scores_wide<W>(lead, tS, Desc{dQ.lo + (TB >> 4) * x, dQ.hi}, kTileBytes, Desc{dK.lo + (HB >> 4) * (e % R), dK.hi},
+            mma_scores_wide<W>(lead, tS, Desc{dQ.lo + (TB >> 4) * x, dQ.hi}, kTileBytes, Desc{dK.lo + (HB >> 4) * in, dK.hi},
                                HSub, id_s);
             mma_commit(lead, sdone + 8 * w);             // the scores, and every product in front of them
             pending |= 1u << w;
           }
         }
-        if (e >= 2) mma_commit(lead, kfree + 8 * ((e - 2) % R));
-        // half tile e - 3, whose products were issued one round ago, makes room for e - 3 + R
-        if (e >= 3 && e - 3 + R < nh) {
-          mbar_wait_warp(kfree + 8 * ((e - 3) % R), ((e - 3) / R) & 1, ctl, &g_attend_status, kErrWaitMma);
-          load_keys(e - 3 + R);
+        if (e >= 2) {
+          mma_commit(lead, kfree + 8 * out);
+          if (++out == R) out = 0;
         }
+        // half tile e - 3, whose products were issued one round ago, makes room for e - 3 + R
+        if (e >= 3) {
+          if (e - 3 + R < nh) {
+            mbar_wait_warp(kfree + 8 * refill, back, ctl, &g_attend_status, kErrWaitMma);
+            load_keys(e - 3 + R, refill);
+          }
+          if (++refill == R) { refill = 0; back ^= 1; }
+        }
+        if (++in == R) { in = 0; phase ^= 1; }
       }
 #pragma unroll
       for (int w = 0; w < 2 * NT; ++w) mma_commit(lead, sdone + 8 * w);              // the last products
@@ -348,7 +384,9 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     float ref = -INFINITY, s = 0.f;
     int turn = 0;
     for (int e = half; e < nh; e += 2) {
-      const int what = (int)uniform(state(tile, h0 + e));
+      const States& z = s_state[tile];
+      const int what = (int)uniform(e >= kStates ? (uint32_t)state(tile, h0 + e)
+                                    : z.any[e / 32] >> (e & 31) & 1 ? 2 - (z.masked[e / 32] >> (e & 31) & 1) : 0u);
       if (what == 0) continue;
       mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
       ++turn;
@@ -445,6 +483,7 @@ template <int D, int STAY> struct AttendBackward {
   static constexpr int kOperands = (int)(2 * kTile + 2 * kRing * kHalf);
   static constexpr int kStats = STAY == 1 ? kRing * 512 : 0;
   static constexpr int kBytes = kOperands + kStats + 512 + 256 + 1024;
+  static_assert(kBytes + (int)sizeof(States) + 64 <= 232448, "shared memory, with what the kernel has of its own");
 };
 
 // Bytes of global memory into shared memory, both on 16-byte boundaries.
@@ -455,12 +494,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 // A warpgroup's step over 64 columns: S at tS, dout . v at tS + 64.  P (keys stay) as bf16 over the scores and dS over the
-// others, both as A operands.  x0: the first passing token, y: the lane's own; st: (lse, delta) of the passing queries.
-template <int STAY, bool CAP, bool BIAS>
-__device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float lin, float pre, int x0, int y, bool edge, float2 own,
-                                              const float4* st) {
+// others, both as A operands.  x0: the first passing token, y: the lane's own; st: (-lse, -lse, -delta, -delta) of pairs of passing
+// queries; own: (-lse, -delta) of the lane's query.  EDGE: masks decide.
+template <int STAY, bool CAP, bool BIAS, bool EDGE>
+__device__ __forceinline__ void backward_tile(uint32_t tS, const Row& r, float lin, float pre, int x0, int y, float2 own, const float4* st) {
   uint2 bits = make_uint2(0, 0);
-  if (edge) bits = STAY == 1 ? query_bits(r, x0, y) : key_bits(r, y, x0);
+  if (EDGE) bits = STAY == 1 ? query_bits(r, x0, y) : key_bits(r, y, x0);
 #pragma unroll
   for (int c0 = 0; c0 < 64; c0 += 32) {
     float v[32], g[32];
@@ -475,30 +514,27 @@ __device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float l
     const float step = STAY == 1 ? -r.slope2 : r.slope2;
     const float first = STAY == 1 ? r.slope2 * (float)(y - x0 - c0) : r.slope2 * (float)(x0 + c0 - y);
     float2 far = make_float2(first, first + step);
+    const float2 two = make_float2(2.f * step, 2.f * step);
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
-      float2 off, delta;                                  // -lse (and the distance's term), -delta
+      float2 off = make_float2(own.x, own.x), delta = make_float2(own.y, own.y);
       if (STAY == 1) {
         const float4 x = st[(c0 + e) >> 1];
-        off = make_float2(-x.x, -x.z);
-        delta = make_float2(-x.y, -x.w);
-      } else {
-        off = make_float2(-own.x, -own.x);
-        delta = make_float2(-own.y, -own.y);
+        off = make_float2(x.x, x.y);
+        delta = make_float2(x.z, x.w);
       }
       if (BIAS) {
-        off = add2(off, edge ? make_float2(-fabsf(far.x), -fabsf(far.y)) : far);
-        far = add2(far, make_float2(2.f * step, 2.f * step));
+        off = add2(off, EDGE ? make_float2(-fabsf(far.x), -fabsf(far.y)) : far);
+        far = add2(far, two);
       }
-      float2 z = fma2(make_float2(v[e], v[e + 1]), mm, off);
+      const float2 z = fma2(make_float2(v[e], v[e + 1]), mm, off);
       float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
-      float2 d = add2(make_float2(g[e], g[e + 1]), delta);
-      d = mul2(p, d);
+      float2 d = mul2(p, add2(make_float2(g[e], g[e + 1]), delta));
       if (CAP) {
-        const float2 t = make_float2(v[e], v[e + 1]), minus = make_float2(-t.x, -t.y);
-        d = mul2(d, fma2(minus, t, make_float2(1.f, 1.f)));
+        const float2 t = make_float2(v[e], v[e + 1]);
+        d = sub2(d, mul2(mul2(t, t), d));
       }
-      if (edge) {
+      if (EDGE) {
         if (!bit_of(bits, c0 + e)) p.x = d.x = 0.f;
         if (!bit_of(bits, c0 + e + 1)) p.y = d.y = 0.f;
       }
@@ -513,7 +549,7 @@ __device__ __forceinline__ void backward_step(uint32_t tS, const Row& r, float l
 
 // grid = rows * ceil(t / 128): dq: batch * heads rows, last queries first; dk, dv: batch * kv_heads rows, first keys first.
 // map_a, map_b: Q and dout (batch * heads rows); map_c, map_d: K and V (batch * kv_heads rows), boxes of 64 rows all.
-// stats: (lse, delta) of every query, padded to whole half tiles with (+inf, 0): (batch * heads, 64 ceil(t / 64)).
+// stats: (-lse, -lse, -delta, -delta) of every pair of queries, padded to whole half tiles with -inf and 0.
 template <int D, int STAY, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_backward_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
@@ -531,6 +567,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
                  pready = alldone + 8;
   Ctl* ctl = reinterpret_cast<Ctl*>(bars + 2 + 2 * R + 2 * NW);
   __shared__ int s_range[2];
+  __shared__ States s_state;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
   const int warp_u = uniform_warp();
@@ -577,6 +614,8 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem), tAcc = tmem + 128 * NW;
   const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0, ne = nh * passes;
+  keep_states(&s_state, nh, warp, F::kThreads / 32, [&](int e) { return state(h0 + e); });
+  __syncthreads();
 
   if (warp_u == 4 * NW) {
     // ------------------------------------------------------------ the warp that issues MMAs
@@ -586,37 +625,46 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
     if (ne > 0) {
       mbar_wait_warp(afull, 0, ctl, &g_attend_status, kErrWaitTma);
       uint32_t pending = 0, flip = 0, started = 0;         // warpgroups with a dS to come, the parity of the next
+      // (counters in place of remainders: this warp's time between two products is what the others wait for)
+      int w = 0, in = 0, out = 0, eh = 0;
+      uint32_t phase = 0, word = 0;
       for (int e = 0; e < ne + NW; ++e) {
-        const int w = e % NW;
         const uint32_t tS = tmem + 128 * w;
+        if ((eh & 31) == 0)
+          word = uniform(eh < kStates ? s_state.any[eh / 32] : __ballot_sync(0xffffffffu, eh + lane < nh && state(h0 + eh + lane) != 0));
         if (pending >> w & 1) {                            // of half tile e - NW
-          const int st = (e - NW) % R;
           mbar_wait_warp(pready + 8 * w, flip >> w & 1, ctl, &g_attend_status, kErrWaitTile);
           flip ^= 1u << w;
           pending &= ~(1u << w);
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)                   // dS times the passing queries (or keys)
-            mma_ts(lead, tAcc, tS + 64 + 8 * kk, dBm, (HB >> 4) * st + 128 * kk, id_a, started | (kk > 0));
+            mma_ts(lead, tAcc, tS + 64 + 8 * kk, dBm, (HB >> 4) * out + 128 * kk, id_a, started | (kk > 0));
           if (STAY == 1) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)                 // P times their dout
-              mma_ts(lead, tAcc + D, tS + 8 * kk, dCm, (HB >> 4) * st + 128 * kk, id_a, started | (kk > 0));
+              mma_ts(lead, tAcc + D, tS + 8 * kk, dCm, (HB >> 4) * out + 128 * kk, id_a, started | (kk > 0));
           }
           started = 1;
         }
-        if (e >= NW) mma_commit(lead, bfree + 8 * ((e - NW) % R));
+        if (e >= NW) {
+          mma_commit(lead, bfree + 8 * out);
+          if (++out == R) out = 0;
+        }
         if (e < ne) {
-          mbar_wait_warp(bfull + 8 * (e % R), (e / R) & 1, ctl, &g_attend_status, kErrWaitTma);
-          if (uniform(state(h0 + e % nh)) != 0) {
+          mbar_wait_warp(bfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
+          if (word >> (eh & 31) & 1) {
             tc_fence_after();
-            mma_scores_wide<W>(lead, tS, dA, kTileBytes, Desc{dB.lo + (HB >> 4) * (e % R), dB.hi}, HSub, id_s);
-            mma_scores_wide<W>(lead, tS + 64, Desc{dA.lo + (TB >> 4), dA.hi}, kTileBytes, Desc{dC.lo + (HB >> 4) * (e % R), dC.hi}, HSub,
+            mma_scores_wide<W>(lead, tS, dA, kTileBytes, Desc{dB.lo + (HB >> 4) * in, dB.hi}, HSub, id_s);
+            mma_scores_wide<W>(lead, tS + 64, Desc{dA.lo + (TB >> 4), dA.hi}, kTileBytes, Desc{dC.lo + (HB >> 4) * in, dC.hi}, HSub,
                                id_s);
             mma_commit(lead, sdone + 8 * w);
             pending |= 1u << w;
           }
         }
+        if (++w == NW) w = 0;
+        if (++in == R) { in = 0; phase ^= 1; }
+        if (++eh == nh) eh = 0;
       }
       mma_commit(lead, alldone);
     }
@@ -635,9 +683,10 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
                            kTileBytes);
     }
     __syncwarp();
+    int st = 0, hh = h0, m = nx;
+    uint32_t phase = 1;
     for (int e = 0; e < ne; ++e) {
-      const int st = e % R, hh = h0 + e % nh, m = nx + e / nh;
-      if (e >= R) mbar_wait_warp(bfree + 8 * st, (e / R - 1) & 1, ctl, &g_attend_status, kErrWaitMma);
+      if (e >= R) mbar_wait_warp(bfree + 8 * st, phase, ctl, &g_attend_status, kErrWaitMma);
       if (lead) {
         mbar_expect_tx(bfull + 8 * st, 2 * HB + (STAY == 1 ? 512 : 0));
         tma_load_rows<W>(sB + HB * st, STAY == 1 ? &map_q : &map_k, hh * 64, m, bfull + 8 * st, HSub);
@@ -645,22 +694,31 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
         if (STAY == 1) bulk_load(sStat + 512 * st, stats + (int64_t)m * padded + hh * 64, 512, bfull + 8 * st);
       }
       __syncwarp();
+      if (++st == R) { st = 0; phase ^= 1; }
+      if (++hh == h0 + nh) { hh = h0; ++m; }
     }
   } else {
     // ------------------------------------------------------------ the compute warps: lane = the staying query or key
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + 128 * wg + lanes;
     const int y = y0 + row, ys = min(y, a.t - 1);
     float2 own = make_float2(0.f, 0.f);
-    if (STAY == 0) own = y < a.t ? stats[(int64_t)n * padded + y] : make_float2(INFINITY, 0.f);
-    int turn = 0;
-    for (int e = wg; e < ne; e += NW) {
-      if (STAY == 1 && BIAS) r.slope2 = a.slopes[head * group + e / nh] * kLog2e;
-      const int hh = h0 + (passes == 1 ? e : e % nh), what = (int)uniform(state(hh));
+    if (STAY == 0) {
+      const float* pair = reinterpret_cast<const float*>(stats + ((int64_t)n * padded + (y & ~1))) + (y & 1);
+      own = y < a.t ? make_float2(pair[0], pair[2]) : make_float2(-INFINITY, 0.f);
+    }
+    int turn = 0, pass = 0, eh = wg;
+    for (int e = wg; e < ne; e += NW, eh += NW) {
+      while (eh >= nh) { eh -= nh; ++pass; }
+      if (STAY == 1 && BIAS) r.slope2 = a.slopes[head * group + pass] * kLog2e;
+      const int hh = h0 + eh;
+      const int what = (int)uniform(eh >= kStates ? (uint32_t)state(hh)
+                                    : s_state.any[eh / 32] >> (eh & 31) & 1 ? 2 - (s_state.masked[eh / 32] >> (eh & 31) & 1) : 0u);
       if (what == 0) continue;
       mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
       ++turn;
       tc_fence_after();
-      backward_step<STAY, CAP, BIAS>(tS, r, lin, pre, hh * 64, ys, what == 1, own, stat + 32 * (e % R));
+      if (what == 1) backward_tile<STAY, CAP, BIAS, true>(tS, r, lin, pre, hh * 64, ys, own, stat + 32 * (e % R));
+      else backward_tile<STAY, CAP, BIAS, false>(tS, r, lin, pre, hh * 64, ys, own, stat + 32 * (e % R));
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(pready + 8 * wg);
@@ -707,7 +765,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
   if (warp == 0) tmem_free(tmem, 512);
 }
 
-// (lse, delta_i = dout_i . out_i) of every query, padded.  D / 8 lanes a row, 16 bytes each.
+// lse and delta_i = dout_i . out_i of every query, padded, as the kernels above read them.  D / 8 lanes a row, 16 bytes each.
 template <int D>
 __global__ void __launch_bounds__(256) attend_stats_kernel(attend::Args a, float2* __restrict__ stats) {
   constexpr int L = D / 8;
@@ -727,7 +785,9 @@ __global__ void __launch_bounds__(256) attend_stats_kernel(attend::Args a, float
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (u == 0 && n < (int64_t)a.batch * a.heads) {
-    stats[at] = real ? make_float2(a.lse[n * a.t + i], s) : make_float2(INFINITY, 0.f);
+    float* pair = reinterpret_cast<float*>(stats + (at & ~(int64_t)1)) + (at & 1);
+    pair[0] = real ? -a.lse[n * a.t + i] : -INFINITY;
+    pair[2] = real ? -s : 0.f;
     if (real) a.delta[n * a.t + i] = s;
   }
 }
