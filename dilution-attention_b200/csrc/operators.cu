@@ -109,10 +109,10 @@ template <int D, int NT> int tc_forward(const attend::Args& a, cudaStream_t st) 
   });
 }
 
-template <int D, int STAY> int tc_backward_half(const attend::Args& a, const AttendMaps& m, const float2* stats, cudaStream_t st) {
-  using F = tc::AttendBackward<D, STAY>;
+template <int D, int STAY, int NW> int tc_backward_half(const attend::Args& a, const AttendMaps& m, const float2* stats, cudaStream_t st) {
+  using F = tc::AttendBackward<D, STAY, NW>;
   return with_score(a, [&](auto cap, auto bias) {
-    auto kernel = tc::attend_backward_kernel<D, STAY, cap(), bias()>;
+    auto kernel = tc::attend_backward_kernel<D, STAY, NW, cap(), bias()>;
     if (int rc = opt_in(kernel, F::kBytes)) return rc;
     LaunchMark mark(STAY ? "attend_dkv" : "attend_dq", st);
     const unsigned grid = (unsigned)((int64_t)a.batch * (STAY ? a.kv_heads : a.heads) * ((a.t + 127) / 128));
@@ -130,8 +130,17 @@ template <int D> int tc_backward(const attend::Args& a, float2* stats, cudaStrea
     tc::attend_stats_kernel<D><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a, stats);
     if (int rc = abi_check_launch("attend_delta")) return rc;
   }
-  if (int rc = tc_backward_half<D, 1>(a, m, stats, st)) return rc;
-  return tc_backward_half<D, 0>(a, m, stats, st);
+  // Heads of 64: two CTAs with a warpgroup each on an SM, whose starts and ends overlap, or one with three.  dk, dv and dq in us,
+  // two / one: n = 148, T = 512 32 + 25 / 40 + 33, T = 1024 77 + 63 / 92 + 76; n = 64, T = 4096 325 + 255 / 318 + 261, T = 8192
+  // 1227 + 938 / 1112 + 914, packed documents of 700 tokens (T = 4096) 156 + 119 / 178 + 145.
+  if constexpr (D == 64) {
+    if (a.docs || a.t <= 4096) {
+      if (int rc = tc_backward_half<D, 1, 1>(a, m, stats, st)) return rc;
+      return tc_backward_half<D, 0, 1>(a, m, stats, st);
+    }
+  }
+  if (int rc = tc_backward_half<D, 1, D == 64 ? 3 : 2>(a, m, stats, st)) return rc;
+  return tc_backward_half<D, 0, 3>(a, m, stats, st);
 }
 
 template <typename T, int D> constexpr bool kOnTensorCores = std::is_same<T, __nv_bfloat16>::value && (D == 64 || D == 128);
@@ -188,6 +197,7 @@ int dilution_attend_forward(const void* q, const void* k, const void* v, int dty
   return with_type(dtype, d, [&](auto type, auto dim) {
     if constexpr (!kOnTensorCores<decltype(type), dim()>) return simt_forward<decltype(type), dim()>(a, st);
     else if constexpr (dim() == 128) return tc_forward<128, 1>(a, st);
+    // two query tiles per CTA / one, two CTAs on an SM, n = 64: T = 2048 83 / 71 us, T = 4096 226 / 208, T = 8192 759 / 773
     else return a.docs == nullptr && a.t >= 8192 ? tc_forward<64, 2>(a, st) : tc_forward<64, 1>(a, st);
   });
 }

@@ -57,21 +57,28 @@ __device__ __forceinline__ int pair_state(const Row& r, int i0, int i1, const Do
 }
 
 // ---- forward -----------------------------------------------------------------------------------------
-// What pairs of tiles have to do is asked once per block and kept for this many half tiles from the first on: two bits each, of
-// 32 half tiles in a word: the warp that issues MMAs has to know in a few cycles, it is what all others wait for.
+// What pairs of tiles have to do is asked once per block and kept for this many half tiles from `base` on: two bits each, of 32
+// half tiles in a word: the warp that issues MMAs has to know in a few cycles, it is what all others wait for.
 constexpr int kStates = 4096;
 struct States {
   uint32_t any[kStates / 32], masked[kStates / 32];
+  __device__ __forceinline__ int of(int e) const { return any[e / 32] >> (e & 31) & 1 ? 2 - (masked[e / 32] >> (e & 31) & 1) : 0; }
 };
-// Whole warps, 32 half tiles at a time; f: the state of a half tile, counted from the first.
-template <typename F> __device__ __forceinline__ void keep_states(States* s, int n, int warp, int warps, F f) {
+// Half tiles [base, end); f: the state of one.  The first and the last + 1 that have anything to do into range[0] and range[1].
+template <typename F> __device__ __forceinline__ void keep_states(States* s, int* range, int base, int end, int warp, int warps, F f) {
   const int lane = threadIdx.x & 31;
-  for (int e = 32 * warp; e < min(n, kStates); e += 32 * warps) {
-    const int what = e + lane < n ? f(e + lane) : 0;
+  for (int e = base + 32 * warp; e < end; e += 32 * warps) {
+    const int what = e + lane < end ? f(e + lane) : 0;
     const uint32_t any = __ballot_sync(0xffffffffu, what != 0), masked = __ballot_sync(0xffffffffu, what == 1);
     if (lane == 0) {
-      s->any[e / 32] = any;
-      s->masked[e / 32] = masked;
+      if (e - base < kStates) {
+        s->any[(e - base) / 32] = any;
+        s->masked[(e - base) / 32] = masked;
+      }
+      if (any) {
+        atomicMin(&range[0], e + __ffs(any) - 1);
+        atomicMax(&range[1], e + 32 - __clz(any));
+      }
     }
   }
 }
@@ -279,28 +286,17 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   __syncwarp();
   if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
   __syncthreads();
-  // half tiles [h0, h1) that any of the CTA's queries sees
+  // half tiles [h0, h0 + nh) that any of the CTA's queries sees
   {
-    const int i1 = min(r.t, (ib + NT) * kTileRows) - 1, top = (attend::key_end(r, i1) + 63) / 64;
-    if (r.ranges == nullptr) {
-      if (tid == 0) { s_range[0] = 0; s_range[1] = top; }
-    } else {
-      for (int hh = tid; hh < top; hh += F::kThreads) {
-        bool any = false;
+    const int top = (attend::key_end(r, min(r.t, (ib + NT) * kTileRows) - 1) + 63) / 64;
 #pragma unroll
-        for (int x = 0; x < NT; ++x) any = any || state(x, hh) != 0;
-        if (any) { atomicMin(&s_range[0], hh); atomicMax(&s_range[1], hh + 1); }
-      }
-    }
+    for (int x = 0; x < NT; ++x) keep_states(&s_state[x], s_range, 0, top, warp, F::kThreads / 32, [&](int hh) { return state(x, hh); });
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem);
   const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0;
-#pragma unroll
-  for (int x = 0; x < NT; ++x) keep_states(&s_state[x], nh, warp, F::kThreads / 32, [&](int e) { return state(x, h0 + e); });
-  __syncthreads();
 
   if (warp_u == 8 * NT) {
     // ------------------------------------------------------------ the issuing warp
@@ -325,10 +321,11 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       int in = 0, out = 0, refill = 0;
       uint32_t phase = 0, back = 0, word[NT];
       for (int e = 0; e < nh + 2; ++e) {
-        if ((e & 31) == 0 && e < nh)
+        const int hh = h0 + e;
+        if (((hh & 31) == 0 || e == 0) && e < nh)
 #pragma unroll
           for (int x = 0; x < NT; ++x)
-            word[x] = uniform(e < kStates ? s_state[x].any[e / 32] : __ballot_sync(0xffffffffu, e + lane < nh && state(x, h0 + e + lane) != 0));
+            word[x] = uniform(hh < kStates ? s_state[x].any[hh / 32] : __ballot_sync(0xffffffffu, (hh & ~31) + lane < h0 + nh && state(x, (hh & ~31) + lane) != 0));
         if (e < nh) mbar_wait_warp(kfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
@@ -343,7 +340,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
             for (int kk = 0; kk < 4; ++kk)               // 16 keys per instruction: 16 rows of 128 B = 128 units
               mma_ts(lead, tS + 64, tS + 8 * kk, dV, (HB >> 4) * out + 128 * kk, id_p, 1);
           }
-          if (e < nh && (word[x] >> (e & 31) & 1)) {
+          if (e < nh && (word[x] >> (hh & 31) & 1)) {
             tc_fence_after();
             mma_scores_wide<W>(lead, tS, Desc{dQ.lo + (TB >> 4) * x, dQ.hi}, kTileBytes, Desc{dK.lo + (HB >> 4) * in, dK.hi},
                                HSub, id_s);
@@ -384,9 +381,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     float ref = -INFINITY, s = 0.f;
     int turn = 0;
     for (int e = half; e < nh; e += 2) {
-      const States& z = s_state[tile];
-      const int what = (int)uniform(e >= kStates ? (uint32_t)state(tile, h0 + e)
-                                    : z.any[e / 32] >> (e & 31) & 1 ? 2 - (z.masked[e / 32] >> (e & 31) & 1) : 0u);
+      const int hh = h0 + e, what = (int)uniform(hh < kStates ? s_state[tile].of(hh) : state(tile, hh));
       if (what == 0) continue;
       mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
       ++turn;
@@ -472,13 +467,13 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
 // ---- backward ------------------------------------------------------------------------------------------
 // STAY 0: queries stay (dq), 1: keys stay (dk, dv).  Staying tile: [Q, dout] or [K, V], rows of 128; passing half tiles: [K, V] or
 // [Q, dout], rows of 64, with the passing queries' (lse, delta).
-template <int D, int STAY> struct AttendBackward {
-  static constexpr int kWg = D == 128 && STAY == 1 ? 2 : 3;
-  static constexpr int kThreads = 128 * kWg + 64;
-  static constexpr int kRing = D == 64 ? 6 : STAY == 1 ? 4 : 5;         // one more than are in work, at least
+template <int D, int STAY, int NW> struct AttendBackward {
+  static constexpr int kThreads = 128 * NW + 64;
+  static constexpr int kRing = D == 64 ? (NW == 1 ? 4 : 6) : STAY == 1 ? 4 : 5;         // one more than are in work, at least
   static constexpr uint32_t kTile = Rows<kForm<D>>::kBytes, kHalf = kTile / 2;
   static constexpr int kAcc = STAY == 1 ? 2 * D : D;                     // accumulator columns
-  static_assert(kWg * 128 + kAcc <= 512, "the warpgroups' scores and the accumulators fit TMEM");
+  static_assert(NW * 128 + kAcc <= 512, "the warpgroups' scores and the accumulators fit TMEM");
+  static constexpr int kTmem = NW * 128 + kAcc <= 256 ? 256 : 512, kPerSm = D == 64 && kTmem == 256 ? 2 : 1;
   // staying tiles | passing tiles [ring] x 2 | (lse, delta) [ring][64] | flags [128] | barriers + control
   static constexpr int kOperands = (int)(2 * kTile + 2 * kRing * kHalf);
   static constexpr int kStats = STAY == 1 ? kRing * 512 : 0;
@@ -550,12 +545,12 @@ __device__ __forceinline__ void backward_tile(uint32_t tS, const Row& r, float l
 // grid = rows * ceil(t / 128): dq: batch * heads rows, last queries first; dk, dv: batch * kv_heads rows, first keys first.
 // map_a, map_b: Q and dout (batch * heads rows); map_c, map_d: K and V (batch * kv_heads rows), boxes of 64 rows all.
 // stats: (-lse, -lse, -delta, -delta) of every pair of queries, padded to whole half tiles with -inf and 0.
-template <int D, int STAY, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_backward_kernel(
+template <int D, int STAY, int NW, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendBackward<D, STAY, NW>::kPerSm) attend_backward_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ attend::Args a, const float2* __restrict__ stats) {
-  using F = AttendBackward<D, STAY>;
-  constexpr int W = kForm<D>, R = F::kRing, NW = F::kWg;
+  using F = AttendBackward<D, STAY, NW>;
+  constexpr int W = kForm<D>, R = F::kRing;
   constexpr uint32_t TB = F::kTile, HB = F::kHalf, HSub = kTileBytes / 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
@@ -597,25 +592,16 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
   }
   if (tid < 128) sFlag[tid] = 0;
   __syncwarp();
-  if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), 512);
+  if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
   __syncthreads();
-  {
-    // passing half tiles [h0, h1) of which any sees the tile (or is seen by it)
-    const int lo = STAY == 1 ? attend::first_query(r, y0) / 64 : 0, hi = STAY == 1 ? padded / 64 : (attend::key_end(r, y1) + 63) / 64;
-    if (r.ranges == nullptr) {
-      if (tid == 0) { s_range[0] = lo; s_range[1] = hi; }
-    } else {
-      for (int hh = lo + tid; hh < hi; hh += F::kThreads)
-        if (state(hh) != 0) { atomicMin(&s_range[0], hh); atomicMax(&s_range[1], hh + 1); }
-    }
-  }
+  // passing half tiles [h0, h0 + nh) of which any sees the tile (or is seen by it)
+  const int base = STAY == 1 ? attend::first_query(r, y0) / 64 : 0;
+  keep_states(&s_state, s_range, base, STAY == 1 ? padded / 64 : (attend::key_end(r, y1) + 63) / 64, warp, F::kThreads / 32, state);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem), tAcc = tmem + 128 * NW;
-  const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0, ne = nh * passes;
-  keep_states(&s_state, nh, warp, F::kThreads / 32, [&](int e) { return state(h0 + e); });
-  __syncthreads();
+  const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : base), nh = (int)uniform(s_range[1] > 0 ? s_range[1] : base) - h0, ne = nh * passes;
 
   if (warp_u == 4 * NW) {
     // ------------------------------------------------------------ the warp that issues MMAs
@@ -630,8 +616,10 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
       uint32_t phase = 0, word = 0;
       for (int e = 0; e < ne + NW; ++e) {
         const uint32_t tS = tmem + 128 * w;
-        if ((eh & 31) == 0)
-          word = uniform(eh < kStates ? s_state.any[eh / 32] : __ballot_sync(0xffffffffu, eh + lane < nh && state(h0 + eh + lane) != 0));
+        const int at = h0 - base + eh;
+        if ((at & 31) == 0 || eh == 0)
+          word = uniform(at < kStates ? s_state.any[at / 32]
+                                      : __ballot_sync(0xffffffffu, (at & ~31) + lane < h0 - base + nh && state(base + (at & ~31) + lane) != 0));
         if (pending >> w & 1) {                            // of half tile e - NW
           mbar_wait_warp(pready + 8 * w, flip >> w & 1, ctl, &g_attend_status, kErrWaitTile);
           flip ^= 1u << w;
@@ -653,7 +641,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
         }
         if (e < ne) {
           mbar_wait_warp(bfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
-          if (word >> (eh & 31) & 1) {
+          if (word >> (at & 31) & 1) {
             tc_fence_after();
             mma_scores_wide<W>(lead, tS, dA, kTileBytes, Desc{dB.lo + (HB >> 4) * in, dB.hi}, HSub, id_s);
             mma_scores_wide<W>(lead, tS + 64, Desc{dA.lo + (TB >> 4), dA.hi}, kTileBytes, Desc{dC.lo + (HB >> 4) * in, dC.hi}, HSub,
@@ -710,9 +698,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
     for (int e = wg; e < ne; e += NW, eh += NW) {
       while (eh >= nh) { eh -= nh; ++pass; }
       if (STAY == 1 && BIAS) r.slope2 = a.slopes[head * group + pass] * kLog2e;
-      const int hh = h0 + eh;
-      const int what = (int)uniform(eh >= kStates ? (uint32_t)state(hh)
-                                    : s_state.any[eh / 32] >> (eh & 31) & 1 ? 2 - (s_state.masked[eh / 32] >> (eh & 31) & 1) : 0u);
+      const int hh = h0 + eh, what = (int)uniform(hh - base < kStates ? s_state.of(hh - base) : state(hh));
       if (what == 0) continue;
       mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
       ++turn;
@@ -762,7 +748,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY>::kThreads, 1) attend_b
   drain_if_aborted(ctl);
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) tmem_free(tmem, 512);
+  if (warp == 0) tmem_free(tmem, F::kTmem);
 }
 
 // lse and delta_i = dout_i . out_i of every query, padded, as the kernels above read them.  D / 8 lanes a row, 16 bytes each.
