@@ -3,6 +3,9 @@
 // holds the scores of rows 4 ty .. 4 ty + 3 and columns tx, tx + 16, .. of a tile, and the accumulators of its rows and
 // features tx, tx + 16, ..  Operand tiles lie in shared memory in fp32 with rows of D + 4 words, so that the 16 rows
 // that a half warp reads at a time start in different banks.  Tiles without a visible pair are passed over.
+// Calls of few blocks share each block between the CTAs of a cluster: every `ranks`-th tile is a CTA's, and what they have
+// accumulated is joined through distributed shared memory, in the ranks' order, each rank finishing a part of the rows.
+// One sequence of 301 tokens, 4 heads of 64 (2 key heads), fp32, forward / dk, dv / dq: 38 / 95 / 38 us by one CTA a block.
 #pragma once
 
 #include "attend_common.cuh"
@@ -79,16 +82,41 @@ __device__ __forceinline__ float max16(float v) {
   return v;
 }
 
+// Accumulators [4][D / 16] of a thread into a [64][D + 4] tile.
+template <int D> __device__ __forceinline__ void put_tile(float* dst, int ty, int tx, const float acc[4][D / 16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) dst[(4 * ty + i) * (D + 4) + tx + 16 * c] = acc[i][c];
+}
+// The rows' sums over the ranks of element x of their tiles.
+__device__ __forceinline__ float over_ranks(const float* x, int ranks) {
+  if (ranks == 1) return *x;
+  float s = 0.f;
+  for (int r = 0; r < ranks; ++r) s += ld_cluster(x, r);
+  return s;
+}
+__device__ __forceinline__ void meet(int ranks) {
+  if (ranks > 1) cluster_sync(); else __syncthreads();
+}
+// f(row) by whole warps for the rank's rows whose flag is set; a row's flag is its thread block's own.
+template <typename F> __device__ __forceinline__ void each_flagged(const int* flag, int first, int last, F f) {
+  __syncthreads();
+  for (int row = first + (int)(threadIdx.x >> 5); row < last; row += kSimtThreads / 32)
+    if (flag[row]) f(row);
+}
+
 template <int D> constexpr int simt_smem(int tiles) { return 4 * (tiles * kTile * (D + 4) + kTile * (kTile + 4)); }
 
-// grid = batch * heads * ceil(t / 64), last query tiles (the longest) first.
+// grid = ranks * batch * heads * ceil(t / 64), last query tiles (the longest) first.
 template <typename T, int D>
-__global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a) {
+__global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a, int ranks) {
   extern __shared__ float sm[];
   float *sQ = sm, *sK = sQ + kTile * (D + 4), *sV = sK + kTile * (D + 4), *sP = sV + kTile * (D + 4);
   const int tiles = (a.t + kTile - 1) / kTile, heads = a.batch * a.heads;
-  const int64_t n = blockIdx.x % heads;
-  const int i0 = (tiles - 1 - (int)(blockIdx.x / heads)) * kTile;
+  const int rank = blockIdx.x % ranks, block = blockIdx.x / ranks;
+  const int64_t n = block % heads;
+  const int i0 = (tiles - 1 - block / heads) * kTile;
   const int b = (int)(n / a.heads), h = (int)(n % a.heads);
   const int64_t nk = (int64_t)b * a.kv_heads + h / (a.heads / a.kv_heads);
   const Row r = make_row(a, b, h);
@@ -105,8 +133,9 @@ __global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a) {
     for (int c = 0; c < D / 16; ++c) o[i][c] = 0.f;
   }
   const int end = key_end(r, min(i0 + kTile, a.t) - 1);
+  int turn = 0;
   for (int j0 = 0; j0 < end; j0 += kTile) {
-    if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1)) continue;
+    if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1) || turn++ % ranks != rank) continue;
     __syncthreads();
     load_tile<T, D>(sK, k, j0, a.t);
     load_tile<T, D>(sV, v, j0, a.t);
@@ -141,33 +170,50 @@ __global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a) {
     __syncwarp();                    // a row's 16 threads are one half warp: P is handed over within it
     tile_accumulate<D>(sP, sV, ty, tx, o);
   }
-  bool bad = false;
+  // [64] maxima, sums and flags over P, the accumulator over K
+  __syncthreads();
+  float *sM = sP, *sL = sP + kTile;
+  int* sFlag = reinterpret_cast<int*>(sP + 2 * kTile);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int qi = i0 + 4 * ty + i;
-    const float sum = sum16(l[i]), inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (qi >= a.t) continue;
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      const float x = o[i][c] * inv;
-      bad = bad || !isfinite(x);
-      reinterpret_cast<T*>(a.out)[(n * a.t + qi) * D + tx + 16 * c] = from_f32<T>(x);
+    const float sum = sum16(l[i]);
+    if (tx == 0) {
+      sM[4 * ty + i] = m[i];
+      sL[4 * ty + i] = sum;
+      sFlag[4 * ty + i] = 0;
     }
-    if (a.lse != nullptr && tx == 0) a.lse[n * a.t + qi] = sum == 0.f ? INFINITY : m[i] + log2f(sum);
   }
-  if (__any_sync(0xffffffffu, bad))          // the 8 rows of this warp
-    for (int x = 0; x < 8; ++x)
-      if (i0 + 8 * (tid >> 5) + x < a.t) redo_forward_row<T, D>(a, b, h, i0 + 8 * (tid >> 5) + x);
+  put_tile<D>(sK, ty, tx, o);
+  meet(ranks);
+  const int part = kTile / ranks, first = rank * part, last = min(first + part, a.t - i0);
+  for (int x = tid; x < (last - first) * D; x += kSimtThreads) {
+    const int row = first + x / D, c = x % D;
+    float top = -INFINITY, sum = 0.f, acc = 0.f;
+    for (int y = 0; y < ranks; ++y) top = fmaxf(top, ranks == 1 ? sM[row] : ld_cluster(sM + row, y));
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int y = 0; y < ranks; ++y) {
+      const float f = exp2f((ranks == 1 ? sM[row] : ld_cluster(sM + row, y)) - ref);
+      sum = fmaf(ranks == 1 ? sL[row] : ld_cluster(sL + row, y), f, sum);
+      acc = fmaf(ranks == 1 ? sK[row * (D + 4) + c] : ld_cluster(sK + row * (D + 4) + c, y), f, acc);
+    }
+    const float out = sum == 0.f ? 0.f : acc / sum;
+    if (!isfinite(out)) sFlag[row] = 1;
+    reinterpret_cast<T*>(a.out)[(n * a.t + i0 + row) * D + c] = from_f32<T>(out);
+    if (a.lse != nullptr && c == 0) a.lse[n * a.t + i0 + row] = sum == 0.f ? INFINITY : top + log2f(sum);
+  }
+  each_flagged(sFlag, first, last, [&](int row) { redo_forward_row<T, D>(a, b, h, i0 + row); });
+  meet(ranks);                       // no CTA leaves while another may read its sums
 }
 
 // dq.  grid as above.
 template <typename T, int D>
-__global__ void __launch_bounds__(kSimtThreads) simt_dq_kernel(Args a) {
+__global__ void __launch_bounds__(kSimtThreads) simt_dq_kernel(Args a, int ranks) {
   extern __shared__ float sm[];
   float *sQ = sm, *sG = sQ + kTile * (D + 4), *sX = sG + kTile * (D + 4), *sP = sX + kTile * (D + 4);
   const int tiles = (a.t + kTile - 1) / kTile, heads = a.batch * a.heads;
-  const int64_t n = blockIdx.x % heads;
-  const int i0 = (tiles - 1 - (int)(blockIdx.x / heads)) * kTile;
+  const int rank = blockIdx.x % ranks, block = blockIdx.x / ranks;
+  const int64_t n = block % heads;
+  const int i0 = (tiles - 1 - block / heads) * kTile;
   const int b = (int)(n / a.heads), h = (int)(n % a.heads);
   const int64_t nk = (int64_t)b * a.kv_heads + h / (a.heads / a.kv_heads);
   const Row r = make_row(a, b, h);
@@ -184,8 +230,9 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dq_kernel(Args a) {
     for (int c = 0; c < D / 16; ++c) dq[i][c] = 0.f;
   }
   const int end = key_end(r, min(i0 + kTile, a.t) - 1);
+  int turn = 0;
   for (int j0 = 0; j0 < end; j0 += kTile) {
-    if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1)) continue;
+    if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1) || turn++ % ranks != rank) continue;
     float s[4][4], g[4][4];
     __syncthreads();
     load_tile<T, D>(sX, row_ptr<T>(a.v, nk, a.t, D), j0, a.t);
@@ -211,32 +258,32 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dq_kernel(Args a) {
     __syncwarp();
     tile_accumulate<D>(sP, sX, ty, tx, dq);
   }
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int qi = i0 + 4 * ty + i;
-    if (qi >= a.t) continue;
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      const float x = dq[i][c] * a.scale;
-      bad = bad || !isfinite(x);
-      reinterpret_cast<T*>(a.dq)[(n * a.t + qi) * D + tx + 16 * c] = from_f32<T>(x);
-    }
+  __syncthreads();
+  int* sFlag = reinterpret_cast<int*>(sP);
+  if (tid < kTile) sFlag[tid] = 0;
+  put_tile<D>(sX, ty, tx, dq);
+  meet(ranks);
+  const int part = kTile / ranks, first = rank * part, last = min(first + part, a.t - i0);
+  for (int x = tid; x < (last - first) * D; x += kSimtThreads) {
+    const int row = first + x / D, c = x % D;
+    const float y = over_ranks(sX + row * (D + 4) + c, ranks) * a.scale;
+    if (!isfinite(y)) sFlag[row] = 1;
+    reinterpret_cast<T*>(a.dq)[(n * a.t + i0 + row) * D + c] = from_f32<T>(y);
   }
-  if (__any_sync(0xffffffffu, bad))
-    for (int x = 0; x < 8; ++x)
-      if (i0 + 8 * (tid >> 5) + x < a.t) redo_dq_row<T, D>(a, b, h, i0 + 8 * (tid >> 5) + x);
+  each_flagged(sFlag, first, last, [&](int row) { redo_dq_row<T, D>(a, b, h, i0 + row); });
+  meet(ranks);
 }
 
 // dk and dv of 64 keys of a key head, over all queries of the heads that share it.  Rows of a tile are keys here.
-// grid = batch * kv_heads * ceil(t / 64), first key tiles (the longest) first.
+// grid = ranks * batch * kv_heads * ceil(t / 64), first key tiles (the longest) first.
 template <typename T, int D>
-__global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a) {
+__global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a, int ranks) {
   extern __shared__ float sm[];
   float *sK = sm, *sV = sK + kTile * (D + 4), *sX = sV + kTile * (D + 4), *sP = sX + kTile * (D + 4);
   const int heads = a.batch * a.kv_heads, group = a.heads / a.kv_heads;
-  const int64_t nk = blockIdx.x % heads;
-  const int j0 = (int)(blockIdx.x / heads) * kTile;
+  const int rank = blockIdx.x % ranks, block = blockIdx.x / ranks;
+  const int64_t nk = block % heads;
+  const int j0 = block / heads * kTile;
   const int b = (int)(nk / a.kv_heads), hk = (int)(nk % a.kv_heads);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   load_tile<T, D>(sK, row_ptr<T>(a.k, nk, a.t, D), j0, a.t);
@@ -246,11 +293,12 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a) {
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
+  int turn = 0;
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     const Row r = make_row(a, b, h);
     const int64_t n = (int64_t)b * a.heads + h;
     for (int i0 = first_query(r, j0) / kTile * kTile; i0 < a.t; i0 += kTile) {
-      if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1)) continue;
+      if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1) || turn++ % ranks != rank) continue;
       float s[4][4], g[4][4];
       const bool full = tile_full(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1);
       __syncthreads();
@@ -290,22 +338,22 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a) {
       tile_accumulate<D>(sP, sX, ty, tx, dk);
     }
   }
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int kj = j0 + 4 * ty + i;
-    if (kj >= a.t) continue;
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      const float x = dk[i][c] * a.scale, y = dv[i][c];
-      bad = bad || !isfinite(x) || !isfinite(y);
-      reinterpret_cast<T*>(a.dk)[(nk * a.t + kj) * D + tx + 16 * c] = from_f32<T>(x);
-      reinterpret_cast<T*>(a.dv)[(nk * a.t + kj) * D + tx + 16 * c] = from_f32<T>(y);
-    }
+  __syncthreads();
+  int* sFlag = reinterpret_cast<int*>(sP);
+  if (tid < kTile) sFlag[tid] = 0;
+  put_tile<D>(sK, ty, tx, dk);
+  put_tile<D>(sV, ty, tx, dv);
+  meet(ranks);
+  const int part = kTile / ranks, first = rank * part, last = min(first + part, a.t - j0);
+  for (int x = tid; x < (last - first) * D; x += kSimtThreads) {
+    const int row = first + x / D, c = x % D;
+    const float y = over_ranks(sK + row * (D + 4) + c, ranks) * a.scale, z = over_ranks(sV + row * (D + 4) + c, ranks);
+    if (!isfinite(y) || !isfinite(z)) sFlag[row] = 1;
+    reinterpret_cast<T*>(a.dk)[(nk * a.t + j0 + row) * D + c] = from_f32<T>(y);
+    reinterpret_cast<T*>(a.dv)[(nk * a.t + j0 + row) * D + c] = from_f32<T>(z);
   }
-  if (__any_sync(0xffffffffu, bad))
-    for (int x = 0; x < 8; ++x)
-      if (j0 + 8 * (tid >> 5) + x < a.t) redo_dkv_row<T, D>(a, b, hk, j0 + 8 * (tid >> 5) + x);
+  each_flagged(sFlag, first, last, [&](int row) { redo_dkv_row<T, D>(a, b, hk, j0 + row); });
+  meet(ranks);
 }
 
 }  // namespace attend

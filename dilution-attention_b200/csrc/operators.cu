@@ -45,13 +45,31 @@ int launch_ranges(const attend::Args& a, cudaStream_t st) {
   return abi_check_launch("attend_ranges");
 }
 
+// CTAs that share a block of `stream` tiles: until every SM has one, or each has two tiles.
+template <typename K> int launch_shared(K kernel, const char* name, int64_t blocks, int64_t stream, int smem, const attend::Args& a,
+                                        cudaStream_t st) {
+  int ranks = 1;
+  while (ranks < 8 && blocks * ranks < 148 && stream >= 2 * ranks) ranks *= 2;
+  if (int rc = opt_in(kernel, smem)) return rc;
+  LaunchMark mark(name, st);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ranks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(blocks * ranks));
+  cfg.blockDim = dim3(attend::kSimtThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, ranks);
+  return e == cudaSuccess ? DILUTION_OK : abi_fail(DILUTION_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+}
+
 template <typename T, int D> int simt_forward(const attend::Args& a, cudaStream_t st) {
-  constexpr int smem = attend::simt_smem<D>(3);
-  if (int rc = opt_in(attend::simt_forward_kernel<T, D>, smem)) return rc;
-  LaunchMark mark("attend_forward", st);
-  const unsigned grid = (unsigned)((int64_t)a.batch * a.heads * doc_spans(a.t));
-  attend::simt_forward_kernel<T, D><<<grid, attend::kSimtThreads, smem, st>>>(a);
-  return abi_check_launch("attend_forward");
+  return launch_shared(attend::simt_forward_kernel<T, D>, "attend_forward", (int64_t)a.batch * a.heads * doc_spans(a.t), doc_spans(a.t),
+                       attend::simt_smem<D>(3), a, st);
 }
 
 template <typename T, int D> int launch_delta(const attend::Args& a, cudaStream_t st) {
@@ -64,18 +82,9 @@ template <typename T, int D> int launch_delta(const attend::Args& a, cudaStream_
 template <typename T, int D> int simt_backward(const attend::Args& a, cudaStream_t st) {
   constexpr int smem = attend::simt_smem<D>(3);
   if (int rc = launch_delta<T, D>(a, st)) return rc;
-  if (int rc = opt_in(attend::simt_dq_kernel<T, D>, smem)) return rc;
-  if (int rc = opt_in(attend::simt_dkv_kernel<T, D>, smem)) return rc;
-  {
-    LaunchMark mark("attend_dkv", st);
-    const unsigned grid = (unsigned)((int64_t)a.batch * a.kv_heads * doc_spans(a.t));
-    attend::simt_dkv_kernel<T, D><<<grid, attend::kSimtThreads, smem, st>>>(a);
-    if (int rc = abi_check_launch("attend_dkv")) return rc;
-  }
-  LaunchMark mark("attend_dq", st);
-  const unsigned grid = (unsigned)((int64_t)a.batch * a.heads * doc_spans(a.t));
-  attend::simt_dq_kernel<T, D><<<grid, attend::kSimtThreads, smem, st>>>(a);
-  return abi_check_launch("attend_dq");
+  if (int rc = launch_shared(attend::simt_dkv_kernel<T, D>, "attend_dkv", (int64_t)a.batch * a.kv_heads * doc_spans(a.t),
+                             doc_spans(a.t) * (a.heads / a.kv_heads), smem, a, st)) return rc;
+  return launch_shared(attend::simt_dq_kernel<T, D>, "attend_dq", (int64_t)a.batch * a.heads * doc_spans(a.t), doc_spans(a.t), smem, a, st);
 }
 
 // ---- the same on the tensor cores

@@ -297,6 +297,8 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem);
   const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0;
+  // nearest keys first: a distance bias has the largest scores there, and later half tiles do not move the reference
+  const int last = h0 + nh - 1;
 
   if (warp_u == 8 * NT) {
     // ------------------------------------------------------------ the issuing warp
@@ -305,8 +307,8 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     auto load_keys = [&](int e, int st) {
       if (!lead) return;
       mbar_expect_tx(kfull + 8 * st, 2 * HB);
-      tma_load_rows<W>(sK + HB * st, &map_k, (h0 + e) * 64, nk, kfull + 8 * st, HSub);
-      tma_load_rows<W>(sV + HB * st, &map_v, (h0 + e) * 64, nk, kfull + 8 * st, HSub);
+      tma_load_rows<W>(sK + HB * st, &map_k, (last - e) * 64, nk, kfull + 8 * st, HSub);
+      tma_load_rows<W>(sV + HB * st, &map_v, (last - e) * 64, nk, kfull + 8 * st, HSub);
     };
     const int tiles = NT == 2 && (ib + 1) * kTileRows < r.t ? 2 : 1;
     if (nh > 0) {
@@ -321,8 +323,8 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       int in = 0, out = 0, refill = 0;
       uint32_t phase = 0, back = 0, word[NT];
       for (int e = 0; e < nh + 2; ++e) {
-        const int hh = h0 + e;
-        if (((hh & 31) == 0 || e == 0) && e < nh)
+        const int hh = last - e;
+        if (((hh & 31) == 31 || e == 0) && e < nh)
 #pragma unroll
           for (int x = 0; x < NT; ++x)
             word[x] = uniform(hh < kStates ? s_state[x].any[hh / 32] : __ballot_sync(0xffffffffu, (hh & ~31) + lane < h0 + nh && state(x, (hh & ~31) + lane) != 0));
@@ -381,12 +383,12 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     float ref = -INFINITY, s = 0.f;
     int turn = 0;
     for (int e = half; e < nh; e += 2) {
-      const int hh = h0 + e, what = (int)uniform(hh < kStates ? s_state[tile].of(hh) : state(tile, hh));
+      const int hh = last - e, what = (int)uniform(hh < kStates ? s_state[tile].of(hh) : state(tile, hh));
       if (what == 0) continue;
       mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
       ++turn;
       tc_fence_after();
-      forward_step<D, CAP, BIAS>(tS, tO, r, lin, pre, (h0 + e) * 64, is, what == 1, ref, s);
+      forward_step<D, CAP, BIAS>(tS, tO, r, lin, pre, hh * 64, is, what == 1, ref, s);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(pready + 8 * wg);

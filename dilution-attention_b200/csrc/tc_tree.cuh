@@ -61,16 +61,17 @@ template <int RK, int RV, int NB> struct StreamBars {
   }
 };
 
-// The warp that copies tiles [first, first + ne) of KT keys and (if V) their values.
+// The warp that copies ne tiles of KT keys and (if V) their values, from tile `last` down: a distance bias has the largest scores
+// there, and later tiles do not move a row's reference.
 template <int D, int KT, int RK, int RV, int NB, bool V>
 __device__ __forceinline__ void stream_tiles(const StreamBars<RK, RV, NB>& bars, const CUtensorMap* map_k, const CUtensorMap* map_v,
-                                             uint32_t ring_k, uint32_t ring_v, int first, int ne, int nk, uint32_t lead) {
+                                             uint32_t ring_k, uint32_t ring_v, int last, int ne, int nk, uint32_t lead) {
   constexpr uint32_t kOne = KT * D * 2;
   auto copy = [&](const CUtensorMap* map, uint32_t dst, int e, uint32_t bar) {
     if (lead) {
       mbar_expect_tx(bar, kOne);
 #pragma unroll
-      for (int x = 0; x < KT / 64; ++x) tma_load_rows<kForm<D>>(dst + 8192 * x, map, (first + e) * KT + 64 * x, nk, bar, KT * 128);
+      for (int x = 0; x < KT / 64; ++x) tma_load_rows<kForm<D>>(dst + 8192 * x, map, (last - e) * KT + 64 * x, nk, bar, KT * 128);
     }
     __syncwarp();
   };
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
   const int nk = blockIdx.z, b = nk / a.kv_heads, hk = nk % a.kv_heads, rows = a.group * a.nodes, r0 = blockIdx.y * 128;
   const int len = (int)uniform(tree::cache_len(a.pos_dev, a.len, a.capacity));
   const int2 keys = tree::chunk_keys(len, a.chunks, blockIdx.x, KT);
-  const int first = keys.x / KT, ne = (keys.y - keys.x + KT - 1) / KT;
+  const int ne = (keys.y - keys.x + KT - 1) / KT, last = keys.x / KT + ne - 1;
 
   if (tid == 0) bars.init();
   // the rows between zeros
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
     tc_fence_after();
     for (int e = 0; e < ne + NB - 1; ++e) {
       if (e < ne) {
-        const int st = e % RK, from = len - (first + e) * KT;
+        const int st = e % RK, from = len - (last - e) * KT;
         const uint32_t tS = tmem + NC * (e % NB);
         mbar_wait_warp(bars.kfull + 8 * st, (e / RK) & 1, ctl, &g_tree_status, kErrWaitTma);
         if (from < KT) {
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
         tc_fence_after();
         if (OUT) {
           mbar_wait_warp(bars.vfull + 8 * st, (y / RV) & 1, ctl, &g_tree_status, kErrWaitTma);
-          const int from = len - (first + y) * KT;
+          const int from = len - (last - y) * KT;
           if (from < KT) {
             zero_rows(smem + F::kBuf + F::kOne * (RK + st), KT, from, SUB);
             fence_async_smem();
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
     mma_commit(lead, bars.alldone);
     __syncwarp();
   } else if (warp_u == 4 * NW + 1) {
-    stream_tiles<D, KT, RK, RV, NB, OUT>(bars, &map_k, &map_v, ring_k, ring_v, first, ne, nk, lead);
+    stream_tiles<D, KT, RK, RV, NB, OUT>(bars, &map_k, &map_v, ring_k, ring_v, last, ne, nk, lead);
   } else {
     // ------------------------------------------------------------ the compute warps: lane = row of a group
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tP = tmem + NC * NB + F::kWgCols * wg + lanes, tO = tP + 64;
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
     }
     float ref = -INFINITY, s = 0.f;
     for (int e = wg; e < ne; e += NW) {
-      const int j0 = (first + e) * KT + NC * g;
+      const int j0 = (last - e) * KT + NC * g;
       mbar_wait_warp(bars.sdone + 8 * (e % NB), (e / NB) & 1, ctl, &g_tree_status, kErrWaitMma);
       // the product of the warpgroup's last tile has read its P~
       if (OUT && e >= NW) mbar_wait_warp(bars.used + 8 * wg, (e / NW - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
   const int rows = DILUTE ? a.nodes : a.group * acc.accepted;
   const int len = (int)uniform(tree::cache_len(a.pos_dev, a.len, a.capacity));
   const int2 keys = tree::chunk_keys(len, a.chunks, blockIdx.x, KT);
-  const int first = keys.x / KT, ne = (keys.y - keys.x + KT - 1) / KT;
+  const int ne = (keys.y - keys.x + KT - 1) / KT, last = keys.x / KT + ne - 1;
 
   if (tid == 0) bars.init();
   tree::make_lineage(&lineage, a.parents + b * a.parent_stride, a.nodes);
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
     const Desc dOnes = make_desc(sOnes, 2048, 1024);
     for (int e = 0; e < ne + NB - 1; ++e) {
       if (e < ne) {
-        const int st = e % RK, from = len - (first + e) * KT;
+        const int st = e % RK, from = len - (last - e) * KT;
         const uint32_t tS = tmem + 64 * (e % NB);
         mbar_wait_warp(bars.kfull + 8 * st, (e / RK) & 1, ctl, &g_tree_status, kErrWaitTma);
         if (from < KT) {
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
         tc_fence_after();
         if (DILUTE) {
           mbar_wait_warp(bars.vfull + 8 * st, (y / RV) & 1, ctl, &g_tree_status, kErrWaitTma);
-          const int from = len - (first + y) * KT;
+          const int from = len - (last - y) * KT;
           if (from < KT) {
             zero_rows(smem + kQ + F::kOne * (RK + st), KT, from, SUB);
             fence_async_smem();
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
     mma_commit(lead, bars.alldone);
     __syncwarp();
   } else if (warp_u == 9) {
-    stream_tiles<D, KT, RK, RV, NB, DILUTE>(bars, &map_k, &map_v, ring_k, ring_v, first, ne, nk, lead);
+    stream_tiles<D, KT, RK, RV, NB, DILUTE>(bars, &map_k, &map_v, ring_k, ring_v, last, ne, nk, lead);
   } else {
     // ------------------------------------------------------------ the compute warps: lane = key
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
     const float lin = cap ? a.cap * kLog2e : a.scale * kLog2e, pre = cap ? a.scale / a.cap : 0.f;
     const uint64_t jumps = walk[0], keeps = walk[1];
     for (int e = wg; e < ne; e += 2) {
-      const int j = (first + e) * KT + row;
+      const int j = (last - e) * KT + row;
       const bool live = j < len;
       const int64_t at = (int64_t)nk * a.capacity + j;
       const float base = live ? a.committed[at] : 0.f;
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
       // the product of the warpgroup's last tile has read its shares
       if (DILUTE && e >= 2) mbar_wait_warp(bars.used + 8 * wg, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
       tc_fence_after();
-      float last = base, total = base;
+      float left = base, total = base;
 #pragma unroll
       for (int c0 = 0; c0 < N; c0 += 16) {
         if (c0 >= rows) break;
@@ -565,15 +566,15 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
           for (int y = 0; y < 16; ++y) {
             if (jumps >> (c0 + y) & 1) {
               const int up = step[c0 + y].up;
-              last = base;
+              left = base;
               if (up >= 0) {
                 tmem_st_wait();
-                tmem_ld1(tS + up, &last);
-                tmem_ld_wait1(&last);
+                tmem_ld1(tS + up, &left);
+                tmem_ld_wait1(&left);
               }
             }
-            d[y] = last = last + v[y];
-            if (keeps >> (c0 + y) & 1) tmem_st1(tS + c0 + y, last);
+            d[y] = left = left + v[y];
+            if (keeps >> (c0 + y) & 1) tmem_st1(tS + c0 + y, left);
           }
 #pragma unroll
           for (int y = 0; y < 16; ++y) v[y] *= fast_rcp(d[y] + a.eps);

@@ -275,18 +275,29 @@ __global__ void __launch_bounds__(kThreads) simt_dilute_kernel(Args a) {
       for (int j = 0; j < 4; ++j) w.s.p[(w.ty + 16 * i) * (kKeys + 4) + w.tx + 16 * j] = exp2f(z[i][j] - lse[i]);
     }
     __syncthreads();
+    // the demand behind every node, by one thread per key; then the shares, by all
     if (threadIdx.x < kKeys) {
       const int key = threadIdx.x, j = j0 + key;
       const float base = j < w.len ? a.committed[w.nk * a.capacity + j] : 0.f;
+      float left = base;
+#pragma unroll 4
       for (int x = 0; x < a.nodes; ++x) {
         const int up = w.s.tree.parent[x];
-        float& bid = w.s.p[x * (kKeys + 4) + key];
-        const float had = up >= 0 ? w.s.had[up * (kKeys + 4) + key] : base, p = bid;
-        w.s.had[x * (kKeys + 4) + key] = had + p;
-        // (a node that does not see the key has no share of it, whatever the demand is)
-        bid = p == 0.f ? 0.f : p / (had + p + a.eps);
+        if (up != x - 1 || up < 0) left = up >= 0 ? w.s.had[up * (kKeys + 4) + key] : base;
+        left += w.s.p[x * (kKeys + 4) + key];
+        w.s.had[x * (kKeys + 4) + key] = left;
       }
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = (w.ty + 16 * i) * (kKeys + 4) + w.tx + 16 * j;
+        const float p = w.s.p[at];
+        // (a node that does not see the key has no share of it, whatever the demand is)
+        if (row(w.ty + 16 * i) >= 0) w.s.p[at] = p == 0.f ? 0.f : p / (w.s.had[at] + a.eps);
+      }
     w.keys(true, j0, range.y, node);
 #pragma unroll
     for (int i = 0; i < RI; ++i)

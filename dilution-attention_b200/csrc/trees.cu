@@ -15,9 +15,9 @@ int trees_read_status(int* code) { return read_status_word(tc::g_tree_status, co
 
 namespace {
 
-// Parts that a key head's keys are cut into.  fp32 FMAs: enough blocks for four on every SM, of 256 keys at least.
+// Parts that a key head's keys are cut into.  fp32 FMAs: enough blocks for four on every SM, of 128 keys at least.
 int simt_chunks(int64_t blocks, int64_t keys) {
-  const int64_t want = (148 * 4 + blocks - 1) / std::max<int64_t>(blocks, 1), most = (keys + 255) / 256;
+  const int64_t want = (148 * 4 + blocks - 1) / std::max<int64_t>(blocks, 1), most = (keys + 127) / 128;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 512}));
 }
 // Tensor cores: as many parts as make the fewest rounds of tiles of 128 keys on the chip's SMs, where a block's start and end take as
