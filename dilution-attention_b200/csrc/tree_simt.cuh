@@ -3,7 +3,7 @@
 // 256 threads walk a chunk of a key head's keys in tiles of 64; 16 RI of its rows are held at a time: thread
 // (ty, tx) = (tid / 16, tid % 16) has rows ty + 16 i and keys tx + 16 j of a tile.  A step's chunks are joined by
 // join_kernel.  What bounds them is the cache's bytes: at RI = 1 a tile of 64 keys takes 16 x 64 x D x 2 FMAs, which the
-// SM does in less time than its share of the memory system needs for the tile; RI = 4 is bound by the FMAs.
+// SM does in less time than its share of the memory system needs for the tile; from RI = 2 on the FMAs are the bound.
 #pragma once
 
 #include "tree_common.cuh"
@@ -103,6 +103,11 @@ template <typename T, int D, int RI> struct Walker {
   }
   // The scores of row r (node % nodes) against the tile's keys from j0 on; -inf where it does not see the key.
   __device__ void scores(int r, int j0, float z[4]) {
+    if (j0 + kKeys <= len && a.cap == 0.f && a.slopes == nullptr) {       // (rows behind the last go nowhere)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[j] *= a.scale * kLog2e;
+      return;
+    }
     const int x = r >= 0 ? r % a.nodes : 0, h = hk * a.group + (r >= 0 ? r / a.nodes : 0);
     const float slope2 = a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
     const int at = s.tree.depth[x];
@@ -172,12 +177,12 @@ __global__ void __launch_bounds__(kThreads) simt_softmax_kernel(Args a) {
     for (int i = 0; i < RI; ++i) {
       w.scores(row(w.ty + 16 * i), j0, z[i]);
       const float top = fmaxf(m[i], max16(fmaxf(fmaxf(z[i][0], z[i][1]), fmaxf(z[i][2], z[i][3]))));
-      const float ref = top == -INFINITY ? 0.f : top, f = exp2f(m[i] - ref);
+      const float ref = top == -INFINITY ? 0.f : top, f = fast_exp2(m[i] - ref);
       m[i] = top;
       l[i] *= f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = exp2f(z[i][j] - ref);
+        const float p = fast_exp2(z[i][j] - ref);
         l[i] += p;
         if (OUT) w.s.p[(w.ty + 16 * i) * (kKeys + 4) + w.tx + 16 * j] = p;
       }
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) simt_dilute_kernel(Args a) {
     for (int i = 0; i < RI; ++i) {
       w.scores(row(w.ty + 16 * i), j0, z[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w.s.p[(w.ty + 16 * i) * (kKeys + 4) + w.tx + 16 * j] = exp2f(z[i][j] - lse[i]);
+      for (int j = 0; j < 4; ++j) w.s.p[(w.ty + 16 * i) * (kKeys + 4) + w.tx + 16 * j] = fast_exp2(z[i][j] - lse[i]);
     }
     __syncthreads();
     // the demand behind every node, by one thread per key; then the shares, by all
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) simt_advance_kernel(Args a, Accept c
         w.scores(r, j0, z[i]);
         const float lse = r >= 0 ? a.lse[w.nk * w.rows + r] : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += exp2f(z[i][j] - lse);
+        for (int j = 0; j < 4; ++j) sum[j] += r >= 0 ? fast_exp2(z[i][j] - lse) : 0.f;
       }
     }
     // the 16 rows of threads, one after the other: the order is fixed

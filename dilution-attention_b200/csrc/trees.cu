@@ -37,7 +37,7 @@ int tc_chunks(int64_t blocks, int64_t keys, int per_sm) {
   return chunks;
 }
 int row_blocks(int rows, int of) { return (rows + of - 1) / of; }
-int simt_row_blocks(int rows) { return rows <= 16 ? 1 : row_blocks(rows, 64); }
+int simt_row_blocks(int rows) { return row_blocks(rows, 64); }
 
 template <typename T, int D> constexpr bool kOnTensorCores = std::is_same<T, __nv_bfloat16>::value && (D == 64 || D == 128);
 
@@ -105,6 +105,14 @@ float* place_scratch(tree::Args& a, void* scratch, int d) {
   a.psum = (float*)(p + s.psum);
   a.pout = (float*)(p + s.pout);
   return (float*)(p + s.shares);
+}
+
+// f(integral_constant<int, RI>()): the fewest rows of 16 that hold `rows` of them, four at most.
+template <typename F> int with_rows(int rows, F f) {
+  if (rows <= 16) return f(std::integral_constant<int, 1>());
+  if (rows <= 32) return f(std::integral_constant<int, 2>());
+  if (rows <= 48) return f(std::integral_constant<int, 3>());
+  return f(std::integral_constant<int, 4>());
 }
 
 template <typename T, int D, int RI, bool OUT> int simt_softmax(const tree::Args& a, cudaStream_t st) {
@@ -254,7 +262,7 @@ int dilution_tree_softmax(const void* q, const void* k_new, const void* v_new, c
     else {
     a.chunks = simt_chunks((int64_t)a.batch * a.kv_heads * simt_row_blocks(rows), tree_keys(a));
     place_scratch(a, scratch, d);
-    if (int rc = rows <= 16 ? simt_softmax<T, dim(), 1, true>(a, st) : simt_softmax<T, dim(), 4, true>(a, st)) return rc;
+    if (int rc = with_rows(rows, [&](auto ri) { return simt_softmax<T, dim(), ri(), true>(a, st); })) return rc;
     return join<T, false>(a, d, st);
     }
   });
@@ -279,14 +287,14 @@ int dilution_tree_dilute(const void* q, const void* k_new, const void* v_new, co
     else {
     a.chunks = simt_chunks((int64_t)a.batch * a.kv_heads * simt_row_blocks(nodes), tree_keys(a));
     place_scratch(a, scratch, d);
-    if (int rc = nodes <= 16 ? simt_softmax<T, dim(), 1, false>(a, st) : simt_softmax<T, dim(), 4, false>(a, st)) return rc;
+    if (int rc = with_rows(nodes, [&](auto ri) { return simt_softmax<T, dim(), ri(), false>(a, st); })) return rc;
     {
       LaunchMark mark("tree_join_stats", st);
       const int64_t all = (int64_t)a.batch * a.kv_heads * nodes;
       tree::join_stats_kernel<<<(unsigned)((all + 7) / 8), 256, 0, st>>>(a);
       if (int rc = abi_check_launch("tree_join_stats")) return rc;
     }
-    if (int rc = nodes <= 16 ? simt_dilute<T, dim(), 1>(a, st) : simt_dilute<T, dim(), 4>(a, st)) return rc;
+    if (int rc = with_rows(nodes, [&](auto ri) { return simt_dilute<T, dim(), ri()>(a, st); })) return rc;
     return join<T, true>(a, d, st);
     }
   });
