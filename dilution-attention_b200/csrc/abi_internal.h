@@ -75,4 +75,22 @@ template <typename F> int with_type(int dtype, int d, F f) {
   return dtype == DILUTION_F32 ? with_d<float>(d, f) : with_d<__nv_bfloat16>(d, f);
 }
 
+// Launch a kernel that may start while the one in front of it in the stream ends (and waits for it itself: wait_for_last).
+template <typename... P, typename... A>
+int launch_early(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, const char* name, const A&... args) {
+  LaunchMark mark(name, st);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? DILUTION_OK : abi_fail(DILUTION_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+}
+
 }  // namespace dil

@@ -149,6 +149,11 @@ __device__ __forceinline__ float ld_cluster(const float* p, int rank) {
   return v;
 }
 
+// Programmatic launches.  A kernel that lets the next one in early, and what the next one calls in front of the first use of the
+// other's results: it returns when that kernel has ended and its writes are visible.
+__device__ __forceinline__ void let_next_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));

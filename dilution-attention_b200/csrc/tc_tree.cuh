@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
   const int2 keys = tree::chunk_keys(len, a.chunks, blockIdx.x, KT);
   const int ne = (keys.y - keys.x + KT - 1) / KT, last = keys.x / KT + ne - 1;
 
+  let_next_in();
   if (tid == 0) bars.init();
   // the rows between zeros
   for (int x = tid; x < F::kBufRows * 8 * SUB; x += F::kThreads) {
@@ -427,32 +428,11 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
   const int2 keys = tree::chunk_keys(len, a.chunks, blockIdx.x, KT);
   const int ne = (keys.y - keys.x + KT - 1) / KT, last = keys.x / KT + ne - 1;
 
+  let_next_in();
   if (tid == 0) bars.init();
   tree::make_lineage(&lineage, a.parents + b * a.parent_stride, a.nodes);
   // row r of the sweep is row q_row(r) of the key head's queries
   auto q_row = [&](int r) { return DILUTE ? r : r / acc.accepted * a.nodes + tree::path_node(a, acc, b, r % acc.accepted); };
-  if (tid < N) {
-    NodeStep s{0.f, -1, 0, 0.f};
-    bool jump = false, keep = false;
-    if (tid < rows) {
-      const int q = q_row(tid);
-      s.lse = a.lse[((int64_t)nk * a.group) * a.nodes + q];
-      if (DILUTE) {
-        s.up = lineage.parent[tid];
-        jump = s.up < 0 || s.up != tid - 1;
-        for (int y = tid + 2; y < a.nodes; ++y) keep = keep || lineage.parent[y] == tid;
-      } else {
-        s.slope2 = a.slopes != nullptr ? a.slopes[hk * a.group + q / a.nodes] * kLog2e : 0.f;
-        s.at = len + lineage.depth[q % a.nodes];
-      }
-    }
-    step[tid] = s;
-    const unsigned active = N < 32 ? (1u << N) - 1 : 0xffffffffu, j = __ballot_sync(active, jump), k = __ballot_sync(active, keep);
-    if (lane == 0) {
-      reinterpret_cast<uint32_t*>(walk)[warp] = j;
-      reinterpret_cast<uint32_t*>(walk)[2 + warp] = k;
-    }
-  }
   for (int x = tid; x < N * 8 * SUB; x += F::kThreads) {
     const int sub = x / (N * 8), r = x / 8 % N, c = x % 8;
     uint4 w = make_uint4(0, 0, 0, 0);
@@ -535,6 +515,31 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const bool cap = a.cap > 0.f;
     const float lin = cap ? a.cap * kLog2e : a.scale * kLog2e, pre = cap ? a.scale / a.cap : 0.f;
+    // what the keys' threads have to know of the rows; their lse may come from a kernel that has not ended yet
+    if (DILUTE) wait_for_last();
+    if (tid < N) {
+      NodeStep s{0.f, -1, 0, 0.f};
+      bool jump = false, keep = false;
+      if (tid < rows) {
+        const int q = q_row(tid);
+        s.lse = a.lse[((int64_t)nk * a.group) * a.nodes + q];
+        if (DILUTE) {
+          s.up = lineage.parent[tid];
+          jump = s.up < 0 || s.up != tid - 1;
+          for (int y = tid + 2; y < a.nodes; ++y) keep = keep || lineage.parent[y] == tid;
+        } else {
+          s.slope2 = a.slopes != nullptr ? a.slopes[hk * a.group + q / a.nodes] * kLog2e : 0.f;
+          s.at = len + lineage.depth[q % a.nodes];
+        }
+      }
+      step[tid] = s;
+      const unsigned active = N < 32 ? (1u << N) - 1 : 0xffffffffu, j = __ballot_sync(active, jump), k = __ballot_sync(active, keep);
+      if (lane == 0) {
+        reinterpret_cast<uint32_t*>(walk)[warp] = j;
+        reinterpret_cast<uint32_t*>(walk)[2 + warp] = k;
+      }
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
     const uint64_t jumps = walk[0], keeps = walk[1];
     for (int e = wg; e < ne; e += 2) {
       const int j = (last - e) * KT + row;

@@ -39,132 +39,153 @@ __device__ __noinline__ float2 redo_stats(const Args& a, int64_t nk, int r, int 
   return make_float2(m, s);
 }
 
-// One block of D threads per row: out and lse of a softmax layer's node.
+// Threads of a block that has a warp for each of n nodes, 8 to 16 of them.
+inline int join_threads(int n) { return 32 * (n < 8 ? 8 : n > 16 ? 16 : n); }
+
+// q, k (and v) of a head's nodes in shared memory, rows of D + 2 elements: an odd number of words.
+template <int D> __device__ __forceinline__ void load_nodes(__nv_bfloat16* dst, const void* src, int64_t first, int n) {
+  const uint32_t* from = reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)src + first * D);
+  for (int x = threadIdx.x; x < n * D / 2; x += blockDim.x)
+    reinterpret_cast<uint32_t*>(dst)[x / (D / 2) * (D / 2 + 1) + x % (D / 2)] = from[x];
+}
+// z[nodes][nodes + 1]: scores of the nodes against the nodes that they see, -inf elsewhere.
 template <int D>
-__global__ void __launch_bounds__(D) join_softmax_kernel(Args a) {
-  __shared__ int up[kMaxNodes], line[kMaxNodes], count;
-  __shared__ float z[kMaxNodes];
-  __shared__ float again[D + 2];
-  const int rows = a.group * a.nodes, c = threadIdx.x, lane = c & 31, warp = c >> 5;
-  const int64_t at = blockIdx.x, nk = at / rows;
-  const int r = (int)(at % rows), x = r % a.nodes, b = (int)(nk / a.kv_heads);
-  if (c < a.nodes) up[c] = a.parents[b * a.parent_stride + c];
-  __syncthreads();
-  if (c == 0) {
-    int n = 0;
-    for (int y = x; y >= 0;) {
-      line[n++] = y;
-      const int p = up[y];
-      y = p >= 0 && p < y ? p : -1;
-    }
-    count = n;
-  }
-  __syncthreads();
-  const int n = count;
-  const float slope2 = a.slopes != nullptr ? a.slopes[(nk % a.kv_heads) * a.group + r / a.nodes] * kLog2e : 0.f;
-  {
-    LaneRow<D> q, k;
-    q.load((const __nv_bfloat16*)a.q + at * D);
-    for (int y = warp; y < n; y += D / 32) {
-      k.load((const __nv_bfloat16*)a.kn + (nk * a.nodes + line[y]) * D);
-      const float s = score<true>(q.dot(k), a.scale, a.cap, slope2, (float)y);
-      if (lane == 0) z[y] = s;
-    }
-  }
-  __syncthreads();
-  const float2* part = a.part + nk * a.chunks * rows + r;
-  float m = -INFINITY;
-  for (int y = 0; y < a.chunks; ++y) m = fmaxf(m, part[(int64_t)y * rows].x);
-  for (int y = 0; y < n; ++y) m = fmaxf(m, z[y]);
-  const float from = m == -INFINITY ? 0.f : m;
-  float s = 0.f, o = 0.f;
-  for (int y = 0; y < a.chunks; ++y) {
-    const float2 p = part[(int64_t)y * rows];
-    const float f = exp2f(p.x - from);
-    s = fmaf(p.y, f, s);
-    o = fmaf(a.pout[((nk * a.chunks + y) * rows + r) * D + c], f, o);
-  }
-  auto nodes = [&]() {
-    for (int y = 0; y < n; ++y) {
-      const float p = exp2f(z[y] - from);
-      s += p;
-      o = fmaf(p, to_f32(((const __nv_bfloat16*)a.vn)[(nk * a.nodes + line[y]) * D + c]), o);
-    }
-  };
-  nodes();
-  if (__syncthreads_or(!isfinite(o / s))) {
-    // as in redo_stats, with the values: warp 0, key by key
-    if (warp == 0) {
-      const int len = cache_len(a.pos_dev, a.len, a.capacity);
-      LaneRow<D> q, k, v, sum;
-      q.load((const __nv_bfloat16*)a.q + at * D);
-      float top = -INFINITY, mass = 0.f;
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) sum.x[e] = 0.f;
-      for (int j = 0; j < len; ++j) {
-        k.load((const __nv_bfloat16*)a.kc + (nk * a.capacity + j) * D);
-        v.load((const __nv_bfloat16*)a.vc + (nk * a.capacity + j) * D);
-        const float s1 = score<true>(q.dot(k), a.scale, a.cap, slope2, (float)(len + n - 1 - j)), now = fmaxf(top, s1);
-        const float base = now == -INFINITY ? 0.f : now, f = exp2f(top - base), p = exp2f(s1 - base);
-        mass = mass * f + p;
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) sum.x[e] = sum.x[e] * f + (p == 0.f ? 0.f : p * v.x[e]);
-        top = now;
+__device__ __forceinline__ void node_scores(float* z, const __nv_bfloat16* q, const __nv_bfloat16* k, const Lineage& tree, const Args& a,
+                                            float slope2) {
+  const int n = a.nodes;
+  for (int x = threadIdx.x; x < n * n; x += blockDim.x) {
+    const int i = x / n, j = x % n;
+    float s = -INFINITY;
+    if (tree.line[i] >> j & 1) {
+      s = 0.f;
+#pragma unroll 8
+      for (int c = 0; c < D / 2; ++c) {
+        const float2 u = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(q)[i * (D / 2 + 1) + c]);
+        const float2 v = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(k)[j * (D / 2 + 1) + c]);
+        s = fmaf(u.x, v.x, s);
+        s = fmaf(u.y, v.y, s);
       }
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) again[lane + 32 * e] = sum.x[e];
-      if (lane == 0) { again[D] = top; again[D + 1] = mass; }
+      s = score<true>(s, a.scale, a.cap, slope2, (float)(tree.depth[i] - tree.depth[j]));
     }
-    __syncthreads();
-    m = again[D];
-    for (int y = 0; y < n; ++y) m = fmaxf(m, z[y]);
-    const float base = m == -INFINITY ? 0.f : m, f = exp2f(again[D] - base);
-    s = again[D + 1] * f;
-    o = again[c] * f;
-    for (int y = 0; y < n; ++y) {
-      const float p = exp2f(z[y] - base);
-      s += p;
-      o = fmaf(p, to_f32(((const __nv_bfloat16*)a.vn)[(nk * a.nodes + line[y]) * D + c]), o);
-    }
+    z[i * (n + 1) + j] = s;
   }
-  reinterpret_cast<__nv_bfloat16*>(a.out)[at * D + c] = from_f32<__nv_bfloat16>(o / s);
-  if (c == 0) a.lse[at] = (m == -INFINITY ? 0.f : m) + log2f(s);
+}
+
+// out and lse of a softmax layer's nodes.  One block per query head, a warp per node (join_threads).
+// Dynamic shared memory: z [nodes][nodes + 1], then q, k, v [nodes][D + 2].
+template <int D> constexpr int join_softmax_smem(int n) { return (n * (n + 1) * 4 + 15) / 16 * 16 + 3 * n * (D + 2) * 2; }
+template <int D>
+__global__ void __launch_bounds__(512) join_softmax_kernel(Args a) {
+  __shared__ Lineage tree;
+  extern __shared__ __align__(16) float z[];
+  const int n = a.nodes, rows = a.group * n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(z + (n * (n + 1) + 3) / 4 * 4);
+  __nv_bfloat16 *k = q + n * (D + 2), *v = k + n * (D + 2);
+  const int64_t head = blockIdx.x, nk = head / a.group;
+  const int h = (int)(head % ((int64_t)a.kv_heads * a.group));
+  const float slope2 = a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
+  load_nodes<D>(q, a.q, head * n, n);
+  load_nodes<D>(k, a.kn, nk * n, n);
+  load_nodes<D>(v, a.vn, nk * n, n);
+  make_lineage(&tree, a.parents + nk / a.kv_heads * a.parent_stride, n);
+  node_scores<D>(z, q, k, tree, a, slope2);
+  __syncthreads();
+  wait_for_last();                    // the chunks' parts
+  constexpr int E = D / 32;
+  for (int x = warp; x < n; x += (int)(blockDim.x >> 5)) {
+    const int r = (int)(head % a.group) * n + x;
+    const float2* part = a.part + nk * a.chunks * rows + r;
+    const float* zx = z + x * (n + 1);
+    float nodes_top = -INFINITY;
+    for (int y = lane; y < n; y += 32) nodes_top = fmaxf(nodes_top, zx[y]);
+    nodes_top = warp_max(nodes_top);
+    float top = nodes_top, s = 0.f, o[E];
+    for (int y = lane; y < a.chunks; y += 32) top = fmaxf(top, part[(int64_t)y * rows].x);
+    top = warp_max(top);
+    float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int y0 = 0; y0 < a.chunks; y0 += 32) {
+      float f = 0.f;
+      if (y0 + lane < a.chunks) {
+        const float2 p = part[(int64_t)(y0 + lane) * rows];
+        f = exp2f(p.x - from);
+        s = fmaf(p.y, f, s);
+      }
+      const float* src = a.pout + ((nk * a.chunks + y0) * rows + r) * D + lane;
+#pragma unroll 4
+      for (int y = 0; y < min(32, a.chunks - y0); ++y) {
+        const float fy = __shfl_sync(0xffffffffu, f, y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(src[(int64_t)y * rows * D + 32 * e], fy, o[e]);
+      }
+    }
+    s = warp_sum(s);
+    auto nodes = [&]() {
+      for (unsigned long long left = tree.line[x]; left; left &= left - 1) {
+        const int y = __ffsll(left) - 1;
+        const float p = exp2f(zx[y] - from);
+        s += p;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(p, to_f32(v[y * (D + 2) + lane + 32 * e]), o[e]);
+      }
+    };
+    nodes();
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) bad = bad || !isfinite(o[e] / s);
+    if (__any_sync(0xffffffffu, bad)) {
+      // key by key, as in redo_stats, with the values
+      const int len = cache_len(a.pos_dev, a.len, a.capacity);
+      LaneRow<D> qr, kr, vr;
+      qr.load((const __nv_bfloat16*)a.q + (head * n + x) * D);
+      float m = -INFINITY;
+      s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
+      for (int j = 0; j < len; ++j) {
+        kr.load((const __nv_bfloat16*)a.kc + (nk * a.capacity + j) * D);
+        vr.load((const __nv_bfloat16*)a.vc + (nk * a.capacity + j) * D);
+        const float s1 = score<true>(qr.dot(kr), a.scale, a.cap, slope2, (float)(len + tree.depth[x] - j)), now = fmaxf(m, s1);
+        const float base = now == -INFINITY ? 0.f : now, f = exp2f(m - base), p = exp2f(s1 - base);
+        s = s * f + p;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * f + (p == 0.f ? 0.f : p * vr.x[e]);
+        m = now;
+      }
+      top = fmaxf(m, nodes_top);
+      from = top == -INFINITY ? 0.f : top;
+      const float f = exp2f(m - from);
+      s *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= f;
+      nodes();
+    }
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (head * n + x) * D + lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[32 * e] = from_f32<__nv_bfloat16>(o[e] / s);
+    if (lane == 0) a.lse[head * n + x] = from + log2f(s);
+  }
 }
 
 // lse of a dilution layer's nodes, and their shares of the nodes' own keys: (batch * heads, nodes, nodes), 0 where a node
 // does not see another.  One block per head.
 template <int D>
-__global__ void __launch_bounds__(256) join_bids_kernel(Args a, float* __restrict__ shares) {
-  constexpr int P = D + 2;                                // a row's pitch in elements: an odd number of words
+__global__ void __launch_bounds__(512) join_bids_kernel(Args a, float* __restrict__ shares) {
   __shared__ Lineage tree;
-  __shared__ __nv_bfloat16 q[kMaxNodes * P], k[kMaxNodes * P];
+  __shared__ __nv_bfloat16 q[kMaxNodes * (D + 2)], k[kMaxNodes * (D + 2)];
   extern __shared__ float z[];                            // [nodes][nodes + 1]
   __shared__ float lse[kMaxNodes];
   const int n = a.nodes, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t nk = blockIdx.x;
-  for (int x = tid; x < n * D / 2; x += 256) {
-    const int row = x / (D / 2), c = x % (D / 2);
-    reinterpret_cast<uint32_t*>(q)[row * (P / 2) + c] = reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)a.q + nk * n * D)[x];
-    reinterpret_cast<uint32_t*>(k)[row * (P / 2) + c] = reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)a.kn + nk * n * D)[x];
-  }
+  load_nodes<D>(q, a.q, nk * n, n);
+  load_nodes<D>(k, a.kn, nk * n, n);
   make_lineage(&tree, a.parents + nk / a.kv_heads * a.parent_stride, n);
-  for (int x = tid; x < n * n; x += 256) {
-    const int i = x / n, j = x % n;
-    float s = -INFINITY;
-    if (tree.line[i] >> j & 1) {
-      s = 0.f;
-      for (int c = 0; c < D / 2; ++c) {
-        const float2 u = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(q)[i * (P / 2) + c]);
-        const float2 v = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(k)[j * (P / 2) + c]);
-        s = fmaf(u.x, v.x, s);
-        s = fmaf(u.y, v.y, s);
-      }
-      s *= a.scale * kLog2e;
-    }
-    z[i * (n + 1) + j] = s;
-  }
+  let_next_in();
+  node_scores<D>(z, q, k, tree, a, 0.f);
   __syncthreads();
-  for (int x = warp; x < n; x += 8) {
+  wait_for_last();                    // the chunks' statistics
+  for (int x = warp; x < n; x += (int)(blockDim.x >> 5)) {
     const float2* part = a.part + nk * a.chunks * n + x;
     float m = -INFINITY, s = 0.f;
     for (int y = lane; y < a.chunks; y += 32) m = fmaxf(m, part[(int64_t)y * n].x);
@@ -216,6 +237,7 @@ __global__ void __launch_bounds__(D) join_dilute_kernel(Args a, const float* __r
   const int64_t at = blockIdx.x, nk = at / n;
   const int x = (int)(at % n);
   float s = 0.f, o = 0.f;
+  wait_for_last();
   for (int y = 0; y < a.chunks; ++y) {
     const int64_t p = (nk * a.chunks + y) * n + x;
     s += a.psum[p];
@@ -239,6 +261,7 @@ __global__ void __launch_bounds__(256) accept_nodes_kernel(Args a, Accept c) {
   const int64_t nk = blockIdx.x;
   const int b = (int)(nk / a.kv_heads), hk = (int)(nk % a.kv_heads), len = cache_len(a.pos_dev, a.len, a.capacity);
   make_lineage(&tree, a.parents + b * a.parent_stride, a.nodes);
+  wait_for_last();
   for (int x = warp; x < c.accepted && (int64_t)len + x < a.capacity; x += 8) {
     const int key = path_node(a, c, b, x);
     const int64_t src = (nk * a.nodes + key) * D, dst = (nk * a.capacity + len + x) * D;

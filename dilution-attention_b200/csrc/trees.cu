@@ -173,9 +173,11 @@ template <int D, int N, bool DILUTE>
 int tc_sweep_rows(const tree::Args& a, const tree::Accept& c, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
   using F = tc::Sweep<D, N, DILUTE>;
   if (int rc = opt_in(tc::sweep_kernel<D, N, DILUTE>, F::kBytes)) return rc;
-  LaunchMark mark(DILUTE ? "tree_dilute" : "tree_advance", st);
-  tc::sweep_kernel<D, N, DILUTE><<<dim3(a.chunks, 1, a.batch * a.kv_heads), F::kThreads, F::kBytes, st>>>(k, v, a, c);
-  return abi_check_launch("tree_sweep");
+  const dim3 grid(a.chunks, 1, a.batch * a.kv_heads);
+  if (DILUTE) return launch_early(tc::sweep_kernel<D, N, DILUTE>, grid, F::kThreads, F::kBytes, st, "tree_dilute", k, v, a, c);
+  LaunchMark mark("tree_advance", st);
+  tc::sweep_kernel<D, N, DILUTE><<<grid, F::kThreads, F::kBytes, st>>>(k, v, a, c);
+  return abi_check_launch("tree_advance");
 }
 template <int D, bool DILUTE>
 int tc_sweep(const tree::Args& a, const tree::Accept& c, int rows, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
@@ -191,9 +193,9 @@ template <int D> int tc_softmax(tree::Args a, void* scratch, cudaStream_t st) {
   a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads * row_blocks(rows, 128), tree_keys(a), tc::Scan<D, 4, true>::kPerSm);
   place_scratch(a, scratch, D);
   if (int rc = tc_scan<D, true>(a, k, v, st)) return rc;
-  LaunchMark mark("tree_join", st);
-  tree::join_softmax_kernel<D><<<(unsigned)((int64_t)a.batch * a.kv_heads * rows), D, 0, st>>>(a);
-  return abi_check_launch("tree_join");
+  if (int rc = opt_in(tree::join_softmax_kernel<D>, tree::join_softmax_smem<D>(tree::kMaxNodes))) return rc;
+  return launch_early(tree::join_softmax_kernel<D>, dim3((unsigned)((int64_t)a.batch * a.kv_heads * a.group)), tree::join_threads(a.nodes),
+                      tree::join_softmax_smem<D>(a.nodes), st, "tree_join", a);
 }
 
 template <int D> int tc_dilute(tree::Args a, void* scratch, cudaStream_t st) {
@@ -203,17 +205,11 @@ template <int D> int tc_dilute(tree::Args a, void* scratch, cudaStream_t st) {
   a.chunks = tc_chunks(heads, tree_keys(a), tc::Sweep<D, 64, true>::kPerSm);
   float* shares = place_scratch(a, scratch, D);
   if (int rc = tc_scan<D, false>(a, k, v, st)) return rc;
-  {
-    LaunchMark mark("tree_join_bids", st);
-    const int smem = a.nodes * (a.nodes + 1) * 4;
-    if (int rc = opt_in(tree::join_bids_kernel<D>, 64 * 65 * 4, 36 * 1024)) return rc;
-    tree::join_bids_kernel<D><<<(unsigned)heads, 256, smem, st>>>(a, shares);
-    if (int rc = abi_check_launch("tree_join_bids")) return rc;
-  }
+  if (int rc = opt_in(tree::join_bids_kernel<D>, 64 * 65 * 4, 36 * 1024)) return rc;
+  if (int rc = launch_early(tree::join_bids_kernel<D>, dim3((unsigned)heads), tree::join_threads(a.nodes), a.nodes * (a.nodes + 1) * 4, st,
+                            "tree_join_bids", a, shares)) return rc;
   if (int rc = tc_sweep<D, true>(a, tree::Accept{}, a.nodes, k, v, st)) return rc;
-  LaunchMark mark("tree_join", st);
-  tree::join_dilute_kernel<D><<<(unsigned)(heads * a.nodes), D, 0, st>>>(a, shares);
-  return abi_check_launch("tree_join");
+  return launch_early(tree::join_dilute_kernel<D>, dim3((unsigned)(heads * a.nodes)), D, 0, st, "tree_join", a, shares);
 }
 
 template <int D> int tc_accept(tree::Args a, const tree::Accept& c, cudaStream_t st) {
@@ -223,6 +219,8 @@ template <int D> int tc_accept(tree::Args a, const tree::Accept& c, cudaStream_t
     a.chunks = tc_chunks((int64_t)a.batch * a.kv_heads, tree_keys(a), 2);
     if (int rc = tc_sweep<D, false>(a, c, a.group * c.accepted, k, v, st)) return rc;
   }
+  // (it starts early behind the sweep alone: what it reads in front of its wait may be another kernel's work otherwise)
+  if (c.advanced) return launch_early(tree::accept_nodes_kernel<D>, dim3((unsigned)(a.batch * a.kv_heads)), 256, 0, st, "tree_append", a, c);
   LaunchMark mark("tree_append", st);
   tree::accept_nodes_kernel<D><<<(unsigned)(a.batch * a.kv_heads), 256, 0, st>>>(a, c);
   return abi_check_launch("tree_append");

@@ -18,6 +18,7 @@ itself, and stands at position len + depth(x) (depth 0 follows the last cached t
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -29,14 +30,20 @@ from .masked import _CODE, _DIMS, aligned, check_slopes, check_softcap, on_devic
 MAX_NODES = 64
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(*sizes) -> int:
+    return _lib.load().dilution_tree_scratch_bytes(*sizes)
+
+
 def _cache(cache, batch, heads, dim, dtype, device):
     """(k, v, capacity, length) of a cache whose rows the kernels read by their addresses."""
     k, v, length = cache["k"], cache["v"], cache["len"]
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != batch or k.shape[1] != heads or k.shape[3] != dim:
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[0] != batch or shape[1] != heads or shape[3] != dim:
         raise ValueError("the caches are (batch, key heads, capacity, head_dim), like the drafted keys")
     if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
         raise ValueError("the caches must have the drafted tokens' dtype and device")
-    capacity = k.shape[2]
+    capacity = shape[2]
     if not 0 <= length <= capacity or capacity < 1:
         raise ValueError(f"length {length} outside cache capacity {capacity}")
     k, v = K._cache_rows(k, batch, heads, capacity, dim), K._cache_rows(v, batch, heads, capacity, dim)
@@ -54,6 +61,12 @@ def _demand(x, batch, heads, capacity, device, name="committed"):
 def _indices(x, batch, name, device):
     """(int32 tensor on the device, stride between sequences, the host's copy or None) of a list, (N,) or (B, N)."""
     host = None
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.int32 and x.is_contiguous() and x.device == device:
+        shape = x.shape
+        if len(shape) == 1:
+            return x, 0, None
+        if len(shape) == 2 and shape[0] == batch:
+            return x, shape[1], None
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         x = torch.as_tensor(x)
         if x.numel() == 0:
@@ -102,14 +115,13 @@ def _draft(q, k, v, cache, parents):
     return draft, sizes, (kc, vc), pos_dev
 
 
-def _buffers(lib, sizes, pos_dev, like, out, scratch):
+def _buffers(sizes, pos_dev, like, out, scratch):
     batch, heads, kv_heads, nodes, dim, capacity, length = sizes
     if out is None:
         out = torch.empty(like.shape, device=like.device, dtype=like.dtype)
     elif out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like q")
-    need = lib.dilution_tree_scratch_bytes(batch, kv_heads, heads // kv_heads, nodes, capacity if pos_dev is not None else length,
-                                           dim)
+    need = _scratch_bytes(batch, kv_heads, heads // kv_heads, nodes, capacity if pos_dev is not None else length, dim)
     if scratch is None or scratch.numel() * scratch.element_size() < need or scratch.data_ptr() % 16:
         scratch = torch.empty(need, device=like.device, dtype=torch.uint8)
     return out, scratch
@@ -131,7 +143,7 @@ def softmax_tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: 
     batch, heads, kv_heads, nodes, dim, capacity, length = sizes
     draft["softcap"], draft["slopes"] = check_softcap(softcap), check_slopes(slopes, heads, q.device)
     lib = _lib.load()
-    out, scratch = _buffers(lib, sizes, pos_dev, q, out, scratch)
+    out, scratch = _buffers(sizes, pos_dev, q, out, scratch)
     with on_device(q.device):
         _lib.check(lib.dilution_tree_softmax(
             draft["q"].data_ptr(), draft["k"].data_ptr(), draft["v"].data_ptr(), kc.data_ptr(), vc.data_ptr(), _CODE[q.dtype], batch,
@@ -155,7 +167,7 @@ def dilution_tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
         raise ValueError("a dilution layer has as many key heads as query heads")
     committed = _demand(cache["committed"], batch, heads, capacity, q.device)
     lib = _lib.load()
-    out, scratch = _buffers(lib, sizes, pos_dev, q, out, scratch)
+    out, scratch = _buffers(sizes, pos_dev, q, out, scratch)
     with on_device(q.device):
         _lib.check(lib.dilution_tree_dilute(
             draft["q"].data_ptr(), draft["k"].data_ptr(), draft["v"].data_ptr(), kc.data_ptr(), vc.data_ptr(), _CODE[q.dtype], batch,
