@@ -140,6 +140,9 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
+// Its halves, for warps that have nothing to say to the other CTAs and work on: each arrives once and waits later.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // A float of CTA `rank`'s shared memory, by its address in this CTA's.
 __device__ __forceinline__ float ld_cluster(const float* p, int rank) {
   uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;

@@ -61,17 +61,17 @@ template <int RK, int RV, int NB> struct StreamBars {
   }
 };
 
-// The warp that copies ne tiles of KT keys and (if V) their values, from tile `last` down: a distance bias has the largest scores
-// there, and later tiles do not move a row's reference.
+// The warp that copies ne tiles of KT keys and (if V) their values: from, from + step, ..  Scans go from the last tile down: a
+// distance bias has the largest scores there, and later tiles do not move a row's reference.
 template <int D, int KT, int RK, int RV, int NB, bool V>
 __device__ __forceinline__ void stream_tiles(const StreamBars<RK, RV, NB>& bars, const CUtensorMap* map_k, const CUtensorMap* map_v,
-                                             uint32_t ring_k, uint32_t ring_v, int last, int ne, int nk, uint32_t lead) {
+                                             uint32_t ring_k, uint32_t ring_v, int from, int step, int ne, int nk, uint32_t lead) {
   constexpr uint32_t kOne = KT * D * 2;
   auto copy = [&](const CUtensorMap* map, uint32_t dst, int e, uint32_t bar) {
     if (lead) {
       mbar_expect_tx(bar, kOne);
 #pragma unroll
-      for (int x = 0; x < KT / 64; ++x) tma_load_rows<kForm<D>>(dst + 8192 * x, map, (last - e) * KT + 64 * x, nk, bar, KT * 128);
+      for (int x = 0; x < KT / 64; ++x) tma_load_rows<kForm<D>>(dst + 8192 * x, map, (from + step * e) * KT + 64 * x, nk, bar, KT * 128);
     }
     __syncwarp();
   };
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
     mma_commit(lead, bars.alldone);
     __syncwarp();
   } else if (warp_u == 4 * NW + 1) {
-    stream_tiles<D, KT, RK, RV, NB, OUT>(bars, &map_k, &map_v, ring_k, ring_v, last, ne, nk, lead);
+    stream_tiles<D, KT, RK, RV, NB, OUT>(bars, &map_k, &map_v, ring_k, ring_v, last, -1, ne, nk, lead);
   } else {
     // ------------------------------------------------------------ the compute warps: lane = row of a group
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tP = tmem + NC * NB + F::kWgCols * wg + lanes, tO = tP + 64;
@@ -385,6 +385,50 @@ struct NodeStep {
   int at;              // an accepted row's position, and the slope of its head
   float slope2;
 };
+
+// Shares of one key (of this lane), whose scores by `rows` nodes are at tS and whose cached demand is base: bf16 into row `row` of
+// the [128][64] tile dst.  jumps: nodes that do not follow the one in front; keeps: nodes whose demand a later one starts from.
+template <int N>
+__device__ __forceinline__ void share_keys(uint32_t tS, int rows, float lin, float eps, float base, bool live, const NodeStep* step,
+                                           uint64_t jumps, uint64_t keeps, uint8_t* dst, int row) {
+  float left = base;
+#pragma unroll
+  for (int c0 = 0; c0 < N; c0 += 16) {
+    if (c0 >= rows) break;
+    float v[16], d[16];
+    uint32_t w[8];
+    __syncwarp();
+    tmem_ld16(tS + c0, v);
+    tmem_ld_wait16(v);
+#pragma unroll
+    for (int y = 0; y < 16; ++y) {
+      v[y] = fast_exp2(fmaf(v[y], lin, -step[c0 + y].lse));
+      if (!live || c0 + y >= rows) v[y] = 0.f;
+    }
+#pragma unroll
+    for (int y = 0; y < 16; ++y) {
+      if (jumps >> (c0 + y) & 1) {
+        const int up = step[c0 + y].up;
+        left = base;
+        if (up >= 0) {
+          tmem_st_wait();
+          tmem_ld1(tS + up, &left);
+          tmem_ld_wait1(&left);
+        }
+      }
+      d[y] = left = left + v[y];
+      if (keeps >> (c0 + y) & 1) tmem_st1(tS + c0 + y, left);
+    }
+#pragma unroll
+    for (int y = 0; y < 16; ++y) v[y] *= fast_rcp(d[y] + eps);
+#pragma unroll
+    for (int y = 0; y < 8; ++y) w[y] = pack_pair(v[2 * y], v[2 * y + 1]);
+    *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  tmem_st_wait();
+  fence_async_smem();
+}
 
 template <int D, int N, bool DILUTE> struct Sweep {
   static constexpr int kKeys = 128, kThreads = 320;
@@ -509,7 +553,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
     mma_commit(lead, bars.alldone);
     __syncwarp();
   } else if (warp_u == 9) {
-    stream_tiles<D, KT, RK, RV, NB, DILUTE>(bars, &map_k, &map_v, ring_k, ring_v, last, ne, nk, lead);
+    stream_tiles<D, KT, RK, RV, NB, DILUTE>(bars, &map_k, &map_v, ring_k, ring_v, last, -1, ne, nk, lead);
   } else {
     // ------------------------------------------------------------ the compute warps: lane = key
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -551,44 +595,17 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
       // the product of the warpgroup's last tile has read its shares
       if (DILUTE && e >= 2) mbar_wait_warp(bars.used + 8 * wg, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
       tc_fence_after();
-      float left = base, total = base;
+      if (DILUTE) {
+        share_keys<N>(tS, rows, lin, a.eps, base, live, step, jumps, keeps, pShare + 16384 * wg, row);
+      } else {
+        float total = base;
 #pragma unroll
-      for (int c0 = 0; c0 < N; c0 += 16) {
-        if (c0 >= rows) break;
-        float v[16];
-        __syncwarp();
-        tmem_ld16(tS + c0, v);
-        tmem_ld_wait16(v);
-        if (DILUTE) {
-          float d[16];
-          uint32_t w[8];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            v[y] = fast_exp2(fmaf(v[y], lin, -step[c0 + y].lse));
-            if (!live || c0 + y >= rows) v[y] = 0.f;
-          }
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            if (jumps >> (c0 + y) & 1) {
-              const int up = step[c0 + y].up;
-              left = base;
-              if (up >= 0) {
-                tmem_st_wait();
-                tmem_ld1(tS + up, &left);
-                tmem_ld_wait1(&left);
-              }
-            }
-            d[y] = left = left + v[y];
-            if (keeps >> (c0 + y) & 1) tmem_st1(tS + c0 + y, left);
-          }
-#pragma unroll
-          for (int y = 0; y < 16; ++y) v[y] *= fast_rcp(d[y] + a.eps);
-#pragma unroll
-          for (int y = 0; y < 8; ++y) w[y] = pack_pair(v[2 * y], v[2 * y + 1]);
-          uint8_t* dst = pShare + 16384 * wg;
-          *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
+        for (int c0 = 0; c0 < N; c0 += 16) {
+          if (c0 >= rows) break;
+          float v[16];
+          __syncwarp();
+          tmem_ld16(tS + c0, v);
+          tmem_ld_wait16(v);
           if (cap) cap_scores<16>(v, pre);
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
@@ -597,12 +614,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
             if (c0 + y < rows) total += fast_exp2(z);
           }
         }
-      }
-      if (DILUTE) {
-        tmem_st_wait();
-        fence_async_smem();
-      } else if (live) {
-        acc.advanced[at] = total;
+        if (live) acc.advanced[at] = total;
       }
       tc_fence_before();
       __syncwarp();
@@ -636,6 +648,358 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
   tc_fence_before();
   __syncthreads();
   if (warp == 0) tmem_free(tmem, F::kTmem);
+}
+
+// ---- a dilution layer's step by clusters -----------------------------------------------------------------
+// scan_kernel and sweep_kernel one after the other, for a head per cluster of eight CTAs: each reads its chunk of keys twice, the
+// second time out of L2; statistics and outputs are joined through distributed shared memory.  The nodes' own keys are dealt out to
+// the CTAs like cached ones.  One launch for the four of a step in chunks (trees.cu has the sizes it is taken for).
+constexpr int kDraftRanks = 8;
+template <int D, int N> struct Draft {
+  static constexpr int kThreads = 320, G = N == 64 ? 2 : 4, kRows = 128 / G, kKeysA = 32 * G;
+  static constexpr uint32_t kOneA = kKeysA * D * 2, kOne = 128 * D * 2;
+  static constexpr int kSpace = D == 64 ? 65536 : 131072, RA = kSpace / (int)kOneA, R = kSpace / (int)kOne / 2, NA = 4, NB = 2;
+  static constexpr int kBufRows = (G - 1) * kRows + 128;
+  static constexpr uint32_t kBufSub = kBufRows * 128, kQSub = N * 128;
+  static constexpr int kBuf = (int)kBufSub * (D / 64), kQ = (N * 128 * (D / 64) + 1023) / 1024 * 1024;
+  static constexpr int kShare = 2 * 16384, kOnes = D == 64 ? 2048 : 4096, kOver = kBuf > kShare + kOnes ? kBuf : kShare + kOnes;
+  static constexpr int kCols = N / kDraftRanks;                          // nodes' keys of a CTA
+  // Q | ring | first the rows between zeros, then shares and ones | z [N][kCols] | steps | statistics of the rows | barriers
+  static constexpr int kZ = N * kCols * 4;
+  static constexpr int kBytes = kQ + kSpace + kOver + kZ + 64 * 16 + 64 * 8 + 640 + 1024;
+  static constexpr int kTmem = 256, kPerSm = ctas_per_sm(kBytes, kTmem);
+  static_assert(StreamBars<RA, 4, NA>::kBytes + StreamBars<R, R, NB>::kBytes + 16 <= 640 && kBytes <= 231000, "shared memory");
+  static_assert(N * D * 4 + 256 <= kSpace, "a chunk's output fits the ring");
+};
+
+// (maximum, sum) of a row over keys [j0, j1), one warp, key by key (tree_join.cuh has the reason).
+template <int D> __device__ __noinline__ float2 redo_chunk_stats(const tree::Args& a, int64_t nk, int r, int j0, int j1) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (nk * a.nodes + r) * D;
+  float m = -INFINITY, s = 0.f;
+  for (int j = j0; j < j1; ++j) {
+    const __nv_bfloat16* k = (const __nv_bfloat16*)a.kc + (nk * a.capacity + j) * D;
+    float z = 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) z = fmaf(to_f32(q[lane + 32 * e]), to_f32(k[lane + 32 * e]), z);
+    z = warp_sum(z) * (a.scale * kLog2e);
+    const float top = fmaxf(m, z), from = top == -INFINITY ? 0.f : top;
+    s = s * exp2f(m - from) + exp2f(z - from);
+    m = top;
+  }
+  return make_float2(m, s);
+}
+
+// grid = heads * 8, clusters of 8
+template <int D, int N>
+__global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                      const __grid_constant__ CUtensorMap map_v,
+                                                                      const __grid_constant__ tree::Args a) {
+  using F = Draft<D, N>;
+  constexpr int SUB = D / 64, G = F::G, KA = F::kKeysA, RA = F::RA, NA = F::NA, R = F::R, NB = F::NB, C = kDraftRanks;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint8_t *pRing = smem + F::kQ, *pOver = pRing + F::kSpace, *pShare = pOver, *pOnes = pOver + F::kShare;
+  const uint32_t sQ = smem_u32(smem), ring = smem_u32(pRing), ring_v = ring + F::kOne * R, sOver = smem_u32(pOver), sOnes = smem_u32(pOnes);
+  float* z = reinterpret_cast<float*>(pOver + F::kOver);                                   // [N][kCols]
+  NodeStep* step = reinterpret_cast<NodeStep*>(z + N * F::kCols);
+  float2* chunk = reinterpret_cast<float2*>(step + 64);                                    // [N] this CTA's (maximum, sum)
+  uint64_t* at_bars = reinterpret_cast<uint64_t*>(chunk + 64);
+  uint32_t* walk = reinterpret_cast<uint32_t*>(at_bars);                                   // jumps, keeps
+  const StreamBars<RA, 4, NA> ba(at_bars + 2);
+  const StreamBars<R, R, NB> bb(at_bars + 2 + StreamBars<RA, 4, NA>::kBytes / 8);
+  Ctl* ctl = ba.ctl;
+  __shared__ tree::Lineage lineage;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
+  const int warp_u = uniform_warp();
+  const uint32_t lead = elect_one();
+  const int rank = blockIdx.x % C, nk = blockIdx.x / C, n = a.nodes;
+  const int len = (int)uniform(tree::cache_len(a.pos_dev, a.len, a.capacity));
+  const int2 keys = tree::chunk_keys(len, C, rank, 128);
+  const int na = (keys.y - keys.x + KA - 1) / KA, last = keys.x / KA + na - 1, ne = (keys.y - keys.x + 127) / 128, first = keys.x / 128;
+
+  if (tid == 0) {
+    ba.init();
+    bb.init();
+  }
+  auto load_row = [&](int r, int sub, int c) {
+    return *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + ((int64_t)nk * n + r) * D + 64 * sub + 8 * c);
+  };
+  for (int x = tid; x < F::kBufRows * 8 * SUB; x += F::kThreads) {
+    const int sub = x / (F::kBufRows * 8), br = x / 8 % F::kBufRows, c = x % 8, r = br - (G - 1) * F::kRows;
+    *reinterpret_cast<uint4*>(pOver + sub * F::kBufSub + swizzled(br, c)) = r >= 0 && r < min(n, F::kRows) ? load_row(r, sub, c) : make_uint4(0, 0, 0, 0);
+  }
+  for (int x = tid; x < N * 8 * SUB; x += F::kThreads) {
+    const int sub = x / (N * 8), r = x / 8 % N, c = x % 8;
+    *reinterpret_cast<uint4*>(smem + sub * F::kQSub + swizzled(r, c)) = r < n ? load_row(r, sub, c) : make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
+  tree::make_lineage(&lineage, a.parents + nk / a.kv_heads * a.parent_stride, n);
+  __syncwarp();
+  if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(ctl->tmem);
+
+  if (warp_u == 8) {
+    // ------------------------------------------------------------ the warp that issues MMAs
+    cluster_arrive();
+    {
+      constexpr uint32_t id_s = instr_desc(128, 32, 0, 0);
+      const Desc dQ = make_desc(sOver, 16, 1024), dK = make_desc(ring, 16, 1024);
+      for (int e = 0; e < na + NA - 1; ++e) {
+        if (e < na) {
+          const int st = e % RA, from = len - (last - e) * KA;
+          mbar_wait_warp(ba.kfull + 8 * st, (e / RA) & 1, ctl, &g_tree_status, kErrWaitTma);
+          if (from < KA) {
+            zero_rows(pRing + F::kOneA * st, KA, from, SUB);
+            fence_async_smem();
+            __syncwarp();
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int s = 0; s < SUB; ++s)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_ss(lead, tmem + 32 * (e % NA), dQ, (F::kBufSub >> 4) * s + 8 * F::kRows * (G - 1 - g) + 2 * kk, dK,
+                       (F::kOneA >> 4) * st + 8 * KA * s + 8 * 32 * g + 2 * kk, id_s, g > 0 || s > 0 || kk > 0);
+          mma_commit(lead, ba.sdone + 8 * (e % NA));
+          mma_commit(lead, ba.kfree + 8 * st);
+        }
+        if (e >= NA - 1) {
+          const int y = e - NA + 1;
+          mbar_wait_warp(ba.ready + 8 * (y % NA), (y / NA) & 1, ctl, &g_tree_status, kErrWaitTile);
+          tc_fence_after();
+        }
+      }
+      mma_commit(lead, ba.alldone);
+    }
+    constexpr uint32_t id_s = instr_desc(128, N, 0, 0), id_o = instr_desc(128, N, 1, 1);
+    const Desc dK = make_desc(ring, 16, 1024), dQ = make_desc(sQ, 16, 1024), dOnes = make_desc(sOnes, 2048, 1024);
+    for (int e = 0; e < ne + NB - 1; ++e) {
+      if (e < ne) {
+        const int st = e % R, from = len - (first + e) * 128;
+        mbar_wait_warp(bb.kfull + 8 * st, (e / R) & 1, ctl, &g_tree_status, kErrWaitTma);
+        if (from < 128) {
+          zero_rows(pRing + F::kOne * st, 128, from, SUB);
+          fence_async_smem();
+          __syncwarp();
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(lead, tmem + 64 * (e % NB), dK, (F::kOne >> 4) * st + 8 * 128 * s + 2 * kk, dQ, (F::kQSub >> 4) * s + 2 * kk, id_s,
+                   s > 0 || kk > 0);
+        mma_commit(lead, bb.sdone + 8 * (e % NB));
+        mma_commit(lead, bb.kfree + 8 * st);
+      }
+      if (e >= NB - 1) {
+        const int y = e - NB + 1, w = y & 1, st = y % R;
+        mbar_wait_warp(bb.ready + 8 * (y % NB), (y / NB) & 1, ctl, &g_tree_status, kErrWaitTile);
+        mbar_wait_warp(bb.vfull + 8 * st, (y / R) & 1, ctl, &g_tree_status, kErrWaitTma);
+        const int from = len - (first + y) * 128;
+        if (from < 128) {
+          zero_rows(pRing + F::kOne * (R + st), 128, from, SUB);
+          fence_async_smem();
+          __syncwarp();
+        }
+        tc_fence_after();
+        const uint32_t v = ring_v + F::kOne * st;
+        const Desc dP = make_desc(smem_u32(pShare) + 16384 * w, 16384, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t at = v + 2048 * kk;
+          mma_ss(lead, tmem + 128, make_desc(at, D == 64 ? sOnes - at : 128 * 128, 1024), 0, dP, 128 * kk, id_o, y > 0 || kk > 0);
+          if (D == 128) mma_ss(lead, tmem + 192, dOnes, 0, dP, 128 * kk, id_o, y > 0 || kk > 0);
+        }
+        mma_commit(lead, bb.vfree + 8 * st);
+        mma_commit(lead, bb.used + 8 * w);
+      }
+    }
+    mma_commit(lead, bb.alldone);
+    __syncwarp();
+    cluster_wait();
+    cluster_sync();
+  } else if (warp_u == 9) {
+    cluster_arrive();
+    stream_tiles<D, KA, RA, 4, NA, false>(ba, &map_k, &map_v, ring, ring, last, -1, na, nk, lead);
+    // (every product has read the first pass's stages)
+    mbar_wait_warp(ba.alldone, 0, ctl, &g_tree_status, kErrWaitMma);
+    stream_tiles<D, 128, R, R, NB, true>(bb, &map_k, &map_v, ring, ring_v, first, 1, ne, nk, lead);
+    cluster_wait();
+    cluster_sync();
+  } else {
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const float lin = a.scale * kLog2e;
+    const int cols = (n - rank + C - 1) / C;                               // nodes rank, rank + 8, ..
+    // scores of the nodes against this CTA's nodes, while the first tiles come
+    for (int x = tid; x < n * cols; x += 256) {
+      const int i = x / cols, c = x % cols, key = rank + C * c;
+      float s = -INFINITY;
+      if (lineage.line[i] >> key & 1) {
+        const uint4* q = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((int64_t)nk * n + i) * D);
+        const uint4* k = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.kn + ((int64_t)nk * n + key) * D);
+        s = 0.f;
+#pragma unroll 4
+        for (int y = 0; y < D / 8; ++y) {
+          const uint4 u = q[y], v = k[y];
+          const __nv_bfloat16 *p = reinterpret_cast<const __nv_bfloat16*>(&u), *w = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) s = fmaf(to_f32(p[t]), to_f32(w[t]), s);
+        }
+        s *= lin;
+      }
+      z[i * F::kCols + c] = s;
+    }
+    // ---------------------------------------------------------- statistics: lane = row of a group
+    float ref = -INFINITY, sum = 0.f;
+    const int g = row / F::kRows;
+    for (int e = wg; e < na; e += 2) {
+      const int j0 = (last - e) * KA + 32 * g;
+      mbar_wait_warp(ba.sdone + 8 * (e % NA), (e / NA) & 1, ctl, &g_tree_status, kErrWaitMma);
+      tc_fence_after();
+      scan_step<D, 32, false>(tmem + 32 * (e % NA) + lanes, 0, 0, lin, 0.f, false, 0.f, 0.f, len - j0, ref, sum);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ba.ready + 8 * (e % NA));
+    }
+    mbar_wait_warp(ba.alldone, 0, ctl, &g_tree_status, kErrWaitMma);
+    tc_fence_after();
+    float2* stat = reinterpret_cast<float2*>(pOver);                        // [2][128], over the rows between zeros
+    stat[wg * 128 + row] = make_float2(ref, sum);
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    for (int x = warp; x < n; x += 8) {
+      float2 p = make_float2(-INFINITY, 0.f);
+      if (lane < 2 * G) p = stat[(lane / G) * 128 + (lane % G) * F::kRows + x];
+      float m = warp_max(p.x);
+      float s = warp_sum(lane < 2 * G ? p.y * fast_exp2(p.x - (m == -INFINITY ? 0.f : m)) : 0.f);
+      if (!isfinite(s) || m == INFINITY) {
+        const float2 again = redo_chunk_stats<D>(a, nk, x, keys.x, keys.y);
+        m = again.x;
+        s = again.y;
+      }
+      const float own = lane < cols ? z[x * F::kCols + lane] : -INFINITY, top = fmaxf(m, warp_max(own)), from = top == -INFINITY ? 0.f : top;
+      s = s * exp2f(m - from) + warp_sum(lane < cols ? exp2f(own - from) : 0.f);
+      if (lane == 0) chunk[x] = make_float2(top, s);
+    }
+    cluster_sync();
+    for (int x = tid; x < F::kShare / 16; x += 256) reinterpret_cast<uint4*>(pShare)[x] = make_uint4(0, 0, 0, 0);
+    for (int x = tid; x < F::kOnes / 16; x += 256)
+      *reinterpret_cast<uint4*>(pOnes + (x >> 7) * 2048 + swizzled((x >> 3) & 15, x & 7)) = make_uint4((x & 7) == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);
+    if (tid < N) {
+      NodeStep s{0.f, -1, 0, 0.f};
+      bool jump = false, keep = false;
+      if (tid < n) {
+        float m[C], t[C], top = -INFINITY, all = 0.f;
+#pragma unroll
+        for (int y = 0; y < C; ++y) {
+          m[y] = ld_cluster(&chunk[tid].x, y);
+          t[y] = ld_cluster(&chunk[tid].y, y);
+          top = fmaxf(top, m[y]);
+        }
+        const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int y = 0; y < C; ++y) all = fmaf(t[y], exp2f(m[y] - from), all);
+        s.lse = from + log2f(all);
+        if (rank == 0) a.lse[(int64_t)nk * n + tid] = s.lse;
+        s.up = lineage.parent[tid];
+        jump = s.up < 0 || s.up != tid - 1;
+        for (int y = tid + 2; y < n; ++y) keep = keep || lineage.parent[y] == tid;
+      }
+      step[tid] = s;
+      const unsigned active = N < 32 ? (1u << N) - 1 : 0xffffffffu, j = __ballot_sync(active, jump), k = __ballot_sync(active, keep);
+      if (lane == 0) {
+        walk[warp] = j;
+        walk[2 + warp] = k;
+      }
+    }
+    fence_async_smem();
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    // ---------------------------------------------------------- shares: lane = key
+    const uint64_t jumps = walk[0] | (N > 32 ? (uint64_t)walk[1] << 32 : 0), keeps = walk[2] | (N > 32 ? (uint64_t)walk[3] << 32 : 0);
+    for (int e = wg; e < ne; e += 2) {
+      const int j = (first + e) * 128 + row;
+      const bool live = j < len;
+      const float base = live ? a.committed[(int64_t)nk * a.capacity + j] : 0.f;
+      mbar_wait_warp(bb.sdone + 8 * (e % NB), (e / NB) & 1, ctl, &g_tree_status, kErrWaitMma);
+      if (e >= 2) mbar_wait_warp(bb.used + 8 * wg, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
+      tc_fence_after();
+      share_keys<N>(tmem + 64 * (e % NB) + lanes, n, lin, a.eps, base, live, step, jumps, keeps, pShare + 16384 * wg, row);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bb.ready + 8 * (e % NB));
+    }
+    mbar_wait_warp(bb.alldone, 0, ctl, &g_tree_status, kErrWaitMma);
+    tc_fence_after();
+    // the chunk's output [N][D] and sums of shares, over the ring
+    float *out = reinterpret_cast<float*>(pRing), *total = out + N * D;
+    if (wg == 0) {
+#pragma unroll
+      for (int c0 = 0; c0 < N; c0 += 16) {
+        float o[16], t[16];
+        __syncwarp();
+        tmem_ld16(tmem + 128 + lanes + c0, o);
+        tmem_ld_wait16(o);
+        if (D == 128) {
+          tmem_ld16(tmem + 192 + lanes + c0, t);
+          tmem_ld_wait16(t);
+        }
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+          if (row < D) out[(c0 + y) * D + row] = ne > 0 ? o[y] : 0.f;
+          if (row == (D == 64 ? 64 : 0)) total[c0 + y] = ne > 0 ? (D == 64 ? o[y] : t[y]) : 0.f;
+        }
+      }
+    } else if (row < cols) {
+      // shares of this CTA's nodes' keys: the demand that a node leaves, then its share, in the place of its score
+      const int key = rank + C * row;
+      for (int x = 0; x < n; ++x) {
+        float& cell = z[x * F::kCols + row];
+        float left = 0.f;
+        if (lineage.line[x] >> key & 1) left = exp2f(cell - step[x].lse) + (lineage.parent[x] >= 0 ? z[lineage.parent[x] * F::kCols + row] : 0.f);
+        cell = left;
+      }
+      for (int x = n - 1; x >= 0; --x) {                 // (children come behind their parents)
+        float& cell = z[x * F::kCols + row];
+        const float had = lineage.parent[x] >= 0 ? z[lineage.parent[x] * F::kCols + row] : 0.f;
+        cell = lineage.line[x] >> key & 1 ? (cell - had == 0.f ? 0.f : (cell - had) / (cell + a.eps)) : 0.f;
+      }
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    for (int x = tid; x < n * D; x += 256) {
+      const int i = x / D, d = x % D;
+      float o = out[x], t = 0.f;
+      for (int c = 0; c < cols; ++c) {
+        const float w = z[i * F::kCols + c];
+        t += w;
+        if (w != 0.f) o = fmaf(w, to_f32(((const __nv_bfloat16*)a.vn)[((int64_t)nk * n + rank + C * c) * D + d]), o);
+      }
+      out[x] = o;
+      if (d == 0) total[i] += t;
+    }
+    cluster_sync();
+    for (int x = tid; x < (n - rank + C - 1) / C * D; x += 256) {
+      const int i = rank + C * (x / D), d = x % D;
+      float o = 0.f, t = 0.f;
+#pragma unroll
+      for (int y = 0; y < C; ++y) {
+        o += ld_cluster(out + i * D + d, y);
+        t += ld_cluster(total + i, y);
+      }
+      reinterpret_cast<__nv_bfloat16*>(a.out)[((int64_t)nk * n + i) * D + d] = from_f32<__nv_bfloat16>(o / (t + a.eps));
+    }
+  }
+  drain_if_aborted(ctl);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_free(tmem, F::kTmem);
+  cluster_sync();                      // no CTA leaves while another may read its output
 }
 
 }  // namespace tc

@@ -198,10 +198,35 @@ template <int D> int tc_softmax(tree::Args a, void* scratch, cudaStream_t st) {
                       tree::join_softmax_smem<D>(a.nodes), st, "tree_join", a);
 }
 
+// A step in one launch, a cluster of eight CTAs per head: for short caches whose clusters all run at once.  24 nodes of heads of 64,
+// one launch / chunks (four launches, with 6 us of timing events each), us: 32 heads, 1024 keys 29 / 53, 4096 keys 35 / 51, 8192 keys
+// 44 / 59; 16 heads, 16384 keys 60 / 69; but 64 heads, 16384 keys 121 / 131 and 256 heads 450 / 370: a CTA's start, its three meetings
+// with the others and its end take about 20 us, which chunks overlap with other chunks' tiles.
+bool by_clusters(const tree::Args& a) { return (int64_t)a.batch * a.kv_heads <= 32 && tree_keys(a) <= 16384; }
+template <int D, int N> int tc_draft(const tree::Args& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  using F = tc::Draft<D, N>;
+  if (int rc = opt_in(tc::draft_kernel<D, N>, F::kBytes)) return rc;
+  LaunchMark mark("tree_draft", st);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = tc::kDraftRanks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(a.batch * a.kv_heads * tc::kDraftRanks));
+  cfg.blockDim = dim3(F::kThreads);
+  cfg.dynamicSmemBytes = F::kBytes;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tc::draft_kernel<D, N>, k, v, a);
+  return e == cudaSuccess ? DILUTION_OK : abi_fail(DILUTION_ERR_CUDA, "tree_draft: %s", cudaGetErrorString(e));
+}
+
 template <int D> int tc_dilute(tree::Args a, void* scratch, cudaStream_t st) {
   CUtensorMap k, v;
   if (int rc = cache_maps(&k, &v, a, D)) return rc;
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
+  if (by_clusters(a)) return a.nodes <= 16 ? tc_draft<D, 16>(a, k, v, st) : a.nodes <= 32 ? tc_draft<D, 32>(a, k, v, st) : tc_draft<D, 64>(a, k, v, st);
   a.chunks = tc_chunks(heads, tree_keys(a), tc::Sweep<D, 64, true>::kPerSm);
   float* shares = place_scratch(a, scratch, D);
   if (int rc = tc_scan<D, false>(a, k, v, st)) return rc;

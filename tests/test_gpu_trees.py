@@ -80,7 +80,7 @@ def check_accept(before, cache, k, v, bids, bids_off, paths, length):
 
 
 @pytest.mark.parametrize("dtype,dim", TYPES)
-@pytest.mark.parametrize("length", [0, 1, 64, 130, 1111])
+@pytest.mark.parametrize("length", [0, 1, 64, 130, 1111, 17000])
 @pytest.mark.parametrize("chain", CHAINS)
 def test_dilution_tree(length, chain, dtype, dim):
     q, k, v, cache = case(1, 3, 3, len(TREE), dim, length, dtype)
