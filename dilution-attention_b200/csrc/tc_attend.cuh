@@ -91,7 +91,8 @@ template <int D, int NT> struct AttendForward {
   static constexpr int kOperands = (int)(NT * kTile + 2 * kRing * kHalf);
   static constexpr int kStats = NT * 2 * 128 * 8, kFlags = NT * 128 * 4;
   static constexpr int kBytes = kOperands + kStats + kFlags + 256 + 1024;
-  static constexpr int kWgCols = 64 + D;
+  static constexpr int kBufs = D == 128 ? 2 : 1;                                   // score buffers of a warpgroup
+  static constexpr int kWgCols = 64 * kBufs + D;
   static constexpr int kTmem = 2 * NT * kWgCols <= 256 ? 256 : 512;
   static_assert(2 * NT * kWgCols <= kTmem, "the warpgroups' columns fit the allocation");
   static_assert(NT * 128 * D * 4 <= (int)(2 * kRing * kHalf), "the merge area fits the ring");
@@ -144,10 +145,10 @@ __device__ __forceinline__ uint2 query_bits(const Row& r, int i0, int j) {
 
 // A warpgroup's step over the 64 scores of keys j0 .. at tS: P~ = 2^(z - reference) as bf16 over the scores, their sum
 // into s.  The reference is the maximum of the first half tile that a row sees and moves where a later one's P~ sum to more
-// than 2^40; only then is the accumulator rescaled.  bf16 has the range of fp32: P~ below that limit keeps 8 bits.
-template <int D, bool CAP, bool BIAS>
+// than 2^40; only then is the accumulator rescaled, once its products are through (settled).  bf16 has the range of fp32: P~ below that limit keeps 8 bits.
+template <int D, bool CAP, bool BIAS, typename Settled>
 __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row& r, float lin, float pre, int j0, int i, bool edge,
-                                             float& ref, float& s) {
+                                             float& ref, float& s, Settled settled) {
   float v[64];
   uint32_t pw[32];
   float ps;
@@ -212,6 +213,7 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
       const bool fresh = __all_sync(0xffffffffu, ref == -INFINITY);        // nothing accumulated yet
       const float f = fast_exp2(ref - (now == -INFINITY ? 0.f : now));
       if (!fresh) {
+        settled();
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           float o[16];
@@ -248,8 +250,10 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   float2* sStat = reinterpret_cast<float2*>(smem + F::kOperands);
   int* sFlag = reinterpret_cast<int*>(smem + F::kOperands + F::kStats);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::kOperands + F::kStats + F::kFlags);
-  const uint32_t qfull = smem_u32(bars), kfull = qfull + 8, kfree = kfull + 8 * R, sdone = kfree + 8 * R, pready = sdone + 16 * NT;
-  Ctl* ctl = reinterpret_cast<Ctl*>(bars + 1 + 2 * R + 4 * NT);
+  constexpr int NB = F::kBufs, NG = 2 * NT;                                        // score buffers, warpgroups
+  const uint32_t qfull = smem_u32(bars), kfull = qfull + 8, kfree = kfull + 8 * R, sdone = kfree + 8 * R, odone = sdone + 8 * NB * NG,
+                 pready = odone + 8 * NG;
+  Ctl* ctl = reinterpret_cast<Ctl*>(bars + 1 + 2 * R + (2 * NB + 1) * NG);
   __shared__ int s_range[2];
   __shared__ States s_state[NT];
 
@@ -278,8 +282,8 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     ctl->abort = 0;
     s_range[0] = INT_MAX;
     s_range[1] = 0;
-    for (int x = 0; x < 1 + 2 * R + 2 * NT; ++x) mbar_init(qfull + 8 * x, 1);        // qfull, kfull, kfree, sdone
-    for (int x = 0; x < 2 * NT; ++x) mbar_init(pready + 8 * x, 4);
+    for (int x = 0; x < 1 + 2 * R + (NB + 1) * NG; ++x) mbar_init(qfull + 8 * x, 1);        // qfull, kfull, kfree, sdone, odone
+    for (int x = 0; x < NB * NG; ++x) mbar_init(pready + 8 * x, 4);      // (of a buffer: a warp may be a half tile ahead of another)
     fence_barrier_init();
   }
   for (int x = tid; x < NT * 128; x += F::kThreads) sFlag[x] = 0;
@@ -318,7 +322,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       }
       for (int e = 0; e < R && e < nh; ++e) load_keys(e, e);
       mbar_wait_warp(qfull, 0, ctl, &g_attend_status, kErrWaitTma);
-      uint32_t pending = 0, flip = 0;                    // warpgroups with a P~ to come, the parity of the next
+      uint32_t pending = 0, flip = 0, side = 0;          // warpgroups with a P~ to come, the parity of the next, the buffer of its scores
       // (counters in place of remainders: this warp's time between two products is what the others wait for)
       int in = 0, out = 0, refill = 0;
       uint32_t phase = 0, back = 0, word[NT];
@@ -332,23 +336,29 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
           const int w = 2 * x + (e & 1);
-          const uint32_t tS = tmem + F::kWgCols * w;
-          if (pending >> w & 1) {                        // of half tile e - 2
-            mbar_wait_warp(pready + 8 * w, flip >> w & 1, ctl, &g_attend_status, kErrWaitTile);
-            flip ^= 1u << w;
-            pending &= ~(1u << w);
+          const uint32_t tW = tmem + F::kWgCols * w;
+          const bool seen = e < nh && (word[x] >> (hh & 31) & 1), old = pending >> w & 1;
+          const int was = side >> w & 1, now = NB == 2 ? was ^ 1 : 0;
+          auto scores = [&]() {
+            tc_fence_after();
+            mma_scores_wide<W>(lead, tW + 64 * now, Desc{dQ.lo + (TB >> 4) * x, dQ.hi}, kTileBytes, Desc{dK.lo + (HB >> 4) * in, dK.hi},
+                               HSub, id_s);
+            mma_commit(lead, sdone + 8 * (NB * w + now));   // the scores, and every product in front of them
+          };
+          if (NB == 2 && seen) scores();                   // into the other buffer, while the arithmetic is at the last ones
+          if (old) {                                       // of half tile e - 2
+            const int bar = NB * w + (NB == 2 ? was : 0);
+            mbar_wait_warp(pready + 8 * bar, flip >> bar & 1, ctl, &g_attend_status, kErrWaitTile);
+            flip ^= 1u << bar;
             tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)               // 16 keys per instruction: 16 rows of 128 B = 128 units
-              mma_ts(lead, tS + 64, tS + 8 * kk, dV, (HB >> 4) * out + 128 * kk, id_p, 1);
+            for (int kk = 0; kk < 4; ++kk)                 // 16 keys per instruction: 16 rows of 128 B = 128 units
+              mma_ts(lead, tW + 64 * NB, tW + 64 * (NB == 2 ? was : 0) + 8 * kk, dV, (HB >> 4) * out + 128 * kk, id_p, 1);
+            if (NB == 2) mma_commit(lead, odone + 8 * w);
           }
-          if (e < nh && (word[x] >> (hh & 31) & 1)) {
-            tc_fence_after();
-            mma_scores_wide<W>(lead, tS, Desc{dQ.lo + (TB >> 4) * x, dQ.hi}, kTileBytes, Desc{dK.lo + (HB >> 4) * in, dK.hi},
-                               HSub, id_s);
-            mma_commit(lead, sdone + 8 * w);             // the scores, and every product in front of them
-            pending |= 1u << w;
-          }
+          if (NB == 1 && seen) scores();
+          pending = seen ? pending | 1u << w : pending & ~(1u << w);
+          if (NB == 2 && seen) side ^= 1u << w;
         }
         if (e >= 2) {
           mma_commit(lead, kfree + 8 * out);
@@ -365,12 +375,13 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
         if (++in == R) { in = 0; phase ^= 1; }
       }
 #pragma unroll
-      for (int w = 0; w < 2 * NT; ++w) mma_commit(lead, sdone + 8 * w);              // the last products
+      for (int w = 0; w < NG; ++w)
+        if (NB == 1) mma_commit(lead, sdone + 8 * w);                                // the last products
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------ the compute warps: lane = query
-    const uint32_t tS = tmem + F::kWgCols * wg + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 64;
+    const uint32_t tS = tmem + F::kWgCols * wg + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 64 * NB;
     {
       uint32_t z[16];
 #pragma unroll
@@ -385,15 +396,27 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     for (int e = half; e < nh; e += 2) {
       const int hh = last - e, what = (int)uniform(hh < kStates ? s_state[tile].of(hh) : state(tile, hh));
       if (what == 0) continue;
-      mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
-      ++turn;
+      // (two buffers: the first scores go to buffer 1)
+      const int side = NB == 2 ? (turn & 1) ^ 1 : 0;
+      mbar_wait_warp(sdone + 8 * (NB * wg + side), (NB == 2 ? turn >> 1 : turn) & 1, ctl, &g_attend_status, kErrWaitMma);
       tc_fence_after();
-      forward_step<D, CAP, BIAS>(tS, tO, r, lin, pre, hh * 64, is, what == 1, ref, s);
+      auto settled = [&]() {                               // the products of the half tiles before this one are through
+        if (NB == 2 && turn > 0) {
+          // (one phase after the other: a wait for the second alone would pass while the first is under way)
+          if (turn > 1) mbar_wait_warp(odone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
+          mbar_wait_warp(odone + 8 * wg, (turn - 1) & 1, ctl, &g_attend_status, kErrWaitMma);
+          tc_fence_after();
+        }
+      };
+      forward_step<D, CAP, BIAS>(tS + 64 * side, tO, r, lin, pre, hh * 64, is, what == 1, ref, s, settled);
+      ++turn;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(pready + 8 * wg);
+      if (lane == 0) mbar_arrive(pready + 8 * (NB * wg + side));
     }
-    if (nh > 0) mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
+    if (NB == 2 && turn > 1) mbar_wait_warp(odone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
+    if (NB == 2 ? turn > 0 : nh > 0)
+      mbar_wait_warp(NB == 2 ? odone + 8 * wg : sdone + 8 * wg, (NB == 2 ? turn - 1 : turn) & 1, ctl, &g_attend_status, kErrWaitMma);
     tc_fence_after();
     // every product has read the ring, which the merge goes over
     asm volatile("bar.sync 1, %0;" ::"n"(256 * NT) : "memory");
