@@ -60,9 +60,9 @@ SIGNATURES = {
     "dilution_variant_decode": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _F, _F, _I, _I, _F, _P, _P, _P, _P]),
     "dilution_attend_ranges_bytes": (_Z, [_L, _L]),
     "dilution_attend_scratch_bytes": (_Z, [_L, _L, _L]),
-    "dilution_attend_forward": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _I, _F, _F, _P, _P, _P, _P, _P, _P, _P]),
+    "dilution_attend_forward": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _I, _F, _F, _P, _P, _P, _P, _P, _P, _P, _P]),
     "dilution_attend_backward": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _I, _F, _F, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
-                                      _P]),
+                                      _P, _P]),
     "dilution_tree_scratch_bytes": (_Z, [_L, _L, _I, _I, _L, _I]),
     "dilution_tree_softmax": (_I, [_P, _P, _P, _P, _P, _I, _L, _L, _I, _I, _L, _L, _P, _I, _F, _F, _P, _P, _L, _P, _P, _P,
                                    _P]),

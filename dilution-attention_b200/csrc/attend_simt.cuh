@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a, int 
     const float out = sum == 0.f ? 0.f : acc / sum;
     if (!isfinite(out)) sFlag[row] = 1;
     reinterpret_cast<T*>(a.out)[(n * a.t + i0 + row) * D + c] = from_f32<T>(out);
+    if (a.rest != nullptr) reinterpret_cast<T*>(a.rest)[(n * a.t + i0 + row) * D + c] = from_f32<T>(left_off<T>(out));
     if (a.lse != nullptr && c == 0) a.lse[n * a.t + i0 + row] = sum == 0.f ? INFINITY : top + log2f(sum);
   }
   each_flagged(sFlag, first, last, [&](int row) { redo_forward_row<T, D>(a, b, h, i0 + row); });

@@ -31,7 +31,8 @@ int check_attend(const char* fn, const attend::Args& a, int dtype, int d) {
   if (!(a.cap >= 0.f) || a.cap > 3e38f || !(a.scale > 0.f))
     return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap finite, 0 for none", fn);
   if (!a.q || !a.k || !a.v || !a.out || (a.docs && !a.ranges)) return abi_fail(DILUTION_ERR_ARG, "%s: null pointer", fn);
-  if (misaligned({a.q, a.k, a.v, a.out, a.dout, a.dq, a.dk, a.dv, a.ranges}))
+  if (a.rest && dtype != DILUTION_BF16) return abi_fail(DILUTION_ERR_ARG, "%s: rest is of bf16 outputs alone", fn);
+  if (misaligned({a.q, a.k, a.v, a.out, a.rest, a.dout, a.dq, a.dk, a.dv, a.ranges}))
     return abi_fail(DILUTION_ERR_ARG, "%s: tensors must be 16-byte aligned", fn);
   return DILUTION_OK;
 }
@@ -75,7 +76,7 @@ template <typename T, int D> int simt_forward(const attend::Args& a, cudaStream_
 template <typename T, int D> int launch_delta(const attend::Args& a, cudaStream_t st) {
   LaunchMark mark("attend_delta", st);
   const int64_t rows = (int64_t)a.batch * a.heads * a.t, threads = rows * D * (int)sizeof(T) / 16;
-  attend::delta_kernel<T, D><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>((const T*)a.dout, (const T*)a.out, rows, a.delta);
+  attend::delta_kernel<T, D><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a, rows);
   return abi_check_launch("attend_delta");
 }
 
@@ -159,12 +160,13 @@ size_t delta_bytes(int64_t batch, int64_t heads, int64_t t) { return (size_t)((b
 
 attend::Args attend_args(const void* q, const void* k, const void* v, int64_t batch, int64_t heads, int64_t kv_heads, int64_t t,
                          float scale, float cap, const float* slopes, const int* documents, const int* prefix, void* ranges,
-                         void* out, float* lse) {
+                         void* out, void* rest, float* lse) {
   attend::Args a{};
   a.q = q;
   a.k = k;
   a.v = v;
   a.out = out;
+  a.rest = rest;
   a.lse = lse;
   a.slopes = slopes;
   a.docs = documents;
@@ -198,8 +200,9 @@ size_t dilution_attend_scratch_bytes(int64_t batch, int64_t heads, int64_t t) {
 
 int dilution_attend_forward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
                             int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
-                            const int* documents, const int* prefix, void* ranges, void* out, float* lse, void* stream) {
-  const attend::Args a = attend_args(q, k, v, batch, heads, kv_heads, t, scale, cap, slopes, documents, prefix, ranges, out, lse);
+                            const int* documents, const int* prefix, void* ranges, void* out, void* rest, float* lse,
+                            void* stream) {
+  const attend::Args a = attend_args(q, k, v, batch, heads, kv_heads, t, scale, cap, slopes, documents, prefix, ranges, out, rest, lse);
   if (int rc = check_attend("dilution_attend_forward", a, dtype, d)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = launch_ranges(a, st)) return rc;
@@ -213,10 +216,10 @@ int dilution_attend_forward(const void* q, const void* k, const void* v, int dty
 
 int dilution_attend_backward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
                              int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
-                             const int* documents, const int* prefix, const void* ranges, const void* out, const float* lse,
-                             const void* dout, void* scratch, void* dq, void* dk, void* dv, void* stream) {
+                             const int* documents, const int* prefix, const void* ranges, const void* out, const void* rest,
+                             const float* lse, const void* dout, void* scratch, void* dq, void* dk, void* dv, void* stream) {
   attend::Args a = attend_args(q, k, v, batch, heads, kv_heads, t, scale, cap, slopes, documents, prefix,
-                               const_cast<void*>(ranges), const_cast<void*>(out), const_cast<float*>(lse));
+                               const_cast<void*>(ranges), const_cast<void*>(out), const_cast<void*>(rest), const_cast<float*>(lse));
   a.dout = dout;
   a.delta = (float*)scratch;
   a.dq = dq;

@@ -1,6 +1,7 @@
 // Softmax attention with caps, biases and masks (attend_common.cuh) on the tensor cores: bf16 heads of 64 and 128.
 // Operand tiles come in by TMA, products are tcgen05.mma with accumulators in TMEM, and the values that a thread forms
-// (P~, dS) go back into TMEM over the scores it has read, as the A operand of the next product.  A warp of its own issues
+// (P~, dS) go back into TMEM over the scores it has read, as the A operand of the next product: in bf16, the operands' type, each
+// off by up to 2^-8 of itself.  References, sums, lse, delta and accumulators are fp32.  A warp of its own issues
 // every copy and MMA.  Which pairs of tiles have anything to do is asked of the documents' ranges, never of a list.
 //
 //   forward : a CTA's query tiles of 128 (two of heads of 64, one of 128) walk over half tiles of 64 keys; two warpgroups per query
@@ -468,11 +469,19 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       for (int c = 0; c < 32; ++c) sum = fmaf(o[c], 0.f, sum);
       bad = bad || sum != 0.f;
       if (i < r.t) {
-        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + ((int64_t)n * a.t + i) * D + kPart * half + c0);
+        const int64_t at = (((int64_t)n * a.t + i) * D + kPart * half + c0) / 8;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          dst[c] = make_uint4(pack_pair(o[8 * c], o[8 * c + 1]), pack_pair(o[8 * c + 2], o[8 * c + 3]),
-                              pack_pair(o[8 * c + 4], o[8 * c + 5]), pack_pair(o[8 * c + 6], o[8 * c + 7]));
+          reinterpret_cast<uint4*>(a.out)[at + c] =
+              make_uint4(pack_pair(o[8 * c], o[8 * c + 1]), pack_pair(o[8 * c + 2], o[8 * c + 3]),
+                         pack_pair(o[8 * c + 4], o[8 * c + 5]), pack_pair(o[8 * c + 6], o[8 * c + 7]));
+        if (a.rest != nullptr) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            reinterpret_cast<uint4*>(a.rest)[at + c] =
+                make_uint4(left_pair(o[8 * c], o[8 * c + 1]), left_pair(o[8 * c + 2], o[8 * c + 3]),
+                           left_pair(o[8 * c + 4], o[8 * c + 5]), left_pair(o[8 * c + 6], o[8 * c + 7]));
+        }
       }
     }
     if (half == 0 && i < r.t && a.lse != nullptr) a.lse[(int64_t)n * a.t + i] = den == 0.f ? INFINITY : m + log2f(den);
@@ -776,7 +785,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
   if (warp == 0) tmem_free(tmem, F::kTmem);
 }
 
-// lse and delta_i = dout_i . out_i of every query, padded, as the kernels above read them.  D / 8 lanes a row, 16 bytes each.
+// lse and delta_i of every query, padded, as the kernels above read them.  D / 8 lanes a row, 16 bytes each.
 template <int D>
 __global__ void __launch_bounds__(256) attend_stats_kernel(attend::Args a, float2* __restrict__ stats) {
   constexpr int L = D / 8;
@@ -784,15 +793,7 @@ __global__ void __launch_bounds__(256) attend_stats_kernel(attend::Args a, float
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L, n = at / padded;
   const int i = (int)(at % padded), u = threadIdx.x % L;
   const bool real = n < (int64_t)a.batch * a.heads && i < a.t;
-  float s = 0.f;
-  if (real) {
-    const int64_t x = (n * a.t + i) * L + u;
-    const uint4 g = reinterpret_cast<const uint4*>(a.dout)[x], o = reinterpret_cast<const uint4*>(a.out)[x];
-    const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(&g);
-    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(&o);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(to_f32(p[e]), to_f32(q[e]), s);
-  }
+  float s = real ? attend::delta_part<__nv_bfloat16>(a, (n * a.t + i) * L + u) : 0.f;
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (u == 0 && n < (int64_t)a.batch * a.heads) {

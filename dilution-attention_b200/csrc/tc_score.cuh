@@ -14,6 +14,12 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return r;
 }
 
+// What the rounding of such a pair leaves off.
+__device__ __forceinline__ uint32_t left_pair(float lo, float hi) {
+  const uint32_t r = pack_pair(lo, hi);
+  return pack_pair(lo - __uint_as_float(r << 16), hi - __uint_as_float(r & 0xffff0000u));
+}
+
 // Head sizes: D / 64 sub-tiles of 64 features (tc_common.cuh).
 template <int D> constexpr int kForm = D == 128 ? kWide128 : kNarrow;
 

@@ -93,7 +93,8 @@ def check_heads(q, k, v):
 
 
 class _SoftmaxAttention(torch.autograd.Function):
-    """Saved for the backward: q, k, v and out as the kernels took them, lse, and the ranges of the documents' ids."""
+    """Saved for the backward: q, k, v and out as the kernels took them, what out's rounding to bf16 left off, lse, and the
+    ranges of the documents' ids."""
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, documents, prefix, softcap):
@@ -106,16 +107,17 @@ class _SoftmaxAttention(torch.autograd.Function):
         train = any(ctx.needs_input_grad[:3])
         q, k, v = (aligned(x) for x in (q, k, v))
         lse = torch.empty(batch, heads, seq, device=q.device, dtype=torch.float32) if train else None
+        rest = torch.empty_like(out) if train and q.dtype == torch.bfloat16 else None
         ranges = None
         if documents is not None:
             ranges = torch.empty(lib.dilution_attend_ranges_bytes(batch, seq), device=q.device, dtype=torch.uint8)
         with on_device(q.device):
             _lib.check(lib.dilution_attend_forward(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _CODE[q.dtype], batch, heads, kv_heads, seq, dim, 1.0 / math.sqrt(dim),
-                softcap, K._ptr(slopes), K._ptr(documents), K._ptr(prefix), K._ptr(ranges), out.data_ptr(), K._ptr(lse),
-                K._stream(q.device)), "dilution_attend_forward")
+                softcap, K._ptr(slopes), K._ptr(documents), K._ptr(prefix), K._ptr(ranges), out.data_ptr(), K._ptr(rest),
+                K._ptr(lse), K._stream(q.device)), "dilution_attend_forward")
         if train:
-            ctx.save_for_backward(q, k, v, out, lse, slopes, documents, prefix, ranges)
+            ctx.save_for_backward(q, k, v, out, rest, lse, slopes, documents, prefix, ranges)
         return out
 
     @staticmethod
@@ -125,7 +127,7 @@ class _SoftmaxAttention(torch.autograd.Function):
         if dout.numel() == 0:
             kv = (batch, kv_heads, seq, dim)
             return dout, dout.new_zeros(kv), dout.new_zeros(kv), None, None, None, None
-        q, k, v, out, lse, slopes, documents, prefix, ranges = ctx.saved_tensors
+        q, k, v, out, rest, lse, slopes, documents, prefix, ranges = ctx.saved_tensors
         lib = _lib.load()
         dout = aligned(dout)
         dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
@@ -133,8 +135,8 @@ class _SoftmaxAttention(torch.autograd.Function):
         with on_device(q.device):
             _lib.check(lib.dilution_attend_backward(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _CODE[q.dtype], batch, heads, kv_heads, seq, dim, 1.0 / math.sqrt(dim),
-                ctx.softcap, K._ptr(slopes), K._ptr(documents), K._ptr(prefix), K._ptr(ranges), out.data_ptr(), lse.data_ptr(),
-                dout.data_ptr(), scratch.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), K._stream(q.device)),
+                ctx.softcap, K._ptr(slopes), K._ptr(documents), K._ptr(prefix), K._ptr(ranges), out.data_ptr(), K._ptr(rest),
+                lse.data_ptr(), dout.data_ptr(), scratch.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), K._stream(q.device)),
                 "dilution_attend_backward")
         return dq, dk, dv, None, None, None, None
 

@@ -400,18 +400,20 @@ int dilution_variant_decode(const void* q1, const void* k1, const void* v1, void
  * j < prefix[b] if prefix (batch) is not NULL, and where documents (batch, t), if not NULL, gives both the same id >= 0.  A
  * query that sees no key has out = 0 and lse = +inf.  With documents, `ranges` is a buffer of
  * dilution_attend_ranges_bytes(batch, t) that the forward fills and the backward reads.  lse (batch, heads, t) fp32: log2 of
- * the sum of 2^(score log2 e), or NULL.
+ * the sum of 2^(score log2 e), or NULL.  rest, for bf16 alone: NULL, or like out: what the rounding of out left off, which the
+ * backward adds to out again (its dq and dk are less exact without, most of all of queries that see a few keys).
  * The backward takes what the forward wrote, dout like out, and scratch of dilution_attend_scratch_bytes(batch, heads, t), 16-byte
  * aligned; dq, dk, dv are like q, k, v.  All results repeat bit for bit. */
 size_t dilution_attend_ranges_bytes(int64_t batch, int64_t t);
 size_t dilution_attend_scratch_bytes(int64_t batch, int64_t heads, int64_t t);
 int dilution_attend_forward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
                             int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
-                            const int* documents, const int* prefix, void* ranges, void* out, float* lse, void* stream);
+                            const int* documents, const int* prefix, void* ranges, void* out, void* rest, float* lse,
+                            void* stream);
 int dilution_attend_backward(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads,
                              int64_t kv_heads, int64_t t, int d, float scale, float cap, const float* slopes,
-                             const int* documents, const int* prefix, const void* ranges, const void* out, const float* lse,
-                             const void* dout, void* scratch, void* dq, void* dk, void* dv, void* stream);
+                             const int* documents, const int* prefix, const void* ranges, const void* out, const void* rest,
+                             const float* lse, const void* dout, void* scratch, void* dq, void* dk, void* dv, void* stream);
 
 /* ---- draft trees over a cache -------------------------------------------------------------------------------------
  * `nodes` (1 to 64) drafted tokens of each sequence: q, out (batch, kv_heads * group, nodes, d), k_new, v_new

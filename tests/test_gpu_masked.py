@@ -103,6 +103,22 @@ def test_heads_that_share_keys(dtype, dim, heads, kv_heads):
     check(inputs(2, heads, kv_heads, 150, dim, dtype))
 
 
+@pytest.mark.parametrize("dim", [16, 32])
+@pytest.mark.parametrize("seq", [1, 2, 7])
+def test_few_keys_and_the_rounding_of_out(seq, dim):
+    """ds = p (dout . v - delta) is a difference; delta is of out before its rounding to bf16.  Off by, next to terms of size
+    e = sum_d |dout_d| (|v_jd| + |out_d|): 2^-16 e for the rounded rest of out (2^-8 of 2^-8), 2^-18 e for 32-bit sums of up to
+    32 + 7 terms and the exponential; and dq's own rounding, 2^-8 of it."""
+    q, k, v, dout = x = inputs(4, 8, 8, seq, dim, torch.bfloat16, seed=11)
+    _, dq, _, _ = call(x)
+    q, k, v, dout = (t.double() for t in x)
+    p = (q @ k.mT / dim ** 0.5).masked_fill(torch.ones(seq, seq, device=DEV).tril() == 0, -torch.inf).softmax(-1)
+    out = p @ v
+    want = p * (dout @ v.mT - (dout * out).sum(-1, keepdim=True)) @ k / dim ** 0.5
+    size = p * (dout.abs() @ v.abs().mT + (dout * out).abs().sum(-1, keepdim=True)) @ k.abs() / dim ** 0.5
+    assert ((dq.double() - want).abs() <= 2 ** -8 * want.abs() + (2 ** -16 + 2 ** -18) * size).all()
+
+
 @pytest.mark.parametrize("dtype,dim", TYPES[:4])
 def test_long_rows(dtype, dim):
     check(inputs(1, 2, 1, 2100, dim, dtype), documents=documents_of(1, 2100, 700, seed=9))

@@ -28,7 +28,7 @@ def message(rc):
 
 def attend(dtype=1, batch=1, heads=2, kv=2, t=8, d=64, scale=0.125, cap=0.0, q=ONE, docs=None, ranges=None, out=ONE):
     lib = load_package()._lib.load()
-    return lib.dilution_attend_forward(q, ONE, ONE, dtype, batch, heads, kv, t, d, scale, cap, None, docs, None, ranges, out, None, None)
+    return lib.dilution_attend_forward(q, ONE, ONE, dtype, batch, heads, kv, t, d, scale, cap, None, docs, None, ranges, out, None, None, None)
 
 
 @pytest.mark.parametrize("change,rc,text", [
@@ -43,8 +43,8 @@ def test_attend_forward(change, rc, text):
 
 def test_attend_backward():
     lib = load_package()._lib.load()
-    args = [ONE, ONE, ONE, 1, 1, 2, 2, 8, 64, 0.125, 0.0, None, None, None, None, ONE, ONE, ONE, ONE, ONE, ONE, ONE, None]
-    for at in (16, 17, 18, 19, 20, 21):
+    args = [ONE, ONE, ONE, 1, 1, 2, 2, 8, 64, 0.125, 0.0, None, None, None, None, ONE, ONE, ONE, ONE, ONE, ONE, ONE, ONE, None]
+    for at in (17, 18, 19, 20, 21, 22):
         rc = lib.dilution_attend_backward(*args[:at], None, *args[at + 1:])
         assert rc == 1 and "null" in message(rc)
 
@@ -195,3 +195,9 @@ def test_a_recorded_decode_refuses_evicted_caches_of_rotated_layers():
     model = SimpleNamespace(config=SimpleNamespace(positional="rope"))
     with pytest.raises(ValueError, match="evicted"):
         lib.GraphedDecode(model, [caches(evicted=3)])
+
+
+def test_rest_is_of_bf16_outputs():
+    lib = load_package()._lib.load()
+    rc = lib.dilution_attend_forward(ONE, ONE, ONE, 0, 1, 2, 2, 8, 64, 0.125, 0.0, None, None, None, None, ONE, ONE, None, None)
+    assert rc == 1 and "rest" in message(rc)
