@@ -26,7 +26,7 @@ int check_attend(const char* fn, const attend::Args& a, int dtype, int d) {
   if (a.batch < 1 || a.heads < 1 || a.kv_heads < 1 || a.t < 1 || a.heads % a.kv_heads != 0)
     return abi_fail(DILUTION_ERR_ARG, "%s: sizes must be positive and kv_heads divide heads (batch=%d heads=%d kv_heads=%d t=%d)", fn,
                     a.batch, a.heads, a.kv_heads, a.t);
-  if (a.t > (1 << 30) || (int64_t)a.batch * a.heads * doc_spans(a.t) >= (int64_t)1 << 31)
+  if (a.t > (1 << 30) || (double)a.batch * a.heads * (double)doc_spans(a.t) >= 2147483648.0)
     return abi_fail(DILUTION_ERR_ARG, "%s: batch * heads * blocks exceeds the grid limit", fn);
   if (!(a.cap >= 0.f) || a.cap > 3e38f || !(a.scale > 0.f))
     return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap finite, 0 for none", fn);

@@ -698,6 +698,8 @@ def _fused_step_cache(self, x1, cache):
     the decode launch; falls back to the model's own method whenever that one
     would not take the kernel path."""
     if not self._kernel_ok(x1) or not self._standard():
+        if cache.get("evicted") and self.rope is not None:
+            raise ValueError("this layer's own cached step rotates by the cache's length, which evicted keys are missing from")
         return self._unfused_step_cache(x1, cache)
     batch = x1.shape[0]
     if cache.get("pos_dev") is not None:       # the position lives on the device (a captured step)

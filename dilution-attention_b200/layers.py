@@ -300,6 +300,8 @@ def _softmax_begin_cache(self, x, capacity=None):
 def _softmax_step_cache(self, x1, cache):
     """CausalSelfAttention.step_cache (model.py:112-117) on the streaming decode kernels."""
     if not x1.is_cuda or (self.d_model // self.n_heads) not in (16, 32, 64, 128):
+        if cache.get("evicted") and self.rope is not None:
+            raise ValueError("this layer's own cached step rotates by the cache's length, which evicted keys are missing from")
         return self._b200_step_cache(x1, cache)
     batch = x1.shape[0]
     if cache.get("pos_dev") is not None:       # the position lives on the device (a captured step)

@@ -122,7 +122,8 @@ def _buffers(sizes, pos_dev, like, out, scratch):
     elif out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like q")
     need = _scratch_bytes(batch, kv_heads, heads // kv_heads, nodes, capacity if pos_dev is not None else length, dim)
-    if scratch is None or scratch.numel() * scratch.element_size() < need or scratch.data_ptr() % 16:
+    if scratch is None or scratch.numel() * scratch.element_size() < need or scratch.data_ptr() % 16 or not scratch.is_contiguous() \
+            or scratch.device != like.device:
         scratch = torch.empty(need, device=like.device, dtype=torch.uint8)
     return out, scratch
 
@@ -135,13 +136,16 @@ def softmax_tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: 
     q: (B, H, N, D), N <= 64; k, v: (B, H_kv, N, D) of the drafted tokens, rotated for their positions len + depth where
     the layer rotates; cache: {"k", "v", "len"} with H_kv heads.  parents: (N,), or (B, N) for a tree of each sequence: the
     earlier node that a node follows, -1 for the last cached token (a device tensor is not checked: any other number counts
-    as -1).  softcap and slopes as in softmax_attention, by the distance of the positions.  out and scratch are optional
-    buffers.  out: (B, H, N, D) in q's dtype; draft is for tree_accept.  The cache is only read; with cache["pos_dev"] its
+    as -1).  softcap and slopes as in softmax_attention, by the distance of the positions (no slopes over a cache that keys
+    were evicted from).  out and scratch are optional buffers.  out: (B, H, N, D) in q's dtype; draft is for tree_accept, and
+    refers to q, k, v and parents: they stay as they are until then.  The cache is only read; with cache["pos_dev"] its
     length is read from the device, so that the step can be recorded into a CUDA graph.
     """
     draft, sizes, (kc, vc), pos_dev = _draft(q, k, v, cache, parents)
     batch, heads, kv_heads, nodes, dim, capacity, length = sizes
     draft["softcap"], draft["slopes"] = check_softcap(softcap), check_slopes(slopes, heads, q.device)
+    if slopes is not None and cache.get("evicted"):
+        raise ValueError("a cache that keys were evicted from does not know its keys' positions, which slopes need")
     lib = _lib.load()
     out, scratch = _buffers(sizes, pos_dev, q, out, scratch)
     with on_device(q.device):
@@ -165,6 +169,8 @@ def dilution_tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
     batch, heads, kv_heads, nodes, dim, capacity, length = sizes
     if kv_heads != heads:
         raise ValueError("a dilution layer has as many key heads as query heads")
+    if cache.get("committed") is None:
+        raise ValueError("a dilution layer's cache holds the committed demand of its keys")
     committed = _demand(cache["committed"], batch, heads, capacity, q.device)
     lib = _lib.load()
     out, scratch = _buffers(sizes, pos_dev, q, out, scratch)

@@ -124,6 +124,20 @@ def test_long_rows(dtype, dim):
     check(inputs(1, 2, 1, 2100, dim, dtype), documents=documents_of(1, 2100, 700, seed=9))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_more_half_tiles_than_a_block_keeps_notes_of(dim):
+    """270000 tokens, which are over 4096 half tiles of keys, in documents of 450: the first and the last ones as rows of their own."""
+    seq, doc, near = 270000, 450, 8
+    docs = (torch.arange(seq, device=DEV) // doc).expand(1, seq).contiguous()
+    x = inputs(1, 2, 1, seq, dim, torch.bfloat16)
+    got = call(x, documents=docs)
+    for first in (0, seq // 2 // doc * doc, seq - near * doc):
+        rows = [t[0, :, first:first + near * doc].unflatten(1, (near, doc)).transpose(0, 1) for t in (*x, *got)]
+        want, off = O.attention(*rows[:4])
+        for a, b, far in zip(rows[4:], want, off):
+            assert ((a.double() - b).abs() <= far + 1e-12).all()
+
+
 @pytest.mark.parametrize("dtype,dim", TYPES[:4])
 @pytest.mark.parametrize("std", [8.0, 40.0])
 def test_peaked_scores(dtype, dim, std):

@@ -288,3 +288,74 @@ def test_two_streams_at_once():
             got.append(lib.dilution_tree_step(q, k, v, cache, tree)[0])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("nodes", [9, 20, 40, 64])
+@pytest.mark.parametrize("dtype,dim", TYPES[:3])
+@pytest.mark.parametrize("batch,heads,length", [(3, 11, 300), (1, 2, 16400)])
+def test_caches_in_chunks(batch, heads, length, nodes, dtype, dim):
+    """More heads, or more keys, than a step by clusters takes: the demand crosses kernels and chunks."""
+    trees = [random_tree(nodes, s) for s in range(batch)]
+    q, k, v, cache = case(batch, heads, heads, nodes, dim, length, dtype)
+    parents = torch.tensor(trees, device=DEV, dtype=torch.int32)
+    lib = load_package()
+    out, draft = lib.dilution_tree_step(q, k, v, cache, parents)
+    want, off, bids, bids_off = O.tree_nodes(q, k, v, cache["k"], cache["v"], length, trees, committed=cache["committed"])
+    within(out, want, off)
+    again, _ = lib.dilution_tree_step(q, k, v, cache, parents)
+    assert torch.equal(out, again)
+    before = clone(cache)
+    lib.tree_accept(cache, draft, [0])
+    check_accept(before, cache, k, v, bids, bids_off, [[0]] * batch, length)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_recorded_step_in_chunks_beside_an_eager_one(dim):
+    """40 heads: the step's launches start early behind one another, in a graph as on a stream."""
+    lib = load_package()
+    tree = random_tree(24, 5)
+    q, k, v, cache = case(2, 20, 20, 24, dim, 900, torch.bfloat16)
+    parents = torch.tensor(tree, device=DEV, dtype=torch.int32)
+    want = lib.dilution_tree_step(q, k, v, cache, parents)[0]
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = lib.dilution_tree_step(q, k, v, cache, parents)[0]
+        graphs.append((graph, got))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for stream, (graph, got) in zip(streams, graphs):
+            got.zero_()
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = lib.dilution_tree_step(q, k, v, cache, parents)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want) and all(torch.equal(got, want) for _, got in graphs)
+
+
+@pytest.mark.parametrize("dtype,dim", TYPES[:3])
+def test_cached_keys_that_are_not_finite(dtype, dim):
+    """A NaN key reaches its own head's rows alone, in either layer and on both of a dilution step's ways."""
+    lib = load_package()
+    for heads in (2, 40):
+        q, k, v, cache = case(1, heads, heads, len(TREE), dim, 150, dtype)
+        clean = [lib.softmax_tree_step(q, k, v, cache, TREE)[0], lib.dilution_tree_step(q, k, v, cache, TREE)[0]]
+        cache["k"][0, 1, 77, 3] = float("nan")
+        got = [lib.softmax_tree_step(q, k, v, cache, TREE)[0], lib.dilution_tree_step(q, k, v, cache, TREE)[0]]
+        others = [h for h in range(heads) if h != 1]
+        for a, b in zip(clean, got):
+            assert b[0, 1].isnan().all() and torch.equal(a[:, others], b[:, others])
+
+
+def test_strided_tokens_and_a_scratch_that_does_not_do():
+    """Rows as a projection leaves them, (B, N, H, D); a scratch that is a view of fewer bytes than it counts is not used."""
+    lib = load_package()
+    q, k, v, cache = case(2, 4, 4, len(TREE), 64, 200, torch.bfloat16)
+    want = lib.softmax_tree_step(q, k, v, cache, TREE)[0]
+    strided = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    scratch = torch.zeros(16, device=DEV, dtype=torch.uint8).expand(1 << 20, 16)
+    assert torch.equal(lib.softmax_tree_step(*strided, cache, TREE, scratch=scratch)[0], want)
+    assert not scratch[0].any()

@@ -201,3 +201,58 @@ def test_rest_is_of_bf16_outputs():
     lib = load_package()._lib.load()
     rc = lib.dilution_attend_forward(ONE, ONE, ONE, 0, 1, 2, 2, 8, 64, 0.125, 0.0, None, None, None, None, ONE, ONE, None, None)
     assert rc == 1 and "rest" in message(rc)
+
+
+def test_attend_sizes_whose_product_wraps():
+    big = (1 << 31) - 1
+    got = attend(batch=big, heads=big, kv=1, t=1 << 30)
+    assert got == 1 and "grid" in message(got)
+
+
+def test_slopes_over_an_evicted_cache():
+    lib = load_package()
+    q, k = fake(1, 4, 3, 64), fake(1, 2, 3, 64)
+    with pytest.raises(ValueError, match="evicted"):
+        lib.softmax_tree_step(q, k, k, caches(evicted=2), [-1, 0, 1], slopes=torch.zeros(4))
+
+
+def test_a_dilution_step_needs_the_demand():
+    q = fake(1, 2, 3, 64)
+    with pytest.raises(ValueError, match="committed"):
+        load_package().dilution_tree_step(q, q, q, caches(), [-1, 0, 1])
+
+
+class Rotated:
+    """A layer of the model as far as the cached steps ask."""
+    rope, d_model, n_heads = object(), 128, 2
+
+    def __init__(self, fast):
+        self.fast = fast
+
+    def _kernel_ok(self, x):
+        return self.fast
+
+    def _standard(self):
+        return True
+
+    def _split_heads(self, x, offset):
+        raise StopIteration(offset)
+
+    def _unfused_step_cache(self, x, cache):
+        raise LookupError
+
+    _b200_step_cache = _unfused_step_cache
+
+
+@pytest.mark.parametrize("name,fused", [("kernels", "_fused_step_cache"), ("layers", "_softmax_step_cache")])
+def test_cached_steps_rotate_by_the_tokens_that_there_have_been(name, fused):
+    step = getattr(getattr(load_package(), name), fused)
+    for evicted, offset in ((0, 8), (5, 13)):
+        with pytest.raises(StopIteration) as stop:
+            step(Rotated(True), fake(1, 1, 128), caches(evicted=evicted))
+        assert stop.value.args == (offset,)
+    # a layer whose own step runs instead: it would rotate by the cache's length
+    with pytest.raises(ValueError, match="evicted"):
+        step(Rotated(False), torch.zeros(1, 1, 128), caches(evicted=5))
+    with pytest.raises(LookupError):
+        step(Rotated(False), torch.zeros(1, 1, 128), caches())
