@@ -401,21 +401,21 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       const int side = NB == 2 ? (turn & 1) ^ 1 : 0;
       mbar_wait_warp(sdone + 8 * (NB * wg + side), (NB == 2 ? turn >> 1 : turn) & 1, ctl, &g_attend_status, kErrWaitMma);
       tc_fence_after();
-      auto settled = [&]() {                               // the products of the half tiles before this one are through
+      // The products of the half tiles before this one are through.  Every turn asks before it lets its own products start, so that the
+      // barrier is never more than one phase from the one asked for, where parities would be taken for one another.
+      auto settled = [&]() {
         if (NB == 2 && turn > 0) {
-          // (one phase after the other: a wait for the second alone would pass while the first is under way)
-          if (turn > 1) mbar_wait_warp(odone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
           mbar_wait_warp(odone + 8 * wg, (turn - 1) & 1, ctl, &g_attend_status, kErrWaitMma);
           tc_fence_after();
         }
       };
       forward_step<D, CAP, BIAS>(tS + 64 * side, tO, r, lin, pre, hh * 64, is, what == 1, ref, s, settled);
+      settled();
       ++turn;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(pready + 8 * (NB * wg + side));
     }
-    if (NB == 2 && turn > 1) mbar_wait_warp(odone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
     if (NB == 2 ? turn > 0 : nh > 0)
       mbar_wait_warp(NB == 2 ? odone + 8 * wg : sdone + 8 * wg, (NB == 2 ? turn - 1 : turn) & 1, ctl, &g_attend_status, kErrWaitMma);
     tc_fence_after();

@@ -147,6 +147,14 @@ def test_peaked_scores(dtype, dim, std):
     check((x[0], (x[1] * ramp).to(dtype), x[2], x[3]))
 
 
+@pytest.mark.parametrize("dtype,dim", TYPES[:4])
+def test_scores_that_grow_with_the_distance(dtype, dim):
+    """By about 90 (in the exponent of 2) over 64 keys: whatever the order of the keys, the reference of a row moves many times."""
+    q, k, v, dout = inputs(1, 2, 1, 700, dim, dtype)
+    far = torch.arange(700, 0, -1, device=DEV)[:, None] * (dim ** -0.5 / 4)
+    check(((q / 8 + 4).to(dtype), (k + far).to(dtype), v, dout))
+
+
 @pytest.mark.parametrize("dtype,dim", TYPES)
 def test_ids_in_any_order(dtype, dim):
     """Documents that interleave: masks inside every tile."""
