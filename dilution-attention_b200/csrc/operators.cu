@@ -141,10 +141,11 @@ template <int D> int tc_backward(const attend::Args& a, float2* stats, cudaStrea
     if (int rc = abi_check_launch("attend_delta")) return rc;
   }
   // Heads of 64: two CTAs with a warpgroup each on an SM, whose starts and ends overlap, or one with three.  dk, dv and dq in us,
-  // two / one: n = 148, T = 512 32 + 25 / 40 + 33, T = 1024 77 + 63 / 92 + 76; n = 64, T = 4096 325 + 255 / 318 + 261, T = 8192
-  // 1227 + 938 / 1112 + 914, packed documents of 700 tokens (T = 4096) 156 + 119 / 178 + 145.
+  // two / one: n = 148, T = 512 25 + 19 / 31 + 24, T = 1024 68 + 54 / 79 + 64; n = 96, T = 2048 144 + 111 / 147 + 121; n = 64, T = 3000
+  // 184 + 149 / 181 + 155, T = 4096 324 + 249 / 294 + 248, T = 8192 1206 + 910 / 1066 + 881; documents of 700 tokens, T = 4096
+  // 120 + 95 / 143 + 115, T = 8192 235 + 185 / 281 + 230.
   if constexpr (D == 64) {
-    if (a.docs || a.t <= 4096) {
+    if (a.docs || a.t <= 2560) {
       if (int rc = tc_backward_half<D, 1, 1>(a, m, stats, st)) return rc;
       return tc_backward_half<D, 0, 1>(a, m, stats, st);
     }

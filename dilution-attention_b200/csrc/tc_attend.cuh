@@ -65,9 +65,10 @@ struct States {
   uint32_t any[kStates / 32], masked[kStates / 32];
   __device__ __forceinline__ int of(int e) const { return any[e / 32] >> (e & 31) & 1 ? 2 - (masked[e / 32] >> (e & 31) & 1) : 0; }
 };
-// Half tiles [base, end); f: the state of one.  The first and the last + 1 that have anything to do into range[0] and range[1].
-template <typename F> __device__ __forceinline__ void keep_states(States* s, int* range, int base, int end, int warp, int warps, F f) {
+// Half tiles [base, end); f: the state of one.  Returns the first and the last + 1 of the warp's that have anything to do.
+template <typename F> __device__ __forceinline__ int2 keep_states(States* s, int base, int end, int warp, int warps, F f) {
   const int lane = threadIdx.x & 31;
+  int2 range = make_int2(INT_MAX, 0);
   for (int e = base + 32 * warp; e < end; e += 32 * warps) {
     const int what = e + lane < end ? f(e + lane) : 0;
     const uint32_t any = __ballot_sync(0xffffffffu, what != 0), masked = __ballot_sync(0xffffffffu, what == 1);
@@ -76,12 +77,16 @@ template <typename F> __device__ __forceinline__ void keep_states(States* s, int
         s->any[(e - base) / 32] = any;
         s->masked[(e - base) / 32] = masked;
       }
-      if (any) {
-        atomicMin(&range[0], e + __ffs(any) - 1);
-        atomicMax(&range[1], e + 32 - __clz(any));
-      }
     }
+    if (any) range = make_int2(min(range.x, e + __ffs(any) - 1), e + 32 - __clz(any));
   }
+  return range;
+}
+// The warps' ranges, put together by every warp.
+__device__ __forceinline__ int2 all_of(const int2* range, int warps) {
+  const int lane = threadIdx.x & 31;
+  const int2 x = lane < warps ? range[lane] : make_int2(INT_MAX, 0);
+  return make_int2((int)uniform(__reduce_min_sync(0xffffffffu, x.x)), (int)uniform(__reduce_max_sync(0xffffffffu, x.y)));
 }
 
 template <int D, int NT> struct AttendForward {
@@ -255,7 +260,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   const uint32_t qfull = smem_u32(bars), kfull = qfull + 8, kfree = kfull + 8 * R, sdone = kfree + 8 * R, odone = sdone + 8 * NB * NG,
                  pready = odone + 8 * NG;
   Ctl* ctl = reinterpret_cast<Ctl*>(bars + 1 + 2 * R + (2 * NB + 1) * NG);
-  __shared__ int s_range[2];
+  __shared__ int2 s_range[F::kThreads / 32];
   __shared__ States s_state[NT];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
@@ -279,10 +284,9 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     return pair_state<BIAS>(r, i0, i0 + kTileRows - 1, dq[x], j0, j0 + 63, dj);
   };
 
+  const int top = (attend::key_end(r, min(r.t, (ib + NT) * kTileRows) - 1) + 63) / 64;
   if (tid == 0) {
     ctl->abort = 0;
-    s_range[0] = INT_MAX;
-    s_range[1] = 0;
     for (int x = 0; x < 1 + 2 * R + (NB + 1) * NG; ++x) mbar_init(qfull + 8 * x, 1);        // qfull, kfull, kfree, sdone, odone
     for (int x = 0; x < NB * NG; ++x) mbar_init(pready + 8 * x, 4);      // (of a buffer: a warp may be a half tile ahead of another)
     fence_barrier_init();
@@ -290,18 +294,22 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   for (int x = tid; x < NT * 128; x += F::kThreads) sFlag[x] = 0;
   __syncwarp();
   if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
-  __syncthreads();
-  // half tiles [h0, h0 + nh) that any of the CTA's queries sees
   {
-    const int top = (attend::key_end(r, min(r.t, (ib + NT) * kTileRows) - 1) + 63) / 64;
+    int2 mine = make_int2(INT_MAX, 0);
 #pragma unroll
-    for (int x = 0; x < NT; ++x) keep_states(&s_state[x], s_range, 0, top, warp, F::kThreads / 32, [&](int hh) { return state(x, hh); });
+    for (int x = 0; x < NT; ++x) {
+      const int2 y = keep_states(&s_state[x], 0, top, warp, F::kThreads / 32, [&](int hh) { return state(x, hh); });
+      mine = make_int2(min(mine.x, y.x), max(mine.y, y.y));
+    }
+    if (lane == 0) s_range[warp] = mine;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem);
-  const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : 0), nh = (int)uniform(s_range[1]) - h0;
+  // half tiles [h0, h0 + nh) that any of the CTA's queries sees
+  const int2 range = all_of(s_range, F::kThreads / 32);
+  const int h0 = range.y > 0 ? range.x : 0, nh = range.y - h0;
   // nearest keys first: a distance bias has the largest scores there, and later half tiles do not move the reference
   const int last = h0 + nh - 1;
 
@@ -512,7 +520,7 @@ template <int D, int STAY, int NW> struct AttendBackward {
   static constexpr int kOperands = (int)(2 * kTile + 2 * kRing * kHalf);
   static constexpr int kStats = STAY == 1 ? kRing * 512 : 0;
   static constexpr int kBytes = kOperands + kStats + 512 + 256 + 1024;
-  static_assert(kBytes + (int)sizeof(States) + 64 <= 232448, "shared memory, with what the kernel has of its own");
+  static_assert(kBytes + (int)sizeof(States) + 256 <= 232448, "shared memory, with what the kernel has of its own");
 };
 
 // Bytes of global memory into shared memory, both on 16-byte boundaries.
@@ -524,11 +532,10 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 // A warpgroup's step over 64 columns: S at tS, dout . v at tS + 64.  P (keys stay) as bf16 over the scores and dS over the
 // others, both as A operands.  x0: the first passing token, y: the lane's own; st: (-lse, -lse, -delta, -delta) of pairs of passing
-// queries; own: (-lse, -delta) of the lane's query.  EDGE: masks decide.
+// queries; own: (-lse, -delta) of the lane's query.  EDGE: bits say which of the passing tokens count.
 template <int STAY, bool CAP, bool BIAS, bool EDGE>
-__device__ __forceinline__ void backward_tile(uint32_t tS, const Row& r, float lin, float pre, int x0, int y, float2 own, const float4* st) {
-  uint2 bits = make_uint2(0, 0);
-  if (EDGE) bits = STAY == 1 ? query_bits(r, x0, y) : key_bits(r, y, x0);
+__device__ __forceinline__ void backward_tile(uint32_t tS, const Row& r, float lin, float pre, int x0, int y, float2 own, const float4* st,
+                                              const uint2& bits) {
 #pragma unroll
   for (int c0 = 0; c0 < 64; c0 += 32) {
     float v[32], g[32];
@@ -595,7 +602,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
   const uint32_t afull = smem_u32(bars), bfull = afull + 8, bfree = bfull + 8 * R, sdone = bfree + 8 * R, alldone = sdone + 8 * NW,
                  pready = alldone + 8;
   Ctl* ctl = reinterpret_cast<Ctl*>(bars + 2 + 2 * R + 2 * NW);
-  __shared__ int s_range[2];
+  __shared__ int2 s_range[F::kThreads / 32];
   __shared__ States s_state;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
@@ -616,26 +623,45 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
     return STAY == 1 ? pair_state<BIAS>(r, x0, x0 + 63, dx, y0, y1, dy) : pair_state<BIAS>(r, y0, y1, dy, x0, x0 + 63, dx);
   };
 
-  if (tid == 0) {
+  const int base = STAY == 1 ? attend::first_query(r, y0) / 64 : 0;
+  const int end = STAY == 1 ? padded / 64 : (attend::key_end(r, y1) + 63) / 64;
+  const int nx = STAY == 1 ? b * a.heads + head * group : b * a.kv_heads + head / group;      // the passing rows, the first of them
+  auto load_passing = [&](int hh, int m, int st) {
+    mbar_expect_tx(bfull + 8 * st, 2 * HB + (STAY == 1 ? 512 : 0));
+    tma_load_rows<W>(sB + HB * st, STAY == 1 ? &map_q : &map_k, hh * 64, m, bfull + 8 * st, HSub);
+    tma_load_rows<W>(sC + HB * st, STAY == 1 ? &map_do : &map_v, hh * 64, m, bfull + 8 * st, HSub);
+    if (STAY == 1) bulk_load(sStat + 512 * st, stats + (int64_t)m * padded + hh * 64, 512, bfull + 8 * st);
+  };
+  // The staying tile, and for keys the queries on the diagonal, are asked for before it is known which others there are.
+  const int ahead = STAY == 1 && y0 >= r.prefix ? min(2, end - base) : 0;
+  if (warp_u == 4 * NW + 1 && lead) {
     ctl->abort = 0;
-    s_range[0] = INT_MAX;
-    s_range[1] = 0;
     for (int x = 0; x < 2 + 2 * R + NW; ++x) mbar_init(afull + 8 * x, 1);        // afull, bfull, bfree, sdone, alldone
     for (int x = 0; x < NW; ++x) mbar_init(pready + 8 * x, 4);
     fence_barrier_init();
+    fence_async_smem();
+    mbar_expect_tx(afull, 2 * TB);
+    // (two boxes of 64 rows for each sub-tile: a box behind the last row reads zeros)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        tma_load_rows<W>(sA + TB * x + HSub * half, STAY == 1 ? (x ? &map_v : &map_k) : (x ? &map_do : &map_q), y0 + 64 * half, n, afull,
+                         kTileBytes);
+    for (int e = 0; e < ahead; ++e) load_passing(base + e, nx, e);
   }
   if (tid < 128) sFlag[tid] = 0;
   __syncwarp();
   if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
-  __syncthreads();
-  // passing half tiles [h0, h0 + nh) of which any sees the tile (or is seen by it)
-  const int base = STAY == 1 ? attend::first_query(r, y0) / 64 : 0;
-  keep_states(&s_state, s_range, base, STAY == 1 ? padded / 64 : (attend::key_end(r, y1) + 63) / 64, warp, F::kThreads / 32, state);
+  const int2 mine = keep_states(&s_state, base, end, warp, F::kThreads / 32, state);
+  if (lane == 0) s_range[warp] = mine;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(ctl->tmem), tAcc = tmem + 128 * NW;
-  const int h0 = (int)uniform(s_range[1] > 0 ? s_range[0] : base), nh = (int)uniform(s_range[1] > 0 ? s_range[1] : base) - h0, ne = nh * passes;
+  // passing half tiles [h0, h0 + nh) of which any sees the tile (or is seen by it), and those that are on their way
+  const int2 range = all_of(s_range, F::kThreads / 32);
+  const int h0 = range.y > 0 && ahead == 0 ? range.x : base, nh = range.y > 0 ? max(range.y, base + ahead) - h0 : 0, ne = nh * passes;
 
   if (warp_u == 4 * NW) {
     // ------------------------------------------------------------ the warp that issues MMAs
@@ -693,28 +719,15 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
     __syncwarp();
   } else if (warp_u == 4 * NW + 1) {
     // ------------------------------------------------------------ the warp that issues copies
-    const int nx = STAY == 1 ? b * a.heads + head * group : b * a.kv_heads + head / group;      // the passing rows, the first of them
-    if (ne > 0 && lead) {
-      mbar_expect_tx(afull, 2 * TB);
-      // (two boxes of 64 rows for each sub-tile: a box behind the last row reads zeros)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-          tma_load_rows<W>(sA + TB * x + HSub * half, STAY == 1 ? (x ? &map_v : &map_k) : (x ? &map_do : &map_q), y0 + 64 * half, n, afull,
-                           kTileBytes);
+    if (ne == 0) {
+      mbar_wait_warp(afull, 0, ctl, &g_attend_status, kErrWaitTma);
+      for (int e = 0; e < ahead; ++e) mbar_wait_warp(bfull + 8 * e, 0, ctl, &g_attend_status, kErrWaitTma);
     }
-    __syncwarp();
     int st = 0, hh = h0, m = nx;
     uint32_t phase = 1;
     for (int e = 0; e < ne; ++e) {
       if (e >= R) mbar_wait_warp(bfree + 8 * st, phase, ctl, &g_attend_status, kErrWaitMma);
-      if (lead) {
-        mbar_expect_tx(bfull + 8 * st, 2 * HB + (STAY == 1 ? 512 : 0));
-        tma_load_rows<W>(sB + HB * st, STAY == 1 ? &map_q : &map_k, hh * 64, m, bfull + 8 * st, HSub);
-        tma_load_rows<W>(sC + HB * st, STAY == 1 ? &map_do : &map_v, hh * 64, m, bfull + 8 * st, HSub);
-        if (STAY == 1) bulk_load(sStat + 512 * st, stats + (int64_t)m * padded + hh * 64, 512, bfull + 8 * st);
-      }
+      if (e >= ahead && lead) load_passing(hh, m, st);
       __syncwarp();
       if (++st == R) { st = 0; phase ^= 1; }
       if (++hh == h0 + nh) { hh = h0; ++m; }
@@ -734,11 +747,29 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
       if (STAY == 1 && BIAS) r.slope2 = a.slopes[head * group + pass] * kLog2e;
       const int hh = h0 + eh, what = (int)uniform(hh - base < kStates ? s_state.of(hh - base) : state(hh));
       if (what == 0) continue;
+      // which pairs count is asked for while the scores are under way; of a masked half tile most warps have all pairs or none
+      uint2 bits = make_uint2(~0u, ~0u);
+      bool edge = what == 1, none = false;
+      if (edge) {
+        bits = STAY == 1 ? query_bits(r, hh * 64, ys) : key_bits(r, ys, hh * 64);
+        none = __all_sync(0xffffffffu, (bits.x | bits.y) == 0);
+        edge = !__all_sync(0xffffffffu, (bits.x & bits.y) == ~0u && (!BIAS || (STAY == 1 ? ys <= hh * 64 : hh * 64 + 63 <= ys)));
+      }
       mbar_wait_warp(sdone + 8 * wg, turn & 1, ctl, &g_attend_status, kErrWaitMma);
       ++turn;
       tc_fence_after();
-      if (what == 1) backward_tile<STAY, CAP, BIAS, true>(tS, r, lin, pre, hh * 64, ys, own, stat + 32 * (e % R));
-      else backward_tile<STAY, CAP, BIAS, false>(tS, r, lin, pre, hh * 64, ys, own, stat + 32 * (e % R));
+      if (none) {
+        uint32_t z[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) z[c] = 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_st16(tS + (c >> 1) * 64 + (c & 1) * 16, z);
+        tmem_st_wait();
+      } else if (edge) {
+        backward_tile<STAY, CAP, BIAS, true>(tS, r, lin, pre, hh * 64, ys, own, stat + 32 * (e % R), bits);
+      } else {
+        backward_tile<STAY, CAP, BIAS, false>(tS, r, lin, pre, hh * 64, ys, own, stat + 32 * (e % R), bits);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(pready + 8 * wg);
