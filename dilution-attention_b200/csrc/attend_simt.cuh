@@ -5,7 +5,8 @@
 // that a half warp reads at a time start in different banks.  Tiles without a visible pair are passed over.
 // Calls of few blocks share each block between the CTAs of a cluster: every `ranks`-th tile is a CTA's, and what they have
 // accumulated is joined through distributed shared memory, in the ranks' order, each rank finishing a part of the rows.
-// One sequence of 301 tokens, 4 heads of 64 (2 key heads), fp32, forward / dk, dv / dq: 38 / 95 / 38 us by one CTA a block.
+// One sequence of 301 tokens, 4 heads of 64 (2 key heads), fp32, forward / dk, dv / dq: 38 / 95 / 38 us by one CTA a block,
+// 23 / 26 / 19 us by clusters, whose length is then a tile's latency (loads, 64 x 64 x D FMAs twice, three barriers).
 #pragma once
 
 #include "attend_common.cuh"

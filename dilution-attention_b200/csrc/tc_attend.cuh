@@ -14,7 +14,9 @@
 //             place of five, and no result depends on an order of atomic additions.
 //
 // What bounds them, per pair of tiles of 128 x 64: 512 cycles for one exponential a score on the special-function unit (16 a
-// clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.
+// clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.  Measured, forward / dk, dv /
+// dq: n = 64, T = 8192, heads of 64 762 / 1066 / 881 us (forward 0.64 of the exponentials' rate); documents of 700 tokens 218 / 235 / 185 us,
+// where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads of 128, capped 760 / 1020 / 800 us.
 #pragma once
 
 #include "attend_common.cuh"

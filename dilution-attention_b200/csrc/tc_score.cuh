@@ -74,10 +74,17 @@ inline EncodeTiled encode_tiled() {
 }
 // (n, t, d) bf16 rows as boxes {64 features, box rows, 1}, 128-byte swizzle; rows past t read as zero.  True: encoded.
 inline bool tile_map(CUtensorMap* map, const void* base, int64_t n, int64_t t, int d, int box) {
-  // the encoder wants a current context, which a thread that has only selected a device (one of autograd's) need not have yet
+  // the encoder wants a current context, which a thread that has only selected a device (one of autograd's) need not have yet; a
+  // thread that has one may be recording a graph, where cudaFree is not allowed
   static thread_local bool bound = false;
   if (!bound) {
-    cudaFree(nullptr);
+    typedef CUresult (*GetCurrent)(CUcontext*);
+    void* get = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    CUcontext current = nullptr;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &get, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess ||
+        ((GetCurrent)get)(&current) != CUDA_SUCCESS || current == nullptr)
+      cudaFree(nullptr);
     bound = true;
   }
   EncodeTiled fn = encode_tiled();

@@ -191,7 +191,7 @@ def tree_accept(cache: dict, draft: dict, path, out: torch.Tensor | None = None)
     by their bids (for a softmax layer: by their attention weights, summed over the heads that share a key head), in place
     or into `out`, a buffer like it whose rows behind the new length are left as they are.  On a host tensor or a list
     the path is checked against the tree; on the device an index outside the tree counts as its nearest node.  With
-    cache["pos_dev"] the caller advances that count.
+    cache["pos_dev"] the caller advances that count (a cache that GraphedDecode steps is closed there first).
     """
     q = draft["q"]
     batch, heads, nodes, dim = q.shape

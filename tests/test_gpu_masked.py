@@ -293,3 +293,42 @@ def test_empty_calls():
     out = load_package().softmax_attention(q, k, k)
     out.sum().backward()
     assert out.shape == q.shape and q.grad.shape == q.shape and k.grad.shape == k.shape
+
+
+def test_a_thread_whose_first_call_is_recorded():
+    """Forward and backward recorded by a thread that has made no call of the library before."""
+    import threading
+    x = inputs(1, 2, 2, 200, 64, torch.bfloat16)
+    want, got, graph = call(x), [], torch.cuda.CUDAGraph()
+    leaves = [t.detach().clone().requires_grad_(True) for t in x[:3]]
+    torch.cuda.synchronize()
+
+    def record():
+        with torch.cuda.graph(graph):
+            out = load_package().softmax_attention(*leaves)
+            got.extend((out, *torch.autograd.grad(out, leaves, x[3])))
+
+    thread = threading.Thread(target=record)
+    thread.start()
+    thread.join()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert len(got) == 4 and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("dim", [32, 64])
+def test_gradients_without_the_rest_of_out(dim):
+    """The C entries with rest NULL: delta is of the rounded out, within the bounds that count that rounding."""
+    lib = load_package()._lib
+    q, k, v, dout = x = inputs(1, 2, 2, 150, dim, torch.bfloat16)
+    out, dq, dk, dv = (torch.empty_like(q) for _ in range(4))
+    lse = torch.empty(1, 2, 150, device=DEV)
+    scratch = torch.empty(lib.load().dilution_attend_scratch_bytes(1, 2, 150), device=DEV, dtype=torch.uint8)
+    head = [q.data_ptr(), k.data_ptr(), v.data_ptr(), lib.BF16, 1, 2, 2, 150, dim, dim ** -0.5, 0.0, None, None, None, None]
+    stream = torch.cuda.current_stream().cuda_stream
+    lib.check(lib.load().dilution_attend_forward(*head, out.data_ptr(), None, lse.data_ptr(), stream), "forward")
+    lib.check(lib.load().dilution_attend_backward(*head, out.data_ptr(), None, lse.data_ptr(), dout.data_ptr(), scratch.data_ptr(),
+                                                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), stream), "backward")
+    want, off = O.attention(*x)
+    for a, b, far in zip((out, dq, dk, dv), want, off):
+        assert ((a.double() - b).abs() <= far + 1e-12).all()
