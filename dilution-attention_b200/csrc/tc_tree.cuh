@@ -10,7 +10,7 @@
 //                 key's demand (a node's demand is its parent's demand and bid; a parent further back is found in the TMEM
 //                 column that its score came from), and out^T += V^T share; or it adds the accepted nodes' bids.
 // What bounds them: the cache's bytes.  256 heads of 64, 24 nodes over 16384 keys: statistics 106 us (0.54 GB, 0.78 of the copy rate), shares
-// and outputs 220 us (1.09 GB, 0.76), five accepted nodes' bids 90 us (0.55 GB, 0.94).  64 key heads whose 128 rows fill the lanes:
+// and outputs 169 us (1.09 GB, 0.98), five accepted nodes' bids 90 us (0.55 GB, 0.94).  64 key heads whose 128 rows fill the lanes:
 // 70 us for 0.27 GB, of which the exponentials need 30.
 // A chunk of a key head's keys per CTA; one warp issues copies, one MMAs, two warpgroups take tiles in turn.
 #pragma once
@@ -381,53 +381,80 @@ __global__ void __launch_bounds__(Scan<D, G, OUT>::kThreads, Scan<D, G, OUT>::kP
 }
 
 // ---- sweep ---------------------------------------------------------------------------------------------
-// What the thread of a key has to know of a row.
-struct NodeStep {
+// What the thread of a key has to know of an accepted row: its lse, its position and the slope of its head.
+struct RowStep {
   float lse;
-  int up;              // the parent, or -1
-  int at;              // an accepted row's position, and the slope of its head
+  int at;
   float slope2;
+  int pad;
 };
+// And of a draft's nodes, in their order: their lse (+inf behind the last: no bids), their parents; as bits, those that follow none (roots) or
+// another than the one in front (far), and those whose demand such a later one starts from (keeps).
+struct Walk {
+  float lse[64];
+  uint8_t up[64];
+  uint32_t roots[2], far[2], keeps[2];
+};
+// Threads 0 .. N - 1, each with its node's lse.
+template <int N> __device__ __forceinline__ void keep_walk(Walk* w, const tree::Lineage& lineage, int nodes, float lse) {
+  const int x = threadIdx.x, up = x < nodes ? lineage.parent[x] : -1;
+  bool keep = false;
+  if (x < nodes)
+    for (int y = x + 2; y < nodes; ++y) keep = keep || lineage.parent[y] == x;
+  w->lse[x] = x < nodes ? lse : INFINITY;
+  w->up[x] = (uint8_t)max(up, 0);
+  const unsigned active = N < 32 ? (1u << N) - 1 : 0xffffffffu;
+  const unsigned root = __ballot_sync(active, up < 0), far = __ballot_sync(active, up >= 0 && up != x - 1), k = __ballot_sync(active, keep);
+  if ((x & 31) == 0) {
+    w->roots[x >> 5] = root;
+    w->far[x >> 5] = far;
+    w->keeps[x >> 5] = k;
+  }
+}
 
 // Shares of one key (of this lane), whose scores by `rows` nodes are at tS and whose cached demand is base: bf16 into row `row` of
-// the [128][64] tile dst.  jumps: nodes that do not follow the one in front; keeps: nodes whose demand a later one starts from.
+// the [128][64] tile dst.  Eight nodes at a time, whose bids and shares have nothing to wait for; their demand is one chain.
+// 256 heads of 64, 24 nodes over 16384 keys, us: 169; 16 at a time, each looked up in shared memory 222; one node 157.
 template <int N>
-__device__ __forceinline__ void share_keys(uint32_t tS, int rows, float lin, float eps, float base, bool live, const NodeStep* step,
-                                           uint64_t jumps, uint64_t keeps, uint8_t* dst, int row) {
+__device__ __forceinline__ void share_keys(uint32_t tS, int rows, float lin, float eps, float base, bool live, const Walk& walk,
+                                           uint8_t* dst, int row) {
   float left = base;
 #pragma unroll
   for (int c0 = 0; c0 < N; c0 += 16) {
     if (c0 >= rows) break;
-    float v[16], d[16];
-    uint32_t w[8];
+    float v[16];
     __syncwarp();
     tmem_ld16(tS + c0, v);
     tmem_ld_wait16(v);
+    const uint32_t roots = walk.roots[c0 / 32] >> (c0 & 31), far = walk.far[c0 / 32] >> (c0 & 31), keeps = walk.keeps[c0 / 32] >> (c0 & 31);
 #pragma unroll
-    for (int y = 0; y < 16; ++y) {
-      v[y] = fast_exp2(fmaf(v[y], lin, -step[c0 + y].lse));
-      if (!live || c0 + y >= rows) v[y] = 0.f;
-    }
+    for (int h = 0; h < 16; h += 8) {
+      if (c0 + h >= rows) break;
+      const float4 l0 = reinterpret_cast<const float4*>(walk.lse + c0 + h)[0], l1 = reinterpret_cast<const float4*>(walk.lse + c0 + h)[1];
+      const uint2 ups = *reinterpret_cast<const uint2*>(walk.up + c0 + h);
+      const float lse[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
+      float p[8], d[8];
 #pragma unroll
-    for (int y = 0; y < 16; ++y) {
-      if (jumps >> (c0 + y) & 1) {
-        const int up = step[c0 + y].up;
-        left = base;
-        if (up >= 0) {
+      for (int y = 0; y < 8; ++y) {
+        p[y] = fast_exp2(fmaf(v[h + y], lin, -lse[y]));
+        if (!live) p[y] = 0.f;
+      }
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        if (roots >> (h + y) & 1) left = base;
+        if (far >> (h + y) & 1) {
           tmem_st_wait();
-          tmem_ld1(tS + up, &left);
+          tmem_ld1(tS + ((y < 4 ? ups.x : ups.y) >> (8 * (y & 3)) & 255), &left);
           tmem_ld_wait1(&left);
         }
+        d[y] = left = left + p[y];
+        if (keeps >> (h + y) & 1) tmem_st1(tS + c0 + h + y, left);
       }
-      d[y] = left = left + v[y];
-      if (keeps >> (c0 + y) & 1) tmem_st1(tS + c0 + y, left);
+      uint32_t w[4];
+#pragma unroll
+      for (int y = 0; y < 8; y += 2) w[y >> 1] = pack_pair(p[y] * fast_rcp(d[y] + eps), p[y + 1] * fast_rcp(d[y + 1] + eps));
+      *reinterpret_cast<uint4*>(dst + swizzled(row, (c0 + h) / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-#pragma unroll
-    for (int y = 0; y < 16; ++y) v[y] *= fast_rcp(d[y] + eps);
-#pragma unroll
-    for (int y = 0; y < 8; ++y) w[y] = pack_pair(v[2 * y], v[2 * y + 1]);
-    *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(dst + swizzled(row, c0 / 8 + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
   }
   tmem_st_wait();
   fence_async_smem();
@@ -459,10 +486,9 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
   uint8_t* smem = align1024(smem_raw);
   uint8_t *pShare = smem + kQ + F::kRingBytes, *pOnes = pShare + F::kShare;
   const uint32_t sQ = smem_u32(smem), ring_k = sQ + kQ, ring_v = ring_k + F::kOne * RK, sShare = smem_u32(pShare), sOnes = smem_u32(pOnes);
-  NodeStep* step = reinterpret_cast<NodeStep*>(pOnes + F::kOnes);
-  uint64_t* walk = reinterpret_cast<uint64_t*>(step + 64);      // bits of the nodes that do not follow the one in front, and of
-                                                                // those whose demand a later node starts from
-  const StreamBars<RK, RV, NB> bars(walk + 32);
+  RowStep* step = reinterpret_cast<RowStep*>(pOnes + F::kOnes);
+  Walk* walk = reinterpret_cast<Walk*>(step);
+  const StreamBars<RK, RV, NB> bars(reinterpret_cast<uint64_t*>(step + 64));
   Ctl* ctl = bars.ctl;
   __shared__ tree::Lineage lineage;
 
@@ -565,41 +591,39 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
     // what the keys' threads have to know of the rows; their lse may come from a kernel that has not ended yet
     if (DILUTE) wait_for_last();
     if (tid < N) {
-      NodeStep s{0.f, -1, 0, 0.f};
-      bool jump = false, keep = false;
-      if (tid < rows) {
-        const int q = q_row(tid);
-        s.lse = a.lse[((int64_t)nk * a.group) * a.nodes + q];
-        if (DILUTE) {
-          s.up = lineage.parent[tid];
-          jump = s.up < 0 || s.up != tid - 1;
-          for (int y = tid + 2; y < a.nodes; ++y) keep = keep || lineage.parent[y] == tid;
-        } else {
+      RowStep s{0.f, 0, 0.f, 0};
+      const int q = tid < rows ? q_row(tid) : 0;
+      if (tid < rows) s.lse = a.lse[((int64_t)nk * a.group) * a.nodes + q];
+      if (DILUTE) {
+        keep_walk<N>(walk, lineage, rows, s.lse);
+      } else {
+        if (tid < rows) {
           s.slope2 = a.slopes != nullptr ? a.slopes[hk * a.group + q / a.nodes] * kLog2e : 0.f;
           s.at = len + lineage.depth[q % a.nodes];
         }
-      }
-      step[tid] = s;
-      const unsigned active = N < 32 ? (1u << N) - 1 : 0xffffffffu, j = __ballot_sync(active, jump), k = __ballot_sync(active, keep);
-      if (lane == 0) {
-        reinterpret_cast<uint32_t*>(walk)[warp] = j;
-        reinterpret_cast<uint32_t*>(walk)[2 + warp] = k;
+        step[tid] = s;
       }
     }
     asm volatile("bar.sync 2, 256;" ::: "memory");
-    const uint64_t jumps = walk[0], keeps = walk[1];
+    // (a key's demand is asked for a turn ahead)
+    auto demand = [&](int e) {
+      const int j = (last - e) * KT + row;
+      return e < ne && j < len ? a.committed[(int64_t)nk * a.capacity + j] : 0.f;
+    };
+    float next = demand(wg);
     for (int e = wg; e < ne; e += 2) {
       const int j = (last - e) * KT + row;
       const bool live = j < len;
       const int64_t at = (int64_t)nk * a.capacity + j;
-      const float base = live ? a.committed[at] : 0.f;
+      const float base = next;
+      next = demand(e + 2);
       const uint32_t tS = tmem + 64 * (e % NB) + lanes;
       mbar_wait_warp(bars.sdone + 8 * (e % NB), (e / NB) & 1, ctl, &g_tree_status, kErrWaitMma);
       // the product of the warpgroup's last tile has read its shares
       if (DILUTE && e >= 2) mbar_wait_warp(bars.used + 8 * wg, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
       tc_fence_after();
       if (DILUTE) {
-        share_keys<N>(tS, rows, lin, a.eps, base, live, step, jumps, keeps, pShare + 16384 * wg, row);
+        share_keys<N>(tS, rows, lin, a.eps, base, live, *walk, pShare + 16384 * wg, row);
       } else {
         float total = base;
 #pragma unroll
@@ -612,7 +636,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
           if (cap) cap_scores<16>(v, pre);
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
-            const NodeStep s = step[c0 + y];
+            const RowStep s = step[c0 + y];
             const float z = fmaf(v[y], lin, -s.lse - s.slope2 * (float)(s.at - j));
             if (c0 + y < rows) total += fast_exp2(z);
           }
@@ -705,10 +729,9 @@ __global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const _
   uint8_t *pRing = smem + F::kQ, *pOver = pRing + F::kSpace, *pShare = pOver, *pOnes = pOver + F::kShare;
   const uint32_t sQ = smem_u32(smem), ring = smem_u32(pRing), ring_v = ring + F::kOne * R, sOver = smem_u32(pOver), sOnes = smem_u32(pOnes);
   float* z = reinterpret_cast<float*>(pOver + F::kOver);                                   // [N][kCols]
-  NodeStep* step = reinterpret_cast<NodeStep*>(z + N * F::kCols);
-  float2* chunk = reinterpret_cast<float2*>(step + 64);                                    // [N] this CTA's (maximum, sum)
+  Walk* walk = reinterpret_cast<Walk*>(z + N * F::kCols);
+  float2* chunk = reinterpret_cast<float2*>(z + N * F::kCols + 256);                                    // [N] this CTA's (maximum, sum)
   uint64_t* at_bars = reinterpret_cast<uint64_t*>(chunk + 64);
-  uint32_t* walk = reinterpret_cast<uint32_t*>(at_bars);                                   // jumps, keeps
   const StreamBars<RA, 4, NA> ba(at_bars + 2);
   const StreamBars<R, R, NB> bb(at_bars + 2 + StreamBars<RA, 4, NA>::kBytes / 8);
   Ctl* ctl = ba.ctl;
@@ -896,8 +919,7 @@ __global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const _
     for (int x = tid; x < F::kOnes / 16; x += 256)
       *reinterpret_cast<uint4*>(pOnes + (x >> 7) * 2048 + swizzled((x >> 3) & 15, x & 7)) = make_uint4((x & 7) == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);
     if (tid < N) {
-      NodeStep s{0.f, -1, 0, 0.f};
-      bool jump = false, keep = false;
+      float lse = 0.f;
       if (tid < n) {
         float m[C], t[C], top = -INFINITY, all = 0.f;
 #pragma unroll
@@ -909,23 +931,14 @@ __global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const _
         const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int y = 0; y < C; ++y) all = fmaf(t[y], exp2f(m[y] - from), all);
-        s.lse = from + log2f(all);
-        if (rank == 0) a.lse[(int64_t)nk * n + tid] = s.lse;
-        s.up = lineage.parent[tid];
-        jump = s.up < 0 || s.up != tid - 1;
-        for (int y = tid + 2; y < n; ++y) keep = keep || lineage.parent[y] == tid;
+        lse = from + log2f(all);
+        if (rank == 0) a.lse[(int64_t)nk * n + tid] = lse;
       }
-      step[tid] = s;
-      const unsigned active = N < 32 ? (1u << N) - 1 : 0xffffffffu, j = __ballot_sync(active, jump), k = __ballot_sync(active, keep);
-      if (lane == 0) {
-        walk[warp] = j;
-        walk[2 + warp] = k;
-      }
+      keep_walk<N>(walk, lineage, n, lse);
     }
     fence_async_smem();
     asm volatile("bar.sync 2, 256;" ::: "memory");
     // ---------------------------------------------------------- shares: lane = key
-    const uint64_t jumps = walk[0] | (N > 32 ? (uint64_t)walk[1] << 32 : 0), keeps = walk[2] | (N > 32 ? (uint64_t)walk[3] << 32 : 0);
     for (int e = wg; e < ne; e += 2) {
       const int j = (first + e) * 128 + row;
       const bool live = j < len;
@@ -933,7 +946,7 @@ __global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const _
       mbar_wait_warp(bb.sdone + 8 * (e % NB), (e / NB) & 1, ctl, &g_tree_status, kErrWaitMma);
       if (e >= 2) mbar_wait_warp(bb.used + 8 * wg, (e / 2 - 1) & 1, ctl, &g_tree_status, kErrWaitMma);
       tc_fence_after();
-      share_keys<N>(tmem + 64 * (e % NB) + lanes, n, lin, a.eps, base, live, step, jumps, keeps, pShare + 16384 * wg, row);
+      share_keys<N>(tmem + 64 * (e % NB) + lanes, n, lin, a.eps, base, live, *walk, pShare + 16384 * wg, row);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bb.ready + 8 * (e % NB));
@@ -965,7 +978,7 @@ __global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const _
       for (int x = 0; x < n; ++x) {
         float& cell = z[x * F::kCols + row];
         float left = 0.f;
-        if (lineage.line[x] >> key & 1) left = exp2f(cell - step[x].lse) + (lineage.parent[x] >= 0 ? z[lineage.parent[x] * F::kCols + row] : 0.f);
+        if (lineage.line[x] >> key & 1) left = exp2f(cell - walk->lse[x]) + (lineage.parent[x] >= 0 ? z[lineage.parent[x] * F::kCols + row] : 0.f);
         cell = left;
       }
       for (int x = n - 1; x >= 0; --x) {                 // (children come behind their parents)
