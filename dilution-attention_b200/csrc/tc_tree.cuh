@@ -9,8 +9,8 @@
 //   sweep_kernel: S^T = K Q^T, lane = key, for what belongs to keys: a thread walks the tree in the nodes' order with its
 //                 key's demand (a node's demand is its parent's demand and bid; a parent further back is found in the TMEM
 //                 column that its score came from), and out^T += V^T share; or it adds the accepted nodes' bids.
-// What bounds them: the cache's bytes.  256 heads of 64, 24 nodes over 16384 keys: statistics 106 us (0.54 GB, 0.78 of the copy rate), shares
-// and outputs 169 us (1.09 GB, 0.98), five accepted nodes' bids 90 us (0.55 GB, 0.94).  64 key heads whose 128 rows fill the lanes:
+// What bounds them: the cache's bytes.  256 heads of 64, 24 nodes over 16384 keys: statistics 96 us (0.54 GB, 0.85 of the copy rate), shares
+// and outputs 169 us (1.09 GB, 0.98), five accepted nodes' bids 86 us (0.55 GB, 0.98).  64 key heads whose 128 rows fill the lanes:
 // 70 us for 0.27 GB, of which the exponentials need 30.
 // A chunk of a key head's keys per CTA; one warp issues copies, one MMAs, two warpgroups take tiles in turn.
 #pragma once
@@ -94,7 +94,9 @@ __device__ __forceinline__ void stream_tiles(const StreamBars<RK, RV, NB>& bars,
 constexpr int ctas_per_sm(int bytes, int tmem) { return 2 * (bytes + 2304) <= 233472 && 2 * tmem <= 512 ? 2 : 1; }
 
 template <int D, int G, bool OUT> struct Scan {
-  static constexpr int kRows = 128 / G, kCols = G == 1 ? 64 : 32, kKeys = kCols * G;
+  // 64 columns a product, or 32 where P~ of several quarters is kept as well.  Statistics alone, 256 heads of 64, 24 nodes over 16384
+  // keys: 32 columns 105 us, 64 columns 96 us: a product of few columns takes the tensor pipe nearly as long.
+  static constexpr int kRows = 128 / G, kCols = G == 1 || !OUT ? 64 : 32, kKeys = kCols * G;
   static constexpr int kWg = OUT && D == 64 ? 1 : 2;                       // warpgroups, which take tiles in turn
   static constexpr int kThreads = 128 * kWg + 64;
   static constexpr uint32_t kOne = kKeys * D * 2;
