@@ -199,7 +199,7 @@ template <int D> int tc_softmax(tree::Args a, void* scratch, cudaStream_t st) {
 }
 
 // A step in one launch, a cluster of eight CTAs per head: for short caches whose clusters all run at once.  24 nodes of heads of 64,
-// one launch / chunks (four launches, with 6 us of timing events each), us: 32 heads, 1024 keys 29 / 53, 4096 keys 35 / 51, 8192 keys
+// one launch / chunks (four launches, with 6 us of timing events each; shares 16 nodes at a time on either side), us: 32 heads, 1024 keys 29 / 53, 4096 keys 35 / 51, 8192 keys
 // 44 / 59; 16 heads, 16384 keys 60 / 69; but 64 heads, 16384 keys 121 / 131 and 256 heads 450 / 370: a CTA's start, its three meetings
 // with the others and its end take about 20 us, which chunks overlap with other chunks' tiles.
 bool by_clusters(const tree::Args& a) { return (int64_t)a.batch * a.kv_heads <= 32 && tree_keys(a) <= 16384; }
