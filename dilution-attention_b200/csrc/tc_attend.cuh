@@ -15,8 +15,8 @@
 //
 // What bounds them, per pair of tiles of 128 x 64: 512 cycles for one exponential a score on the special-function unit (16 a
 // clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.  Measured, forward / dk, dv /
-// dq: n = 64, T = 8192, heads of 64 762 / 1066 / 881 us (forward 0.64 of the exponentials' rate); documents of 700 tokens 218 / 235 / 185 us,
-// where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads of 128, capped 760 / 1020 / 800 us.
+// dq: n = 64, T = 8192, heads of 64 762 / 1066 / 881 us (forward 0.64 of the exponentials' rate); documents of 700 tokens 220 / 235 / 185 us,
+// where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads of 128, capped 817 / 1020 / 800 us.
 #pragma once
 
 #include "attend_common.cuh"
@@ -95,9 +95,9 @@ template <int D, int NT> struct AttendForward {
   static constexpr int kThreads = 256 * NT + 32;
   static constexpr int kRing = D == 64 && NT == 1 ? 5 : D == 64 ? 8 : 5;           // half tiles of K and V
   static constexpr uint32_t kTile = Rows<kForm<D>>::kBytes, kHalf = kTile / 2;
-  // Q[NT] | K[ring] | V[ring] | merge statistics [NT][2][128] float2 | flags [NT][128] | barriers + control
+  // Q[NT] | K[ring] | V[ring] | merge statistics [NT][2][128] float2, float | flags [NT][128] | barriers + control
   static constexpr int kOperands = (int)(NT * kTile + 2 * kRing * kHalf);
-  static constexpr int kStats = NT * 2 * 128 * 8, kFlags = NT * 128 * 4;
+  static constexpr int kStats = NT * 2 * 128 * 12, kFlags = NT * 128 * 4;
   static constexpr int kBytes = kOperands + kStats + kFlags + 256 + 1024;
   static constexpr int kBufs = D == 128 ? 2 : 1;                                   // score buffers of a warpgroup
   static constexpr int kWgCols = 64 * kBufs + D;
@@ -151,15 +151,16 @@ __device__ __forceinline__ uint2 query_bits(const Row& r, int i0, int j) {
   return m;
 }
 
-// A warpgroup's step over the 64 scores of keys j0 .. at tS: P~ = 2^(z - reference) as bf16 over the scores, their sum
-// into s.  The reference is the maximum of the first half tile that a row sees and moves where a later one's P~ sum to more
+// A warpgroup's step over the 64 scores of keys j0 .. at tS: P~ = 2^(z - reference) as bf16 over the scores, their sum into s, and that
+// of the rounded ones, which out is divided by, into sr: the rounding of a P~ that a row is mostly made of then cancels (dq, dk of
+// capped scores of deviation 3 against 64 bits by norm 0.0028 with one sum, 0.0025 with two; 767 -> 817 us at B2 H16 T8192 d128).  The reference is the maximum of the first half tile that a row sees and moves where a later one's P~ sum to more
 // than 2^40; only then is the accumulator rescaled, once its products are through (settled).  bf16 has the range of fp32: P~ below that limit keeps 8 bits.
 template <int D, bool CAP, bool BIAS, typename Settled>
 __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row& r, float lin, float pre, int j0, int i, bool edge,
-                                             float& ref, float& s, Settled settled) {
+                                             float& ref, float& s, float& sr, Settled settled) {
   float v[64];
   uint32_t pw[32];
-  float ps;
+  float ps, pr;
   bool some = true;                  // the row sees any of the keys
   // the scores as z = mul v + add + step e, masked ones -inf
   auto fetch = [&]() {
@@ -184,7 +185,7 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
   const float add = BIAS && !edge ? r.slope2 * (float)(j0 - i) : 0.f;
   auto exponentials = [&](float mul, float add, float step) {
     const float2 mm = make_float2(mul, mul), four = make_float2(4.f * step, 4.f * step);
-    float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+    float2 a0 = make_float2(0.f, 0.f), a1 = a0, b0 = a0;
     float2 o0 = make_float2(add, BIAS ? add + step : add), o1 = BIAS ? make_float2(add + 2.f * step, add + 3.f * step) : o0;
 #pragma unroll
     for (int e = 0; e < 64; e += 4) {
@@ -196,11 +197,14 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
       const float2 p0 = make_float2(fast_exp2(z0.x), fast_exp2(z0.y)), p1 = make_float2(fast_exp2(z1.x), fast_exp2(z1.y));
       a0 = add2(a0, p0);
       a1 = add2(a1, p1);
-      pw[e >> 1] = pack_pair(p0.x, p0.y);
-      pw[(e >> 1) + 1] = pack_pair(p1.x, p1.y);
+      const uint32_t w0 = pack_pair(p0.x, p0.y), w1 = pack_pair(p1.x, p1.y);
+      b0 = add2(b0, add2(unpack_pair(w0), unpack_pair(w1)));
+      pw[e >> 1] = w0;
+      pw[(e >> 1) + 1] = w1;
     }
     const float2 a = add2(a0, a1);
     ps = a.x + a.y;
+    pr = b0.x + b0.y;
   };
   fetch();
   bool slow = __any_sync(0xffffffffu, ref == -INFINITY && some);
@@ -234,11 +238,13 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
         }
       }
       s *= f;
+      sr *= f;
       ref = now;
     }
     exponentials(1.f, ref == -INFINITY ? 0.f : -ref, 0.f);
   }
   s += ps;
+  sr += pr;
   tmem_st16(tS, pw);
   tmem_st16(tS + 16, pw + 16);
   tmem_st_wait();
@@ -402,7 +408,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       tmem_st_wait();
     }
     const int tile = NT == 2 ? wg >> 1 : 0, half = wg & 1, i = (ib + tile) * kTileRows + row, is = min(i, r.t - 1);
-    float ref = -INFINITY, s = 0.f;
+    float ref = -INFINITY, s = 0.f, sr = 0.f;
     int turn = 0;
     for (int e = half; e < nh; e += 2) {
       const int hh = last - e, what = (int)uniform(hh < kStates ? s_state[tile].of(hh) : state(tile, hh));
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
           tc_fence_after();
         }
       };
-      forward_step<D, CAP, BIAS>(tS + 64 * side, tO, r, lin, pre, hh * 64, is, what == 1, ref, s, settled);
+      forward_step<D, CAP, BIAS>(tS + 64 * side, tO, r, lin, pre, hh * 64, is, what == 1, ref, s, sr, settled);
       settled();
       ++turn;
       tc_fence_before();
@@ -435,7 +441,9 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     constexpr int kPart = D / 2;
     float* sX = reinterpret_cast<float*>(smem + NT * TB) + tile * 128 * D;           // [2][128][kPart]
     float2* stat = sStat + 256 * tile;
+    float* rounded = reinterpret_cast<float*>(sStat + NT * 256) + 256 * tile;
     stat[half * 128 + row] = make_float2(ref, s);
+    rounded[half * 128 + row] = sr;
     float* give = sX + ((1 - half) * 128 + row) * kPart;
     __syncwarp();
 #pragma unroll
@@ -455,7 +463,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
     const float2 other = stat[(1 - half) * 128 + row];
     const float m = fmaxf(ref, other.x), base = m == -INFINITY ? 0.f : m;
     const float f_own = fast_exp2(ref - base), f_oth = fast_exp2(other.x - base);
-    const float den = s * f_own + other.y * f_oth, inv = den == 0.f ? 0.f : 1.f / den;
+    const float den = s * f_own + other.y * f_oth, by = sr * f_own + rounded[(1 - half) * 128 + row] * f_oth, inv = by == 0.f ? 0.f : 1.f / by;
     __syncwarp();
     const float a_own = f_own * inv, a_oth = f_oth * inv;
     const float* take = sX + (half * 128 + row) * kPart;

@@ -14,10 +14,11 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return r;
 }
 
+__device__ __forceinline__ float2 unpack_pair(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 // What the rounding of such a pair leaves off.
 __device__ __forceinline__ uint32_t left_pair(float lo, float hi) {
-  const uint32_t r = pack_pair(lo, hi);
-  return pack_pair(lo - __uint_as_float(r << 16), hi - __uint_as_float(r & 0xffff0000u));
+  const float2 r = unpack_pair(pack_pair(lo, hi));
+  return pack_pair(lo - r.x, hi - r.y);
 }
 
 // Head sizes: D / 64 sub-tiles of 64 features (tc_common.cuh).
