@@ -105,15 +105,15 @@ template <typename F> int with_score(const attend::Args& a, F f) {
   return a.slopes ? f(std::false_type(), std::true_type()) : f(std::false_type(), std::false_type());
 }
 
-template <int D, int NT> int tc_forward(const attend::Args& a, cudaStream_t st) {
-  using F = tc::AttendForward<D, NT>;
+template <int D> int tc_forward(const attend::Args& a, cudaStream_t st) {
+  using F = tc::AttendForward<D>;
   AttendMaps m;
   if (int rc = attend_maps(m, a, D, 128, 64)) return rc;
   return with_score(a, [&](auto cap, auto bias) {
-    auto kernel = tc::attend_forward_kernel<D, NT, cap(), bias()>;
+    auto kernel = tc::attend_forward_kernel<D, cap(), bias()>;
     if (int rc = opt_in(kernel, F::kBytes)) return rc;
     LaunchMark mark("attend_forward", st);
-    const unsigned grid = (unsigned)((int64_t)a.batch * a.heads * ((a.t + 128 * NT - 1) / (128 * NT)));
+    const unsigned grid = (unsigned)((int64_t)a.batch * a.heads * ((a.t + 127) / 128));
     kernel<<<grid, F::kThreads, F::kBytes, st>>>(m.q, m.k, m.v, a);
     return abi_check_launch("attend_forward");
   });
@@ -209,9 +209,7 @@ int dilution_attend_forward(const void* q, const void* k, const void* v, int dty
   if (int rc = launch_ranges(a, st)) return rc;
   return with_type(dtype, d, [&](auto type, auto dim) {
     if constexpr (!kOnTensorCores<decltype(type), dim()>) return simt_forward<decltype(type), dim()>(a, st);
-    else if constexpr (dim() == 128) return tc_forward<128, 1>(a, st);
-    // two query tiles per CTA / one, two CTAs on an SM, n = 64: T = 2048 83 / 71 us, T = 4096 226 / 208, T = 8192 759 / 773
-    else return a.docs == nullptr && a.t >= 8192 ? tc_forward<64, 2>(a, st) : tc_forward<64, 1>(a, st);
+    else return tc_forward<dim()>(a, st);
   });
 }
 

@@ -4,8 +4,7 @@
 // off by up to 2^-8 of itself.  References, sums, lse, delta and accumulators are fp32.  A warp of its own issues
 // every copy and MMA.  Which pairs of tiles have anything to do is asked of the documents' ranges, never of a list.
 //
-//   forward : a CTA's query tiles of 128 (two of heads of 64, one of 128) walk over half tiles of 64 keys; two warpgroups per query
-//             tile take them in turn.  lane = query: reference, sum and accumulator of a row belong to one thread and
+//   forward : a CTA's query tile of 128 walks over half tiles of 64 keys; two warpgroups take them in turn.  lane = query: reference, sum and accumulator of a row belong to one thread and
 //             warpgroup, and are merged once at the end.
 //   backward: one kernel for both halves.  A tile of 128 stays (dq: queries with their dout; dk, dv: keys with their values),
 //             half tiles of 64 of the other kind stream past; kWg warpgroups take them in turn, and accumulators in TMEM
@@ -15,8 +14,8 @@
 //
 // What bounds them, per pair of tiles of 128 x 64: 512 cycles for one exponential a score on the special-function unit (16 a
 // clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.  Measured, forward / dk, dv /
-// dq: n = 64, T = 8192, heads of 64 762 / 1066 / 881 us (forward 0.64 of the exponentials' rate); documents of 700 tokens 220 / 235 / 185 us,
-// where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads of 128, capped 817 / 1020 / 800 us.
+// dq: n = 64, T = 8192, heads of 64 773 / 1066 / 881 us (forward 0.62 of the exponentials' rate); documents of 700 tokens 220 / 235 / 185 us,
+// where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads of 128, capped 830 / 1020 / 795 us.
 #pragma once
 
 #include "attend_common.cuh"
@@ -91,19 +90,18 @@ __device__ __forceinline__ int2 all_of(const int2* range, int warps) {
   return make_int2((int)uniform(__reduce_min_sync(0xffffffffu, x.x)), (int)uniform(__reduce_max_sync(0xffffffffu, x.y)));
 }
 
-template <int D, int NT> struct AttendForward {
-  static constexpr int kThreads = 256 * NT + 32;
-  static constexpr int kRing = D == 64 && NT == 1 ? 5 : D == 64 ? 8 : 5;           // half tiles of K and V
+template <int D> struct AttendForward {
+  static constexpr int kThreads = 256 + 32, kRing = 5;                              // half tiles of K and V
   static constexpr uint32_t kTile = Rows<kForm<D>>::kBytes, kHalf = kTile / 2;
-  // Q[NT] | K[ring] | V[ring] | merge statistics [NT][2][128] float2, float | flags [NT][128] | barriers + control
-  static constexpr int kOperands = (int)(NT * kTile + 2 * kRing * kHalf);
-  static constexpr int kStats = NT * 2 * 128 * 12, kFlags = NT * 128 * 4;
+  // Q | K[ring] | V[ring] | merge statistics [2][128] float2, float | flags [128] | barriers + control
+  static constexpr int kOperands = (int)(kTile + 2 * kRing * kHalf);
+  static constexpr int kStats = 2 * 128 * 12, kFlags = 128 * 4;
   static constexpr int kBytes = kOperands + kStats + kFlags + 256 + 1024;
   static constexpr int kBufs = D == 128 ? 2 : 1;                                   // score buffers of a warpgroup
   static constexpr int kWgCols = 64 * kBufs + D;
-  static constexpr int kTmem = 2 * NT * kWgCols <= 256 ? 256 : 512;
-  static_assert(2 * NT * kWgCols <= kTmem, "the warpgroups' columns fit the allocation");
-  static_assert(NT * 128 * D * 4 <= (int)(2 * kRing * kHalf), "the merge area fits the ring");
+  static constexpr int kTmem = 2 * kWgCols <= 256 ? 256 : 512;
+  static_assert(2 * kWgCols <= kTmem, "the warpgroups' columns fit the allocation");
+  static_assert(128 * D * 4 <= (int)(2 * kRing * kHalf), "the merge area fits the ring");
 };
 
 constexpr float kAttendLimit = 1099511627776.f;      // 2^40: a half tile whose P~ sum to more moves the reference
@@ -153,8 +151,10 @@ __device__ __forceinline__ uint2 query_bits(const Row& r, int i0, int j) {
 
 // A warpgroup's step over the 64 scores of keys j0 .. at tS: P~ = 2^(z - reference) as bf16 over the scores, their sum into s, and that
 // of the rounded ones, which out is divided by, into sr: the rounding of a P~ that a row is mostly made of then cancels (dq, dk of
-// capped scores of deviation 3 against 64 bits by norm 0.0028 with one sum, 0.0025 with two; 767 -> 817 us at B2 H16 T8192 d128).  The reference is the maximum of the first half tile that a row sees and moves where a later one's P~ sum to more
-// than 2^40; only then is the accumulator rescaled, once its products are through (settled).  bf16 has the range of fp32: P~ below that limit keeps 8 bits.
+// capped scores of deviation 3 against 64 bits by norm 0.0028 with one sum, 0.0025 with two; 767 -> 830 us at B2 H16 T8192 d128).
+// The reference is the maximum of the first half tile that a row sees and moves where a later one's P~ sum to more than 2^40; only
+// then is the accumulator rescaled, once its products are through (settled).  bf16 has the range of fp32: P~ below that limit
+// keeps 8 bits.
 template <int D, bool CAP, bool BIAS, typename Settled>
 __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row& r, float lin, float pre, int j0, int i, bool edge,
                                              float& ref, float& s, float& sr, Settled settled) {
@@ -185,7 +185,7 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
   const float add = BIAS && !edge ? r.slope2 * (float)(j0 - i) : 0.f;
   auto exponentials = [&](float mul, float add, float step) {
     const float2 mm = make_float2(mul, mul), four = make_float2(4.f * step, 4.f * step);
-    float2 a0 = make_float2(0.f, 0.f), a1 = a0, b0 = a0;
+    float2 a0 = make_float2(0.f, 0.f), b0 = a0;
     float2 o0 = make_float2(add, BIAS ? add + step : add), o1 = BIAS ? make_float2(add + 2.f * step, add + 3.f * step) : o0;
 #pragma unroll
     for (int e = 0; e < 64; e += 4) {
@@ -195,15 +195,13 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
         o1 = add2(o1, four);
       }
       const float2 p0 = make_float2(fast_exp2(z0.x), fast_exp2(z0.y)), p1 = make_float2(fast_exp2(z1.x), fast_exp2(z1.y));
-      a0 = add2(a0, p0);
-      a1 = add2(a1, p1);
+      a0 = add2(a0, add2(p0, p1));
       const uint32_t w0 = pack_pair(p0.x, p0.y), w1 = pack_pair(p1.x, p1.y);
       b0 = add2(b0, add2(unpack_pair(w0), unpack_pair(w1)));
       pw[e >> 1] = w0;
       pw[(e >> 1) + 1] = w1;
     }
-    const float2 a = add2(a0, a1);
-    ps = a.x + a.y;
+    ps = a0.x + a0.y;
     pr = b0.x + b0.y;
   };
   fetch();
@@ -250,67 +248,54 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
   tmem_st_wait();
 }
 
-// grid = batch * heads * ceil(t / (128 NT)), last queries (the longest rows) first.
-template <int D, int NT, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT == 1 ? 2 : 1) attend_forward_kernel(
+// grid = batch * heads * ceil(t / 128), last queries (the longest rows) first.
+template <int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(AttendForward<D>::kThreads, D == 64 ? 2 : 1) attend_forward_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
     const __grid_constant__ attend::Args a) {
-  using F = AttendForward<D, NT>;
+  using F = AttendForward<D>;
   constexpr int W = kForm<D>, R = F::kRing;
   constexpr uint32_t TB = F::kTile, HB = F::kHalf, HSub = kTileBytes / 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
-  const uint32_t sQ = smem_u32(smem), sK = sQ + NT * TB, sV = sK + R * HB;
+  const uint32_t sQ = smem_u32(smem), sK = sQ + TB, sV = sK + R * HB;
   float2* sStat = reinterpret_cast<float2*>(smem + F::kOperands);
   int* sFlag = reinterpret_cast<int*>(smem + F::kOperands + F::kStats);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::kOperands + F::kStats + F::kFlags);
-  constexpr int NB = F::kBufs, NG = 2 * NT;                                        // score buffers, warpgroups
+  constexpr int NB = F::kBufs, NG = 2;                                        // score buffers, warpgroups
   const uint32_t qfull = smem_u32(bars), kfull = qfull + 8, kfree = kfull + 8 * R, sdone = kfree + 8 * R, odone = sdone + 8 * NB * NG,
                  pready = odone + 8 * NG;
   Ctl* ctl = reinterpret_cast<Ctl*>(bars + 1 + 2 * R + (2 * NB + 1) * NG);
   __shared__ int2 s_range[F::kThreads / 32];
-  __shared__ States s_state[NT];
+  __shared__ States s_state;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = tid >> 7, row = tid & 127;
   const int warp_u = uniform_warp();
   const uint32_t lead = elect_one();
-  const int heads = a.batch * a.heads, blocks = (a.t + NT * kTileRows - 1) / (NT * kTileRows);
-  const int n = (int)(blockIdx.x % heads), ib = (blocks - 1 - (int)(blockIdx.x / heads)) * NT;
+  const int heads = a.batch * a.heads, blocks = (a.t + kTileRows - 1) / kTileRows;
+  const int n = (int)(blockIdx.x % heads), i0 = (blocks - 1 - (int)(blockIdx.x / heads)) * kTileRows;
   const int b = n / a.heads, h = n % a.heads, nk = b * a.kv_heads + h / (a.heads / a.kv_heads);
   const Row r = attend::make_row(a, b, h);
   const float lin = CAP ? r.cap2 : r.pre, pre = CAP ? a.scale / a.cap : 0.f;
-  Docs dq[NT];
-#pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    const int i0 = (ib + x) * kTileRows;
-    dq[x] = r.ranges != nullptr && i0 < r.t ? docs_of(r, i0, i0 + kTileRows - 1) : Docs{INT_MAX, -1, -1};
-  }
-  auto state = [&](int x, int hh) {                     // of query tile x and half tile hh
-    const int i0 = (ib + x) * kTileRows, j0 = hh * 64;
-    if (i0 >= r.t) return 0;
+  const Docs dq = r.ranges != nullptr ? docs_of(r, i0, i0 + kTileRows - 1) : Docs{INT_MAX, -1, -1};
+  auto state = [&](int hh) {                            // of half tile hh
+    const int j0 = hh * 64;
     const Docs dj = r.ranges != nullptr ? docs_of(r, j0, j0 + 63) : Docs{INT_MAX, -1, -1};
-    return pair_state<BIAS>(r, i0, i0 + kTileRows - 1, dq[x], j0, j0 + 63, dj);
+    return pair_state<BIAS>(r, i0, i0 + kTileRows - 1, dq, j0, j0 + 63, dj);
   };
 
-  const int top = (attend::key_end(r, min(r.t, (ib + NT) * kTileRows) - 1) + 63) / 64;
+  const int top = (attend::key_end(r, min(r.t, i0 + kTileRows) - 1) + 63) / 64;
   if (tid == 0) {
     ctl->abort = 0;
     for (int x = 0; x < 1 + 2 * R + (NB + 1) * NG; ++x) mbar_init(qfull + 8 * x, 1);        // qfull, kfull, kfree, sdone, odone
     for (int x = 0; x < NB * NG; ++x) mbar_init(pready + 8 * x, 4);      // (of a buffer: a warp may be a half tile ahead of another)
     fence_barrier_init();
   }
-  for (int x = tid; x < NT * 128; x += F::kThreads) sFlag[x] = 0;
+  if (tid < 128) sFlag[tid] = 0;
   __syncwarp();
   if (warp == 0) tmem_alloc(smem_u32(&ctl->tmem), F::kTmem);
-  {
-    int2 mine = make_int2(INT_MAX, 0);
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      const int2 y = keep_states(&s_state[x], 0, top, warp, F::kThreads / 32, [&](int hh) { return state(x, hh); });
-      mine = make_int2(min(mine.x, y.x), max(mine.y, y.y));
-    }
-    if (lane == 0) s_range[warp] = mine;
-  }
+  const int2 mine = keep_states(&s_state, 0, top, warp, F::kThreads / 32, state);
+  if (lane == 0) s_range[warp] = mine;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -321,7 +306,7 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
   // nearest keys first: a distance bias has the largest scores there, and later half tiles do not move the reference
   const int last = h0 + nh - 1;
 
-  if (warp_u == 8 * NT) {
+  if (warp_u == 8) {
     // ------------------------------------------------------------ the issuing warp
     constexpr uint32_t id_s = instr_desc(128, 64, 0, 0), id_p = instr_desc(128, D, 0, 1);
     const Desc dQ = make_desc(sQ, 16, 1024), dK = make_desc(sK, 16, 1024), dV = make_desc(sV, HSub, 1024);
@@ -331,52 +316,47 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       tma_load_rows<W>(sK + HB * st, &map_k, (last - e) * 64, nk, kfull + 8 * st, HSub);
       tma_load_rows<W>(sV + HB * st, &map_v, (last - e) * 64, nk, kfull + 8 * st, HSub);
     };
-    const int tiles = NT == 2 && (ib + 1) * kTileRows < r.t ? 2 : 1;
     if (nh > 0) {
       if (lead) {
-        mbar_expect_tx(qfull, tiles * TB);
-        for (int x = 0; x < tiles; ++x) tma_load_rows<W>(sQ + TB * x, &map_q, (ib + x) * kTileRows, n, qfull);
+        mbar_expect_tx(qfull, TB);
+        tma_load_rows<W>(sQ, &map_q, i0, n, qfull);
       }
       for (int e = 0; e < R && e < nh; ++e) load_keys(e, e);
       mbar_wait_warp(qfull, 0, ctl, &g_attend_status, kErrWaitTma);
       uint32_t pending = 0, flip = 0, side = 0;          // warpgroups with a P~ to come, the parity of the next, the buffer of its scores
       // (counters in place of remainders: this warp's time between two products is what the others wait for)
       int in = 0, out = 0, refill = 0;
-      uint32_t phase = 0, back = 0, word[NT];
+      uint32_t phase = 0, back = 0, word = 0;
       for (int e = 0; e < nh + 2; ++e) {
         const int hh = last - e;
         if (((hh & 31) == 31 || e == 0) && e < nh)
-#pragma unroll
-          for (int x = 0; x < NT; ++x)
-            word[x] = uniform(hh < kStates ? s_state[x].any[hh / 32] : __ballot_sync(0xffffffffu, (hh & ~31) + lane < h0 + nh && state(x, (hh & ~31) + lane) != 0));
+          word = uniform(hh < kStates ? s_state.any[hh / 32]
+                                      : __ballot_sync(0xffffffffu, (hh & ~31) + lane < h0 + nh && state((hh & ~31) + lane) != 0));
         if (e < nh) mbar_wait_warp(kfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
+        const int w = e & 1;
+        const uint32_t tW = tmem + F::kWgCols * w;
+        const bool seen = e < nh && (word >> (hh & 31) & 1), old = pending >> w & 1;
+        const int was = side >> w & 1, now = NB == 2 ? was ^ 1 : 0;
+        auto scores = [&]() {
+          tc_fence_after();
+          mma_scores_wide<W>(lead, tW + 64 * now, dQ, kTileBytes, Desc{dK.lo + (HB >> 4) * in, dK.hi},
+                             HSub, id_s);
+          mma_commit(lead, sdone + 8 * (NB * w + now));   // the scores, and every product in front of them
+        };
+        if (NB == 2 && seen) scores();                   // into the other buffer, while the arithmetic is at the last ones
+        if (old) {                                       // of half tile e - 2
+          const int bar = NB * w + (NB == 2 ? was : 0);
+          mbar_wait_warp(pready + 8 * bar, flip >> bar & 1, ctl, &g_attend_status, kErrWaitTile);
+          flip ^= 1u << bar;
+          tc_fence_after();
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          const int w = 2 * x + (e & 1);
-          const uint32_t tW = tmem + F::kWgCols * w;
-          const bool seen = e < nh && (word[x] >> (hh & 31) & 1), old = pending >> w & 1;
-          const int was = side >> w & 1, now = NB == 2 ? was ^ 1 : 0;
-          auto scores = [&]() {
-            tc_fence_after();
-            mma_scores_wide<W>(lead, tW + 64 * now, Desc{dQ.lo + (TB >> 4) * x, dQ.hi}, kTileBytes, Desc{dK.lo + (HB >> 4) * in, dK.hi},
-                               HSub, id_s);
-            mma_commit(lead, sdone + 8 * (NB * w + now));   // the scores, and every product in front of them
-          };
-          if (NB == 2 && seen) scores();                   // into the other buffer, while the arithmetic is at the last ones
-          if (old) {                                       // of half tile e - 2
-            const int bar = NB * w + (NB == 2 ? was : 0);
-            mbar_wait_warp(pready + 8 * bar, flip >> bar & 1, ctl, &g_attend_status, kErrWaitTile);
-            flip ^= 1u << bar;
-            tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)                 // 16 keys per instruction: 16 rows of 128 B = 128 units
-              mma_ts(lead, tW + 64 * NB, tW + 64 * (NB == 2 ? was : 0) + 8 * kk, dV, (HB >> 4) * out + 128 * kk, id_p, 1);
-            if (NB == 2) mma_commit(lead, odone + 8 * w);
-          }
-          if (NB == 1 && seen) scores();
-          pending = seen ? pending | 1u << w : pending & ~(1u << w);
-          if (NB == 2 && seen) side ^= 1u << w;
+          for (int kk = 0; kk < 4; ++kk)                 // 16 keys per instruction: 16 rows of 128 B = 128 units
+            mma_ts(lead, tW + 64 * NB, tW + 64 * (NB == 2 ? was : 0) + 8 * kk, dV, (HB >> 4) * out + 128 * kk, id_p, 1);
+          if (NB == 2) mma_commit(lead, odone + 8 * w);
         }
+        if (NB == 1 && seen) scores();
+        pending = seen ? pending | 1u << w : pending & ~(1u << w);
+        if (NB == 2 && seen) side ^= 1u << w;
         if (e >= 2) {
           mma_commit(lead, kfree + 8 * out);
           if (++out == R) out = 0;
@@ -407,11 +387,11 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       for (int c = 0; c < D / 16; ++c) tmem_st16(tO + 16 * c, z);
       tmem_st_wait();
     }
-    const int tile = NT == 2 ? wg >> 1 : 0, half = wg & 1, i = (ib + tile) * kTileRows + row, is = min(i, r.t - 1);
+    const int half = wg & 1, i = i0 + row, is = min(i, r.t - 1);
     float ref = -INFINITY, s = 0.f, sr = 0.f;
     int turn = 0;
     for (int e = half; e < nh; e += 2) {
-      const int hh = last - e, what = (int)uniform(hh < kStates ? s_state[tile].of(hh) : state(tile, hh));
+      const int hh = last - e, what = (int)uniform(hh < kStates ? s_state.of(hh) : state(hh));
       if (what == 0) continue;
       // (two buffers: the first scores go to buffer 1)
       const int side = NB == 2 ? (turn & 1) ^ 1 : 0;
@@ -436,13 +416,12 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       mbar_wait_warp(NB == 2 ? odone + 8 * wg : sdone + 8 * wg, (NB == 2 ? turn - 1 : turn) & 1, ctl, &g_attend_status, kErrWaitMma);
     tc_fence_after();
     // every product has read the ring, which the merge goes over
-    asm volatile("bar.sync 1, %0;" ::"n"(256 * NT) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(256) : "memory");
     // Each of a tile's two warpgroups finishes half of the features: it hands the other half of its accumulator over.
     constexpr int kPart = D / 2;
-    float* sX = reinterpret_cast<float*>(smem + NT * TB) + tile * 128 * D;           // [2][128][kPart]
-    float2* stat = sStat + 256 * tile;
-    float* rounded = reinterpret_cast<float*>(sStat + NT * 256) + 256 * tile;
-    stat[half * 128 + row] = make_float2(ref, s);
+    float* sX = reinterpret_cast<float*>(smem + TB);                                 // [2][128][kPart]
+    float* rounded = reinterpret_cast<float*>(sStat + 256);
+    sStat[half * 128 + row] = make_float2(ref, s);
     rounded[half * 128 + row] = sr;
     float* give = sX + ((1 - half) * 128 + row) * kPart;
     __syncwarp();
@@ -455,12 +434,9 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       for (int c = 0; c < 8; ++c)
         reinterpret_cast<float4*>(give + c0)[c ^ (row & 7)] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
     }
-    auto meet = [tile] {
-      if (NT == 1 || tile == 0) asm volatile("bar.sync 2, 256;" ::: "memory");
-      else asm volatile("bar.sync 3, 256;" ::: "memory");
-    };
+    auto meet = [] { asm volatile("bar.sync 2, 256;" ::: "memory"); };
     meet();
-    const float2 other = stat[(1 - half) * 128 + row];
+    const float2 other = sStat[(1 - half) * 128 + row];
     const float m = fmaxf(ref, other.x), base = m == -INFINITY ? 0.f : m;
     const float f_own = fast_exp2(ref - base), f_oth = fast_exp2(other.x - base);
     const float den = s * f_own + other.y * f_oth, by = sr * f_own + rounded[(1 - half) * 128 + row] * f_oth, inv = by == 0.f ? 0.f : 1.f / by;
@@ -503,12 +479,12 @@ __global__ void __launch_bounds__(AttendForward<D, NT>::kThreads, D == 64 && NT 
       }
     }
     if (half == 0 && i < r.t && a.lse != nullptr) a.lse[(int64_t)n * a.t + i] = den == 0.f ? INFINITY : m + log2f(den);
-    if (bad && i < r.t) sFlag[tile * 128 + row] = 1;
+    if (bad && i < r.t) sFlag[row] = 1;
     meet();
     // (both warpgroups have written their halves; a warp's rows are its own lanes', every other one of them)
-    unsigned again = __ballot_sync(0xffffffffu, sFlag[tile * 128 + row] != 0) & (half ? 0xaaaaaaaau : 0x55555555u);
+    unsigned again = __ballot_sync(0xffffffffu, sFlag[row] != 0) & (half ? 0xaaaaaaaau : 0x55555555u);
     for (; again; again &= again - 1)
-      attend::redo_forward_row<__nv_bfloat16, D>(a, b, h, (ib + tile) * kTileRows + (row & 96) + __ffs(again) - 1);
+      attend::redo_forward_row<__nv_bfloat16, D>(a, b, h, i0 + (row & 96) + __ffs(again) - 1);
   }
   drain_if_aborted(ctl);
   tc_fence_before();

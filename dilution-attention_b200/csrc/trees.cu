@@ -198,11 +198,14 @@ template <int D> int tc_softmax(tree::Args a, void* scratch, cudaStream_t st) {
                       tree::join_softmax_smem<D>(a.nodes), st, "tree_join", a);
 }
 
-// A step in one launch, a cluster of eight CTAs per head: for short caches whose clusters all run at once.  24 nodes of heads of 64,
-// one launch / chunks (four launches, with 6 us of timing events each; shares 16 nodes at a time on either side), us: 32 heads, 1024 keys 29 / 53, 4096 keys 35 / 51, 8192 keys
-// 44 / 59; 16 heads, 16384 keys 60 / 69; but 64 heads, 16384 keys 121 / 131 and 256 heads 450 / 370: a CTA's start, its three meetings
-// with the others and its end take about 20 us, which chunks overlap with other chunks' tiles.
-bool by_clusters(const tree::Args& a) { return (int64_t)a.batch * a.kv_heads <= 32 && tree_keys(a) <= 16384; }
+// A step in one launch, a cluster of eight CTAs per head: for short caches whose clusters all run at once (a CTA of heads of 128 has an
+// SM to itself, and clusters of them do not share one).  24 nodes, one launch / chunks (four launches that start early), both replayed from
+// a graph, us.  Heads of 64: 1 head, 1024 keys 25 / 29, 8192 keys 35 / 33; 8 heads, 1024 27 / 31, 8192 37 / 41; 16 heads, 1024 29 / 35, 8192
+// 41 / 41, 16384 57 / 51; 32 heads, 1024 30 / 37, 8192 45 / 53; 64 heads, 4096 64 / 51.  Heads of 128: 1 head, 1024 29 / 31, 8192 43 / 35;
+// 8 heads, 1024 29 / 33, 4096 35 / 35; 16 heads, 512 51 / 33; 32 heads, 8192 115 / 66.
+template <int D> bool by_clusters(const tree::Args& a) {
+  return (int64_t)a.batch * a.kv_heads <= (D == 64 ? 32 : 8) && tree_keys(a) <= (D == 64 ? 8192 : 4096) + tree::kMaxNodes;
+}
 template <int D, int N> int tc_draft(const tree::Args& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
   using F = tc::Draft<D, N>;
   if (int rc = opt_in(tc::draft_kernel<D, N>, F::kBytes)) return rc;
@@ -226,7 +229,7 @@ template <int D> int tc_dilute(tree::Args a, void* scratch, cudaStream_t st) {
   CUtensorMap k, v;
   if (int rc = cache_maps(&k, &v, a, D)) return rc;
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
-  if (by_clusters(a)) return a.nodes <= 16 ? tc_draft<D, 16>(a, k, v, st) : a.nodes <= 32 ? tc_draft<D, 32>(a, k, v, st) : tc_draft<D, 64>(a, k, v, st);
+  if (by_clusters<D>(a)) return a.nodes <= 16 ? tc_draft<D, 16>(a, k, v, st) : a.nodes <= 32 ? tc_draft<D, 32>(a, k, v, st) : tc_draft<D, 64>(a, k, v, st);
   a.chunks = tc_chunks(heads, tree_keys(a), tc::Sweep<D, 64, true>::kPerSm);
   float* shares = place_scratch(a, scratch, D);
   if (int rc = tc_scan<D, false>(a, k, v, st)) return rc;
