@@ -1,4 +1,5 @@
-// extern "C" entry points of masked softmax attention and of eviction.  Argument validation, kernel selection and launches; declarations in include/dilution_b200.h.
+// extern "C" entry points of masked softmax attention and of eviction.  Argument validation, kernel selection and launches;
+// declarations in include/dilution_b200.h.
 
 #include <algorithm>
 #include <cstdint>

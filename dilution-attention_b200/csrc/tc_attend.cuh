@@ -4,8 +4,8 @@
 // off by up to 2^-8 of itself.  References, sums, lse, delta and accumulators are fp32.  A warp of its own issues
 // every copy and MMA.  Which pairs of tiles have anything to do is asked of the documents' ranges, never of a list.
 //
-//   forward : a CTA's query tile of 128 walks over half tiles of 64 keys; two warpgroups take them in turn.  lane = query: reference, sum and accumulator of a row belong to one thread and
-//             warpgroup, and are merged once at the end.
+//   forward : a CTA's query tile of 128 walks over half tiles of 64 keys; two warpgroups take them in turn.  lane = query:
+//             reference, sums and accumulator of a row belong to one thread and warpgroup, and are merged once at the end.
 //   backward: one kernel for both halves.  A tile of 128 stays (dq: queries with their dout; dk, dv: keys with their values),
 //             half tiles of 64 of the other kind stream past; kWg warpgroups take them in turn, and accumulators in TMEM
 //             are shared by all of them.  dq: lane = query.  dk, dv: lane = key, and nothing is reduced across CTAs: the heads
@@ -13,9 +13,10 @@
 //             place of five, and no result depends on an order of atomic additions.
 //
 // What bounds them, per pair of tiles of 128 x 64: 512 cycles for one exponential a score on the special-function unit (16 a
-// clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.  Measured, forward / dk, dv /
-// dq: n = 64, T = 8192, heads of 64 773 / 1066 / 881 us (forward 0.62 of the exponentials' rate); documents of 700 tokens 220 / 235 / 185 us,
-// where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads of 128, capped 830 / 1020 / 795 us.
+// clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.  Measured, forward /
+// dk, dv / dq in us: n = 64, T = 8192, heads of 64 773 / 1066 / 881 (forward 0.62 of the exponentials' rate), documents of 700
+// tokens 220 / 235 / 185, where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads
+// of 128, capped 830 / 1020 / 795.
 #pragma once
 
 #include "attend_common.cuh"

@@ -9,9 +9,9 @@
 //   sweep_kernel: S^T = K Q^T, lane = key, for what belongs to keys: a thread walks the tree in the nodes' order with its
 //                 key's demand (a node's demand is its parent's demand and bid; a parent further back is found in the TMEM
 //                 column that its score came from), and out^T += V^T share; or it adds the accepted nodes' bids.
-// What bounds them: the cache's bytes.  256 heads of 64, 24 nodes over 16384 keys: statistics 96 us (0.54 GB, 0.85 of the copy rate), shares
-// and outputs 169 us (1.09 GB, 0.98), five accepted nodes' bids 86 us (0.55 GB, 0.98).  64 key heads whose 128 rows fill the lanes:
-// 70 us for 0.27 GB, of which the exponentials need 30.
+// What bounds them: the cache's bytes.  256 heads of 64, 24 nodes over 16384 keys: statistics 96 us (0.54 GB, 0.85 of the copy
+// rate), shares and outputs 169 us (1.09 GB, 0.98), five accepted nodes' bids 86 us (0.55 GB, 0.98).  64 key heads whose 128 rows
+// fill the lanes: 70 us for 0.27 GB, of which the exponentials need 30.
 // A chunk of a key head's keys per CTA; one warp issues copies, one MMAs, two warpgroups take tiles in turn.
 #pragma once
 
@@ -390,8 +390,8 @@ struct RowStep {
   float slope2;
   int pad;
 };
-// And of a draft's nodes, in their order: their lse (+inf behind the last: no bids), their parents; as bits, those that follow none (roots) or
-// another than the one in front (far), and those whose demand such a later one starts from (keeps).
+// And of a draft's nodes, in their order: their lse (+inf behind the last: no bids), their parents; as bits, those that follow
+// none (roots) or another than the one in front (far), and those whose demand such a later one starts from (keeps).
 struct Walk {
   float lse[64];
   uint8_t up[64];
