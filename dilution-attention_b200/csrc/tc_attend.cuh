@@ -533,9 +533,11 @@ __device__ __forceinline__ void backward_tile(uint32_t tS, const Row& r, float l
     if (CAP) cap_scores<32>(v, pre);
     uint32_t pw[16], gw[16];
     const float2 mm = make_float2(lin, lin);
-    // the distance's term of column e: first + step * e (one sign throughout, except in masked tiles)
-    const float step = STAY == 1 ? -r.slope2 : r.slope2;
-    const float first = STAY == 1 ? r.slope2 * (float)(y - x0 - c0) : r.slope2 * (float)(x0 + c0 - y);
+    // the distance's term of column e: first + step * e; in masked tiles, whose distances have both signs, these are the plain
+    // distances, and the slope, of either sign itself, comes to their size
+    const float by = EDGE ? 1.f : r.slope2, step = STAY == 1 ? -by : by;
+    const float first = by * (float)(STAY == 1 ? y - x0 - c0 : x0 + c0 - y);
+    const float2 slope = make_float2(-r.slope2, -r.slope2);
     float2 far = make_float2(first, first + step);
     const float2 two = make_float2(2.f * step, 2.f * step);
 #pragma unroll
@@ -547,7 +549,7 @@ __device__ __forceinline__ void backward_tile(uint32_t tS, const Row& r, float l
         delta = make_float2(x.z, x.w);
       }
       if (BIAS) {
-        off = add2(off, EDGE ? make_float2(-fabsf(far.x), -fabsf(far.y)) : far);
+        off = EDGE ? fma2(make_float2(fabsf(far.x), fabsf(far.y)), slope, off) : add2(off, far);
         far = add2(far, two);
       }
       const float2 z = fma2(make_float2(v[e], v[e + 1]), mm, off);
