@@ -99,13 +99,12 @@ __device__ __forceinline__ bool tile_full(const Row& r, int i0, int i1, int j0, 
 }
 
 // (z, 1 - (c / cap)^2) of q . k: the score in the log2 domain and what the gradient of the capped score is multiplied by.
-// EXACT: CUDA's tanhf (fp32 tensors).  Otherwise tanh x = 1 - 2 / (1 + e^2x) from two special-function operations: an
-// error of 2e-7 of the cap, where bf16 scores carry 2^-9 of themselves; e^2x = inf gives 1.
+// EXACT: CUDA's tanhf (fp32 tensors), otherwise tanh_score.
 template <bool EXACT>
 __device__ __forceinline__ float2 score(const Row& r, float dot, int i, int j) {
   float z, slack = 1.f;
   if (r.cap2 > 0.f) {
-    const float u = EXACT ? tanhf(dot * r.pre * (0.5f * kLn2)) : fmaf(-2.f, fast_rcp(1.f + fast_exp2(dot * r.pre)), 1.f);
+    const float x = dot * r.pre * (0.5f * kLn2), u = EXACT ? tanhf(x) : tanh_score(x);
     z = r.cap2 * u;
     slack = fmaf(-u, u, 1.f);
   } else {

@@ -157,6 +157,20 @@ __device__ __forceinline__ float ld_cluster(const float* p, int rank) {
 __device__ __forceinline__ void let_next_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// tanh of a capped score next to bf16 operands, to 3e-7 of the value below 1 and 4e-7 past it, where 1 - 2 / (1 + e^2x) from two
+// special-function operations cancels nothing (e^2x = inf gives 1).  Below 1 it would be off by 2e-7 of the CAP, however small the
+// score: x + x^3 P(x^2) there, a least-maximum fit of degree 5 (8e-8).
+__device__ constexpr float kTanh[6] = {-0.3333301842212677f, 0.133268341422081f, -0.053518135100603104f,
+                                       0.02039860375225544f, -0.006294633727520704f, 0.0010702026775106788f};
+__device__ __forceinline__ float tanh_past_one(float x) { return fmaf(-2.f, fast_rcp(1.f + fast_exp2(x * (2.f * kLog2e))), 1.f); }
+__device__ __forceinline__ float tanh_score(float x) {
+  const float y = x * x;
+  float p = kTanh[5];
+#pragma unroll
+  for (int i = 4; i >= 0; --i) p = fmaf(p, y, kTanh[i]);
+  return fabsf(x) <= 1.f ? fmaf(x, p * y, x) : tanh_past_one(x);
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));

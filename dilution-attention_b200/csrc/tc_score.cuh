@@ -25,16 +25,14 @@ __device__ __forceinline__ uint32_t left_pair(float lo, float hi) {
 template <int D> constexpr int kForm = D == 128 ? kWide128 : kNarrow;
 
 // ---- scores ----------------------------------------------------------------------------------------
-// tanh of two values, |x| <= 1: x + x^3 P(x^2) with a least-maximum fit of degree 5, 1.6e-7 relative.  Nine packed instructions,
-// where the two special-function operations of a value take 16 cycles of a warp's quarter.
+// tanh of two values, |x| <= 1 (tanh_score).  Nine packed instructions, where the two special-function operations of a value take 16
+// cycles of a warp's quarter.
 __device__ __forceinline__ float2 tanh_poly2(float2 x) {
   auto both = [](float c) { return make_float2(c, c); };
   const float2 y = mul2(x, x);
-  float2 p = fma2(y, both(0.0010702026775106788f), both(-0.006294633727520704f));
-  p = fma2(p, y, both(0.02039860375225544f));
-  p = fma2(p, y, both(-0.053518135100603104f));
-  p = fma2(p, y, both(0.133268341422081f));
-  p = fma2(p, y, both(-0.3333301842212677f));
+  float2 p = both(kTanh[5]);
+#pragma unroll
+  for (int i = 4; i >= 0; --i) p = fma2(p, y, both(kTanh[i]));
   p = mul2(p, y);
   return fma2(x, p, x);
 }

@@ -86,8 +86,7 @@ template <bool EXACT>
 __device__ __forceinline__ float score(float dot, float scale, float cap, float slope2, float far) {
   float z;
   if (cap > 0.f)
-    z = cap * kLog2e * (EXACT ? tanhf(dot * scale / cap)
-                              : fmaf(-2.f, fast_rcp(1.f + fast_exp2(dot * (scale * 2.f * kLog2e / cap))), 1.f));
+    z = cap * kLog2e * (EXACT ? tanhf(dot * scale / cap) : tanh_score(dot * (scale / cap)));
   else
     z = dot * (scale * kLog2e);
   return fmaf(-slope2, far, z);

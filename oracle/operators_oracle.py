@@ -3,7 +3,11 @@
 `bound` arrays are worst cases by arithmetic, element by element.  u is what one rounding of a formed value (a probability,
 a share, a score's gradient, an output) is off by at most, relative to the value: 2^-8 for bf16.  For fp32 kernels u stands
 for all the roundings of a sum of n terms, n 2^-24.  Scores are fp32 sums of D products: off by at most
-(D + 8) 2^-24 sum |q k| each, which every probability carries as a relative error (`slack`)."""
+(D + 8) 2^-24 sum |q k| each, which every probability carries as a relative error (`slack`).
+
+A capped score is off by at most 4e-7 min(cap, |s|) next to bf16, s the score in front of the cap: below the cap tanh is x + x^3 P(x^2),
+whose fit (8e-8), argument (two roundings), polynomial (0.33 2^-23) and last rounding come to 3e-7 of x; past it 1 - 2 / (1 + e^2x), whose
+exponential (2^-22, times 0.12 at x = -1), reciprocal (2^-23) and sums come to 3.7e-7 of the cap."""
 
 from __future__ import annotations
 
@@ -47,8 +51,9 @@ def attention(q, k, v, dout=None, softcap=None, slopes=None, documents=None, pre
             qs, ks, vs = (torch.where(torch.isfinite(x), x, 0.0) for x in (q64[b, h], k64[b, g], v64[b, g]))
             c = qs @ ks.T * scale
             size = qs.abs() @ ks.abs().T * scale
-            t = torch.zeros_like(c)
+            t, capped = torch.zeros_like(c), 0.0
             if softcap is not None:
+                capped = 4e-7 * c.abs().clamp(max=softcap)
                 t = torch.tanh(c / softcap)
                 c = softcap * t
             a = c if slopes is None else c - slopes[h].double() * far
@@ -57,8 +62,8 @@ def attention(q, k, v, dout=None, softcap=None, slopes=None, documents=None, pre
             e = torch.exp(a - torch.where(torch.isfinite(top), top, 0.0))
             mass = e.sum(-1, keepdim=True)
             p = e / torch.where(mass > 0, mass, 1.0)
-            # a score's error, also through the cap (2e-7 of it next to bf16) and the distance's product
-            wrong = (dim + 8) * 2.0 ** -24 * size + (4e-7 * softcap if softcap else 0.0) + 2.0 ** -22 * torch.where(see, a.abs(), 0.0)
+            # a score's error, also through the cap and the distance's product
+            wrong = (dim + 8) * 2.0 ** -24 * size + capped + 2.0 ** -22 * torch.where(see, a.abs(), 0.0)
             slack = 2 * wrong.masked_fill(~see, 0.0).amax(-1, keepdim=True) + 2.0 ** -20
             out = p @ vs
             spread = p @ vs.abs()
@@ -111,12 +116,14 @@ def tree_nodes(q, k, v, cache_k, cache_v, length, parents, softcap=None, slopes=
                 at = torch.tensor(seen, device=q.device)
                 s = keys[at] @ q[b, h, x].double() * dim ** -0.5
                 size = keys[at].abs() @ q[b, h, x].double().abs() * dim ** -0.5
+                capped = 0.0
                 if softcap is not None:
+                    capped = 4e-7 * s.abs().clamp(max=softcap)
                     s = softcap * torch.tanh(s / softcap)
                 if slopes is not None:
                     s = s - slopes[h].double() * torch.arange(len(seen) - 1, -1, -1, device=q.device)
                 p = torch.softmax(s, 0)
-                slack = 2 * ((dim + 8) * 2.0 ** -24 * size + (4e-7 * softcap if softcap else 0.0) + 2.0 ** -22 * s.abs()).amax() + 2.0 ** -20
+                slack = 2 * ((dim + 8) * 2.0 ** -24 * size + capped + 2.0 ** -22 * s.abs()).amax() + 2.0 ** -20
                 bids[b, h, x, at] = p
                 bids_off[b, h, x, at] = slack * p
                 if committed is None:
