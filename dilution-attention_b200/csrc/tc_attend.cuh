@@ -169,7 +169,7 @@ __device__ __forceinline__ void forward_step(uint32_t tS, uint32_t tO, const Row
     tmem_ld32(tS + 32, v + 32);
     tmem_ld_wait(v);
     tmem_ld_wait(v + 32);
-    if (CAP) cap_scores<64>(v, pre);
+    if (CAP) cap_scores<64>(v, pre, r.cap2 > kWideCap * kLog2e);
     if (edge) {
       const uint2 m = key_bits(r, i, j0);
       some = (m.x | m.y) != 0;
@@ -530,7 +530,7 @@ __device__ __forceinline__ void backward_tile(uint32_t tS, const Row& r, float l
     tmem_ld32(tS + 64 + c0, g);
     tmem_ld_wait(v);
     tmem_ld_wait(g);
-    if (CAP) cap_scores<32>(v, pre);
+    if (CAP) cap_scores<32>(v, pre, r.cap2 > kWideCap * kLog2e);
     uint32_t pw[16], gw[16];
     const float2 mm = make_float2(lin, lin);
     // the distance's term of column e: first + step * e; in masked tiles, whose distances have both signs, these are the plain

@@ -36,17 +36,15 @@ __device__ __forceinline__ float2 tanh_poly2(float2 x) {
   p = mul2(p, y);
   return fma2(x, p, x);
 }
-// v = tanh(v * pre) of N products q . k.  pre: scale / cap.
-template <int N> __device__ __forceinline__ void cap_scores(float* v, float pre) {
+// v = tanh(v * pre) of N products q . k.  pre: scale / cap.  Where a score of the warp is past the cap all take the form for those, which
+// is off by 4e-7 of the cap: at most 4e-4 of a score up to caps of 1024, a tenth of what the rounding of P~ may be.  wide: larger
+// caps, each score by its own size.  (That for all caps: B2 H16 T8192, heads of 128, scores past a cap of 5, forward 1087 -> 1830 us.)
+template <int N> __device__ __forceinline__ void cap_scores(float* v, float pre, bool wide) {
   float top = 0.f;
 #pragma unroll
   for (int e = 0; e < N; e += 2) top = fmaxf(top, fmaxf(fabsf(v[e]), fabsf(v[e + 1])));
   // (fmaxf passes over a NaN, which comes through either form)
-  if (__any_sync(0xffffffffu, top * pre > 1.f)) {
-    const float twice = pre * 2.f * kLog2e;
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = fmaf(-2.f, fast_rcp(1.f + fast_exp2(v[e] * twice)), 1.f);
-  } else {
+  if (!__any_sync(0xffffffffu, top * pre > 1.f)) {
     const float2 pp = make_float2(pre, pre);
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
@@ -54,8 +52,16 @@ template <int N> __device__ __forceinline__ void cap_scores(float* v, float pre)
       v[e] = t.x;
       v[e + 1] = t.y;
     }
+  } else if (wide) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = tanh_score(v[e] * pre);
+  } else {
+    const float twice = pre * 2.f * kLog2e;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = fmaf(-2.f, fast_rcp(1.f + fast_exp2(v[e] * twice)), 1.f);
   }
 }
+constexpr float kWideCap = 1024.f;
 
 // ---- tensor maps -----------------------------------------------------------------------------------
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -127,7 +127,7 @@ __device__ __forceinline__ void scan_step(uint32_t tS, uint32_t tP, uint32_t tO,
     if (N == 64) tmem_ld32(tS + 32, v + (N - 32));
     tmem_ld_wait(v);
     if (N == 64) tmem_ld_wait(v + (N - 32));
-    if (cap) cap_scores<N>(v, pre);
+    if (cap) cap_scores<N>(v, pre, lin > kWideCap * kLog2e);
     if (valid < N) {
 #pragma unroll
       for (int e = 0; e < N; ++e) v[e] = e < valid ? v[e] : -INFINITY;
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(320, Sweep<D, N, DILUTE>::kPerSm) sweep_kernel
           __syncwarp();
           tmem_ld16(tS + c0, v);
           tmem_ld_wait16(v);
-          if (cap) cap_scores<16>(v, pre);
+          if (cap) cap_scores<16>(v, pre, lin > kWideCap * kLog2e);
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
             const RowStep s = step[c0 + y];

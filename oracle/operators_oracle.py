@@ -7,7 +7,8 @@ for all the roundings of a sum of n terms, n 2^-24.  Scores are fp32 sums of D p
 
 A capped score is off by at most 4e-7 min(cap, |s|) next to bf16, s the score in front of the cap: below the cap tanh is x + x^3 P(x^2),
 whose fit (8e-8), argument (two roundings), polynomial (0.33 2^-23) and last rounding come to 3e-7 of x; past it 1 - 2 / (1 + e^2x), whose
-exponential (2^-22, times 0.12 at x = -1), reciprocal (2^-23) and sums come to 3.7e-7 of the cap."""
+exponential (2^-22, times 0.12 at x = -1), reciprocal (2^-23) and sums come to 3.7e-7 of the cap.  Up to caps of 1024 a score below the
+cap may take the second form, off by that much of the cap (`cap_error`): a tenth of a probability's rounding."""
 
 from __future__ import annotations
 
@@ -33,6 +34,10 @@ def _unit(dtype, terms):
     return 2.0 ** -8 if dtype == torch.bfloat16 else (terms + 64) * 2.0 ** -24
 
 
+def cap_error(s, softcap):
+    return 4e-7 * (softcap if softcap <= 1024 else s.abs().clamp(max=softcap))
+
+
 def attention(q, k, v, dout=None, softcap=None, slopes=None, documents=None, prefix=None):
     """((out, dq, dk, dv), bounds) of masked softmax attention, or (out,) and its bound without dout."""
     dtype, (batch, heads, seq, dim) = q.dtype, q.shape
@@ -53,7 +58,7 @@ def attention(q, k, v, dout=None, softcap=None, slopes=None, documents=None, pre
             size = qs.abs() @ ks.abs().T * scale
             t, capped = torch.zeros_like(c), 0.0
             if softcap is not None:
-                capped = 4e-7 * c.abs().clamp(max=softcap)
+                capped = cap_error(c, softcap)
                 t = torch.tanh(c / softcap)
                 c = softcap * t
             a = c if slopes is None else c - slopes[h].double() * far
@@ -118,7 +123,7 @@ def tree_nodes(q, k, v, cache_k, cache_v, length, parents, softcap=None, slopes=
                 size = keys[at].abs() @ q[b, h, x].double().abs() * dim ** -0.5
                 capped = 0.0
                 if softcap is not None:
-                    capped = 4e-7 * s.abs().clamp(max=softcap)
+                    capped = cap_error(s, softcap)
                     s = softcap * torch.tanh(s / softcap)
                 if slopes is not None:
                     s = s - slopes[h].double() * torch.arange(len(seen) - 1, -1, -1, device=q.device)

@@ -34,3 +34,21 @@ def test_tree_steps(cap, dtype, dim):
     taken, far = (x[:, :, [0, 1, 3]][..., :150].unflatten(1, (2, 2)).sum((2, 3)) for x in (bids, bids_off))
     taken = taken + before[:, :, :150].double()
     within(cache["committed"][:, :, :150], taken, far + 2.0 ** -18 * taken + 1e-9)
+
+
+@pytest.mark.parametrize("dtype,dim", TYPES)
+@pytest.mark.parametrize("cap", [1e4, 1e6])
+def test_a_row_past_the_cap_beside_ordinary_ones(cap, dtype, dim):
+    """One query in 40 has scores beyond the cap; its neighbours' stay as exact as without it."""
+    q, k, v, dout = inputs(1, 2, 2, 200, dim, dtype)
+    q[:, :, ::40] *= 8 * cap
+    check((q, k, v, dout), softcap=cap)
+
+
+@pytest.mark.parametrize("dtype,dim", TYPES)
+@pytest.mark.parametrize("cap", [1e4, 1e6])
+def test_a_node_past_the_cap_beside_ordinary_ones(cap, dtype, dim):
+    q, k, v, cache = case(1, 2, 2, len(TREE), dim, 150, dtype)
+    q[:, :, 5] *= 8 * cap
+    out, _ = load_package().softmax_tree_step(q, k, v, cache, TREE, softcap=cap)
+    within(out, *O.tree_nodes(q, k, v, cache["k"], cache["v"], 150, TREE, softcap=cap)[:2])
