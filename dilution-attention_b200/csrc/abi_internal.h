@@ -44,6 +44,8 @@ template <typename W> int read_status_word(const W& word, int* code) {
 }
 
 inline bool valid_d(int d) { return d == 16 || d == 32 || d == 64 || d == 128; }
+// A cap of the scores, or 0 for none: what it divides and multiplies stays inside fp32.
+inline bool valid_cap(float cap) { return cap == 0.f || (cap >= 1e-30f && cap <= 1e38f); }
 inline bool misaligned(std::initializer_list<const void*> ps) {
   uintptr_t x = 0;
   for (const void* p : ps) x |= (uintptr_t)p;

@@ -29,8 +29,8 @@ int check_attend(const char* fn, const attend::Args& a, int dtype, int d) {
                     a.batch, a.heads, a.kv_heads, a.t);
   if (a.t > (1 << 30) || (double)a.batch * a.heads * (double)doc_spans(a.t) >= 2147483648.0)
     return abi_fail(DILUTION_ERR_ARG, "%s: batch * heads * blocks exceeds the grid limit", fn);
-  if (!(a.cap >= 0.f) || a.cap > 3e38f || !(a.scale > 0.f))
-    return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap finite, 0 for none", fn);
+  if (!valid_cap(a.cap) || !(a.scale > 0.f))
+    return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap in [1e-30, 1e38], or 0 for none", fn);
   if (!a.q || !a.k || !a.v || !a.out || (a.docs && !a.ranges)) return abi_fail(DILUTION_ERR_ARG, "%s: null pointer", fn);
   if (a.rest && dtype != DILUTION_BF16) return abi_fail(DILUTION_ERR_ARG, "%s: rest is of bf16 outputs alone", fn);
   if (misaligned({a.q, a.k, a.v, a.out, a.rest, a.dout, a.dq, a.dk, a.dv, a.ranges}))

@@ -67,8 +67,8 @@ int check_tree(const char* fn, const tree::Args& a, int64_t length, int dtype, i
     return abi_fail(DILUTION_ERR_ARG, "%s: a tree has 1 to %d nodes, not %d", fn, tree::kMaxNodes, a.nodes);
   if (a.capacity < 1 || a.capacity > (1 << 30) || length < 0 || length > a.capacity)
     return abi_fail(DILUTION_ERR_ARG, "%s: length %lld outside cache capacity %lld", fn, (long long)length, (long long)a.capacity);
-  if (!(a.cap >= 0.f) || a.cap > 3e38f || !(a.scale > 0.f))
-    return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap finite, 0 for none", fn);
+  if (!valid_cap(a.cap) || !(a.scale > 0.f))
+    return abi_fail(DILUTION_ERR_ARG, "%s: scale must be positive and cap in [1e-30, 1e38], or 0 for none", fn);
   if (!a.q || !a.kn || !a.vn || !a.kc || !a.vc || !a.parents || !a.lse) return abi_fail(DILUTION_ERR_ARG, "%s: null pointer", fn);
   if (misaligned({a.q, a.kn, a.vn, a.kc, a.vc}))
     return abi_fail(DILUTION_ERR_ARG, "%s: q, drafted keys and values and caches must be 16-byte aligned", fn);

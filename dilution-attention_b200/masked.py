@@ -43,8 +43,8 @@ def check_softcap(softcap) -> float:
     if softcap is None:
         return 0.0
     softcap = float(softcap)
-    if not (softcap > 0.0 and math.isfinite(softcap)):
-        raise ValueError("softcap must be a positive number, or None")
+    if not 1e-30 <= softcap <= 1e38:
+        raise ValueError("softcap must be a number from 1e-30 to 1e38, or None")
     return softcap
 
 
@@ -149,7 +149,7 @@ def softmax_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softcap
     q: (B, H, T, D); k, v: (B, H_kv, T, D) with H_kv dividing H, query head h on key head h // (H / H_kv); all float32
     or all bfloat16, D in {16, 32, 64, 128}, any strides.  Returns (B, H, T, D) in q's dtype.
 
-    softcap: scores go through softcap * tanh(s / softcap).  slopes: (H,), constants.  documents: (B, T) int32 or int64
+    softcap: scores go through softcap * tanh(s / softcap), from 1e-30 to 1e38.  slopes: (H,), constants of either sign.  documents: (B, T) int32 or int64
     ids below 2^31; a token sees its own document alone, and one with a negative id (padding) sees and is seen by nothing:
     its output and its gradients are zero, and what its rows hold does not matter.  prefix: (B,) integers or one for all;
     the first `prefix` tokens are seen by every token of their sequence (and document).

@@ -395,8 +395,8 @@ int dilution_variant_decode(const void* q1, const void* k1, const void* v1, void
 
 /* ---- masked softmax attention (no counterpart in the reference, whose softmax layers are causal only) -----------
  * q, out (batch, heads, t, d); k, v (batch, kv_heads, t, d), query head h on key head h / (heads / kv_heads); dtype
- * of all of them DILUTION_F32 or DILUTION_BF16, 16-byte aligned.  Scores scale q.k, through cap * tanh(x / cap) if cap > 0,
- * minus slopes[h] * |i - j| if slopes (heads fp32) is not NULL.  Query i of a sequence sees key j where j <= i, or
+ * of all of them DILUTION_F32 or DILUTION_BF16, 16-byte aligned.  Scores scale q.k, through cap * tanh(x / cap) if cap is not 0
+ * (1e-30 to 1e38), minus slopes[h] * |i - j| if slopes (heads fp32) is not NULL.  Query i of a sequence sees key j where j <= i, or
  * j < prefix[b] if prefix (batch) is not NULL, and where documents (batch, t), if not NULL, gives both the same id >= 0.  A
  * query that sees no key has out = 0 and lse = +inf.  With documents, `ranges` is a buffer of
  * dilution_attend_ranges_bytes(batch, t) that the forward fills and the backward reads.  lse (batch, heads, t) fp32: log2 of

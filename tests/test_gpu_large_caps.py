@@ -52,3 +52,10 @@ def test_a_node_past_the_cap_beside_ordinary_ones(cap, dtype, dim):
     q[:, :, 5] *= 8 * cap
     out, _ = load_package().softmax_tree_step(q, k, v, cache, TREE, softcap=cap)
     within(out, *O.tree_nodes(q, k, v, cache["k"], cache["v"], 150, TREE, softcap=cap)[:2])
+
+
+@pytest.mark.parametrize("dtype,dim", TYPES)
+@pytest.mark.parametrize("cap", [1e-30, 1e-3])
+def test_small_caps(cap, dtype, dim):
+    """All weights alike: nothing is left of the scores."""
+    check(inputs(1, 2, 1, 150, dim, dtype), softcap=cap, documents=documents_of(1, 150, 60, seed=1, pad=9))
