@@ -24,6 +24,7 @@ from . import _lib
 from . import kernels as K
 
 _DIMS = (16, 32, 64, 128)
+_INT_MAX = 2 ** 31 - 1
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
@@ -64,11 +65,13 @@ def check_slopes(slopes, heads, device):
 
 
 def _integers(x, shape, name, device):
-    """int32 on the device, in one of the given shapes."""
+    """int32 on the device, in the given shape; anything below 0 is as good as -1 here, and nothing wraps."""
     if not isinstance(x, torch.Tensor) or x.dtype not in (torch.int32, torch.int64) or x.shape != shape:
         raise ValueError(f"{name} must be an int32 or int64 tensor of shape {tuple(shape)}")
     if x.device != device:
         raise ValueError(f"{name} must be on q's device")
+    if x.dtype == torch.int64:
+        x = x.clamp(-1, _INT_MAX)
     return x.to(torch.int32).contiguous()
 
 
@@ -161,6 +164,6 @@ def softmax_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softcap
         documents = _integers(documents, (batch, seq), "documents", q.device)
     if prefix is not None:
         if isinstance(prefix, int):
-            prefix = torch.full((batch,), prefix, device=q.device, dtype=torch.int32)
+            prefix = torch.full((batch,), min(max(prefix, 0), _INT_MAX), device=q.device, dtype=torch.int32)
         prefix = _integers(prefix, (batch,), "prefix", q.device)
     return _SoftmaxAttention.apply(q, k, v, slopes, documents, prefix, softcap)
