@@ -79,6 +79,8 @@ def _indices(x, batch, name, device):
     if x.device != device:
         raise ValueError(f"{name} must be on q's device (or on the host)")
     stride = x.shape[1] if x.dim() == 2 else 0
+    if x.dtype == torch.int64:                 # (what lies outside every tree may not wrap into one)
+        x = x.clamp(-1, MAX_NODES)
     return x.to(torch.int32).contiguous(), stride, host
 
 

@@ -6,7 +6,9 @@ from __future__ import annotations
 import pytest
 import torch
 
+from conftest import load_package
 from test_gpu_masked import DEV, call, inputs
+from test_gpu_trees import case
 
 pytestmark = pytest.mark.gpu
 BIG = 1 << 32
@@ -24,3 +26,13 @@ def test_documents_and_prefixes(dim):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     for prefix, same in ((1 << 40, 150), (-(1 << 40), 0)):
         assert all(torch.equal(a, b) for a, b in zip(call(x, prefix=prefix), call(x, prefix=same)))
+
+
+def test_parents_and_paths():
+    lib = load_package()
+    q, k, v, cache = case(1, 2, 2, 5, 64, 100, torch.bfloat16)
+    got, draft = lib.dilution_tree_step(q, k, v, cache, torch.tensor([BIG, BIG, BIG + 1, 2 - BIG, 3], device=DEV))
+    want, _ = lib.dilution_tree_step(q, k, v, cache, [-1, -1, -1, -1, 3])
+    assert torch.equal(got, want)
+    lib.tree_accept(cache, draft, torch.tensor([-BIG + 3, BIG + 2], device=DEV))
+    assert torch.equal(cache["k"][:, :, 100], k[:, :, 0]) and torch.equal(cache["k"][:, :, 101], k[:, :, 4])
