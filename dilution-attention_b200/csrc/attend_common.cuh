@@ -23,9 +23,9 @@ namespace attend {
 constexpr int kSpan = 64;      // tokens per entry of the document ranges
 
 // Documents of a span of tokens.  lo, hi: smallest and largest id that is not negative (INT_MAX, -1: none);
-// pure: every token of the span has the one id lo.
+// pure: every token of the span has the one id lo; holes: some have a negative id.
 struct DocRange {
-  int lo, hi, pure, pad;
+  int lo, hi, pure, holes;
 };
 
 struct Args {
@@ -119,38 +119,64 @@ template <typename T> __device__ __forceinline__ const T* row_ptr(const void* ba
 
 // ---- single rows, a warp each ------------------------------------------------------------------
 // A masked pair adds 0 times a value to its row's accumulator in the tile kernels, which is NaN where that value is not
-// finite (a padded token's, or a later one's).  A kernel whose finished rows are not finite computes them again here, where
-// masked pairs are passed over: no cost to calls whose values are finite, some milliseconds to others.
-// Lane l holds features l, l + 32, ...
-template <typename T, int D> struct WarpRow {
-  static constexpr int E = (D + 31) / 32;
-  float x[E];
-  __device__ __forceinline__ void load(const T* p, int lane) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = lane + 32 * e < D ? to_f32(p[lane + 32 * e]) : 0.f;
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = 0.f;
-  }
-  __device__ __forceinline__ void fma(float f, const WarpRow& o) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = fmaf(f, o.x[e], x[e]);
-  }
-  __device__ __forceinline__ float dot(const WarpRow& o) const {
+// finite.  Values of padding (a negative id) are zeros in their tiles; a later token's or another document's are not, since rows of
+// the same tile may see them.  So a kernel whose finished rows are not finite asks here whether any such value is behind it, and only
+// then computes the row again, with masked pairs passed over: no cost to calls whose values are finite, little to those whose rows are
+// no numbers by right, and to the rows of a tile with such a value a walk over their pairs, a warp a row.  16 bytes of a row a lane, so
+// that a warp has several rows at once, kSteps times; each group of lanes keeps sums of its own, which are joined at the end.  (lse
+// has no such products and stays as it is.)  B1 H4 T4096 heads of 64, forward and backward, us: finite 380; a NaN in key 0 342, in
+// key 2000 2080, in all of dout 264, in query 2000 2550, in a token of padding 276.
+template <typename T, int D> struct Lanes {
+  static constexpr int E = 16 / (int)sizeof(T), L = D / E, R = 32 / L;      // elements of a lane, lanes of a row, rows at once
+  static constexpr int kSteps = 4, kRows = R * kSteps;
+  int part, own;                                                            // the lane's elements, its row
+  __device__ __forceinline__ Lanes() : part((int)(threadIdx.x & 31) % L), own((int)(threadIdx.x & 31) / L) {}
+  __device__ __forceinline__ uint4 load(const T* rows, int row) const { return reinterpret_cast<const uint4*>(rows + (int64_t)row * D)[part]; }
+  __device__ __forceinline__ float of(const uint4& u, int e) const { return to_f32(reinterpret_cast<const T*>(&u)[e]); }
+  // x . y, in each of a row's lanes
+  __device__ __forceinline__ float dot(const uint4& x, const uint4& y) const {
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(x[e], o.x[e], s);
-    return warp_sum(s);
-  }
-  __device__ __forceinline__ void store(T* p, int lane, float f) const {
+    for (int e = 0; e < E; ++e) s = fmaf(of(x, e), of(y, e), s);
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (lane + 32 * e < D) p[lane + 32 * e] = from_f32<T>(x[e] * f);
+    for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
   }
-  __device__ __forceinline__ void round() {        // as the stored tensor holds it
+  static __device__ __forceinline__ float over_rows(float s) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = to_f32(from_f32<T>(x[e]));
+    for (int o = L; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+  }
+};
+template <typename T, int D> struct LaneSums : Lanes<T, D> {
+  using B = Lanes<T, D>;
+  float x[B::E] = {};
+  __device__ __forceinline__ void scale(float f) {
+#pragma unroll
+    for (int e = 0; e < B::E; ++e) x[e] *= f;
+  }
+  __device__ __forceinline__ void add(float f, const uint4& u) {
+#pragma unroll
+    for (int e = 0; e < B::E; ++e) x[e] = fmaf(f, this->of(u, e), x[e]);
+  }
+  // No feature of the row is a number any more.
+  __device__ __forceinline__ bool no_number() const {
+    unsigned bits = 0;
+#pragma unroll
+    for (int e = 0; e < B::E; ++e) bits |= (x[e] != x[e] ? 1u : 0u) << e;
+#pragma unroll
+    for (int o = B::L; o < 32; o <<= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, o);
+    return __all_sync(0xffffffffu, bits == (1u << B::E) - 1);
+  }
+  __device__ __forceinline__ void join(float f) {
+#pragma unroll
+    for (int e = 0; e < B::E; ++e) x[e] = B::over_rows(x[e]) * f;
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    uint4 u;
+#pragma unroll
+    for (int e = 0; e < B::E; ++e) reinterpret_cast<T*>(&u)[e] = from_f32<T>(x[e]);
+    if (this->own == 0) reinterpret_cast<uint4*>(p)[this->part] = u;
   }
 };
 
@@ -158,93 +184,220 @@ template <typename T, int D> struct WarpRow {
 __device__ __forceinline__ int key_end(const Row& r, int i) { return min(r.t, max(i + 1, r.prefix)); }
 __device__ __forceinline__ int first_query(const Row& r, int j) { return j < r.prefix ? 0 : j; }
 
+// Whether a token that the row's tile has had to do with, but the row does not see, holds a value that is not finite.  Half tiles
+// [h0, h1); visited(h): the tile has had to do with half tile h; bad(x): token x is such a one.
+template <typename V, typename B> __device__ __forceinline__ bool masked_not_finite(int h0, int h1, V visited, B bad) {
+  const int lane = threadIdx.x & 31;
+  for (int h = h0; h < h1; h += 32)
+    for (unsigned todo = __ballot_sync(0xffffffffu, h + lane < h1 && visited(h + lane)); todo; todo &= todo - 1) {
+      const int x = (h + __ffs(todo) - 1) * 64 + lane;
+      if (__any_sync(0xffffffffu, bad(x) || bad(x + 32))) return true;
+    }
+  return false;
+}
+template <typename T, int D> __device__ __forceinline__ bool finite_row(const T* p) {
+  constexpr int N = 16 / (int)sizeof(T);
+  float s = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < D / N; ++c) {
+    const uint4 w = reinterpret_cast<const uint4*>(p)[c];
+#pragma unroll
+    for (int e = 0; e < N; ++e) s = fmaf(to_f32(reinterpret_cast<const T*>(&w)[e]), 0.f, s);
+  }
+  return s == 0.f;
+}
+// Of query i, over `rows` of the keys (a tile of the tensor-core kernels; the others' are half of one).
+template <typename T, int D> __device__ __forceinline__ bool masked_keys_not_finite(const Row& r, int i, const T* rows) {
+  const int i0 = i & ~127;
+  return masked_not_finite(r.docs != nullptr ? 0 : max(i + 1, r.prefix) / 64, (key_end(r, i0 + 127) + 63) / 64,
+                           [&](int h) { return tile_visible(r, i0, i0 + 127, 64 * h, 64 * h + 63); },
+                           [&](int j) { return j < r.t && !sees(r, i, j) && !finite_row<T, D>(rows + (int64_t)j * D); });
+}
+
 // What the rounding of x to T leaves off.
 template <typename T> __device__ __forceinline__ float left_off(float x) { return x - to_f32(from_f32<T>(x)); }
 
 template <typename T, int D>
-__device__ __noinline__ void redo_forward_row(const Args& a, int b, int h, int i) {
+__device__ __forceinline__ void redo_forward_row(const Args& a, int b, int h, int i) {
   const Row r = make_row(a, b, h);
-  const int lane = threadIdx.x & 31, hk = h / (a.heads / a.kv_heads);
+  const int hk = h / (a.heads / a.kv_heads);
   const int64_t n = (int64_t)b * a.heads + h, nk = (int64_t)b * a.kv_heads + hk;
   const T* k = row_ptr<T>(a.k, nk, a.t, D);
   const T* v = row_ptr<T>(a.v, nk, a.t, D);
-  WarpRow<T, D> q, o, x;
-  q.load(row_ptr<T>(a.q, n, a.t, D) + (int64_t)i * D, lane);
+  if (!masked_keys_not_finite<T, D>(r, i, v)) return;
+  LaneSums<T, D> o;
+  constexpr int U = o.kSteps;
+  const uint4 q = o.load(row_ptr<T>(a.q, n, a.t, D), i);
   float m = -INFINITY, s = 0.f;
-  o.zero();
   const int end = key_end(r, i);
-  for (int j = 0; j < end; ++j) {
-    if (!sees(r, i, j)) continue;
-    x.load(k + (int64_t)j * D, lane);
-    const float z = score<sizeof(T) == 4>(r, q.dot(x), i, j).x;
-    const float top = fmaxf(m, z);
-    const float ref = top == -INFINITY ? 0.f : top, f = exp2f(m - ref), p = exp2f(z - ref);
-    x.load(v + (int64_t)j * D, lane);
-    s = fmaf(s, f, p);
+  for (int j0 = 0; j0 < end; j0 += o.kRows) {
+    bool see[U], any = false;
 #pragma unroll
-    for (int e = 0; e < o.E; ++e) o.x[e] = o.x[e] * f + (p == 0.f ? 0.f : p * x.x[e]);
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * o.R + o.own;
+      see[u] = j < end && sees(r, i, j);
+      any = any || see[u];
+    }
+    if (!__any_sync(0xffffffffu, any)) continue;
+    uint4 x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = min(j0 + u * o.R + o.own, end - 1);
+      x[u] = o.load(k, j);
+      y[u] = o.load(v, j);
+    }
+    float z[U], top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float dot = o.dot(q, x[u]);
+      z[u] = see[u] ? score<sizeof(T) == 4>(r, dot, i, j0 + u * o.R + o.own).x : -INFINITY;
+      top = fmaxf(top, z[u]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top, f = exp2f(m - ref);
     m = top;
+    s *= f;
+    o.scale(f);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (see[u]) {
+        const float p = exp2f(z[u] - ref);
+        s += p;
+        o.add(p, y[u]);
+      }
+    if (o.no_number()) break;
   }
-  const float f = s == 0.f ? 0.f : 1.f / s;
-  o.store(reinterpret_cast<T*>(a.out) + (n * a.t + i) * D, lane, f);
+  // the groups' sums against one maximum
+  float top = m;
+#pragma unroll
+  for (int l = o.L; l < 32; l <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, l));
+  const float f = exp2f(m - (top == -INFINITY ? 0.f : top));
+  s = o.over_rows(s * f);
+  o.scale(f);
+  o.join(s == 0.f ? 0.f : 1.f / s);
+  o.store(reinterpret_cast<T*>(a.out) + (n * a.t + i) * D);
   if (a.rest != nullptr) {
 #pragma unroll
-    for (int e = 0; e < o.E; ++e) o.x[e] = left_off<T>(o.x[e] * f);
-    o.store(reinterpret_cast<T*>(a.rest) + (n * a.t + i) * D, lane, 1.f);
+    for (int e = 0; e < o.E; ++e) o.x[e] = left_off<T>(o.x[e]);
+    o.store(reinterpret_cast<T*>(a.rest) + (n * a.t + i) * D);
   }
-  if (a.lse != nullptr && lane == 0) a.lse[n * a.t + i] = s == 0.f ? INFINITY : m + log2f(s);
 }
 
 template <typename T, int D>
-__device__ __noinline__ void redo_dq_row(const Args& a, int b, int h, int i) {
+__device__ __forceinline__ void redo_dq_row(const Args& a, int b, int h, int i) {
   const Row r = make_row(a, b, h);
-  const int lane = threadIdx.x & 31, hk = h / (a.heads / a.kv_heads);
+  const int hk = h / (a.heads / a.kv_heads);
   const int64_t n = (int64_t)b * a.heads + h, nk = (int64_t)b * a.kv_heads + hk;
   const T* k = row_ptr<T>(a.k, nk, a.t, D);
   const T* v = row_ptr<T>(a.v, nk, a.t, D);
-  WarpRow<T, D> q, g, acc, x;
-  q.load(row_ptr<T>(a.q, n, a.t, D) + (int64_t)i * D, lane);
-  g.load(row_ptr<T>(a.dout, n, a.t, D) + (int64_t)i * D, lane);
-  acc.zero();
+  if (!masked_keys_not_finite<T, D>(r, i, k)) return;
+  LaneSums<T, D> acc;
+  constexpr int U = acc.kSteps;
+  const uint4 q = acc.load(row_ptr<T>(a.q, n, a.t, D), i), g = acc.load(row_ptr<T>(a.dout, n, a.t, D), i);
   const float lse = a.lse[n * a.t + i], delta = a.delta[n * a.t + i];
   const int end = key_end(r, i);
-  for (int j = 0; j < end; ++j) {
-    if (!sees(r, i, j)) continue;
-    x.load(v + (int64_t)j * D, lane);
-    const float dp = g.dot(x);
-    x.load(k + (int64_t)j * D, lane);
-    const float2 z = score<sizeof(T) == 4>(r, q.dot(x), i, j);
-    const float p = exp2f(z.x - lse);
-    if (p != 0.f) acc.fma(p * (dp - delta) * z.y, x);
+  for (int j0 = 0; j0 < end; j0 += acc.kRows) {
+    bool see[U], any = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * acc.R + acc.own;
+      see[u] = j < end && sees(r, i, j);
+      any = any || see[u];
+    }
+    if (!__any_sync(0xffffffffu, any)) continue;
+    uint4 x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = min(j0 + u * acc.R + acc.own, end - 1);
+      x[u] = acc.load(k, j);
+      y[u] = acc.load(v, j);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float dot = acc.dot(q, x[u]), dp = acc.dot(g, y[u]);
+      if (see[u]) {
+        const float2 z = score<sizeof(T) == 4>(r, dot, i, j0 + u * acc.R + acc.own);
+        acc.add(exp2f(z.x - lse) * (dp - delta) * z.y, x[u]);
+      }
+    }
+    if (acc.no_number()) break;
   }
-  acc.store(reinterpret_cast<T*>(a.dq) + (n * a.t + i) * D, lane, a.scale);
+  acc.join(a.scale);
+  acc.store(reinterpret_cast<T*>(a.dq) + (n * a.t + i) * D);
 }
 
 template <typename T, int D>
-__device__ __noinline__ void redo_dkv_row(const Args& a, int b, int hk, int j) {
-  const int lane = threadIdx.x & 31, group = a.heads / a.kv_heads;
+__device__ __forceinline__ void redo_dkv_row(const Args& a, int b, int hk, int j) {
+  const int group = a.heads / a.kv_heads;
   const int64_t nk = (int64_t)b * a.kv_heads + hk;
-  WarpRow<T, D> k, v, dk, dv, q, g;
-  k.load(row_ptr<T>(a.k, nk, a.t, D) + (int64_t)j * D, lane);
-  v.load(row_ptr<T>(a.v, nk, a.t, D) + (int64_t)j * D, lane);
-  dk.zero();
-  dv.zero();
-  for (int h = hk * group; h < (hk + 1) * group; ++h) {
+  bool redo = false;
+  for (int h = hk * group; h < (hk + 1) * group && !redo; ++h) {
     const Row r = make_row(a, b, h);
     const int64_t n = (int64_t)b * a.heads + h;
-    for (int i = first_query(r, j); i < a.t; ++i) {
-      if (!sees(r, i, j)) continue;
-      q.load(row_ptr<T>(a.q, n, a.t, D) + (int64_t)i * D, lane);
-      g.load(row_ptr<T>(a.dout, n, a.t, D) + (int64_t)i * D, lane);
-      const float2 z = score<sizeof(T) == 4>(r, q.dot(k), i, j);
-      const float p = exp2f(z.x - a.lse[n * a.t + i]), dp = g.dot(v);
-      if (p == 0.f) continue;
-      dv.fma(p, g);
-      dk.fma(p * (dp - a.delta[n * a.t + i]) * z.y, q);
+    const T* q = row_ptr<T>(a.q, n, a.t, D);
+    const T* g = row_ptr<T>(a.dout, n, a.t, D);
+    const int j0 = j & ~127;
+    redo = masked_not_finite(
+        first_query(r, j0) / 64, ((r.docs != nullptr ? a.t : j) + 63) / 64,
+        [&](int x) { return tile_visible(r, 64 * x, 64 * x + 63, j0, j0 + 127); },
+        [&](int i) { return i < a.t && !sees(r, i, j) && !(finite_row<T, D>(q + (int64_t)i * D) && finite_row<T, D>(g + (int64_t)i * D)); });
+  }
+  if (!redo) return;
+  LaneSums<T, D> dk, dv;
+  constexpr int U = dk.kSteps / 2;
+  const uint4 k = dk.load(row_ptr<T>(a.k, nk, a.t, D), j), v = dk.load(row_ptr<T>(a.v, nk, a.t, D), j);
+  bool done = false;
+  for (int h = hk * group; h < (hk + 1) * group && !done; ++h) {
+    const Row r = make_row(a, b, h);
+    const int64_t n = (int64_t)b * a.heads + h;
+    const T* q = row_ptr<T>(a.q, n, a.t, D);
+    const T* g = row_ptr<T>(a.dout, n, a.t, D);
+    for (int i0 = first_query(r, j); i0 < a.t && !done; i0 += dk.R * U) {
+      bool see[U], any = false;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        see[u] = sees(r, i0 + u * dk.R + dk.own, j);
+        any = any || see[u];
+      }
+      if (!__any_sync(0xffffffffu, any)) continue;
+      uint4 x[U], y[U];
+      float lse[U], delta[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u * dk.R + dk.own, a.t - 1);
+        x[u] = dk.load(q, i);
+        y[u] = dk.load(g, i);
+        lse[u] = a.lse[n * a.t + i];
+        delta[u] = a.delta[n * a.t + i];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float dot = dk.dot(k, x[u]), dp = dk.dot(v, y[u]);
+        if (see[u]) {
+          const float2 z = score<sizeof(T) == 4>(r, dot, i0 + u * dk.R + dk.own, j);
+          const float p = exp2f(z.x - lse[u]);
+          dv.add(p, y[u]);
+          dk.add(p * (dp - delta[u]) * z.y, x[u]);
+        }
+      }
+      done = dk.no_number() && dv.no_number();
     }
   }
-  dk.store(reinterpret_cast<T*>(a.dk) + (nk * a.t + j) * D, lane, a.scale);
-  dv.store(reinterpret_cast<T*>(a.dv) + (nk * a.t + j) * D, lane, 1.f);
+  dk.join(a.scale);
+  dv.join(1.f);
+  dk.store(reinterpret_cast<T*>(a.dk) + (nk * a.t + j) * D);
+  dv.store(reinterpret_cast<T*>(a.dv) + (nk * a.t + j) * D);
+}
+
+// The rows first + bit of `rows`, one after the other, by a warp.  A call of its own: nothing of it may cost the kernels registers.
+enum Redo { kRedoForward, kRedoDq, kRedoDkv };
+template <Redo WHAT, typename T, int D> __device__ __noinline__ void redo_rows(const Args& a, int b, int h, int first, unsigned rows) {
+#pragma unroll 1
+  for (; rows; rows &= rows - 1) {
+    const int x = first + __ffs(rows) - 1;
+    if (WHAT == kRedoForward) redo_forward_row<T, D>(a, b, h, x);
+    else if (WHAT == kRedoDq) redo_dq_row<T, D>(a, b, h, x);
+    else redo_dkv_row<T, D>(a, b, h, x);
+  }
 }
 
 // ---- what runs in front of the passes ----------------------------------------------------------
@@ -265,7 +418,7 @@ __global__ void __launch_bounds__(256) doc_ranges_kernel(const int* __restrict__
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   neg = __any_sync(0xffffffffu, neg);
-  if (lane == 0) ranges[at] = DocRange{lo, hi, !neg && lo == hi, 0};
+  if (lane == 0) ranges[at] = DocRange{lo, hi, !neg && lo == hi, neg};
 }
 
 // dout . (out + rest) of 16 bytes of each, in 32 bits.  (An out beyond bf16's range has no rest: inf - inf.)

@@ -17,14 +17,14 @@ namespace attend {
 constexpr int kTile = 64;
 constexpr int kSimtThreads = 256;
 
-// Rows [r0, r0 + 64) of a (t, D) matrix into a tile, zeros behind the last.
+// Rows [r0, r0 + 64) of a (t, D) matrix into a tile, zeros behind the last and in place of padding (docs, if not null, below 0).
 template <typename T, int D>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, int r0, int t) {
+__device__ __forceinline__ void load_tile(float* dst, const T* src, int r0, int t, const int* docs) {
   constexpr int E = 16 / sizeof(T);
   for (int x = threadIdx.x; x < kTile * D / E; x += kSimtThreads) {
     const int row = x / (D / E), c = x % (D / E) * E;
     uint4 w = make_uint4(0, 0, 0, 0);
-    if (r0 + row < t) w = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + row) * D + c);
+    if (r0 + row < t && (docs == nullptr || docs[r0 + row] >= 0)) w = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + row) * D + c);
     const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
     for (int i = 0; i < E; ++i) dst[row * (D + 4) + c + i] = to_f32(e[i]);
@@ -100,11 +100,12 @@ __device__ __forceinline__ float over_ranks(const float* x, int ranks) {
 __device__ __forceinline__ void meet(int ranks) {
   if (ranks > 1) cluster_sync(); else __syncthreads();
 }
-// f(row) by whole warps for the rank's rows whose flag is set; a row's flag is its thread block's own.
-template <typename F> __device__ __forceinline__ void each_flagged(const int* flag, int first, int last, F f) {
+// The rank's rows whose flag is set once more, by whole warps; a row's flag is its thread block's own.
+template <Redo WHAT, typename T, int D>
+__device__ __forceinline__ void redo_flagged(const Args& a, int b, int h, int r0, const int* flag, int first, int last) {
   __syncthreads();
   for (int row = first + (int)(threadIdx.x >> 5); row < last; row += kSimtThreads / 32)
-    if (flag[row]) f(row);
+    if (flag[row]) redo_rows<WHAT, T, D>(a, b, h, r0 + row, 1u);
 }
 
 template <int D> constexpr int simt_smem(int tiles) { return 4 * (tiles * kTile * (D + 4) + kTile * (kTile + 4)); }
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a, int 
   const T* k = row_ptr<T>(a.k, nk, a.t, D);
   const T* v = row_ptr<T>(a.v, nk, a.t, D);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  load_tile<T, D>(sQ, row_ptr<T>(a.q, n, a.t, D), i0, a.t);
+  load_tile<T, D>(sQ, row_ptr<T>(a.q, n, a.t, D), i0, a.t, nullptr);
   float m[4], l[4], o[4][D / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -138,8 +139,8 @@ __global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a, int 
   for (int j0 = 0; j0 < end; j0 += kTile) {
     if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1) || turn++ % ranks != rank) continue;
     __syncthreads();
-    load_tile<T, D>(sK, k, j0, a.t);
-    load_tile<T, D>(sV, v, j0, a.t);
+    load_tile<T, D>(sK, k, j0, a.t, nullptr);
+    load_tile<T, D>(sV, v, j0, a.t, r.docs);
     __syncthreads();
     float s[4][4];
     tile_scores<D>(sQ, sK, ty, tx, s);
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_forward_kernel(Args a, int 
     if (a.rest != nullptr) reinterpret_cast<T*>(a.rest)[(n * a.t + i0 + row) * D + c] = from_f32<T>(left_off<T>(out));
     if (a.lse != nullptr && c == 0) a.lse[n * a.t + i0 + row] = sum == 0.f ? INFINITY : top + log2f(sum);
   }
-  each_flagged(sFlag, first, last, [&](int row) { redo_forward_row<T, D>(a, b, h, i0 + row); });
+  redo_flagged<kRedoForward, T, D>(a, b, h, i0, sFlag, first, last);
   meet(ranks);                       // no CTA leaves while another may read its sums
 }
 
@@ -220,8 +221,8 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dq_kernel(Args a, int ranks
   const int64_t nk = (int64_t)b * a.kv_heads + h / (a.heads / a.kv_heads);
   const Row r = make_row(a, b, h);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  load_tile<T, D>(sQ, row_ptr<T>(a.q, n, a.t, D), i0, a.t);
-  load_tile<T, D>(sG, row_ptr<T>(a.dout, n, a.t, D), i0, a.t);
+  load_tile<T, D>(sQ, row_ptr<T>(a.q, n, a.t, D), i0, a.t, nullptr);
+  load_tile<T, D>(sG, row_ptr<T>(a.dout, n, a.t, D), i0, a.t, nullptr);
   float lse[4], delta[4], dq[4][D / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -237,11 +238,11 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dq_kernel(Args a, int ranks
     if (!tile_visible(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1) || turn++ % ranks != rank) continue;
     float s[4][4], g[4][4];
     __syncthreads();
-    load_tile<T, D>(sX, row_ptr<T>(a.v, nk, a.t, D), j0, a.t);
+    load_tile<T, D>(sX, row_ptr<T>(a.v, nk, a.t, D), j0, a.t, r.docs);
     __syncthreads();
     tile_scores<D>(sG, sX, ty, tx, g);
     __syncthreads();
-    load_tile<T, D>(sX, row_ptr<T>(a.k, nk, a.t, D), j0, a.t);
+    load_tile<T, D>(sX, row_ptr<T>(a.k, nk, a.t, D), j0, a.t, r.docs);
     __syncthreads();
     tile_scores<D>(sQ, sX, ty, tx, s);
     const bool full = tile_full(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1);
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dq_kernel(Args a, int ranks
     if (!isfinite(y)) sFlag[row] = 1;
     reinterpret_cast<T*>(a.dq)[(n * a.t + i0 + row) * D + c] = from_f32<T>(y);
   }
-  each_flagged(sFlag, first, last, [&](int row) { redo_dq_row<T, D>(a, b, h, i0 + row); });
+  redo_flagged<kRedoDq, T, D>(a, b, h, i0, sFlag, first, last);
   meet(ranks);
 }
 
@@ -288,8 +289,8 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a, int rank
   const int j0 = block / heads * kTile;
   const int b = (int)(nk / a.kv_heads), hk = (int)(nk % a.kv_heads);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  load_tile<T, D>(sK, row_ptr<T>(a.k, nk, a.t, D), j0, a.t);
-  load_tile<T, D>(sV, row_ptr<T>(a.v, nk, a.t, D), j0, a.t);
+  load_tile<T, D>(sK, row_ptr<T>(a.k, nk, a.t, D), j0, a.t, nullptr);
+  load_tile<T, D>(sV, row_ptr<T>(a.v, nk, a.t, D), j0, a.t, nullptr);
   float dk[4][D / 16], dv[4][D / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -304,11 +305,11 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a, int rank
       float s[4][4], g[4][4];
       const bool full = tile_full(r, i0, i0 + kTile - 1, j0, j0 + kTile - 1);
       __syncthreads();
-      load_tile<T, D>(sX, row_ptr<T>(a.q, n, a.t, D), i0, a.t);
+      load_tile<T, D>(sX, row_ptr<T>(a.q, n, a.t, D), i0, a.t, r.docs);
       __syncthreads();
       tile_scores<D>(sK, sX, ty, tx, s);
       __syncthreads();
-      load_tile<T, D>(sX, row_ptr<T>(a.dout, n, a.t, D), i0, a.t);
+      load_tile<T, D>(sX, row_ptr<T>(a.dout, n, a.t, D), i0, a.t, r.docs);
       __syncthreads();
       tile_scores<D>(sV, sX, ty, tx, g);
 #pragma unroll
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a, int rank
       __syncwarp();
       tile_accumulate<D>(sP, sX, ty, tx, dv);
       __syncthreads();
-      load_tile<T, D>(sX, row_ptr<T>(a.q, n, a.t, D), i0, a.t);
+      load_tile<T, D>(sX, row_ptr<T>(a.q, n, a.t, D), i0, a.t, r.docs);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_dkv_kernel(Args a, int rank
     reinterpret_cast<T*>(a.dk)[(nk * a.t + j0 + row) * D + c] = from_f32<T>(y);
     reinterpret_cast<T*>(a.dv)[(nk * a.t + j0 + row) * D + c] = from_f32<T>(z);
   }
-  each_flagged(sFlag, first, last, [&](int row) { redo_dkv_row<T, D>(a, b, hk, j0 + row); });
+  redo_flagged<kRedoDkv, T, D>(a, b, hk, j0, sFlag, first, last);
   meet(ranks);
 }
 

@@ -32,20 +32,23 @@ using attend::Row;
 // ---- which pairs of tiles ------------------------------------------------------------------------
 struct Docs {
   int lo, hi, id;          // smallest and largest id, and the one id of all tokens or -1
+  bool holes;              // there is padding among them
 };
 __device__ __forceinline__ Docs docs_of(const Row& r, int i0, int i1) {
-  Docs d{INT_MAX, -1, -1};
+  Docs d{INT_MAX, -1, -1, false};
   bool pure = true;
   for (int s = i0 / attend::kSpan; s <= min(i1, r.t - 1) / attend::kSpan; ++s) {
     const attend::DocRange x = r.ranges[s];
     d.lo = min(d.lo, x.lo);
     d.hi = max(d.hi, x.hi);
     pure = pure && x.pure;
+    d.holes = d.holes || x.holes;
   }
   if (pure && d.lo == d.hi) d.id = d.lo;
   return d;
 }
-// 0: no query of [i0, i1] sees a key of [j0, j1]; 2: each sees each; 1: masks decide.  BIAS: distances of one sign only are
+// 0: no query of [i0, i1] sees a key of [j0, j1]; 2: each sees each; 1: masks decide (the kernels' lambdas: 3 where the half tile that
+// passes has padding).  BIAS: distances of one sign only are
 // left to the kernels' common path.  Rows behind the last token count as seen where they do no harm: queries, and keys
 // of a tile that stays; j1 is the last key that matters then.
 template <bool BIAS>
@@ -61,11 +64,14 @@ __device__ __forceinline__ int pair_state(const Row& r, int i0, int i1, const Do
 
 // ---- forward -----------------------------------------------------------------------------------------
 // What pairs of tiles have to do is asked once per block and kept for this many half tiles from `base` on: two bits each, of 32
-// half tiles in a word: the warp that issues MMAs has to know in a few cycles, it is what all others wait for.
+// half tiles in a word: the warp that issues MMAs has to know in a few cycles, it is what all others wait for.  masked: states 1 and
+// 3; seen: states 1 and 2.
 constexpr int kStates = 4096;
 struct States {
-  uint32_t any[kStates / 32], masked[kStates / 32];
-  __device__ __forceinline__ int of(int e) const { return any[e / 32] >> (e & 31) & 1 ? 2 - (masked[e / 32] >> (e & 31) & 1) : 0; }
+  uint32_t seen[kStates / 32], masked[kStates / 32];
+  __device__ __forceinline__ int of(int e) const { return masked[e / 32] >> (e & 31) & 1 ? 1 : (seen[e / 32] >> (e & 31) & 1) * 2; }
+  __device__ __forceinline__ uint32_t any(int e) const { return seen[e / 32] | masked[e / 32]; }
+  __device__ __forceinline__ uint32_t holes(int e) const { return masked[e / 32] & ~seen[e / 32]; }
 };
 // Half tiles [base, end); f: the state of one.  Returns the first and the last + 1 of the warp's that have anything to do.
 template <typename F> __device__ __forceinline__ int2 keep_states(States* s, int base, int end, int warp, int warps, F f) {
@@ -73,12 +79,11 @@ template <typename F> __device__ __forceinline__ int2 keep_states(States* s, int
   int2 range = make_int2(INT_MAX, 0);
   for (int e = base + 32 * warp; e < end; e += 32 * warps) {
     const int what = e + lane < end ? f(e + lane) : 0;
-    const uint32_t any = __ballot_sync(0xffffffffu, what != 0), masked = __ballot_sync(0xffffffffu, what == 1);
-    if (lane == 0) {
-      if (e - base < kStates) {
-        s->any[(e - base) / 32] = any;
-        s->masked[(e - base) / 32] = masked;
-      }
+    const uint32_t any = __ballot_sync(0xffffffffu, what != 0), masked = __ballot_sync(0xffffffffu, what & 1);
+    const uint32_t seen = __ballot_sync(0xffffffffu, what == 1 || what == 2);
+    if (lane == 0 && e - base < kStates) {
+      s->seen[(e - base) / 32] = seen;
+      s->masked[(e - base) / 32] = masked;
     }
     if (any) range = make_int2(min(range.x, e + __ffs(any) - 1), e + 32 - __clz(any));
   }
@@ -89,6 +94,20 @@ __device__ __forceinline__ int2 all_of(const int2* range, int warps) {
   const int lane = threadIdx.x & 31;
   const int2 x = lane < warps ? range[lane] : make_int2(INT_MAX, 0);
   return make_int2((int)uniform(__reduce_min_sync(0xffffffffu, x.x)), (int)uniform(__reduce_max_sync(0xffffffffu, x.y)));
+}
+
+// Zeros for the padding among the 64 tokens (of `tokens` left) with ids docs, in their half tile of SUB sub-tiles: what the values of padding are
+// multiplied by is 0, which makes no number of those that are not finite.  One warp, in front of the half tile's products.
+template <int SUB> __device__ __noinline__ void zero_holes(uint8_t* tile, const int* docs, int tokens) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int x = 32 * half + lane;
+    for (uint32_t left = __ballot_sync(0xffffffffu, x < tokens && docs[x] < 0); left; left &= left - 1) {
+      const int row = 32 * half + __ffs(left) - 1;
+      if (lane < 8 * SUB) *reinterpret_cast<uint4*>(tile + (lane >> 3) * (kTileBytes / 2) + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
 }
 
 template <int D> struct AttendForward {
@@ -278,11 +297,12 @@ __global__ void __launch_bounds__(AttendForward<D>::kThreads, D == 64 ? 2 : 1) a
   const int b = n / a.heads, h = n % a.heads, nk = b * a.kv_heads + h / (a.heads / a.kv_heads);
   const Row r = attend::make_row(a, b, h);
   const float lin = CAP ? r.cap2 : r.pre, pre = CAP ? a.scale / a.cap : 0.f;
-  const Docs dq = r.ranges != nullptr ? docs_of(r, i0, i0 + kTileRows - 1) : Docs{INT_MAX, -1, -1};
+  const Docs dq = r.ranges != nullptr ? docs_of(r, i0, i0 + kTileRows - 1) : Docs{INT_MAX, -1, -1, false};
   auto state = [&](int hh) {                            // of half tile hh
     const int j0 = hh * 64;
-    const Docs dj = r.ranges != nullptr ? docs_of(r, j0, j0 + 63) : Docs{INT_MAX, -1, -1};
-    return pair_state<BIAS>(r, i0, i0 + kTileRows - 1, dq, j0, j0 + 63, dj);
+    const Docs dj = r.ranges != nullptr ? docs_of(r, j0, j0 + 63) : Docs{INT_MAX, -1, -1, false};
+    const int what = pair_state<BIAS>(r, i0, i0 + kTileRows - 1, dq, j0, j0 + 63, dj);
+    return what == 1 && dj.holes ? 3 : what;
   };
 
   const int top = (attend::key_end(r, min(r.t, i0 + kTileRows) - 1) + 63) / 64;
@@ -327,13 +347,22 @@ __global__ void __launch_bounds__(AttendForward<D>::kThreads, D == 64 ? 2 : 1) a
       uint32_t pending = 0, flip = 0, side = 0;          // warpgroups with a P~ to come, the parity of the next, the buffer of its scores
       // (counters in place of remainders: this warp's time between two products is what the others wait for)
       int in = 0, out = 0, refill = 0;
-      uint32_t phase = 0, back = 0, word = 0;
+      uint32_t phase = 0, back = 0, word = 0, hole = 0;
       for (int e = 0; e < nh + 2; ++e) {
         const int hh = last - e;
-        if (((hh & 31) == 31 || e == 0) && e < nh)
-          word = uniform(hh < kStates ? s_state.any[hh / 32]
-                                      : __ballot_sync(0xffffffffu, (hh & ~31) + lane < h0 + nh && state((hh & ~31) + lane) != 0));
-        if (e < nh) mbar_wait_warp(kfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
+        if (((hh & 31) == 31 || e == 0) && e < nh) {
+          const int x = (hh & ~31) + lane, what = hh < kStates || x >= h0 + nh ? 0 : state(x);
+          word = uniform(hh < kStates ? s_state.any(hh) : __ballot_sync(0xffffffffu, what != 0));
+          hole = uniform(hh < kStates ? s_state.holes(hh) : __ballot_sync(0xffffffffu, what == 3));
+        }
+        if (e < nh) {
+          mbar_wait_warp(kfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
+          if (hole >> (hh & 31) & 1) {
+            zero_holes<D / 64>(smem + TB + R * HB + HB * in, r.docs + hh * 64, r.t - hh * 64);
+            fence_async_smem();
+            __syncwarp();
+          }
+        }
         const int w = e & 1;
         const uint32_t tW = tmem + F::kWgCols * w;
         const bool seen = e < nh && (word >> (hh & 31) & 1), old = pending >> w & 1;
@@ -406,7 +435,7 @@ __global__ void __launch_bounds__(AttendForward<D>::kThreads, D == 64 ? 2 : 1) a
           tc_fence_after();
         }
       };
-      forward_step<D, CAP, BIAS>(tS + 64 * side, tO, r, lin, pre, hh * 64, is, what == 1, ref, s, sr, settled);
+      forward_step<D, CAP, BIAS>(tS + 64 * side, tO, r, lin, pre, hh * 64, is, what & 1, ref, s, sr, settled);
       settled();
       ++turn;
       tc_fence_before();
@@ -484,8 +513,7 @@ __global__ void __launch_bounds__(AttendForward<D>::kThreads, D == 64 ? 2 : 1) a
     meet();
     // (both warpgroups have written their halves; a warp's rows are its own lanes', every other one of them)
     unsigned again = __ballot_sync(0xffffffffu, sFlag[row] != 0) & (half ? 0xaaaaaaaau : 0x55555555u);
-    for (; again; again &= again - 1)
-      attend::redo_forward_row<__nv_bfloat16, D>(a, b, h, i0 + (row & 96) + __ffs(again) - 1);
+    if (again) attend::redo_rows<attend::kRedoForward, __nv_bfloat16, D>(a, b, h, i0 + (row & 96), again);
   }
   drain_if_aborted(ctl);
   tc_fence_before();
@@ -501,6 +529,7 @@ template <int D, int STAY, int NW> struct AttendBackward {
   static constexpr int kRing = D == 64 ? (NW == 1 ? 4 : 6) : STAY == 1 ? 4 : 5;         // one more than are in work, at least
   static constexpr uint32_t kTile = Rows<kForm<D>>::kBytes, kHalf = kTile / 2;
   static constexpr int kAcc = STAY == 1 ? 2 * D : D;                     // accumulator columns
+  static constexpr bool kHoles = D == 128 || NW == 1;                    // (heads of 64 with documents, and so with padding, take NW = 1)
   static_assert(NW * 128 + kAcc <= 512, "the warpgroups' scores and the accumulators fit TMEM");
   static constexpr int kTmem = NW * 128 + kAcc <= 256 ? 256 : 512, kPerSm = D == 64 && kTmem == 256 ? 2 : 1;
   // staying tiles | passing tiles [ring] x 2 | (lse, delta) [ring][64] | flags [128] | barriers + control
@@ -605,11 +634,12 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
   const int passes = STAY == 1 ? group : 1;                      // heads whose queries pass
   Row r = attend::make_row(a, b, STAY == 1 ? head * group : head);
   const float lin = CAP ? r.cap2 : r.pre, pre = CAP ? a.scale / a.cap : 0.f;
-  const Docs dy = r.ranges != nullptr ? docs_of(r, y0, y1) : Docs{INT_MAX, -1, -1};
+  const Docs dy = r.ranges != nullptr ? docs_of(r, y0, y1) : Docs{INT_MAX, -1, -1, false};
   auto state = [&](int hh) {                                     // of the tile and passing half tile hh
     const int x0 = hh * 64;
-    const Docs dx = r.ranges != nullptr ? docs_of(r, x0, x0 + 63) : Docs{INT_MAX, -1, -1};
-    return STAY == 1 ? pair_state<BIAS>(r, x0, x0 + 63, dx, y0, y1, dy) : pair_state<BIAS>(r, y0, y1, dy, x0, x0 + 63, dx);
+    const Docs dx = r.ranges != nullptr ? docs_of(r, x0, x0 + 63) : Docs{INT_MAX, -1, -1, false};
+    const int what = STAY == 1 ? pair_state<BIAS>(r, x0, x0 + 63, dx, y0, y1, dy) : pair_state<BIAS>(r, y0, y1, dy, x0, x0 + 63, dx);
+    return F::kHoles && what == 1 && dx.holes ? 3 : what;
   };
 
   const int base = STAY == 1 ? attend::first_query(r, y0) / 64 : 0;
@@ -662,13 +692,15 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
       uint32_t pending = 0, flip = 0, started = 0;         // warpgroups with a dS to come, the parity of the next
       // (counters in place of remainders: this warp's time between two products is what the others wait for)
       int w = 0, in = 0, out = 0, eh = 0;
-      uint32_t phase = 0, word = 0;
+      uint32_t phase = 0, word = 0, hole = 0;
       for (int e = 0; e < ne + NW; ++e) {
         const uint32_t tS = tmem + 128 * w;
         const int at = h0 - base + eh;
-        if ((at & 31) == 0 || eh == 0)
-          word = uniform(at < kStates ? s_state.any[at / 32]
-                                      : __ballot_sync(0xffffffffu, (at & ~31) + lane < h0 - base + nh && state(base + (at & ~31) + lane) != 0));
+        if ((at & 31) == 0 || eh == 0) {
+          const int x = (at & ~31) + lane, what = at < kStates || x >= h0 - base + nh ? 0 : state(base + x);
+          word = uniform(at < kStates ? s_state.any(at) : __ballot_sync(0xffffffffu, what != 0));
+          if (F::kHoles) hole = uniform(at < kStates ? s_state.holes(at) : __ballot_sync(0xffffffffu, what == 3));
+        }
         if (pending >> w & 1) {                            // of half tile e - NW
           mbar_wait_warp(pready + 8 * w, flip >> w & 1, ctl, &g_attend_status, kErrWaitTile);
           flip ^= 1u << w;
@@ -691,6 +723,12 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
         if (e < ne) {
           mbar_wait_warp(bfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
           if (word >> (at & 31) & 1) {
+            if (F::kHoles && hole >> (at & 31) & 1) {
+              zero_holes<D / 64>(smem + 2 * TB + HB * in, r.docs + (base + at) * 64, r.t - (base + at) * 64);
+              if (STAY == 1) zero_holes<D / 64>(smem + 2 * TB + R * HB + HB * in, r.docs + (base + at) * 64, r.t - (base + at) * 64);
+              fence_async_smem();
+              __syncwarp();
+            }
             tc_fence_after();
             mma_scores_wide<W>(lead, tS, dA, kTileBytes, Desc{dB.lo + (HB >> 4) * in, dB.hi}, HSub, id_s);
             mma_scores_wide<W>(lead, tS + 64, Desc{dA.lo + (TB >> 4), dA.hi}, kTileBytes, Desc{dC.lo + (HB >> 4) * in, dC.hi}, HSub,
@@ -738,7 +776,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
       if (what == 0) continue;
       // which pairs count is asked for while the scores are under way; of a masked half tile most warps have all pairs or none
       uint2 bits = make_uint2(~0u, ~0u);
-      bool edge = what == 1, none = false;
+      bool edge = what & 1, none = false;
       if (edge) {
         bits = STAY == 1 ? query_bits(r, hh * 64, ys) : key_bits(r, ys, hh * 64);
         none = __all_sync(0xffffffffu, (bits.x | bits.y) == 0);
@@ -793,11 +831,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
     asm volatile("bar.sync 1, %0;" ::"n"(128 * NW) : "memory");
     // rows that are not finite, each by one warp: rows and warps are told apart by their number modulo the warpgroups
     unsigned again = __ballot_sync(0xffffffffu, sFlag[row] != 0 && row % NW == wg);
-    for (; again; again &= again - 1) {
-      const int z = y0 + (row & 96) + __ffs(again) - 1;
-      if (STAY == 0) attend::redo_dq_row<__nv_bfloat16, D>(a, b, head, z);
-      else attend::redo_dkv_row<__nv_bfloat16, D>(a, b, head, z);
-    }
+    if (again) attend::redo_rows<STAY == 0 ? attend::kRedoDq : attend::kRedoDkv, __nv_bfloat16, D>(a, b, head, y0 + (row & 96), again);
   }
   drain_if_aborted(ctl);
   tc_fence_before();
