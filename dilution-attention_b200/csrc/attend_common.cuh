@@ -15,7 +15,7 @@
 
 #include <climits>
 
-#include "common.cuh"
+#include "lane_rows.cuh"
 
 namespace dil {
 namespace attend {
@@ -122,64 +122,9 @@ template <typename T> __device__ __forceinline__ const T* row_ptr(const void* ba
 // finite.  Values of padding (a negative id) are zeros in their tiles; a later token's or another document's are not, since rows of
 // the same tile may see them.  So a kernel whose finished rows are not finite asks here whether any such value is behind it, and only
 // then computes the row again, with masked pairs passed over: no cost to calls whose values are finite, little to those whose rows are
-// no numbers by right, and to the rows of a tile with such a value a walk over their pairs, a warp a row.  16 bytes of a row a lane, so
-// that a warp has several rows at once, kSteps times; each group of lanes keeps sums of its own, which are joined at the end.  (lse
-// has no such products and stays as it is.)  B1 H4 T4096 heads of 64, forward and backward, us: finite 380; a NaN in key 0 342, in
+// no numbers by right, and to the rows of a tile with such a value a walk over their pairs (lane_rows.cuh).  (lse has no such products
+// and stays as it is.)  B1 H4 T4096 heads of 64, forward and backward, us: finite 380; a NaN in key 0 342, in
 // key 2000 2080, in all of dout 264, in query 2000 2550, in a token of padding 276.
-template <typename T, int D> struct Lanes {
-  static constexpr int E = 16 / (int)sizeof(T), L = D / E, R = 32 / L;      // elements of a lane, lanes of a row, rows at once
-  static constexpr int kSteps = 4, kRows = R * kSteps;
-  int part, own;                                                            // the lane's elements, its row
-  __device__ __forceinline__ Lanes() : part((int)(threadIdx.x & 31) % L), own((int)(threadIdx.x & 31) / L) {}
-  __device__ __forceinline__ uint4 load(const T* rows, int row) const { return reinterpret_cast<const uint4*>(rows + (int64_t)row * D)[part]; }
-  __device__ __forceinline__ float of(const uint4& u, int e) const { return to_f32(reinterpret_cast<const T*>(&u)[e]); }
-  // x . y, in each of a row's lanes
-  __device__ __forceinline__ float dot(const uint4& x, const uint4& y) const {
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(of(x, e), of(y, e), s);
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-  }
-  static __device__ __forceinline__ float over_rows(float s) {
-#pragma unroll
-    for (int o = L; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-  }
-};
-template <typename T, int D> struct LaneSums : Lanes<T, D> {
-  using B = Lanes<T, D>;
-  float x[B::E] = {};
-  __device__ __forceinline__ void scale(float f) {
-#pragma unroll
-    for (int e = 0; e < B::E; ++e) x[e] *= f;
-  }
-  __device__ __forceinline__ void add(float f, const uint4& u) {
-#pragma unroll
-    for (int e = 0; e < B::E; ++e) x[e] = fmaf(f, this->of(u, e), x[e]);
-  }
-  // No feature of the row is a number any more.
-  __device__ __forceinline__ bool no_number() const {
-    unsigned bits = 0;
-#pragma unroll
-    for (int e = 0; e < B::E; ++e) bits |= (x[e] != x[e] ? 1u : 0u) << e;
-#pragma unroll
-    for (int o = B::L; o < 32; o <<= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, o);
-    return __all_sync(0xffffffffu, bits == (1u << B::E) - 1);
-  }
-  __device__ __forceinline__ void join(float f) {
-#pragma unroll
-    for (int e = 0; e < B::E; ++e) x[e] = B::over_rows(x[e]) * f;
-  }
-  __device__ __forceinline__ void store(T* p) const {
-    uint4 u;
-#pragma unroll
-    for (int e = 0; e < B::E; ++e) reinterpret_cast<T*>(&u)[e] = from_f32<T>(x[e]);
-    if (this->own == 0) reinterpret_cast<uint4*>(p)[this->part] = u;
-  }
-};
-
 // Keys that query i may see end at key_end, queries that may see key j begin at first_query.
 __device__ __forceinline__ int key_end(const Row& r, int i) { return min(r.t, max(i + 1, r.prefix)); }
 __device__ __forceinline__ int first_query(const Row& r, int j) { return j < r.prefix ? 0 : j; }
@@ -267,9 +212,7 @@ __device__ __forceinline__ void redo_forward_row(const Args& a, int b, int h, in
     if (o.no_number()) break;
   }
   // the groups' sums against one maximum
-  float top = m;
-#pragma unroll
-  for (int l = o.L; l < 32; l <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, l));
+  const float top = o.max_over_rows(m);
   const float f = exp2f(m - (top == -INFINITY ? 0.f : top));
   s = o.over_rows(s * f);
   o.scale(f);

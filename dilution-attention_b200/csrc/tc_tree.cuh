@@ -701,24 +701,6 @@ template <int D, int N> struct Draft {
   static_assert(N * D * 4 + 256 <= kSpace, "a chunk's output fits the ring");
 };
 
-// (maximum, sum) of a row over keys [j0, j1), one warp, key by key (tree_join.cuh has the reason).
-template <int D> __device__ __noinline__ float2 redo_chunk_stats(const tree::Args& a, int64_t nk, int r, int j0, int j1) {
-  const int lane = threadIdx.x & 31;
-  const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (nk * a.nodes + r) * D;
-  float m = -INFINITY, s = 0.f;
-  for (int j = j0; j < j1; ++j) {
-    const __nv_bfloat16* k = (const __nv_bfloat16*)a.kc + (nk * a.capacity + j) * D;
-    float z = 0.f;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) z = fmaf(to_f32(q[lane + 32 * e]), to_f32(k[lane + 32 * e]), z);
-    z = warp_sum(z) * (a.scale * kLog2e);
-    const float top = fmaxf(m, z), from = top == -INFINITY ? 0.f : top;
-    s = s * exp2f(m - from) + exp2f(z - from);
-    m = top;
-  }
-  return make_float2(m, s);
-}
-
 // grid = heads * 8, clusters of 8
 template <int D, int N>
 __global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const __grid_constant__ CUtensorMap map_k,
@@ -908,7 +890,7 @@ __global__ void __launch_bounds__(320, Draft<D, N>::kPerSm) draft_kernel(const _
       float m = warp_max(p.x);
       float s = warp_sum(lane < 2 * G ? p.y * fast_exp2(p.x - (m == -INFINITY ? 0.f : m)) : 0.f);
       if (!isfinite(s) || m == INFINITY) {
-        const float2 again = redo_chunk_stats<D>(a, nk, x, keys.x, keys.y);
+        const float2 again = tree::redo_stats<D>(a, nk, x, 0, 0.f, keys.x, keys.y);
         m = again.x;
         s = again.y;
       }

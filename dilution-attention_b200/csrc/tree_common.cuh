@@ -5,7 +5,7 @@
 // row r is node r % N of head r / N.  Keys are numbered [0, len) in the cache and len + x for node x.
 #pragma once
 
-#include "common.cuh"
+#include "lane_rows.cuh"
 
 namespace dil {
 namespace tree {
@@ -90,6 +90,97 @@ __device__ __forceinline__ float score(float dot, float scale, float cap, float 
   else
     z = dot * (scale * kLog2e);
   return fmaf(-slope2, far, z);
+}
+
+// A row that came out as no number, of a bf16 cache on the tensor cores: the block-diagonal scores of a scan multiply zeros with what
+// another quarter's keys hold, and its zero weights another quarter's values, infinities included.  These walk over the cached keys
+// [j0, j1) again, one warp a row (lane_rows.cuh), and end where nothing is a number any more.  Row r of key head nk, at position `at`.
+// 8 heads of 64, 12 nodes over 16384 keys, us: softmax step 53, with the last key or value infinite or NaN 1410, with the first key NaN
+// 54; dilution step 59, 930 and 59.
+template <int D> __device__ __noinline__ float2 redo_stats(const Args& a, int64_t nk, int r, int at, float slope2, int j0, int j1) {
+  using L = Lanes<__nv_bfloat16, D>;
+  const L l;
+  constexpr int U = 2 * L::kSteps;
+  const __nv_bfloat16* k = (const __nv_bfloat16*)a.kc + nk * a.capacity * D;
+  const uint4 q = l.load((const __nv_bfloat16*)a.q + (nk * a.group * a.nodes + r) * D, 0);
+  float m = -INFINITY, s = 0.f;
+  for (int j = j0; j < j1; j += U * L::R) {
+    uint4 x[U];
+    float z[U], top = m, sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = l.load(k, min(j + u * L::R + l.own, j1 - 1));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = j + u * L::R + l.own;
+      const float dot = l.dot(q, x[u]);
+      z[u] = key < j1 ? score<true>(dot, a.scale, a.cap, slope2, (float)(at - key)) : -INFINITY;
+      top = fmaxf(top, z[u]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum += exp2f(z[u] - ref);
+    s = s * exp2f(m - ref) + sum;
+    m = top;
+    if (__any_sync(0xffffffffu, s != s)) return make_float2(m, NAN);
+  }
+  const float top = L::max_over_rows(m);
+  return make_float2(top, L::over_rows(s * exp2f(m - (top == -INFINITY ? 0.f : top))));
+}
+// The same with values: P V's features lane, lane + 32, .. as well, against that maximum.  (Where it ends early m and s are of the keys
+// until then.)
+template <int D> struct Redone {
+  float m, s, o[D / 32];
+};
+template <int D> __device__ __noinline__ Redone<D> redo_softmax(const Args& a, int64_t nk, int r, int at, float slope2, int j0, int j1) {
+  using L = Lanes<__nv_bfloat16, D>;
+  constexpr int U = L::kSteps;
+  LaneSums<__nv_bfloat16, D> sums;
+  const __nv_bfloat16 *k = (const __nv_bfloat16*)a.kc + nk * a.capacity * D, *v = (const __nv_bfloat16*)a.vc + nk * a.capacity * D;
+  const uint4 q = sums.load((const __nv_bfloat16*)a.q + (nk * a.group * a.nodes + r) * D, 0);
+  float m = -INFINITY, s = 0.f;
+  for (int j = j0; j < j1; j += U * L::R) {
+    uint4 x[U], y[U];
+    float z[U], top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = min(j + u * L::R + sums.own, j1 - 1);
+      x[u] = sums.load(k, key);
+      y[u] = sums.load(v, key);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = j + u * L::R + sums.own;
+      const float dot = sums.dot(q, x[u]);
+      z[u] = key < j1 ? score<true>(dot, a.scale, a.cap, slope2, (float)(at - key)) : -INFINITY;
+      top = fmaxf(top, z[u]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top, f = exp2f(m - ref);
+    m = top;
+    s *= f;
+    sums.scale(f);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j + u * L::R + sums.own < j1) {
+        const float p = exp2f(z[u] - ref);
+        s += p;
+        sums.add(p, y[u]);
+      }
+    if (__any_sync(0xffffffffu, s != s) || sums.no_number()) break;
+  }
+  const float top = L::max_over_rows(m), f = exp2f(m - (top == -INFINITY ? 0.f : top));
+  s = L::over_rows(s * f);
+  sums.scale(f);
+  sums.join(1.f);
+  const int lane = threadIdx.x & 31;
+  Redone<D> got{top, s, {}};
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e)
+#pragma unroll
+    for (int c = 0; c < L::E; ++c) {
+      const float x = __shfl_sync(0xffffffffu, sums.x[c], (lane + 32 * e) / L::E);
+      if (lane % L::E == c) got.o[e] = x;
+    }
+  return got;
 }
 
 // The accepted branch: what tree_accept writes.  path: (batch or 1, accepted) nodes.

@@ -22,23 +22,6 @@ template <int D> struct LaneRow {
   }
 };
 
-// (maximum, sum) of a row over the cached keys, one warp, key by key.  For rows whose statistics came out as no number: the
-// block-diagonal scores of the scan multiply zeros with what another quarter's keys hold, infinities included.
-template <int D>
-__device__ __noinline__ float2 redo_stats(const Args& a, int64_t nk, int r, int depth, float slope2, int len) {
-  LaneRow<D> q, k;
-  q.load((const __nv_bfloat16*)a.q + (nk * a.group * a.nodes + r) * D);
-  float m = -INFINITY, s = 0.f;
-  for (int j = 0; j < len; ++j) {
-    k.load((const __nv_bfloat16*)a.kc + (nk * a.capacity + j) * D);
-    const float z = score<true>(q.dot(k), a.scale, a.cap, slope2, (float)(len + depth - j)), top = fmaxf(m, z);
-    const float from = top == -INFINITY ? 0.f : top;
-    s = s * exp2f(m - from) + exp2f(z - from);
-    m = top;
-  }
-  return make_float2(m, s);
-}
-
 // Threads of a block that has a warp for each of n nodes, 8 to 16 of them.
 inline int join_threads(int n) { return 32 * (n < 8 ? 8 : n > 16 ? 16 : n); }
 
@@ -131,40 +114,26 @@ __global__ void __launch_bounds__(512) join_softmax_kernel(Args a) {
       }
     };
     nodes();
+    float lse = from + log2f(s);
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) bad = bad || !isfinite(o[e] / s);
     if (__any_sync(0xffffffffu, bad)) {
-      // key by key, as in redo_stats, with the values
       const int len = cache_len(a.pos_dev, a.len, a.capacity);
-      LaneRow<D> qr, kr, vr;
-      qr.load((const __nv_bfloat16*)a.q + (head * n + x) * D);
-      float m = -INFINITY;
-      s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-      for (int j = 0; j < len; ++j) {
-        kr.load((const __nv_bfloat16*)a.kc + (nk * a.capacity + j) * D);
-        vr.load((const __nv_bfloat16*)a.vc + (nk * a.capacity + j) * D);
-        const float s1 = score<true>(qr.dot(kr), a.scale, a.cap, slope2, (float)(len + tree.depth[x] - j)), now = fmaxf(m, s1);
-        const float base = now == -INFINITY ? 0.f : now, f = exp2f(m - base), p = exp2f(s1 - base);
-        s = s * f + p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + (p == 0.f ? 0.f : p * vr.x[e]);
-        m = now;
-      }
-      top = fmaxf(m, nodes_top);
+      const Redone<D> again = redo_softmax<D>(a, nk, r, len + tree.depth[x], slope2, 0, len);
+      top = fmaxf(again.m, nodes_top);
       from = top == -INFINITY ? 0.f : top;
-      const float f = exp2f(m - from);
-      s *= f;
+      const float f = exp2f(again.m - from);
+      s = again.s * f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] *= f;
+      for (int e = 0; e < E; ++e) o[e] = again.o[e] * f;
       nodes();
+      if (!isfinite(lse)) lse = from + log2f(s);        // (it stands where the values alone were no numbers)
     }
     __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (head * n + x) * D + lane;
 #pragma unroll
     for (int e = 0; e < E; ++e) out[32 * e] = from_f32<__nv_bfloat16>(o[e] / s);
-    if (lane == 0) a.lse[head * n + x] = from + log2f(s);
+    if (lane == 0) a.lse[head * n + x] = lse;
   }
 }
 
@@ -197,7 +166,7 @@ __global__ void __launch_bounds__(512) join_bids_kernel(Args a, float* __restric
     s = warp_sum(s);
     if (!isfinite(s) || !isfinite(m)) {
       const int len = cache_len(a.pos_dev, a.len, a.capacity);
-      const float2 p = redo_stats<D>(a, nk, x, tree.depth[x], 0.f, len);
+      const float2 p = redo_stats<D>(a, nk, x, len + tree.depth[x], 0.f, 0, len);
       m = p.x;
       s = p.y;
     }
