@@ -24,6 +24,7 @@
 
 #include "once_per_device.cuh"
 #include "tc_common.cuh"
+#include "tensor_maps.cuh"
 
 namespace dil {
 namespace tc {
@@ -35,34 +36,6 @@ inline bool supported(int dtype, int precision, int d, int64_t q_offset) {
 }
 
 // ---------------------------------------------------------------- host: tensor maps
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return (EncodeTiledFn)p;
-  }();
-  return fn;
-}
-
-// cuTensorMapEncodeTiled is a driver entry point and wants a current context.  A thread that
-// has only selected the device (an autograd engine thread calling the backward first) may
-// not have one yet: a runtime call that touches the device binds the primary context.
-inline void ensure_context() {
-  static thread_local bool bound = false;
-  if (!bound) {
-    cudaFree(nullptr);
-    bound = true;
-  }
-}
-
 // Encoded maps are kept: a map depends only on (base, n, t, element type, box), and the same
 // tensors come back on every step of a training loop or every pass of a forward.
 struct MapKey {
@@ -105,8 +78,8 @@ inline int make_map(CUtensorMap* map, const void* base, int64_t n, int64_t t, ch
                     int feat = kHeadDim, int box_rows = kTileRows) {
   const MapKey key{base, n, t, 0, box_rows, feat};
   if (map_cache().find(key, map)) return 0;
-  ensure_context();
-  EncodeTiledFn fn = encode_fn();
+  bind_context();
+  EncodeTiled fn = encode_tiled();
   if (!fn) {
     snprintf(err, errlen, "cuTensorMapEncodeTiled is not available from the driver");
     return 3;
@@ -136,8 +109,8 @@ inline int make_map_f32(CUtensorMap* map, const void* base, int64_t n, int64_t t
                         int feat = kHeadDim, int box_rows = kTileRows, bool swizzle = true) {
   const MapKey key{base, n, t, swizzle ? 1 : 2, box_rows, feat};
   if (map_cache().find(key, map)) return 0;
-  ensure_context();
-  EncodeTiledFn fn = encode_fn();
+  bind_context();
+  EncodeTiled fn = encode_tiled();
   if (!fn) {
     snprintf(err, errlen, "cuTensorMapEncodeTiled is not available from the driver");
     return 3;

@@ -4,6 +4,7 @@
 
 #include "common.cuh"
 #include "tc_common.cuh"
+#include "tensor_maps.cuh"
 
 namespace dil {
 namespace tc {
@@ -64,34 +65,9 @@ template <int N> __device__ __forceinline__ void cap_scores(float* v, float pre,
 constexpr float kWideCap = 1024.f;
 
 // ---- tensor maps -----------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                CUtensorMapFloatOOBfill);
-inline EncodeTiled encode_tiled() {
-  static EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return (EncodeTiled)p;
-  }();
-  return fn;
-}
 // (n, t, d) bf16 rows as boxes {64 features, box rows, 1}, 128-byte swizzle; rows past t read as zero.  True: encoded.
 inline bool tile_map(CUtensorMap* map, const void* base, int64_t n, int64_t t, int d, int box) {
-  // the encoder wants a current context, which a thread that has only selected a device (one of autograd's) need not have yet; a
-  // thread that has one may be recording a graph, where cudaFree is not allowed
-  static thread_local bool bound = false;
-  if (!bound) {
-    typedef CUresult (*GetCurrent)(CUcontext*);
-    void* get = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    CUcontext current = nullptr;
-    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &get, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess ||
-        ((GetCurrent)get)(&current) != CUDA_SUCCESS || current == nullptr)
-      cudaFree(nullptr);
-    bound = true;
-  }
+  bind_context();
   EncodeTiled fn = encode_tiled();
   const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)t, (cuuint64_t)n};
   const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)t * d * 2};
