@@ -1,4 +1,4 @@
-"""softmax_attention with slopes of either sign: the bias is -slope |i - j| in every tile, masked or not, forward and backward.  Heads of
+"""softmax_attention and softmax_tree_step with slopes of either sign: the bias is -slope |i - j| in every tile, masked or not, forward and backward.  Heads of
 64 above 2560 tokens without documents have backward kernels of their own, which these lengths reach as well."""
 
 from __future__ import annotations
@@ -7,7 +7,9 @@ import pytest
 import torch
 
 from conftest import load_package
+from oracle import operators_oracle as O
 from test_gpu_masked import DEV, TYPES, call, check, documents_of, inputs
+from test_gpu_trees import CHAINS, TREE, case, check_accept, clone, within
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +58,17 @@ def test_a_prefix_that_is_one_number():
     want = call(x, prefix=torch.tensor([90, 90], device=DEV))
     assert all(torch.equal(a, b) for a, b in zip(want, call(x, prefix=90)))
     assert load_package().softmax_attention(*x[:3], prefix=0).shape == x[0].shape
+
+
+@pytest.mark.parametrize("dtype,dim", TYPES)
+@pytest.mark.parametrize("length", [0, 150, 5000])
+def test_trees_with_slopes_of_both_signs(length, dtype, dim):
+    """Over a cache: with a negative slope the first keys have the largest scores, which a scan comes to last."""
+    q, k, v, cache = case(1, 4, 2, len(TREE), dim, length, dtype)
+    slopes = torch.tensor([-0.25, 0.5, -0.001, 0.01], device=DEV)
+    out, draft = load_package().softmax_tree_step(q, k, v, cache, TREE, slopes=slopes)
+    want, off, bids, bids_off = O.tree_nodes(q, k, v, cache["k"], cache["v"], length, TREE, slopes=slopes)
+    within(out, want, off)
+    before, path = clone(cache), CHAINS["leaf"]
+    load_package().tree_accept(cache, draft, path)
+    check_accept(before, cache, k, v, bids, bids_off, [path], length)
