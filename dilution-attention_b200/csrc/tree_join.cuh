@@ -58,7 +58,7 @@ __device__ __forceinline__ void node_scores(float* z, const __nv_bfloat16* q, co
 // Dynamic shared memory: z [nodes][nodes + 1], then q, k, v [nodes][D + 2].
 template <int D> constexpr int join_softmax_smem(int n) { return (n * (n + 1) * 4 + 15) / 16 * 16 + 3 * n * (D + 2) * 2; }
 template <int D>
-__global__ void __launch_bounds__(512) join_softmax_kernel(Args a) {
+__global__ void __launch_bounds__(512, 2) join_softmax_kernel(Args a) {
   __shared__ Lineage tree;
   extern __shared__ __align__(16) float z[];
   const int n = a.nodes, rows = a.group * n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -75,17 +75,34 @@ __global__ void __launch_bounds__(512) join_softmax_kernel(Args a) {
   __syncthreads();
   wait_for_last();                    // the chunks' parts
   constexpr int E = D / 32;
-  for (int x = warp; x < n; x += (int)(blockDim.x >> 5)) {
+  const int warps = (int)(blockDim.x >> 5);
+  auto nodes_max = [&](int x) {
+    float top = -INFINITY;
+    for (int y = lane; y < n; y += 32) top = fmaxf(top, z[x * (n + 1) + y]);
+    return warp_max(top);
+  };
+  auto join_nodes = [&](int x, float from, float& s, float* o) {
+    for (unsigned long long left = tree.line[x]; left; left &= left - 1) {
+      const int y = __ffsll(left) - 1;
+      const float p = exp2f(z[x * (n + 1) + y] - from);
+      s += p;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(p, to_f32(v[y * (D + 2) + lane + 32 * e]), o[e]);
+    }
+  };
+  auto store = [&](int x, float s, const float* o) {
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (head * n + x) * D + lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[32 * e] = from_f32<__nv_bfloat16>(o[e] / s);
+  };
+  unsigned again = 0;                 // of the warp's nodes
+  for (int x = warp; x < n; x += warps) {
     const int r = (int)(head % a.group) * n + x;
     const float2* part = a.part + nk * a.chunks * rows + r;
-    const float* zx = z + x * (n + 1);
-    float nodes_top = -INFINITY;
-    for (int y = lane; y < n; y += 32) nodes_top = fmaxf(nodes_top, zx[y]);
-    nodes_top = warp_max(nodes_top);
-    float top = nodes_top, s = 0.f, o[E];
+    float top = nodes_max(x), s = 0.f, o[E];
     for (int y = lane; y < a.chunks; y += 32) top = fmaxf(top, part[(int64_t)y * rows].x);
     top = warp_max(top);
-    float from = top == -INFINITY ? 0.f : top;
+    const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
     for (int y0 = 0; y0 < a.chunks; y0 += 32) {
@@ -104,43 +121,33 @@ __global__ void __launch_bounds__(512) join_softmax_kernel(Args a) {
       }
     }
     s = warp_sum(s);
-    auto nodes = [&]() {
-      for (unsigned long long left = tree.line[x]; left; left &= left - 1) {
-        const int y = __ffsll(left) - 1;
-        const float p = exp2f(zx[y] - from);
-        s += p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(p, to_f32(v[y * (D + 2) + lane + 32 * e]), o[e]);
-      }
-    };
-    nodes();
-    float lse = from + log2f(s);
+    join_nodes(x, from, s, o);
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) bad = bad || !isfinite(o[e] / s);
-    if (__any_sync(0xffffffffu, bad)) {
-      const int len = cache_len(a.pos_dev, a.len, a.capacity);
-      const Redone<D> again = redo_softmax<D>(a, nk, r, len + tree.depth[x], slope2, 0, len);
-      top = fmaxf(again.m, nodes_top);
-      from = top == -INFINITY ? 0.f : top;
-      const float f = exp2f(again.m - from);
-      s = again.s * f;
+    if (__any_sync(0xffffffffu, bad)) again |= 1u << x / warps;
+    store(x, s, o);
+    if (lane == 0) a.lse[head * n + x] = from + log2f(s);
+  }
+  // rows that are no numbers, over the cached keys again; behind all others, whose registers the walk does not cost there
+  for (; again; again &= again - 1) {
+    const int x = warp + warps * (__ffs(again) - 1), r = (int)(head % a.group) * n + x, len = cache_len(a.pos_dev, a.len, a.capacity);
+    const Redone<D> got = redo_softmax<D>(a, nk, r, len + tree.depth[x], slope2, 0, len);
+    const float top = fmaxf(got.m, nodes_max(x)), from = top == -INFINITY ? 0.f : top, f = exp2f(got.m - from);
+    float s = got.s * f, o[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = again.o[e] * f;
-      nodes();
-      if (!isfinite(lse)) lse = from + log2f(s);        // (it stands where the values alone were no numbers)
-    }
-    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (head * n + x) * D + lane;
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[32 * e] = from_f32<__nv_bfloat16>(o[e] / s);
-    if (lane == 0) a.lse[head * n + x] = lse;
+    for (int e = 0; e < E; ++e) o[e] = got.o[e] * f;
+    join_nodes(x, from, s, o);
+    store(x, s, o);
+    // (lse stands where the values alone were no numbers)
+    if (lane == 0 && !isfinite(a.lse[head * n + x])) a.lse[head * n + x] = from + log2f(s);
   }
 }
 
 // lse of a dilution layer's nodes, and their shares of the nodes' own keys: (batch * heads, nodes, nodes), 0 where a node
 // does not see another.  One block per head.
 template <int D>
-__global__ void __launch_bounds__(512) join_bids_kernel(Args a, float* __restrict__ shares) {
+__global__ void __launch_bounds__(512, 2) join_bids_kernel(Args a, float* __restrict__ shares) {
   __shared__ Lineage tree;
   __shared__ __nv_bfloat16 q[kMaxNodes * (D + 2)], k[kMaxNodes * (D + 2)];
   extern __shared__ float z[];                            // [nodes][nodes + 1]
@@ -154,22 +161,8 @@ __global__ void __launch_bounds__(512) join_bids_kernel(Args a, float* __restric
   node_scores<D>(z, q, k, tree, a, 0.f);
   __syncthreads();
   wait_for_last();                    // the chunks' statistics
-  for (int x = warp; x < n; x += (int)(blockDim.x >> 5)) {
-    const float2* part = a.part + nk * a.chunks * n + x;
-    float m = -INFINITY, s = 0.f;
-    for (int y = lane; y < a.chunks; y += 32) m = fmaxf(m, part[(int64_t)y * n].x);
-    m = warp_max(m);
-    for (int y = lane; y < a.chunks; y += 32) {
-      const float2 p = part[(int64_t)y * n];
-      s = fmaf(p.y, exp2f(p.x - (m == -INFINITY ? 0.f : m)), s);
-    }
-    s = warp_sum(s);
-    if (!isfinite(s) || !isfinite(m)) {
-      const int len = cache_len(a.pos_dev, a.len, a.capacity);
-      const float2 p = redo_stats<D>(a, nk, x, len + tree.depth[x], 0.f, 0, len);
-      m = p.x;
-      s = p.y;
-    }
+  const int warps = (int)(blockDim.x >> 5);
+  auto finish = [&](int x, float m, float s) {          // with the nodes that x sees
     float top = m;
     for (int y = lane; y < n; y += 32) top = fmaxf(top, z[x * (n + 1) + y]);
     top = warp_max(top);
@@ -181,6 +174,25 @@ __global__ void __launch_bounds__(512) join_bids_kernel(Args a, float* __restric
       lse[x] = from + log2f(s);
       a.lse[nk * n + x] = lse[x];
     }
+  };
+  unsigned again = 0;                 // of the warp's nodes: those whose statistics are no numbers
+  for (int x = warp; x < n; x += warps) {
+    const float2* part = a.part + nk * a.chunks * n + x;
+    float m = -INFINITY, s = 0.f;
+    for (int y = lane; y < a.chunks; y += 32) m = fmaxf(m, part[(int64_t)y * n].x);
+    m = warp_max(m);
+    for (int y = lane; y < a.chunks; y += 32) {
+      const float2 p = part[(int64_t)y * n];
+      s = fmaf(p.y, exp2f(p.x - (m == -INFINITY ? 0.f : m)), s);
+    }
+    s = warp_sum(s);
+    if (!isfinite(s) || m == INFINITY) again |= 1u << x / warps;
+    finish(x, m, s);
+  }
+  for (; again; again &= again - 1) {
+    const int x = warp + warps * (__ffs(again) - 1), len = cache_len(a.pos_dev, a.len, a.capacity);
+    const float2 p = redo_stats<D>(a, nk, x, len + tree.depth[x], 0.f, 0, len);
+    finish(x, p.x, p.y);
   }
   __syncthreads();
   // a key's demand through the tree, in the nodes' order: what a node leaves stands where its score stood
