@@ -13,10 +13,12 @@
 //             place of five, and no result depends on an order of atomic additions.
 //
 // What bounds them, per pair of tiles of 128 x 64: 512 cycles for one exponential a score on the special-function unit (16 a
-// clock), and 128 (heads of 64: 64) cycles for each product on the tensor pipe: 2 forward, 3 and 4 backward.  Measured, forward /
-// dk, dv / dq in us: n = 64, T = 8192, heads of 64 773 / 1066 / 881 (forward 0.62 of the exponentials' rate), documents of 700
-// tokens 220 / 235 / 185, where a block of a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads
-// of 128, capped 830 / 1020 / 795.
+// clock), and 256 (heads of 64: 128) cycles for each product on the tensor pipe, 8192 operations a clock: 2 forward, 4 for dk and dv, 3
+// for dq.  So heads of 64 are bound by the exponentials forward and for dq and by both alike for dk and dv, heads of 128 by both
+// alike forward and by the tensor pipe in the backward (1024 and 768 cycles).  Measured, forward / dk, dv / dq in us: n = 64, T = 8192,
+// heads of 64 774 / 1079 / 896 (forward 0.62 of the exponentials' rate), documents of 700 tokens 231 / 246 / 196, where a block of
+// a few half tiles is mostly its start and its end; n = 32 (8 key heads), T = 8192, heads of 128, capped 834 / 1030 / 840 (0.39 / 0.64 /
+// 0.58 of the burst rate of a large bf16 product for the products that they take).
 #pragma once
 
 #include "attend_common.cuh"
@@ -96,18 +98,25 @@ __device__ __forceinline__ int2 all_of(const int2* range, int warps) {
   return make_int2((int)uniform(__reduce_min_sync(0xffffffffu, x.x)), (int)uniform(__reduce_max_sync(0xffffffffu, x.y)));
 }
 
-// Zeros for the padding among the 64 tokens (of `tokens` left) with ids docs, in their half tile of SUB sub-tiles: what the values of padding are
-// multiplied by is 0, which makes no number of those that are not finite.  One warp, in front of the half tile's products.
-template <int SUB> __device__ __noinline__ void zero_holes(uint8_t* tile, const int* docs, int tokens) {
-  const int lane = threadIdx.x & 31;
+// Zeros for the padding among the 64 tokens (of `tokens` left) with ids docs, in their half tiles of SUB sub-tiles, two of them if `both`
+// and that many bytes apart: what the values of padding are multiplied by is 0, which makes no number of those that are not
+// finite.  One warp, in front of the half tile's products.
+template <int SUB> __device__ __noinline__ void zero_holes(uint8_t* tile, uint32_t apart, bool both, const int* docs, int tokens) {
+  const int lane = threadIdx.x & 31, id0 = lane < tokens ? docs[lane] : 0, id1 = lane + 32 < tokens ? docs[lane + 32] : 0;
+  const uint32_t low = __ballot_sync(0xffffffffu, id0 < 0), high = __ballot_sync(0xffffffffu, id1 < 0);
+#pragma unroll 4
+  for (int x = lane; x < 64 * 8; x += 32) {              // 16 bytes of a row's 128 in a sub-tile
+    const int row = x >> 3;
+    if (!((row < 32 ? low : high) >> (row & 31) & 1)) continue;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int x = 32 * half + lane;
-    for (uint32_t left = __ballot_sync(0xffffffffu, x < tokens && docs[x] < 0); left; left &= left - 1) {
-      const int row = 32 * half + __ffs(left) - 1;
-      if (lane < 8 * SUB) *reinterpret_cast<uint4*>(tile + (lane >> 3) * (kTileBytes / 2) + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    for (int sub = 0; sub < SUB; ++sub) {
+      uint8_t* at = tile + sub * (kTileBytes / 2) + 16 * x;
+      *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+      if (both) *reinterpret_cast<uint4*>(at + apart) = make_uint4(0, 0, 0, 0);
     }
   }
+  fence_async_smem();
+  __syncwarp();
 }
 
 template <int D> struct AttendForward {
@@ -358,9 +367,7 @@ __global__ void __launch_bounds__(AttendForward<D>::kThreads, D == 64 ? 2 : 1) a
         if (e < nh) {
           mbar_wait_warp(kfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
           if (hole >> (hh & 31) & 1) {
-            zero_holes<D / 64>(smem + TB + R * HB + HB * in, r.docs + hh * 64, r.t - hh * 64);
-            fence_async_smem();
-            __syncwarp();
+            zero_holes<D / 64>(smem + TB + R * HB + HB * in, 0, false, r.docs + hh * 64, r.t - hh * 64);
           }
         }
         const int w = e & 1;
@@ -724,10 +731,7 @@ __global__ void __launch_bounds__(AttendBackward<D, STAY, NW>::kThreads, AttendB
           mbar_wait_warp(bfull + 8 * in, phase, ctl, &g_attend_status, kErrWaitTma);
           if (word >> (at & 31) & 1) {
             if (F::kHoles && hole >> (at & 31) & 1) {
-              zero_holes<D / 64>(smem + 2 * TB + HB * in, r.docs + (base + at) * 64, r.t - (base + at) * 64);
-              if (STAY == 1) zero_holes<D / 64>(smem + 2 * TB + R * HB + HB * in, r.docs + (base + at) * 64, r.t - (base + at) * 64);
-              fence_async_smem();
-              __syncwarp();
+              zero_holes<D / 64>(smem + 2 * TB + HB * in, R * HB, STAY == 1, r.docs + (base + at) * 64, r.t - (base + at) * 64);
             }
             tc_fence_after();
             mma_scores_wide<W>(lead, tS, dA, kTileBytes, Desc{dB.lo + (HB >> 4) * in, dB.hi}, HSub, id_s);
