@@ -72,7 +72,8 @@ def attention(q, k, v, dout=None, softcap=None, slopes=None, documents=None, pre
             slack = 2 * wrong.masked_fill(~see, 0.0).amax(-1, keepdim=True) + 2.0 ** -20
             out = p @ vs
             spread = p @ vs.abs()
-            far_out = (u + slack) * spread + u * out.abs()
+            # weights off by e_j each, divided by their own sum, leave sum p_j e_j (v_j - out), at most u (spread + |out|); out's rounding is u |out|
+            far_out = (u + slack) * spread + 2 * u * out.abs()
             got[0][b, h], off[0][b, h] = out, far_out
             if dout is None:
                 continue
