@@ -60,6 +60,21 @@ def test_a_prefix_that_is_one_number():
     assert load_package().softmax_attention(*x[:3], prefix=0).shape == x[0].shape
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_arguments_in_other_forms(dtype):
+    """Slopes of other types and as a list, documents and prefixes that are views with strides."""
+    x = inputs(2, 4, 2, 150, 64, torch.bfloat16)
+    slopes = torch.tensor([-0.25, 0.125, 0.5, -0.0625], device=DEV)
+    docs = documents_of(2, 150, 40, seed=3, pad=5)
+    prefix = torch.tensor([20, 90], device=DEV)
+    want = call(x, slopes=slopes, documents=docs, prefix=prefix)
+    strided = torch.stack((docs, docs + 7), 2).transpose(0, 1).contiguous().transpose(0, 1)[..., 0]
+    apart = torch.stack((prefix, prefix + 1), 1)[:, 0]
+    assert not strided.is_contiguous() and not apart.is_contiguous()
+    for some in (slopes.to(dtype), slopes.tolist(), slopes.to(dtype)[:, None].expand(4, 2)[:, 1]):
+        assert all(torch.equal(a, b) for a, b in zip(want, call(x, slopes=some, documents=strided, prefix=apart)))
+
+
 @pytest.mark.parametrize("dtype,dim", TYPES)
 @pytest.mark.parametrize("length", [0, 150, 5000])
 def test_trees_with_slopes_of_both_signs(length, dtype, dim):

