@@ -124,7 +124,8 @@ template <typename T> __device__ __forceinline__ const T* row_ptr(const void* ba
 // then computes the row again, with masked pairs passed over: no cost to calls whose values are finite, little to those whose rows are
 // no numbers by right, and to the rows of a tile with such a value a walk over their pairs (lane_rows.cuh).  (lse has no such products
 // and stays as it is.)  B1 H4 T4096 heads of 64, forward and backward, us: finite 380; a NaN in key 0 342, in
-// key 2000 2080, in all of dout 264, in query 2000 2550, in a token of padding 276.
+// key 2000 2080, in all of dout 264, in query 2000 2550, in the first token's dout 4620, in a token of padding 276.
+
 // Keys that query i may see end at key_end, queries that may see key j begin at first_query.
 __device__ __forceinline__ int key_end(const Row& r, int i) { return min(r.t, max(i + 1, r.prefix)); }
 __device__ __forceinline__ int first_query(const Row& r, int j) { return j < r.prefix ? 0 : j; }

@@ -11,7 +11,9 @@ template <typename T, int D> struct Lanes {
   static constexpr int kSteps = 4, kRows = R * kSteps;
   int part, own;                                                            // the lane's elements, its row
   __device__ __forceinline__ Lanes() : part((int)(threadIdx.x & 31) % L), own((int)(threadIdx.x & 31) / L) {}
-  __device__ __forceinline__ uint4 load(const T* rows, int row) const { return reinterpret_cast<const uint4*>(rows + (int64_t)row * D)[part]; }
+  __device__ __forceinline__ uint4 load(const T* rows, int row) const {
+    return reinterpret_cast<const uint4*>(rows + (int64_t)row * D)[part];
+  }
   __device__ __forceinline__ float of(const uint4& u, int e) const { return to_f32(reinterpret_cast<const T*>(&u)[e]); }
   // x . y, in each of a row's lanes
   __device__ __forceinline__ float dot(const uint4& x, const uint4& y) const {
